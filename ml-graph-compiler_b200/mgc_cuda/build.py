@@ -11,12 +11,13 @@ from __future__ import annotations
 
 import hashlib
 import os
+import re
 import shutil
 import subprocess
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
-from mgc_cuda import _reference  # noqa: F401
-from ml_graph_compiler.errors import CodegenError
+from mgc_cuda._errors import CodegenError
 
 PACKAGE_DIR = Path(__file__).resolve().parent
 SRC_DIR = PACKAGE_DIR.parent / "csrc"
@@ -66,17 +67,24 @@ def library_path() -> Path:
     return LIB_DIR / LIB_NAME
 
 
-def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the library if the sources changed; return its path."""
-    flags = nvcc_flags()
-    key = source_key(flags)
-    lib = library_path()
-    stamp = lib.with_suffix(".key")
-    if not force and lib.exists() and stamp.exists() and stamp.read_text().strip() == key:
-        return lib
-    LIB_DIR.mkdir(parents=True, exist_ok=True)
-    tmp = lib.with_name(f"{LIB_NAME}.tmp{os.getpid()}")
-    cmd = [find_nvcc(), *flags, str(SRC_DIR / "mgc_cuda.cu"), "-o", str(tmp)]
+def _object_key(source: Path, flags: list[str]) -> str:
+    """Key of one source file's object: its text, that of every header it includes, the flags."""
+    seen: dict[Path, bytes] = {}
+    todo = [source]
+    while todo:
+        path = todo.pop()
+        if path in seen:
+            continue
+        seen[path] = path.read_bytes()
+        for name in re.findall(rb'^\s*#include\s+"([^"]+)"', seen[path], flags=re.M):
+            todo += [d / name.decode() for d in (SRC_DIR, INCLUDE_DIR) if (d / name.decode()).exists()]
+    h = hashlib.sha256(" ".join(flags).encode())
+    for path in sorted(seen):
+        h.update(path.name.encode() + seen[path])
+    return h.hexdigest()[:20]
+
+
+def _run(cmd: list[str], verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd))
     proc = subprocess.run(cmd, capture_output=True, text=True, check=False)
@@ -84,6 +92,36 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         raise CodegenError(f"nvcc failed:\n{' '.join(cmd)}\n{proc.stderr[-6000:]}")
     if verbose and proc.stderr:
         print(proc.stderr[-6000:])
+
+
+def _compile(source: Path, flags: list[str], force: bool, verbose: bool) -> Path:
+    """The object of one source file, compiled if its key changed."""
+    obj = LIB_DIR / f"{source.stem}.o"
+    stamp = LIB_DIR / f"{source.stem}.o.key"
+    key = _object_key(source, flags)
+    if not force and obj.exists() and stamp.exists() and stamp.read_text().strip() == key:
+        return obj
+    tmp = obj.with_name(f"{obj.name}.tmp{os.getpid()}")
+    _run([find_nvcc(), *(f for f in flags if f != "-shared"), "-c", str(source), "-o", str(tmp)], verbose)
+    tmp.replace(obj)
+    stamp.write_text(key + "\n")
+    return obj
+
+
+def build(force: bool = False, verbose: bool = False) -> Path:
+    """Compile the library if the sources changed (its source files side by side); return its path."""
+    flags = nvcc_flags()
+    key = source_key(flags)
+    lib = library_path()
+    stamp = lib.with_suffix(".key")
+    if not force and lib.exists() and stamp.exists() and stamp.read_text().strip() == key:
+        return lib
+    LIB_DIR.mkdir(parents=True, exist_ok=True)
+    units = sorted(SRC_DIR.glob("*.cu"))
+    with ThreadPoolExecutor(max_workers=len(units)) as pool:
+        objects = list(pool.map(lambda u: _compile(u, flags, force, verbose), units))
+    tmp = lib.with_name(f"{LIB_NAME}.tmp{os.getpid()}")
+    _run([find_nvcc(), *flags, *map(str, objects), "-o", str(tmp)], verbose)
     tmp.replace(lib)
     stamp.write_text(key + "\n")
     return lib

@@ -23,86 +23,11 @@ from typing import Any
 import numpy as np
 
 from mgc_cuda import _reference  # noqa: F401
-from mgc_cuda import build as _build
 from mgc_cuda.lowering import BLOB_ALIGN, Chunk, Launch, LoweredModel, input_slice_plan, lower_graph
-from ml_graph_compiler.errors import CodegenError, GraphError
+from mgc_cuda.native import SIGNATURES, check, last_error, library  # noqa: F401
+from ml_graph_compiler.errors import GraphError
 from ml_graph_compiler.ir import Graph, TensorType, numpy_dtype
 from ml_graph_compiler.memory import Strategy
-
-_LIB: ctypes.CDLL | None = None
-_LIB_LOCK = threading.Lock()
-
-# Every symbol include/mgc_cuda.h declares, with its ctypes signature.
-_VP, _I, _I64, _F, _D = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_double
-SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
-    "mgc_cuda_abi_version": (_I, []),
-    "mgc_cuda_last_error": (ctypes.c_char_p, []),
-    "mgc_cuda_device_supported": (_I, [_I]),
-    "mgc_cuda_create": (_I, [_VP, _I, _VP, _I64, _VP, _I64, _I64, _I64, _VP, _I, _VP, _I, _I, ctypes.POINTER(_VP)]),
-    "mgc_cuda_run": (_I, [_VP, _VP, _VP]),
-    "mgc_cuda_run_device": (_I, [_VP, _I]),
-    "mgc_cuda_set_input_chunks": (_I, [_VP, _I, _I, _I64, _VP, _I]),
-    "mgc_cuda_input_ptr": (_VP, [_VP, _I]),
-    "mgc_cuda_output_ptr": (_VP, [_VP, _I]),
-    "mgc_cuda_stream": (_VP, [_VP]),
-    "mgc_cuda_profile": (_I, [_VP, ctypes.POINTER(_D), _I]),
-    "mgc_cuda_launch_count": (_I, [_VP]),
-    "mgc_cuda_gemm_paths": (_I, [_VP, ctypes.POINTER(ctypes.c_int32), _I]),
-    "mgc_cuda_arena_bytes": (_I64, [_VP]),
-    "mgc_cuda_weights_bytes": (_I64, [_VP]),
-    "mgc_cuda_destroy": (None, [_VP]),
-    "mgc_cuda_execute": (_I, [_VP, _I, _VP, _I64, _VP, _VP]),
-    "mgc_cuda_gemm": (
-        _I,
-        [_I, _I, _I, _I, _VP, _I64, _I64, _I64, _VP, _I64, _I64, _I64, _VP, _I64, _I64, _F, _VP, _I, _VP,
-         _I64, _I64, _F, _I, _F, _F, _I, _VP],
-    ),
-    "mgc_cuda_conv_nhwc": (
-        _I,
-        [_I] * 15 + [_VP, _VP, _VP, _VP, _I, _F, _F, _VP, _I, _VP],
-    ),
-    "mgc_cuda_conv_nhwc_noalloc": (_I, [_I] * 15 + [_VP, _VP, _VP, _VP, _I, _F, _F, _VP, _VP]),
-    "mgc_cuda_depthwise_nhwc": (_I, [_I] * 14 + [_VP, _VP, _VP, _VP, _I, _F, _F, _VP, _VP]),
-    "mgc_cuda_pool_nhwc": (_I, [_I] * 18 + [_VP, _VP, _VP]),
-    "mgc_cuda_reduce_mid": (_I, [_I, _I64, _I64, _I64, _VP, _VP, _VP]),
-    "mgc_cuda_softmax": (_I, [_I64, _I64, _I64, _VP, _VP, _I, _VP]),
-    "mgc_cuda_layer_norm": (_I, [_I64, _I64, _VP, _VP, _VP, _F, _VP, _VP]),
-}
-
-
-def library(path: str | Path | None = None) -> ctypes.CDLL:
-    """Load libmgc_cuda.so (building it first if its sources changed) and declare signatures."""
-    global _LIB
-    with _LIB_LOCK:
-        if _LIB is not None and path is None:
-            return _LIB
-        lib_path = Path(path) if path is not None else _build.library_path()
-        if path is None and not lib_path.exists():
-            lib_path = _build.build()
-        lib = ctypes.CDLL(str(lib_path))
-        for name, (res, args) in SIGNATURES.items():
-            fn = getattr(lib, name)
-            fn.restype = res
-            fn.argtypes = args
-        if path is None:
-            _LIB = lib
-        return lib
-
-
-def last_error(lib: ctypes.CDLL | None = None) -> str:
-    raw = (lib or library()).mgc_cuda_last_error()
-    return raw.decode() if raw else ""
-
-
-def check(status: int, what: str, lib: ctypes.CDLL | None = None) -> None:
-    """Raise the reference's exception types for a non-zero ABI status."""
-    if status == 0:
-        return
-    msg = last_error(lib)
-    if status == 1:
-        raise GraphError(msg or "compiled model reported an out-of-range Gather index")
-    raise CodegenError(f"{what} failed with status {status}: {msg}")
-
 
 @dataclass
 class CudaCompileReport:

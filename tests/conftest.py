@@ -22,6 +22,26 @@ def pytest_configure(config: pytest.Config) -> None:
     config.addinivalue_line("markers", "slow: whole benchmark-size models")
 
 
+class _Module(pytest.Module):
+    """A test module; skipped, with the reason, when the reference compiler it imports is absent
+    (the kernel-ABI tests of the paged-cache operators need none)."""
+
+    def collect(self):  # type: ignore[no-untyped-def]
+        try:
+            return list(super().collect())
+        except self.CollectError as e:
+            if REFERENCE_MISSING in str(e):
+                pytest.skip("the reference compiler is not installed", allow_module_level=True)
+            raise
+
+
+REFERENCE_MISSING = "the reference compiler this backend plugs into) is not importable"
+
+
+def pytest_pycollect_makemodule(module_path: Path, parent: pytest.Collector) -> pytest.Module:
+    return _Module.from_parent(parent, path=module_path)
+
+
 def gpu_available() -> bool:
     try:
         import torch
