@@ -60,7 +60,9 @@ enum {
     MGC_I32 = 3,
     MGC_I8 = 4,
     MGC_U8 = 5,
-    MGC_BOOL = 6
+    MGC_BOOL = 6,
+    MGC_F16 = 7,  /* half and bfloat16: the paged-cache operators only (the graph's types end */
+    MGC_BF16 = 8  /* at MGC_BOOL) */
 };
 
 /* ---- activations fused into epilogues (mgc_runtime.h:93-101, ops.py:894-911) ---------------- */
@@ -302,6 +304,81 @@ int mgc_cuda_softmax(int64_t outer, int64_t n, int64_t inner, const float *x, fl
                      int log_softmax, void *stream);
 int mgc_cuda_layer_norm(int64_t rows, int64_t cols, const float *x, const float *scale,
                         const float *bias, float eps, float *y, void *stream);
+
+/* ---- paged cache of keys and values ------------------------------------------------------------
+ * No counterpart in the reference, whose compiled GPT-2 recomputes every token of a fixed length.
+ * The cache is two arrays of pages, k and v, of the same strides: channel c of head h of token t of
+ * page n at k[n * page_stride + t * token_stride + h * head_stride + c] (strides in elements). A
+ * batch is `batch` sequences whose new tokens are packed along one axis of `tokens` rows:
+ * sequence b has rows q_starts[b] .. q_starts[b + 1] - 1 and, these included, kv_lens[b] cached
+ * positions, position p in row p % page_size of page block_table[b * table_stride + p / page_size].
+ * Its i-th new token is at position kv_lens[b] - (q_starts[b + 1] - q_starts[b]) + i. block_table,
+ * kv_lens and q_starts are device arrays that only the kernels read. A page number outside
+ * [0, pages), a position past table_pages pages or one past the rotation table sets *status_dev (when
+ * not NULL) to MGC_CUDA_GATHER_OOB; nothing is read or written there. All fields are 8 bytes wide. */
+typedef struct {
+    void *k, *v;
+    int64_t pages, page_stride, token_stride, head_stride;
+    int64_t dtype;       /* of the pages: MGC_F32, MGC_F16 or MGC_BF16 */
+    int64_t kv_heads, head_dim, page_size;
+    const int32_t *block_table;
+    int64_t table_stride, table_pages;  /* entries between sequences' rows; entries of a row */
+    const int32_t *kv_lens, *q_starts;  /* [batch], [batch + 1] */
+    int64_t batch, tokens;
+    int32_t *status_dev;
+} mgc_cuda_paged;
+
+/* mgc_cuda_kv_append: writes the new tokens' keys and values into their cache positions, channels
+ * [0, rot) of every key rotated by its position p on the way; with q, the rotated queries go to
+ * q_out. Pair i of the rotated channels (i and i + rot/2, or 2i and 2i + 1 when `interleaved`):
+ *   x1' = x1 cos[p][i] - x2 sin[p][i],   x2' = x2 cos[p][i] + x1 sin[p][i],
+ * cos and sin fp32 tables of `positions` rows of rot/2 values, table_row elements apart. rot 0:
+ * no rotation. The sources are of src_dtype, the pages' type or MGC_F32; q_out is of the pages'
+ * type and may be q itself (same strides, src_dtype the pages' type). Arithmetic in fp32, rounded
+ * once. A token at a negative position (more new tokens than cached positions) is not cached, and
+ * its query is copied unrotated. */
+typedef struct {
+    mgc_cuda_paged paged;
+    int64_t src_dtype;
+    const void *k;
+    int64_t k_token_stride, k_head_stride;
+    const void *v;
+    int64_t v_token_stride, v_head_stride;
+    const void *q;  /* NULL: no queries */
+    int64_t q_token_stride, q_head_stride, q_heads;
+    void *q_out;
+    int64_t qo_token_stride, qo_head_stride;
+    const float *cos, *sin;
+    int64_t table_row, positions, rot, interleaved;
+} mgc_cuda_kv_append_args;
+
+int mgc_cuda_kv_append(const mgc_cuda_kv_append_args *args, void *stream);
+
+/* mgc_cuda_paged_attention: out[t][h] = sum_j w_j v_j, w the softmax over the visible positions j of
+ * scale * q[t][h] . k_j, key head h / (q_heads / kv_heads). Visible to a token at position p:
+ * j < kv_lens[b]; with `causal`, j <= p; with window > 0 (causal only), j > p - window. A token
+ * with no visible position gets zeros. q and out are of the pages' type. Cache rows that no token of
+ * their sequence may see are not used, whatever they hold. max_q and max_kv bound the sequences' new
+ * tokens and positions (host values that size the launch; a longer sequence sets *status_dev to
+ * MGC_CUDA_BAD_ARGUMENT and its rows past the bound are left unwritten or see only the bound's
+ * keys). `workspace` holds partial results when the keys of a row are split over several blocks:
+ * mgc_cuda_paged_attention_workspace says how many bytes (0: none), for the current device. A wait
+ * that runs out sets *status_dev to MGC_CUDA_TIMEOUT. */
+typedef struct {
+    mgc_cuda_paged paged;
+    const void *q;
+    int64_t q_token_stride, q_head_stride, q_heads;
+    void *out;
+    int64_t o_token_stride, o_head_stride;
+    int64_t max_q, max_kv;
+    double scale;
+    int64_t causal, window;
+    void *workspace;
+    int64_t workspace_bytes;
+} mgc_cuda_paged_attention_args;
+
+int mgc_cuda_paged_attention(const mgc_cuda_paged_attention_args *args, void *stream);
+int64_t mgc_cuda_paged_attention_workspace(const mgc_cuda_paged_attention_args *args);
 
 #ifdef __cplusplus
 }

@@ -53,6 +53,9 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "mgc_cuda_reduce_mid": (_I, [_I, _I64, _I64, _I64, _VP, _VP, _VP]),
     "mgc_cuda_softmax": (_I, [_I64, _I64, _I64, _VP, _VP, _I, _VP]),
     "mgc_cuda_layer_norm": (_I, [_I64, _I64, _VP, _VP, _VP, _F, _VP, _VP]),
+    "mgc_cuda_kv_append": (_I, [_VP, _VP]),
+    "mgc_cuda_paged_attention": (_I, [_VP, _VP]),
+    "mgc_cuda_paged_attention_workspace": (_I64, [_VP]),
 }
 
 
