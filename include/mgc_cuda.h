@@ -37,6 +37,7 @@ enum {
     MGC_CUDA_BAD_ARGUMENT = 2,   /* malformed launch list, size mismatch, unsupported parameter */
     MGC_CUDA_UNSUPPORTED = 3,    /* a launch kind / dtype / shape this build has no kernel for */
     MGC_CUDA_TIMEOUT = 4,        /* a bounded device wait gave up (kernel returned early) */
+    MGC_CUDA_NEEDS_WORKSPACE = 5, /* the call needs a larger workspace; nothing ran */
     MGC_CUDA_CUDA_ERROR = 100    /* >= 100: 100 + cudaError_t of the failing CUDA call */
 };
 
@@ -358,12 +359,13 @@ int mgc_cuda_kv_append(const mgc_cuda_kv_append_args *args, void *stream);
  * scale * q[t][h] . k_j, key head h / (q_heads / kv_heads). Visible to a token at position p:
  * j < kv_lens[b]; with `causal`, j <= p; with window > 0 (causal only), j > p - window. A token
  * with no visible position gets zeros. q and out are of the pages' type. Cache rows that no token of
- * their sequence may see are not used, whatever they hold. max_q and max_kv bound the sequences' new
- * tokens and positions (host values that size the launch; a longer sequence sets *status_dev to
- * MGC_CUDA_BAD_ARGUMENT and its rows past the bound are left unwritten or see only the bound's
- * keys). `workspace` holds partial results when the keys of a row are split over several blocks:
- * mgc_cuda_paged_attention_workspace says how many bytes (0: none), for the current device. A wait
- * that runs out sets *status_dev to MGC_CUDA_TIMEOUT. */
+ * their sequence may see are not used, whatever they hold. max_q and max_kv, the longest sequence's
+ * new tokens and positions, are host values that size the launch: longer sequences are computed
+ * too, by fewer blocks than they could use. `workspace` (16-byte aligned) holds partial results when
+ * a row's keys are split over many blocks; when it is smaller than
+ * mgc_cuda_paged_attention_workspace says (0 for most calls), the call returns
+ * MGC_CUDA_NEEDS_WORKSPACE and nothing runs. A wait that runs out sets *status_dev to
+ * MGC_CUDA_TIMEOUT. */
 typedef struct {
     mgc_cuda_paged paged;
     const void *q;

@@ -1,38 +1,14 @@
-// Attention of new tokens over a paged cache.
-//
-//   o_t[h] = sum_j w_j v_j,   w = softmax over the visible positions j of scale * q_t[h] . k_j
-// computed in one pass over the keys with the running maximum m and sum l of the softmax:
-//   m' = max(m, s_j),  l' = l e^(m - m') + e^(s_j - m'),  o' = o e^(m - m') + e^(s_j - m') v_j,
-// exponentials in base 2 (scale carries log2 e), everything in fp32.
+// Attention of new tokens over a paged cache: the kernel for unaligned operands, the choice of
+// kernel and the launch.
 #pragma once
 
-#include "paged_common.cuh"
+#include "paged_mma.cuh"
 
 namespace mgc {
 namespace paged {
 
-struct AttendParams {
-    Batch batch;
-    const void *k_pages, *v_pages;
-    long long page_stride, token_stride, head_stride;
-    const void *q;
-    void *out;
-    long long q_ts, q_hs, o_ts, o_hs;
-    int tokens, q_heads, kv_heads, group, head_dim;
-    int causal, window;
-    float scale_log2;  // scale * log2 e
-};
-
-constexpr int MAX_HEAD_DIM = 256;
-
-// Visible positions [lo, hi) of a token at position pos of a sequence of n positions.
-__device__ __forceinline__ void visible(const AttendParams &p, int n, int pos, int &lo, int &hi) {
-    hi = p.causal ? min(n, pos + 1) : n;
-    lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-}
-
-// One warp per (token, query head), lane l holding channels l, l + 32, ...: any type, head width,
-// stride and page size.
+// One warp per (token, query head), lane l holding channels l, l + 32, ...: what the tiled kernels
+// do not take (head widths that are no multiple of 16 bytes, unaligned rows).
 template <typename T>
 __global__ void __launch_bounds__(128) paged_attention_row_kernel(const __grid_constant__ AttendParams p) {
     constexpr int C = MAX_HEAD_DIM / 32;
@@ -87,13 +63,8 @@ __global__ void __launch_bounds__(128) paged_attention_row_kernel(const __grid_c
     }
 }
 
-inline int64_t attend_workspace(const mgc_cuda_paged_attention_args &a) {
-    (void)a;
-    return 0;
-}
-
-inline int attend(const mgc_cuda_paged_attention_args &a, cudaStream_t stream) {
-    const char *what = "mgc_cuda_paged_attention";
+// ---- host side ---------------------------------------------------------------------------------
+inline int check_attend(const mgc_cuda_paged_attention_args &a, const char *what) {
     const mgc_cuda_paged &c = a.paged;
     MGC_CHECK(check_paged(c, what));
     if (c.tokens > 0 && c.batch > 0 && (!a.q || !a.out)) return fail(MGC_CUDA_BAD_ARGUMENT, "%s: q or out is NULL", what);
@@ -107,6 +78,109 @@ inline int attend(const mgc_cuda_paged_attention_args &a, cudaStream_t stream) {
         return fail(MGC_CUDA_BAD_ARGUMENT, "%s: a window of %lld needs causal attention", what, (long long)a.window);
     if (!(a.scale > 0.0) || a.scale > 1e30) return fail(MGC_CUDA_BAD_ARGUMENT, "%s: scale %g", what, a.scale);
     if (a.max_q < 0 || a.max_kv < 0) return fail(MGC_CUDA_BAD_ARGUMENT, "%s: negative bound", what);
+    return MGC_CUDA_OK;
+}
+
+// How a call runs: which kernel, its row tile and how its keys are split.
+struct Plan {
+    bool mma = false;
+    int wm = 1;         // 16-row warps of a row tile
+    int row_tiles = 1, splits = 1;
+    bool clustered = false;
+    int64_t workspace = 0;
+};
+
+constexpr int MIN_SPLIT_KEYS = 128;  // below this a split's start and merge outweigh its loads
+
+inline Plan plan_of(const mgc_cuda_paged_attention_args &a) {
+    const mgc_cuda_paged &c = a.paged;
+    Plan s;
+    const int es = elem_size(c.dtype), chunk = 16 / es;
+    auto rows16 = [&](const void *q, int64_t x, int64_t y, int64_t z) {
+        return aligned(q, 16) && x * es % 16 == 0 && y * es % 16 == 0 && z * es % 16 == 0;
+    };
+    // 16-byte rows everywhere; anything else takes the row kernel
+    s.mma = c.head_dim % chunk == 0 && rows16(c.k, c.page_stride, c.token_stride, c.head_stride) &&
+            rows16(c.v, 0, 0, 0) && rows16(a.q, a.q_token_stride, a.q_head_stride, 0) &&
+            rows16(a.out, a.o_token_stride, a.o_head_stride, 0);
+    if (!s.mma) return s;
+    const int64_t group = a.q_heads / c.kv_heads;
+    int64_t max_q = a.max_q < 1 ? 1 : a.max_q > c.tokens ? c.tokens : a.max_q;
+    const int64_t rows = max_q * group;
+    s.wm = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    s.row_tiles = (int)ceil_div(rows, 16 * s.wm);
+    const int64_t units = c.batch * c.kv_heads * s.row_tiles;
+    // enough parts for two blocks per SM; three times that for batches, whose sequences differ
+    const int64_t target = 2ll * sm_count() * (c.batch > 1 ? 3 : 1);
+    int64_t most = a.max_kv;
+    if (a.window > 0 && a.window + max_q < most) most = a.window + max_q;
+    int64_t splits = units >= target ? 1 : ceil_div(target, units);
+    if (splits > most / MIN_SPLIT_KEYS) splits = most / MIN_SPLIT_KEYS;
+    if (splits > 128) splits = 128;
+    if (splits < 1) splits = 1;
+    if (splits > MAX_CLUSTER && c.batch > 1) splits = MAX_CLUSTER;
+    s.splits = (int)splits;
+    s.clustered = splits > 1 && splits <= MAX_CLUSTER;
+    if (splits > 1 && !s.clustered)
+        s.workspace = splits * c.tokens * a.q_heads * (c.head_dim * 4 + 8);
+    return s;
+}
+
+inline int64_t attend_workspace(const mgc_cuda_paged_attention_args &a) {
+    if (check_attend(a, "mgc_cuda_paged_attention_workspace") != MGC_CUDA_OK) return -1;
+    return a.paged.tokens == 0 || a.paged.batch == 0 ? 0 : plan_of(a).workspace;
+}
+
+template <typename T, int DP, int WM, int WN> inline int launch_mma(const AttendParams &p, int64_t blocks, cudaStream_t stream) {
+    using C = MmaConfig<T, DP, WM, WN>;
+    auto kernel = paged_attention_mma_kernel<T, DP, WM, WN>;
+    MGC_CHECK(raise_smem_ceiling((const void *)kernel));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)blocks, (unsigned)p.splits);
+    cfg.blockDim = dim3(C::THREADS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = attr[0].val.clusterDim.z = 1;
+    attr[0].val.clusterDim.y = (unsigned)p.splits;
+    cfg.attrs = attr;
+    cfg.numAttrs = p.clustered ? 1 : 0;
+    MGC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+    if (p.splits == 1 || p.clustered) return MGC_CUDA_OK;
+    // the combine kernel's blocks may be set up while the parts finish; it waits for them itself
+    cudaLaunchConfig_t comb{};
+    comb.gridDim = dim3((unsigned)ceil_div((int64_t)p.tokens * p.q_heads, 4));
+    comb.blockDim = dim3(128);
+    comb.stream = stream;
+    cudaLaunchAttribute dep[1];
+    dep[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    dep[0].val.programmaticStreamSerializationAllowed = 1;
+    comb.attrs = dep;
+    comb.numAttrs = 1;
+    MGC_CHECK_CUDA(cudaLaunchKernelEx(&comb, paged_combine_kernel<T>, p));
+    return MGC_CUDA_OK;
+}
+
+template <typename T, int DP> inline int launch_mma_rows(const AttendParams &p, int wm, int64_t blocks, cudaStream_t stream) {
+    if (wm == 1) return launch_mma<T, DP, 1, 4>(p, blocks, stream);
+    if (wm == 2) return launch_mma<T, DP, 2, 2>(p, blocks, stream);
+    return launch_mma<T, DP, 4, 1>(p, blocks, stream);
+}
+
+// Head widths are padded to the next of these (zero channels).
+template <typename T> inline int launch_mma_width(const AttendParams &p, int wm, int64_t blocks, cudaStream_t stream) {
+    if (p.head_dim <= 32) return launch_mma_rows<T, 32>(p, wm, blocks, stream);
+    if (p.head_dim <= 64) return launch_mma_rows<T, 64>(p, wm, blocks, stream);
+    if (p.head_dim <= 96) return launch_mma_rows<T, 96>(p, wm, blocks, stream);
+    if (p.head_dim <= 128) return launch_mma_rows<T, 128>(p, wm, blocks, stream);
+    return launch_mma_rows<T, 256>(p, wm, blocks, stream);
+}
+
+inline int attend(const mgc_cuda_paged_attention_args &a, cudaStream_t stream) {
+    const char *what = "mgc_cuda_paged_attention";
+    const mgc_cuda_paged &c = a.paged;
+    MGC_CHECK(check_attend(a, what));
     if (c.tokens == 0 || c.batch == 0) return MGC_CUDA_OK;
     AttendParams p;
     p.batch = batch_of(c);
@@ -119,6 +193,24 @@ inline int attend(const mgc_cuda_paged_attention_args &a, cudaStream_t stream) {
     p.causal = a.causal != 0;
     p.window = (int)(a.window > 0x3FFFFFFF ? 0x3FFFFFFF : a.window);
     p.scale_log2 = (float)(a.scale * 1.4426950408889634074);
+    p.max_positions = (int)(c.table_pages * c.page_size);
+    const Plan s = plan_of(a);
+    p.row_tiles = s.row_tiles; p.splits = s.splits; p.clustered = s.clustered;
+    p.part = nullptr; p.part_ml = nullptr;
+    if (s.workspace) {
+        if (!a.workspace || a.workspace_bytes < s.workspace || !aligned(a.workspace, 16))
+            return fail(MGC_CUDA_NEEDS_WORKSPACE, "%s: needs %lld bytes of workspace (16-byte aligned), got %lld", what,
+                        (long long)s.workspace, (long long)(a.workspace ? a.workspace_bytes : 0));
+        p.part = static_cast<float *>(a.workspace);
+        p.part_ml = reinterpret_cast<float2 *>(p.part + (int64_t)s.splits * p.tokens * p.q_heads * p.head_dim);
+    }
+    if (s.mma) {
+        const int64_t blocks = c.batch * c.kv_heads * s.row_tiles;
+        if (blocks > 0x7FFFFFFF) return fail(MGC_CUDA_UNSUPPORTED, "%s: %lld blocks", what, (long long)blocks);
+        if (c.dtype == MGC_F32) return launch_mma_width<float>(p, s.wm, blocks, stream);
+        if (c.dtype == MGC_F16) return launch_mma_width<__half>(p, s.wm, blocks, stream);
+        return launch_mma_width<__nv_bfloat16>(p, s.wm, blocks, stream);
+    }
     const dim3 grid((unsigned)p.tokens, (unsigned)ceil_div(p.q_heads, 4));
     if (c.dtype == MGC_F32) paged_attention_row_kernel<float><<<grid, 128, 0, stream>>>(p);
     else if (c.dtype == MGC_F16) paged_attention_row_kernel<__half><<<grid, 128, 0, stream>>>(p);

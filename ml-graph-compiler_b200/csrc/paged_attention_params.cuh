@@ -1,0 +1,42 @@
+// Parameters of the paged attention kernels.
+//
+//   o_t[h] = sum_j w_j v_j,   w = softmax over the visible positions j of scale * q_t[h] . k_j
+// computed in one pass over the keys with the running maximum m and sum l of the softmax:
+//   m' = max(m, s_j),  l' = l e^(m - m') + e^(s_j - m'),  o' = o e^(m - m') + e^(s_j - m') v_j,
+// exponentials in base 2 (scale carries log2 e), statistics and sums in fp32.
+#pragma once
+
+#include "paged_common.cuh"
+
+namespace mgc {
+namespace paged {
+
+struct AttendParams {
+    Batch batch;
+    const void *k_pages, *v_pages;
+    long long page_stride, token_stride, head_stride;
+    const void *q;
+    void *out;
+    long long q_ts, q_hs, o_ts, o_hs;
+    int tokens, q_heads, kv_heads, group, head_dim;
+    int causal, window;
+    float scale_log2;  // scale * log2 e
+    int max_positions;  // positions a row of the block table can hold
+    // kernels that tile rows and split keys
+    int row_tiles;      // row tiles per (sequence, key head) in the grid
+    int splits;         // parts of a tile's keys
+    int clustered;      // the parts are one cluster; else their partial results go to part, part_ml
+    float *part;        // [splits][tokens][q_heads][head_dim], relative to the part's maximum
+    float2 *part_ml;    // [splits][tokens][q_heads]: maximum, sum
+};
+
+constexpr int MAX_HEAD_DIM = 256;
+
+// Visible positions [lo, hi) of a token at position pos of a sequence of n positions.
+__device__ __forceinline__ void visible(const AttendParams &p, int n, int pos, int &lo, int &hi) {
+    hi = p.causal ? min(n, pos + 1) : n;
+    lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+}
+
+}  // namespace paged
+}  // namespace mgc

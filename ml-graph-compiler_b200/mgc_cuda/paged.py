@@ -23,7 +23,6 @@ the caller may pass and hand to ``check_status`` when it next synchronises.
 from __future__ import annotations
 
 import struct
-from ctypes import addressof, create_string_buffer
 
 import torch
 
@@ -31,9 +30,15 @@ from mgc_cuda._errors import CodegenError, GraphError
 from mgc_cuda.native import check, library
 
 _DTYPES = {torch.float32: 0, torch.float16: 7, torch.bfloat16: 8}  # MGC_F32, MGC_F16, MGC_BF16
+_I32, _NEEDS_WORKSPACE = torch.int32, 5  # MGC_CUDA_NEEDS_WORKSPACE
 _PAGED = "6q4q5q2qq"
 _APPEND = struct.Struct("=" + _PAGED + "q" + "3q3q4q3q2q4q")
 _ATTEND = struct.Struct("=" + _PAGED + "4q3q2qd2q2q")
+
+
+# the current stream of a device as an integer, without building a stream object (3 us a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _fail(what: str, why: str) -> None:
@@ -43,58 +48,58 @@ def _fail(what: str, why: str) -> None:
 def _paged(what, k_cache, v_cache, block_table, kv_lens, q_starts, tokens, status):
     """The fields of mgc_cuda_paged, checked as far as the C side cannot (types, devices, shapes)."""
     dtype, device = k_cache.dtype, k_cache.device
-    if dtype not in _DTYPES or v_cache.dtype != dtype:
+    if dtype not in _DTYPES or v_cache.dtype is not dtype:
         _fail(what, f"pages of {dtype} and {v_cache.dtype}: both float32, float16 or bfloat16")
-    if device.type != "cuda":
+    shape, strides = k_cache.shape, k_cache.stride()
+    if len(shape) != 4 or v_cache.shape != shape or v_cache.stride() != strides:
+        _fail(what, f"caches {tuple(shape)} and {tuple(v_cache.shape)}: two [pages, page_size, kv_heads, head_dim] of "
+                    "the same strides")
+    if not k_cache.is_cuda:
         _fail(what, f"the cache is on {device}")
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or v_cache.stride() != k_cache.stride():
-        _fail(what, f"caches {tuple(k_cache.shape)} and {tuple(v_cache.shape)}: two [pages, page_size, kv_heads, "
-                    "head_dim] of the same strides")
-    pages, page_size, kv_heads, head_dim = k_cache.shape
-    ps, ts, hs, cs = k_cache.stride()
+    pages, page_size, kv_heads, head_dim = shape
+    ps, ts, hs, cs = strides
     if cs != 1 and head_dim > 1:
         _fail(what, "the cache's channels are not contiguous")
-    i32 = torch.int32
-    if block_table.dtype != i32 or kv_lens.dtype != i32 or q_starts.dtype != i32:
+    if block_table.dtype is not _I32 or kv_lens.dtype is not _I32 or q_starts.dtype is not _I32:
         _fail(what, "block_table, kv_lens and q_starts are int32")
-    batch = kv_lens.shape[0]
-    table_stride, unit = block_table.stride()
-    if (block_table.dim() != 2 or kv_lens.dim() != 1 or q_starts.dim() != 1 or block_table.shape[0] != batch
-            or q_starts.shape[0] != batch + 1 or (unit != 1 and block_table.shape[1] > 1)
-            or not kv_lens.is_contiguous() or not q_starts.is_contiguous()):
-        _fail(what, f"block_table {tuple(block_table.shape)}, kv_lens {tuple(kv_lens.shape)}, q_starts "
-                    f"{tuple(q_starts.shape)}: [batch, n], [batch], [batch + 1], contiguous rows")
+    table, table_strides, lens, starts = block_table.shape, block_table.stride(), kv_lens.shape, q_starts.shape
+    batch = lens[0] if len(lens) == 1 else -1
+    if (len(table) != 2 or batch < 0 or len(starts) != 1 or table[0] != batch or starts[0] != batch + 1
+            or (table_strides[1] != 1 and table[1] > 1) or not kv_lens.is_contiguous() or not q_starts.is_contiguous()):
+        _fail(what, f"block_table {tuple(table)}, kv_lens {tuple(lens)}, q_starts {tuple(starts)}: [batch, n], [batch], "
+                    "[batch + 1], contiguous rows")
     if v_cache.device != device or block_table.device != device or kv_lens.device != device or q_starts.device != device:
         _fail(what, "the tensors are on several devices")
     at = 0
     if status is not None:
-        if status.dtype != i32 or status.numel() != 1 or status.device != device:
+        if status.dtype is not _I32 or status.numel() != 1 or status.device != device:
             _fail(what, "status is one int32 on the cache's device")
         at = status.data_ptr()
     return (k_cache.data_ptr(), v_cache.data_ptr(), pages, ps, ts, hs, _DTYPES[dtype], kv_heads, head_dim, page_size,
-            block_table.data_ptr(), table_stride, block_table.shape[1], kv_lens.data_ptr(), q_starts.data_ptr(),
-            batch, tokens, at)
+            block_table.data_ptr(), table_strides[0], table[1], kv_lens.data_ptr(), q_starts.data_ptr(), batch, tokens, at)
 
 
 def _rows(what, name, x, tokens, heads, dim, device):
     """(pointer, token stride, head stride) of a packed [tokens, heads, head_dim] operand."""
-    if x.dim() != 3 or x.shape[0] != tokens or (heads and x.shape[1] != heads) or x.shape[2] != dim:
-        _fail(what, f"{name} {tuple(x.shape)}: [{tokens}, {heads or 'heads'}, {dim}]")
+    shape, strides = x.shape, x.stride()
+    if len(shape) != 3 or shape[0] != tokens or (heads and shape[1] != heads) or shape[2] != dim:
+        _fail(what, f"{name} {tuple(shape)}: [{tokens}, {heads or 'heads'}, {dim}]")
     if x.device != device:
         _fail(what, f"{name} is on {x.device}, the cache on {device}")
-    ts, hs, cs = x.stride()
-    if cs != 1 and dim > 1:
+    if strides[2] != 1 and dim > 1:
         _fail(what, f"{name}'s channels are not contiguous")
-    return x.data_ptr(), ts, hs
+    return x.data_ptr(), strides[0], strides[1]
 
 
-def _call(fn, what, layout, fields, device):
-    buf = create_string_buffer(layout.pack(*fields), layout.size)
-    if device.index == torch.cuda.current_device():
-        check(fn(addressof(buf), torch.cuda.current_stream().cuda_stream), what)
+def _call(fn, what, args, device):
+    """The C call on the device's current stream."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = fn(args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            check(fn(addressof(buf), torch.cuda.current_stream().cuda_stream), what)
+            status = fn(args, _raw_stream(index))
+    return status
 
 
 def kv_append(
@@ -134,7 +139,7 @@ def kv_append(
         fields += (0, 0, 0, 0, 0, 0, 0)
     else:
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=k_cache.dtype, device=device)
+            q_out = q.new_empty(q.shape, dtype=k_cache.dtype)
         elif q_out.dtype != k_cache.dtype or q_out.shape != q.shape:
             _fail(what, f"q_out {tuple(q_out.shape)} of {q_out.dtype}")
         fields += (*_rows(what, "q", q, tokens, 0, dim, device), q.shape[1],
@@ -150,7 +155,9 @@ def kv_append(
             _fail(what, f"cos {tuple(cos.shape)} and sin {tuple(sin.shape)}: float32 [positions, rot / 2] on the cache's "
                         "device, of the same strides")
         fields += (cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.shape[0], 2 * cos.shape[1], int(interleaved))
-    _call(library().mgc_cuda_kv_append, what, _APPEND, fields, device)
+    status_code = _call(library().mgc_cuda_kv_append, what, _APPEND.pack(*fields), device)
+    if status_code:
+        check(status_code, what)
     return q_out if q is not None else None
 
 
@@ -184,15 +191,24 @@ def paged_attention(
     if q.dtype != dtype:
         _fail(what, f"q of {q.dtype} over a cache of {dtype}")
     if out is None:
-        out = torch.empty(q.shape, dtype=dtype, device=device)
+        out = q.new_empty(q.shape)
     elif out.dtype != dtype or out.shape != q.shape:
         _fail(what, f"out {tuple(out.shape)} of {out.dtype}")
     q_ptr, q_ts, q_hs = _rows(what, "q", q, tokens, 0, dim, device)
     fields = (*paged, q_ptr, q_ts, q_hs, q.shape[1], *_rows(what, "out", out, tokens, 0, dim, device),
               tokens if max_q is None else max_q,
               block_table.shape[1] * k_cache.shape[1] if max_kv is None else max_kv,
-              dim ** -0.5 if scale is None else scale, int(causal), window, 0, 0)
-    _call(library().mgc_cuda_paged_attention, what, _ATTEND, fields, device)
+              dim ** -0.5 if scale is None else scale, int(causal), window)
+    lib = library()
+    status_code = _call(lib.mgc_cuda_paged_attention, what, _ATTEND.pack(*fields, 0, 0), device)
+    if status_code == _NEEDS_WORKSPACE:
+        # few rows over many keys: partial results of the keys' parts, from torch's stream-ordered
+        # allocator (the block returns to this stream's pool after the call)
+        need = lib.mgc_cuda_paged_attention_workspace(_ATTEND.pack(*fields, 0, 0))
+        space = q.new_empty(need, dtype=torch.uint8)
+        status_code = _call(lib.mgc_cuda_paged_attention, what, _ATTEND.pack(*fields, space.data_ptr(), need), device)
+    if status_code:
+        check(status_code, what)
     return out
 
 
