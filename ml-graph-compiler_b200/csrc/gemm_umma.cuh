@@ -35,8 +35,6 @@
 // through its cta_group::2 MMAs.
 #pragma once
 
-#include <cuda.h>
-#include <cudaTypedefs.h>
 #include <stdlib.h>
 #include <string.h>
 
@@ -45,6 +43,7 @@
 #include "common.cuh"
 #include "gemm_simt.cuh"
 #include "kernels_norm.cuh"
+#include "umma_ptx.cuh"
 
 namespace mgc {
 namespace umma {
@@ -52,7 +51,6 @@ namespace umma {
 constexpr int BM = 128;
 constexpr int BK = 32;                       // fp32 elements per K block: one 128-byte swizzle row
 constexpr uint32_t A_TILE_BYTES = BM * BK * 4;
-constexpr long long WAIT_LIMIT_CYCLES = 1ll << 31;  // ~1.1 s at 1.9 GHz
 
 // TF32 mode accumulates a tile's whole K in TMEM. Measured on ResNet-50 (batch 4 against the
 // float64 oracle): promoting the accumulator to fp32 registers every 1, 2, 4 or 8 K blocks, or
@@ -126,210 +124,6 @@ struct Params {
     int gap_hw;
 };
 
-// ---- PTX wrappers -----------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t smem_addr(const void *p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-__device__ __forceinline__ void mbar_init(uint64_t *bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(count) : "memory");
-}
-
-__device__ __forceinline__ void mbar_expect_tx(uint64_t *bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes)
-                 : "memory");
-}
-
-__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
-}
-
-__device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}\n"
-        : "=r"(done)
-        : "r"(smem_addr(bar)), "r"(parity)
-        : "memory");
-    return done != 0;
-}
-
-// Non-blocking test of the same (the thread never suspends); the result is read later, so the
-// test's latency overlaps whatever the thread issues meanwhile.
-__device__ __forceinline__ bool mbar_test_wait(uint64_t *bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}\n"
-        : "=r"(done)
-        : "r"(smem_addr(bar)), "r"(parity)
-        : "memory");
-    return done != 0;
-}
-
-// Bounded wait for the phase with parity `parity` to complete. Returns false on timeout.
-__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const long long t0 = clock64();
-    while (!mbar_try_wait(bar, parity)) {
-        if (clock64() - t0 > WAIT_LIMIT_CYCLES) return false;
-    }
-    return true;
-}
-
-__device__ __forceinline__ void fence_barrier_init() {
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-}
-
-__device__ __forceinline__ void fence_proxy_async_smem() {
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
-
-__device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, uint64_t *bar, int x, int y) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4}], [%2];"
-        ::"r"(smem_addr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(bar)), "r"(x), "r"(y)
-        : "memory");
-}
-
-__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, uint64_t *bar, int x, int y, int z) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5}], [%2];"
-        ::"r"(smem_addr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(bar)), "r"(x), "r"(y), "r"(z)
-        : "memory");
-}
-
-__device__ __forceinline__ void tma_load_im2col_4d(void *dst, const CUtensorMap *map, uint64_t *bar, int c, int w,
-                                                   int h, int n, uint16_t off_w, uint16_t off_h) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.im2col.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5, %6}], [%2], {%7, %8};"
-        ::"r"(smem_addr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(bar)), "r"(c), "r"(w), "r"(h),
-        "r"(n), "h"(off_w), "h"(off_h)
-        : "memory");
-}
-
-__device__ __forceinline__ void tma_load_5d(void *dst, const CUtensorMap *map, uint64_t *bar, int x, int y, int z,
-                                            int w, int v) {
-    asm volatile(
-        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
-        ::"r"(smem_addr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(bar)), "r"(x), "r"(y), "r"(z),
-        "r"(w), "r"(v)
-        : "memory");
-}
-
-// ---- CTA pairs (cta_group::2) ------------------------------------------------------------------
-// A pair of CTAs (a cluster of two) computes one 256-row tile: each CTA loads its own 128 rows of
-// A and one plane of B (rank 0 the TF32 part, rank 1 the residual) into the same shared-memory
-// offsets, and rank 0 issues MMAs with M = 256 that read both CTAs' operands and write each CTA's
-// rows into its own TMEM. Every load of the pair completes on rank 0's stage barrier.
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t cluster_index() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%clusterid.x;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t cluster_count() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%nclusterid.x;" : "=r"(r));
-    return r;
-}
-// Address of the same shared variable in the pair's rank-0 CTA (shared::cluster window).
-__device__ __forceinline__ uint32_t leader_addr(const void *p) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_addr(p)));
-    return r;
-}
-// All threads of both CTAs; orders barrier initialisation before any remote arrive, and every
-// remote access before either CTA exits.
-__device__ __forceinline__ void cluster_sync_all() {
-    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
-__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-__device__ __forceinline__ void tma_load_2d_pair(void *dst, const CUtensorMap *map, uint32_t bar, int x, int y) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4}], [%2];"
-        ::"r"(smem_addr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
-        : "memory");
-}
-__device__ __forceinline__ void tma_load_3d_pair(void *dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5}], [%2];"
-        ::"r"(smem_addr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
-        : "memory");
-}
-__device__ __forceinline__ void tma_load_im2col_4d_pair(void *dst, const CUtensorMap *map, uint32_t bar, int c, int w,
-                                                        int h, int n, uint16_t off_w, uint16_t off_h) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.im2col.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5, %6}], [%2], {%7, %8};"
-        ::"r"(smem_addr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c), "r"(w), "r"(h), "r"(n),
-        "h"(off_w), "h"(off_h)
-        : "memory");
-}
-
-// Plain bulk copy of `bytes` (a multiple of 16, both addresses 16-byte aligned) from global to
-// this CTA's shared memory, completing on `bar`.
-__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
-    asm volatile(
-        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-        ::"r"(smem_addr(dst)), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_addr(bar))
-        : "memory");
-}
-
-// Warm the TMA unit's descriptor cache with a tensor map (kernel-parameter copies included).
-__device__ __forceinline__ void prefetch_tmap(const CUtensorMap *map) {
-    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
-}
-
-__device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, uint64_t *bar, int x, int y, int z, int w) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5, %6}], [%2];"
-        ::"r"(smem_addr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
-        : "memory");
-}
-
-__device__ __forceinline__ void tma_store_4d(const CUtensorMap *map, const void *src, int x, int y, int z, int w) {
-    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
-                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(src)), "r"(x), "r"(y), "r"(z), "r"(w)
-                 : "memory");
-}
-
-__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, const void *src, int x, int y) {
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
-                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(src)), "r"(x), "r"(y)
-                 : "memory");
-}
-
-__device__ __forceinline__ void tma_store_commit_and_wait() {
-    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-}
-
-__device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-
-// Every committed store of this thread has finished reading shared memory.
-__device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-// Every committed store group but the most recent one has read its shared memory.
-__device__ __forceinline__ void tma_store_wait_read_but_one() {
-    asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-}
-
 // Epilogue warps: two per TMEM lane quadrant, each taking half of the tile's columns.
 constexpr int EPI_THREADS = 256;
 // A TMA instruction holds its issuing thread for ~350 cycles (measured, any box size), so A and
@@ -341,216 +135,11 @@ constexpr int THREADS = 64 + EPI_THREADS + 32;  // A producer, MMA, eight epilog
 // Barrier among the epilogue threads only (named barrier 1).
 __device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-__device__ __forceinline__ void tmem_alloc(uint32_t *slot, uint32_t cols) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(slot)),
-                 "r"(cols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-
-__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t cols) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
-}
-
-// Pair forms: warp 1 of both CTAs allocates (and frees) the same columns in each CTA's TMEM.
-__device__ __forceinline__ void tmem_alloc_pair(uint32_t *slot, uint32_t cols) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(slot)),
-                 "r"(cols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-}
-
-__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t cols) {
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
-}
-
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-// K-major operand in 128B-swizzled rows of 128 bytes, 8-row groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
-    return (uint64_t)((saddr >> 4) & 0x3FFFu)      // start address
-           | ((uint64_t)1 << 16)                    // leading byte offset (unused for swizzled K-major)
-           | ((uint64_t)(1024 >> 4) << 32)          // stride byte offset: 8 rows x 128 B
-           | ((uint64_t)1 << 46)                    // descriptor version (sm_100)
-           | ((uint64_t)2 << 61);                   // 128-byte swizzle
-}
-
-// K-major operand without swizzle, in core matrices of 8 rows x 16 bytes (rows 16 bytes apart):
-// `lbo` bytes between core matrices adjacent in K, `sbo` bytes between those adjacent in M / N.
-__device__ __forceinline__ uint64_t plain_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-    return (uint64_t)((saddr >> 4) & 0x3FFFu)
-           | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16)
-           | ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32)
-           | ((uint64_t)1 << 46);                   // descriptor version (sm_100); layout 0: no swizzle
-}
-
 // Tap-packed A tile (narrow-channel convolutions): the K block's 32 fp32 columns are eight
 // 16-byte column groups, each an im2col box of 128 output pixels x 4 channels at one filter tap,
 // stored box after box (128 rows x 16 bytes = 2 KB each). Core matrices: 128 bytes apart along M,
 // 2 KB apart along K.
 constexpr uint32_t PACKED_BOX_BYTES = BM * 16;
-
-// kind::tf32, fp32 accumulate, both operands K-major; M = 128 (one CTA) or 256 (a CTA pair).
-__host__ __device__ constexpr uint32_t instr_desc_tf32(int n, int m = BM) {
-    return (1u << 4)                 // D format f32
-           | (2u << 7)               // A format tf32
-           | (2u << 10)              // B format tf32
-           | ((uint32_t)(n >> 3) << 17)
-           | ((uint32_t)(m >> 4) << 24);
-}
-
-__device__ __forceinline__ void mma_tf32(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                         uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n\t}\n"
-        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
-__device__ __forceinline__ void mma_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
-                 : "memory");
-}
-
-// Pair MMA (issued by rank 0): A rows 0-127 from rank 0's shared memory and 128-255 from rank 1's,
-// B rows [0, N/2) from rank 0 and [N/2, N) from rank 1; D rows land in each CTA's own TMEM.
-__device__ __forceinline__ void mma_tf32_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                              uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::tf32 [%0], %1, %2, %3, p;\n\t}\n"
-        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
-// Arrive on `bar` (same offset) in both CTAs of the pair once the pair MMAs issued so far complete.
-__device__ __forceinline__ void mma_commit_pair(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                 ::"r"(smem_addr(bar)), "h"((uint16_t)3)
-                 : "memory");
-}
-
-__device__ __forceinline__ void mma_commit_pair_local(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
-                 : "memory");
-}
-
-// A K block's four MMAs (K = 8 each) issued back to back from one asm block, with the test of
-// the next stage's barrier between the first and the second. tcgen05.mma holds the issuing
-// thread until the tensor pipe takes it, so any instruction between two MMAs adds to the
-// block's time; every descriptor is computed before the first. first_acc: whether the first
-// MMA accumulates. Returns the barrier test.
-#define MGC_MMA4_BODY(GROUP, A0, A1, A2, A3, B0, B1, B2, B3, EXTRA)                                       \
-    "{\n\t.reg .pred p, t, q;\n\t"                                                                      \
-    "setp.ne.b32 p, %12, 0;\n\t"                                                                         \
-    "setp.eq.b32 t, %12, %12;\n\t"                                                                       \
-    "tcgen05.mma.cta_group::" GROUP ".kind::tf32 [%1], " A0 ", " B0 ", %11, p;\n\t"                      \
-    "mbarrier.test_wait.parity.shared::cta.b64 q, [%13], %14;\n\t"                                      \
-    EXTRA                                                                                                 \
-    "tcgen05.mma.cta_group::" GROUP ".kind::tf32 [%1], " A1 ", " B1 ", %11, t;\n\t"                      \
-    "tcgen05.mma.cta_group::" GROUP ".kind::tf32 [%1], " A2 ", " B2 ", %11, t;\n\t"                      \
-    "tcgen05.mma.cta_group::" GROUP ".kind::tf32 [%1], " A3 ", " B3 ", %11, t;\n\t"                      \
-    "selp.u32 %0, 1, 0, q;\n\t}\n"
-
-template <int PAIR>
-__device__ __forceinline__ bool mma_block4(uint32_t d, const uint64_t (&ad)[4], const uint64_t (&bd)[4], uint32_t idesc,
-                                           uint32_t first_acc, uint64_t *next_bar, uint32_t next_parity) {
-    uint32_t ready;
-    if (PAIR)
-        asm volatile(MGC_MMA4_BODY("2", "%2", "%3", "%4", "%5", "%6", "%7", "%8", "%9", "")
-                     : "=r"(ready)
-                     : "r"(d), "l"(ad[0]), "l"(ad[1]), "l"(ad[2]), "l"(ad[3]), "l"(bd[0]), "l"(bd[1]), "l"(bd[2]),
-                       "l"(bd[3]), "r"(0), "r"(idesc), "r"(first_acc), "r"(smem_addr(next_bar)), "r"(next_parity)
-                     : "memory");
-    else
-        asm volatile(MGC_MMA4_BODY("1", "%2", "%3", "%4", "%5", "%6", "%7", "%8", "%9", "")
-                     : "=r"(ready)
-                     : "r"(d), "l"(ad[0]), "l"(ad[1]), "l"(ad[2]), "l"(ad[3]), "l"(bd[0]), "l"(bd[1]), "l"(bd[2]),
-                       "l"(bd[3]), "r"(0), "r"(idesc), "r"(first_acc), "r"(smem_addr(next_bar)), "r"(next_parity)
-                     : "memory");
-    return ready != 0;
-}
-
-// Wide pair: per K step the B_hi and the B_lo MMA into one accumulator (eight MMAs).
-__device__ __forceinline__ bool mma_block4_wide(uint32_t d, const uint64_t (&ad)[4], const uint64_t (&bd)[4],
-                                                const uint64_t (&bld)[4], uint32_t idesc, uint32_t first_acc,
-                                                uint64_t *next_bar, uint32_t next_parity) {
-    uint32_t ready;
-    asm volatile(
-        "{\n\t.reg .pred p, t, q;\n\t"
-        "setp.ne.b32 p, %15, 0;\n\t"
-        "setp.eq.b32 t, %15, %15;\n\t"
-        "tcgen05.mma.cta_group::2.kind::tf32 [%1], %2, %6, %14, p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 q, [%16], %17;\n\t"
-        "tcgen05.mma.cta_group::2.kind::tf32 [%1], %2, %10, %14, t;\n\t"
-        "tcgen05.mma.cta_group::2.kind::tf32 [%1], %3, %7, %14, t;\n\t"
-        "tcgen05.mma.cta_group::2.kind::tf32 [%1], %3, %11, %14, t;\n\t"
-        "tcgen05.mma.cta_group::2.kind::tf32 [%1], %4, %8, %14, t;\n\t"
-        "tcgen05.mma.cta_group::2.kind::tf32 [%1], %4, %12, %14, t;\n\t"
-        "tcgen05.mma.cta_group::2.kind::tf32 [%1], %5, %9, %14, t;\n\t"
-        "tcgen05.mma.cta_group::2.kind::tf32 [%1], %5, %13, %14, t;\n\t"
-        "selp.u32 %0, 1, 0, q;\n\t}\n"
-        : "=r"(ready)
-        : "r"(d), "l"(ad[0]), "l"(ad[1]), "l"(ad[2]), "l"(ad[3]), "l"(bd[0]), "l"(bd[1]), "l"(bd[2]), "l"(bd[3]),
-          "l"(bld[0]), "l"(bld[1]), "l"(bld[2]), "l"(bld[3]), "r"(idesc), "r"(first_acc), "r"(smem_addr(next_bar)),
-          "r"(next_parity)
-        : "memory");
-    return ready != 0;
-}
-
-// 16 consecutive fp32 columns of this thread's TMEM lane.
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
-}
-
-__device__ __forceinline__ float4 lds4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
-    return v;
-}
-
-__device__ __forceinline__ void sts4(uint32_t addr, float4 v) {
-    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
-                 : "memory");
-}
-
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-
-__device__ __forceinline__ long long ceil_div_dev(long long a, long long b) { return (a + b - 1) / b; }
-
-__device__ __forceinline__ void set_error(int *err, int code) {
-    if (err) atomicExch(err, code);
-}
-
-// Round fp32 to the nearest TF32 value (10 explicit mantissa bits; ties away from zero), the
-// rounding a TFLOAT32 tensor map applies on load.
-__device__ __forceinline__ float tf32_hi(float x) {
-    uint32_t b = __float_as_uint(x);
-    uint32_t r = (b + 0x1000u) & 0xFFFFE000u;
-    return ((b & 0x7F800000u) == 0x7F800000u) ? x : __uint_as_float(r);
-}
-
-// 32 consecutive fp32 columns of this thread's TMEM lane (no wait).
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-}
 
 // Position in a ring of N slots (shared-memory stages, TMEM buffers): the slot, the parity of
 // the current lap, and whether the ring has wrapped (a slot's previous use must then be waited
@@ -573,8 +162,6 @@ struct RingPos {
         return r;
     }
 };
-
-constexpr uint32_t SMEM_LIMIT = 232448;  // dynamic shared memory per block on sm_100 (227 KB)
 
 // RB: B-resident variant. The CTA keeps one N tile for its whole life and loads that tile's B
 // panel (every K block, hi and lo) into shared memory once; the stages then carry A only.
@@ -1635,20 +1222,6 @@ __global__ void __launch_bounds__(256) split_reduce_f64_kernel(const double *par
 }
 
 // ---- host side ---------------------------------------------------------------------------------
-inline PFN_cuTensorMapEncodeTiled_v12000 encode_tiled_fn() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-    if (!fn) {
-        cudaDriverEntryPointQueryResult q;
-        void *ptr = nullptr;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
-        else
-            cudaGetLastError();
-    }
-    return fn;
-}
-
 inline PFN_cuTensorMapEncodeIm2col_v12000 encode_im2col_fn() {
     static PFN_cuTensorMapEncodeIm2col_v12000 fn = nullptr;
     if (!fn) {
