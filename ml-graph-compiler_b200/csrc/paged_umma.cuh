@@ -30,6 +30,9 @@
 #include "paged_mma.cuh"
 #include "umma_ptx.cuh"
 
+#ifndef MGC_POLY
+#define MGC_POLY 0
+#endif
 namespace mgc {
 namespace paged {
 
@@ -37,7 +40,6 @@ using umma::mbar_arrive;
 using umma::mbar_expect_tx;
 using umma::mbar_init;
 using umma::mbar_wait;
-using umma::mma_commit;
 using umma::smem_addr;
 using umma::sw128_desc;
 using umma::tc_fence_after;
@@ -54,7 +56,8 @@ template <int DP> struct UmmaConfig {
     static constexpr uint32_t TILE = HALVES * HALF;   // a Q, K or V tile
     static constexpr int STAGES = DP == 64 ? 8 : 5;
     static constexpr uint32_t SMEM = 1024 + 2 * TILE + STAGES * TILE;
-    // two softmax warpgroups, then a warpgroup of the MMA warp, the load warp and two idle ones.
+    // two softmax warpgroups, then a warpgroup of the MMA warp (8), the load warp (9), one that zeroes
+    // rows of V (10) and an idle one.
     // 384 threads launch with 168 registers each (64,512); the split keeps that sum:
     // 256 x 224 + 128 x 56
     static constexpr int THREADS = 384;
@@ -63,17 +66,29 @@ template <int DP> struct UmmaConfig {
 };
 
 // D = A B with A in TMEM (16-bit values packed in pairs along K) or shared memory.
-__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
-        : "memory");
+// Executed by the lane whose `e` is set (elect_one); the whole warp calls.
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r;
 }
-__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_f16_ss(uint32_t e, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
-        : "memory");
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(e) : "memory");
+}
+__device__ __forceinline__ void mma_f16_ts(uint32_t e, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(e) : "memory");
+}
+__device__ __forceinline__ void commit_if(uint32_t e, uint64_t *bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n"
+        ::"r"(smem_addr(bar)), "r"(e) : "memory");
 }
 // MN-major operand of 16-bit elements in 128B-swizzled rows of 64 (M / N) elements, consecutive K
 // rows 128 bytes apart: 8-row groups 1024 bytes apart along K, 64-element blocks `lbo` bytes apart.
@@ -95,6 +110,50 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
           "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
           "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
         : "memory");
+}
+// Two fp32 operations in one instruction (sm_100).
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+// 2^x for x <= 2^7 on the FMA pipe: x = n + f, n the nearest whole number (taken from the low bits of
+// x + 1.5 * 2^23), 2^f by the polynomial of least largest relative error on [-1/2, 1/2] (found by
+// exchange: 7.5e-5 of degree 3, 2.7e-6 of degree 4, below the rounding of the weights to bf16 and
+// f16), n added to the exponent field. Below 2^-126 it stays at 2^-126.
+template <typename T> __device__ __forceinline__ float2 exp2_poly(float2 x) {
+    constexpr float MAGIC = 12582912.0f;
+    x.x = fmaxf(x.x, -126.0f);
+    x.y = fmaxf(x.y, -126.0f);
+    const float2 t = add2(x, make_float2(MAGIC, MAGIC)), n = add2(t, make_float2(-MAGIC, -MAGIC));
+    const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
+    float2 e;
+    if (std::is_same<T, __nv_bfloat16>::value) {
+        e = fma2(f, make_float2(5.517166853e-02f, 5.517166853e-02f), make_float2(2.426111251e-01f, 2.426111251e-01f));
+        e = fma2(e, f, make_float2(6.932609677e-01f, 6.932609677e-01f));
+        e = fma2(e, f, make_float2(9.999280572e-01f, 9.999280572e-01f));
+    } else {
+        e = fma2(f, make_float2(9.570102207e-03f, 9.570102207e-03f), make_float2(5.591785908e-02f, 5.591785908e-02f));
+        e = fma2(e, f, make_float2(2.402474433e-01f, 2.402474433e-01f));
+        e = fma2(e, f, make_float2(6.931217909e-01f, 6.931217909e-01f));
+        e = fma2(e, f, make_float2(9.999992847e-01f, 9.999992847e-01f));
+    }
+    return make_float2(__int_as_float(__float_as_int(e.x) + (__float_as_int(t.x) << 23)),
+                       __int_as_float(__float_as_int(e.y) + (__float_as_int(t.y) << 23)));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -156,12 +215,14 @@ template <typename T, int DP>
 __global__ void __launch_bounds__(UmmaConfig<DP>::THREADS, 1)
 paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid_constant__ UmmaMaps maps) {
     using C = UmmaConfig<DP>;
+    constexpr int POLY = MGC_POLY;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t full[C::STAGES], empty[C::STAGES], q_full[2], s_full[2], p_full[2], o_full[2];
+    __shared__ __align__(8) uint64_t full[C::STAGES], empty[C::STAGES], q_full[2], s_full[2], p_half[2], p_full[2], o_full[2];
+    __shared__ __align__(8) uint64_t z_ask, z_done;
     __shared__ uint32_t tslot;
     uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *sQ = base, *ring = base + 2 * C::TILE;
-    const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = (int)threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
     unsigned u = blockIdx.x;
     const int split = (int)blockIdx.y;
     const int kh = (int)(u % (unsigned)p.kv_heads);
@@ -179,11 +240,14 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
             mbar_init(&empty[s], 1);
         }
         for (int x = 0; x < 2; ++x) {
-            mbar_init(&q_full[x], 128);
+            mbar_init(&q_full[x], 4);
             mbar_init(&s_full[x], 1);
-            mbar_init(&p_full[x], 128);
+            mbar_init(&p_half[x], 4);
+            mbar_init(&p_full[x], 4);
             mbar_init(&o_full[x], 1);
         }
+        mbar_init(&z_ask, 1);
+        mbar_init(&z_done, 1);
         umma::fence_barrier_init();
         umma::prefetch_tmap(&maps.k);
         umma::prefetch_tmap(&maps.v);
@@ -193,8 +257,18 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
     __syncthreads();
     tc_fence_after();
     const uint32_t tbase = tslot;
-    // a warp's bounded wait; a wait that runs out ends its role, and every role that waits for it
+    // A warp's bounded waits, polled by one lane or by all. A wait that runs out ends its role, and
+    // every role that waits for it.
     auto wait = [&](uint64_t *bar, uint32_t parity) {
+        int ok = 1;
+        if (lane == 0) ok = mbar_wait(bar, parity);
+        ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
+        __syncwarp();
+        if (ok) return true;
+        umma::set_error(p.batch.status, MGC_CUDA_TIMEOUT);
+        return false;
+    };
+    auto waitw = [&](uint64_t *bar, uint32_t parity) {
         if (__all_sync(0xFFFFFFFFu, mbar_wait(bar, parity))) return true;
         umma::set_error(p.batch.status, MGC_CUDA_TIMEOUT);
         return false;
@@ -247,10 +321,16 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
             }
         } else if (warp == 8) {
             // ---------------- MMA ----------------
+            // The tensor pipe takes an MMA only when the one before is nearly done, so whatever
+            // stands between two of them is time lost. The warp runs this code converged, with one
+            // elected lane's predicate on the MMAs: descriptors then live in uniform registers and
+            // a chain of products issues without a gap (a loop of one lane's branch took 1.25-1.55
+            // times as long for the same products).
             int slot = 0;
-            uint32_t lap = 0, q_phase = 0, p_phase = 0;  // p_phase: bit x of row tile x
+            uint32_t lap = 0, q_phase = 0, z_phase = 0, phase0 = 0, phase1 = 0;
             bool ok = true;
             constexpr uint32_t id_s = idesc_f16<T>(128, 0), id_o = idesc_f16<T>(DP, 1);
+            const uint32_t e = elect_one(), tb = __shfl_sync(0xFFFFFFFFu, tbase, 0);
             auto step = [&]() {
                 if (++slot == C::STAGES) {
                     slot = 0;
@@ -258,80 +338,97 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                 }
             };
             auto scores = [&](int x, int stage) {
-                uint64_t a = sw128_desc(smem_addr(sQ + x * C::TILE)), k = sw128_desc(smem_addr(ring + stage * C::TILE));
-                asm volatile("" : "+l"(a), "+l"(k));  // computed here, not kept in registers around the loops
+                const uint64_t a = sw128_desc(smem_addr(sQ) + x * C::TILE), k = sw128_desc(smem_addr(ring) + stage * C::TILE);
 #pragma unroll
                 for (int ks = 0; ks < DP / 16; ++ks) {
                     const uint32_t at = ((uint32_t)(ks >> 2) * C::HALF + (uint32_t)(ks & 3) * 32u) >> 4;
-                    mma_f16_ss(tbase + C::S_COL + x * 128, a + at, k + at, id_s, ks > 0);
+                    mma_f16_ss(e, tb + C::S_COL + x * 128, a + at, k + at, id_s, ks > 0);
                 }
-                mma_commit(&s_full[x]);
+                commit_if(e, &s_full[x]);
             };
             for (int tile = tile0; ok && tile * 256 < nq * p.group; tile += p.row_tiles) {
                 const Item w = umma_item(p, n, nq, tile, split);
-                ok = ok && wait(&q_full[0], q_phase) && wait(&q_full[1], q_phase);
+                ok = waitw(&q_full[0], q_phase) && waitw(&q_full[1], q_phase);
                 q_phase ^= 1u;
-                tc_fence_after();
-                if (w.tiles > 0) {
-                    ok = ok && wait(&full[slot], lap);
+                if (ok && w.tiles > 0) {
+                    ok = waitw(&full[slot], lap);
                     tc_fence_after();
-                    if (ok && lane == 0) {
+                    if (ok) {
                         if (w.need0 > 0) scores(0, slot);
                         if (w.need1 > 0) scores(1, slot);
-                        mma_commit(&empty[slot]);
+                        commit_if(e, &empty[slot]);
                     }
-                    __syncwarp();
                     step();
                 }
                 for (int j = 0; ok && j < w.tiles; ++j) {
                     const int vs = slot;
-                    ok = ok && wait(&full[vs], lap);
+                    ok = waitw(&full[vs], lap);
                     step();
                     const int ks = slot;
                     const bool more = j + 1 < w.tiles;
-                    if (more) {
-                        ok = ok && wait(&full[ks], lap);
-                        step();
-                    }
-                    // rows of V outside [first, hi): zeros
                     const int key0 = w.lo + j * 128;
                     if (ok && (key0 < w.first || key0 + 128 > w.hi)) {
-                        const int r0 = max(w.first - key0, 0), r1 = min(w.hi - key0, 128);
-#pragma unroll 1
-                        for (int x = lane; x < 128 * C::HALVES * 8; x += 32) {
-                            const int r = (x >> 3) & 127;
-                            if (r < r0 || r >= r1)
-                                *reinterpret_cast<uint4 *>(ring + vs * C::TILE + (x >> 10) * C::HALF + r * 128 + (x & 7) * 16) =
-                                    make_uint4(0, 0, 0, 0);
-                        }
-                        umma::fence_proxy_async_smem();
+                        // rows of V that no row sees: warp 10 zeroes them
+                        if (lane == 0) mbar_arrive(&z_ask);
                         __syncwarp();
+                        ok = waitw(&z_done, z_phase);
+                        z_phase ^= 1u;
                     }
-#pragma unroll 1
-                    for (int x = 0; x < 2; ++x) {
-                        if (ok && j < w.need(x)) {
-                            ok = wait(&p_full[x], (p_phase >> x) & 1u);
-                            p_phase ^= 1u << x;
-                            tc_fence_after();
-                            if (ok && lane == 0) {
-                                uint64_t v = mn128_desc(smem_addr(ring + vs * C::TILE), C::HALF);
-                                asm volatile("" : "+l"(v));
+                    if (more) {
+                        ok = ok && waitw(&full[ks], lap);
+                        step();
+                    }
+                    const uint64_t v = mn128_desc(smem_addr(ring) + vs * C::TILE, C::HALF);
 #pragma unroll
-                                for (int kk = 0; kk < 8; ++kk)
-                                    mma_f16_ts(tbase + C::O_COL + x * DP, tbase + C::S_COL + x * 128 + kk * 8, v + kk * (2048 >> 4),
-                                               id_o, j > 0 || kk > 0);
-                                if (x == 1 || j >= w.need1) mma_commit(&empty[vs]);
-                                if (j + 1 < w.need(x)) scores(x, ks);
-                                else mma_commit(&o_full[x]);
-                            }
-                            __syncwarp();
-                        } else if (ok && x == 1 && j >= w.need0 && lane == 0) {
-                            mma_commit(&empty[vs]);  // no row tile used it
-                        }
+                    for (int x = 0; x < 2; ++x) {
+                        if (!ok || j >= w.need(x)) continue;
+                        const uint32_t o = tb + C::O_COL + x * DP, w16 = tb + C::S_COL + x * 128;
+                        uint32_t &phase = x ? phase1 : phase0;
+                        ok = waitw(&p_half[x], phase);
+                        if (!ok) continue;
+                        tc_fence_after();
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk) mma_f16_ts(e, o, w16 + kk * 8, v + kk * (2048 >> 4), id_o, j > 0 || kk > 0);
+                        ok = waitw(&p_full[x], phase);
+                        phase ^= 1u;
+                        if (!ok) continue;
+                        tc_fence_after();
+#pragma unroll
+                        for (int kk = 4; kk < 8; ++kk) mma_f16_ts(e, o, w16 + kk * 8, v + kk * (2048 >> 4), id_o, 1);
+                        if (j + 1 < w.need(x)) scores(x, ks);
+                        else commit_if(e, &o_full[x]);
                     }
-                    if (ok && more && lane == 0) mma_commit(&empty[ks]);
-                    __syncwarp();
+                    if (ok) {
+                        commit_if(e, &empty[vs]);
+                        if (more) commit_if(e, &empty[ks]);
+                    }
                 }
+            }
+        } else if (warp == 10) {
+            // ---------------- zero rows of V, when the MMA warp asks ----------------
+            int slot = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int tile = tile0; ok && tile * 256 < nq * p.group; tile += p.row_tiles) {
+                const Item w = umma_item(p, n, nq, tile, split);
+                for (int j = 0; ok && j < w.tiles; ++j) {
+                    const int vs = (slot + 2 * j + 1) % C::STAGES, key0 = w.lo + j * 128;
+                    if (key0 >= w.first && key0 + 128 <= w.hi) continue;
+                    ok = wait(&z_ask, phase);
+                    phase ^= 1u;
+                    if (!ok) break;
+                    const int r0 = max(w.first - key0, 0), r1 = min(w.hi - key0, 128);
+                    for (int i = lane; i < 128 * C::HALVES * 8; i += 32) {
+                        const int r = (i >> 3) & 127;
+                        if (r < r0 || r >= r1)
+                            *reinterpret_cast<uint4 *>(ring + vs * C::TILE + (i >> 10) * C::HALF + r * 128 + (i & 7) * 16) =
+                                make_uint4(0, 0, 0, 0);
+                    }
+                    umma::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&z_done);
+                }
+                slot = (slot + 2 * w.tiles) % C::STAGES;
             }
         }
     } else {
@@ -358,7 +455,8 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                     *reinterpret_cast<uint4 *>(q + (c >> 3) * C::HALF + (((c & 7) ^ (r & 7)) << 4)) = v;
                 }
                 umma::fence_proxy_async_smem();
-                mbar_arrive(&q_full[x]);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full[x]);
             }
             const RowRange see = row_range(p, n, nq, row);
             float m = -INFINITY, l = 0.0f;  // m: the (lazy) reference of the weights, scaled
@@ -369,16 +467,17 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                 if (!ok) break;
                 tc_fence_after();
                 float s[128];
+                uint32_t t[32];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    uint32_t t[32];
                     umma::tmem_ld32(ts + c * 32, t);
 #pragma unroll
                     for (int i = 0; i < 32; ++i) s[c * 32 + i] = __uint_as_float(t[i]);
                 }
                 umma::tmem_wait_ld();
                 const int key0 = w.lo + j * 128;
-                if (__any_sync(0xFFFFFFFFu, live && (key0 < see.lo || key0 + 128 > see.hi))) {
+                const bool edge = __any_sync(0xFFFFFFFFu, live && (key0 < see.lo || key0 + 128 > see.hi));
+                if (edge) {
                     const int from = see.lo - key0, to_ = see.hi - key0;
 #pragma unroll
                     for (int i = 0; i < 128; ++i)
@@ -386,7 +485,12 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                 }
                 float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int i = 4; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], s[i]);
+                for (int i = 4; i < 124; i += 8) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top[e] = max3(top[e], s[i + 2 * e], s[i + 2 * e + 1]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], s[124 + e]);
                 const float mt = __fmul_rn(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), p.scale_log2);
                 // grown by more than 2^8 (or the first finite maximum): move the reference
                 const bool grow = mt > m + 8.0f;
@@ -405,24 +509,35 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                 }
                 if (grow) m = mt;
                 const float y = m == -INFINITY ? 0.0f : m;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), y2 = make_float2(-y, -y);
+                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                // POLY of every 8 pairs by the polynomial: the exponential unit alone would bound the tile
+                auto weights = [&](auto poly) {
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t t[32];
+                    for (int c = 0; c < 2; ++c) {  // the first 64 keys' products start while the others' weights are made
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const float a = ex2(fmaf(s[c * 64 + 2 * i], p.scale_log2, -y));
-                        const float e = ex2(fmaf(s[c * 64 + 2 * i + 1], p.scale_log2, -y));
-                        sum[i & 1] += a;
-                        sum[2 + (i & 1)] += e;
-                        t[i] = pack2<T>(a, e);
+                        for (int i = 0; i < 32; ++i) {
+                            float2 e = fma2(make_float2(s[c * 64 + 2 * i], s[c * 64 + 2 * i + 1]), scale2, y2);
+                            if ((i & 7) < decltype(poly)::value) {
+                                e = exp2_poly<T>(e);
+                            } else {
+                                e.x = ex2(e.x);
+                                e.y = ex2(e.y);
+                            }
+                            sum[i & 1] = add2(sum[i & 1], e);
+                            t[i] = pack2<T>(e.x, e.y);
+                        }
+                        tmem_st32(ts + c * 32, t);
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(c ? &p_full[x] : &p_half[x]);
                     }
-                    tmem_st32(ts + c * 32, t);
-                }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tmem_wait_st();
-                tc_fence_before();
-                mbar_arrive(&p_full[x]);
+                };
+                if (edge) weights(std::integral_constant<int, 0>{});  // masked scores: exact zeros
+                else weights(std::integral_constant<int, POLY>{});
+                sum[0] = add2(sum[0], sum[1]);
+                l += sum[0].x + sum[0].y;
             }
             if (need > 0) {
                 ok = ok && wait(&o_full[x], o_phase);
