@@ -33,6 +33,9 @@
 #ifndef MGC_POLY
 #define MGC_POLY 0
 #endif
+#ifndef MGC_WAITK
+#define MGC_WAITK "try_wait"
+#endif
 namespace mgc {
 namespace paged {
 
@@ -157,6 +160,23 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Bounded wait of a converged warp, polled by the elected lane only.
+__device__ __forceinline__ bool poll(uint32_t e, uint64_t *bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %3, 0;\n\tsetp.ne.b32 p, 0, 0;\n\t"
+        "@q mbarrier." MGC_WAITK ".parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(done) : "r"(smem_addr(bar)), "r"(parity), "r"(e) : "memory");
+    return __any_sync(0xFFFFFFFFu, done != 0);
+}
+__device__ __forceinline__ bool warp_wait(uint32_t e, uint64_t *bar, uint32_t parity) {
+    if (poll(e, bar, parity)) return true;
+    const long long t0 = clock64();
+    while (!poll(e, bar, parity))
+        if (__any_sync(0xFFFFFFFFu, clock64() - t0 > umma::WAIT_LIMIT_CYCLES)) return false;
+    return true;
+}
+
 // Tensor maps of the pages: {head_dim, page_size, kv_heads, pages}.
 inline bool umma_maps(UmmaMaps *m, const mgc_cuda_paged &c) {
     auto fn = umma::encode_tiled_fn();
@@ -257,19 +277,10 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
     __syncthreads();
     tc_fence_after();
     const uint32_t tbase = tslot;
-    // A warp's bounded waits, polled by one lane or by all. A wait that runs out ends its role, and
-    // every role that waits for it.
+    // A wait that runs out ends its role, and every role that waits for it.
+    const uint32_t e = elect_one();
     auto wait = [&](uint64_t *bar, uint32_t parity) {
-        int ok = 1;
-        if (lane == 0) ok = mbar_wait(bar, parity);
-        ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
-        __syncwarp();
-        if (ok) return true;
-        umma::set_error(p.batch.status, MGC_CUDA_TIMEOUT);
-        return false;
-    };
-    auto waitw = [&](uint64_t *bar, uint32_t parity) {
-        if (__all_sync(0xFFFFFFFFu, mbar_wait(bar, parity))) return true;
+        if (warp_wait(e, bar, parity)) return true;
         umma::set_error(p.batch.status, MGC_CUDA_TIMEOUT);
         return false;
     };
@@ -330,7 +341,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
             uint32_t lap = 0, q_phase = 0, z_phase = 0, phase0 = 0, phase1 = 0;
             bool ok = true;
             constexpr uint32_t id_s = idesc_f16<T>(128, 0), id_o = idesc_f16<T>(DP, 1);
-            const uint32_t e = elect_one(), tb = __shfl_sync(0xFFFFFFFFu, tbase, 0);
+            const uint32_t tb = __shfl_sync(0xFFFFFFFFu, tbase, 0);
             auto step = [&]() {
                 if (++slot == C::STAGES) {
                     slot = 0;
@@ -348,10 +359,10 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
             };
             for (int tile = tile0; ok && tile * 256 < nq * p.group; tile += p.row_tiles) {
                 const Item w = umma_item(p, n, nq, tile, split);
-                ok = waitw(&q_full[0], q_phase) && waitw(&q_full[1], q_phase);
+                ok = wait(&q_full[0], q_phase) && wait(&q_full[1], q_phase);
                 q_phase ^= 1u;
                 if (ok && w.tiles > 0) {
-                    ok = waitw(&full[slot], lap);
+                    ok = wait(&full[slot], lap);
                     tc_fence_after();
                     if (ok) {
                         if (w.need0 > 0) scores(0, slot);
@@ -362,7 +373,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                 }
                 for (int j = 0; ok && j < w.tiles; ++j) {
                     const int vs = slot;
-                    ok = waitw(&full[vs], lap);
+                    ok = wait(&full[vs], lap);
                     step();
                     const int ks = slot;
                     const bool more = j + 1 < w.tiles;
@@ -371,11 +382,11 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                         // rows of V that no row sees: warp 10 zeroes them
                         if (lane == 0) mbar_arrive(&z_ask);
                         __syncwarp();
-                        ok = waitw(&z_done, z_phase);
+                        ok = wait(&z_done, z_phase);
                         z_phase ^= 1u;
                     }
                     if (more) {
-                        ok = ok && waitw(&full[ks], lap);
+                        ok = ok && wait(&full[ks], lap);
                         step();
                     }
                     const uint64_t v = mn128_desc(smem_addr(ring) + vs * C::TILE, C::HALF);
@@ -384,12 +395,12 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                         if (!ok || j >= w.need(x)) continue;
                         const uint32_t o = tb + C::O_COL + x * DP, w16 = tb + C::S_COL + x * 128;
                         uint32_t &phase = x ? phase1 : phase0;
-                        ok = waitw(&p_half[x], phase);
+                        ok = wait(&p_half[x], phase);
                         if (!ok) continue;
                         tc_fence_after();
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk) mma_f16_ts(e, o, w16 + kk * 8, v + kk * (2048 >> 4), id_o, j > 0 || kk > 0);
-                        ok = waitw(&p_full[x], phase);
+                        ok = wait(&p_full[x], phase);
                         phase ^= 1u;
                         if (!ok) continue;
                         tc_fence_after();
@@ -517,15 +528,15 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                     for (int c = 0; c < 2; ++c) {  // the first 64 keys' products start while the others' weights are made
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
-                            float2 e = fma2(make_float2(s[c * 64 + 2 * i], s[c * 64 + 2 * i + 1]), scale2, y2);
+                            float2 z = fma2(make_float2(s[c * 64 + 2 * i], s[c * 64 + 2 * i + 1]), scale2, y2);
                             if ((i & 7) < decltype(poly)::value) {
-                                e = exp2_poly<T>(e);
+                                z = exp2_poly<T>(z);
                             } else {
-                                e.x = ex2(e.x);
-                                e.y = ex2(e.y);
+                                z.x = ex2(z.x);
+                                z.y = ex2(z.y);
                             }
-                            sum[i & 1] = add2(sum[i & 1], e);
-                            t[i] = pack2<T>(e.x, e.y);
+                            sum[i & 1] = add2(sum[i & 1], z);
+                            t[i] = pack2<T>(z.x, z.y);
                         }
                         tmem_st32(ts + c * 32, t);
                         tmem_wait_st();
