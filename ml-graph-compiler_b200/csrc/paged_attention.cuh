@@ -86,6 +86,7 @@ struct Plan {
     bool mma = false, umma = false;
     int wm = 1;         // 16-row warps of a row tile
     int row_tiles = 1, splits = 1;
+    int ctas = 0;       // of the tcgen05 kernel
     bool clustered = false;
     int64_t workspace = 0;
 };
@@ -107,16 +108,10 @@ inline Plan plan_of(const mgc_cuda_paged_attention_args &a) {
     const int64_t group = a.q_heads / c.kv_heads;
     int64_t max_q = a.max_q < 1 ? 1 : a.max_q > c.tokens ? c.tokens : a.max_q;
     const int64_t rows = max_q * group;
-    if (rows > 64 && umma_fits(c)) {
+    if (rows > 64 && umma_fits(c) && c.batch * ceil_div(rows, 256) < 0x7FFFFFFF) {
         s.umma = true;
-        s.row_tiles = (int)ceil_div(rows, 256);
-        const int64_t units = c.batch * c.kv_heads * s.row_tiles;
-        int64_t most = a.max_kv, splits = units >= sm_count() ? 1 : sm_count() / units;
-        if (a.window > 0 && a.window + max_q < most) most = a.window + max_q;
-        if (splits > most / 512) splits = most / 512;
-        if (splits < 1) splits = 1;
-        s.splits = (int)splits;
-        if (splits > 1) s.workspace = splits * c.tokens * a.q_heads * (c.head_dim * 4 + 8);
+        s.ctas = sm_count();
+        s.workspace = (int64_t)s.ctas * (2 * 256 * (c.head_dim * 4 + 8) + sizeof(CutUnit));
         return s;
     }
     s.wm = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
@@ -143,33 +138,33 @@ inline int64_t attend_workspace(const mgc_cuda_paged_attention_args &a) {
     return a.paged.tokens == 0 || a.paged.batch == 0 ? 0 : plan_of(a).workspace;
 }
 
-template <typename T> inline int launch_combine(const AttendParams &p, cudaStream_t stream) {
-    // the combine kernel's blocks may be set up while the parts finish; it waits for them itself
-    cudaLaunchConfig_t comb{};
-    comb.gridDim = dim3((unsigned)ceil_div((int64_t)p.tokens * p.q_heads, 4));
-    comb.blockDim = dim3(128);
-    comb.stream = stream;
+// A combine kernel's blocks may be set up while the kernel before finishes; they wait for it themselves.
+template <typename K> inline int launch_after(K kernel, dim3 grid, const AttendParams &p, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(128);
+    cfg.stream = stream;
     cudaLaunchAttribute dep[1];
     dep[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     dep[0].val.programmaticStreamSerializationAllowed = 1;
-    comb.attrs = dep;
-    comb.numAttrs = 1;
-    MGC_CHECK_CUDA(cudaLaunchKernelEx(&comb, paged_combine_kernel<T>, p));
+    cfg.attrs = dep;
+    cfg.numAttrs = 1;
+    MGC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
     return MGC_CUDA_OK;
 }
 
-template <typename T> inline int launch_umma(const AttendParams &p, const mgc_cuda_paged &c, int64_t blocks, cudaStream_t stream) {
+template <typename T> inline int launch_umma(const AttendParams &p, const mgc_cuda_paged &c, int ctas, cudaStream_t stream) {
     UmmaMaps maps;
     memset(&maps, 0, sizeof maps);
     if (!umma_maps(&maps, c)) return fail(MGC_CUDA_UNSUPPORTED, "mgc_cuda_paged_attention: tensor map encoding failed");
     auto go = [&](auto kernel, uint32_t smem, int threads) -> int {
         MGC_CHECK(raise_smem_ceiling((const void *)kernel));
-        kernel<<<dim3((unsigned)blocks, (unsigned)p.splits), threads, smem, stream>>>(p, maps);
+        kernel<<<(unsigned)ctas, threads, smem, stream>>>(p, maps);
         return check_launch("paged_attention_umma_kernel");
     };
     MGC_CHECK(p.head_dim <= 64 ? go(paged_attention_umma_kernel<T, 64>, UmmaConfig<64>::SMEM, UmmaConfig<64>::THREADS)
                                : go(paged_attention_umma_kernel<T, 128>, UmmaConfig<128>::SMEM, UmmaConfig<128>::THREADS));
-    return p.splits == 1 ? MGC_CUDA_OK : launch_combine<T>(p, stream);
+    return launch_after(paged_combine_units_kernel<T>, dim3((unsigned)ctas, 32), p, stream);
 }
 
 template <typename T, int DP, int WM, int WN> inline int launch_mma(const AttendParams &p, int64_t blocks, cudaStream_t stream) {
@@ -188,7 +183,8 @@ template <typename T, int DP, int WM, int WN> inline int launch_mma(const Attend
     cfg.attrs = attr;
     cfg.numAttrs = p.clustered ? 1 : 0;
     MGC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
-    return p.splits == 1 || p.clustered ? MGC_CUDA_OK : launch_combine<T>(p, stream);
+    if (p.splits == 1 || p.clustered) return MGC_CUDA_OK;
+    return launch_after(paged_combine_kernel<T>, dim3((unsigned)ceil_div((int64_t)p.tokens * p.q_heads, 4)), p, stream);
 }
 
 template <typename T, int DP> inline int launch_mma_rows(const AttendParams &p, int wm, int64_t blocks, cudaStream_t stream) {
@@ -225,19 +221,21 @@ inline int attend(const mgc_cuda_paged_attention_args &a, cudaStream_t stream) {
     p.max_positions = (int)(c.table_pages * c.page_size);
     const Plan s = plan_of(a);
     p.row_tiles = s.row_tiles; p.splits = s.splits; p.clustered = s.clustered;
-    p.part = nullptr; p.part_ml = nullptr;
+    p.part = nullptr; p.part_ml = nullptr; p.cut = nullptr;
     if (s.workspace) {
         if (!a.workspace || a.workspace_bytes < s.workspace || !aligned(a.workspace, 16))
             return fail(MGC_CUDA_NEEDS_WORKSPACE, "%s: needs %lld bytes of workspace (16-byte aligned), got %lld", what,
                         (long long)s.workspace, (long long)(a.workspace ? a.workspace_bytes : 0));
         p.part = static_cast<float *>(a.workspace);
-        p.part_ml = reinterpret_cast<float2 *>(p.part + (int64_t)s.splits * p.tokens * p.q_heads * p.head_dim);
+        const int64_t rows = s.umma ? (int64_t)s.ctas * 2 * 256 : (int64_t)s.splits * p.tokens * p.q_heads;
+        p.part_ml = reinterpret_cast<float2 *>(p.part + rows * p.head_dim);
+        p.cut = reinterpret_cast<CutUnit *>(p.part_ml + rows);
     }
     if (s.mma) {
         const int64_t blocks = c.batch * c.kv_heads * s.row_tiles;
         if (blocks > 0x7FFFFFFF) return fail(MGC_CUDA_UNSUPPORTED, "%s: %lld blocks", what, (long long)blocks);
         if (s.umma)
-            return c.dtype == MGC_F16 ? launch_umma<__half>(p, c, blocks, stream) : launch_umma<__nv_bfloat16>(p, c, blocks, stream);
+            return c.dtype == MGC_F16 ? launch_umma<__half>(p, c, s.ctas, stream) : launch_umma<__nv_bfloat16>(p, c, s.ctas, stream);
         if (c.dtype == MGC_F32) return launch_mma_width<float>(p, s.wm, blocks, stream);
         if (c.dtype == MGC_F16) return launch_mma_width<__half>(p, s.wm, blocks, stream);
         return launch_mma_width<__nv_bfloat16>(p, s.wm, blocks, stream);

@@ -11,6 +11,12 @@
 namespace mgc {
 namespace paged {
 
+// A unit of rows whose first piece ended CTA c's stretch of work (one per CTA at most): its pieces
+// are c's second slot of partial results and the first slots of the next pieces - 1 CTAs.
+struct CutUnit {
+    int h, b, t, pieces;
+};
+
 struct AttendParams {
     Batch batch;
     const void *k_pages, *v_pages;
@@ -28,6 +34,8 @@ struct AttendParams {
     int clustered;      // the parts are one cluster; else their partial results go to part, part_ml
     float *part;        // [splits][tokens][q_heads][head_dim], relative to the part's maximum
     float2 *part_ml;    // [splits][tokens][q_heads]: maximum, sum
+    // the tcgen05 kernel: part and part_ml are [CTA][2][256] rows of pieces, and
+    CutUnit *cut;       // [CTA]
 };
 
 constexpr int MAX_HEAD_DIM = 256;

@@ -204,31 +204,168 @@ inline bool umma_fits(const mgc_cuda_paged &c) {
            c.page_stride < most;
 }
 
-// The keys of one CTA's work item: [lo, hi) in tiles of 128 from lo, `tiles` of them, and how many
-// of those row tile x needs (rows of the first tile stop earlier under a causal mask).
+// ---- work: 256-row units in a fixed order, cut evenly over the CTAs ---------------------------------
+// A unit is (key head, sequence, 256 query rows) and is as long as it has key tiles (at least 1). All
+// units lie end to end, key head by key head; CTA c takes the c-th of gridDim.x equal stretches. A
+// stretch that ends inside a unit cuts it (unless a piece would be below MIN_PIECE tiles): each piece
+// leaves its rows' partial results, and paged_combine_units_kernel adds them in order. 256 equal
+// units on 148 SMs would otherwise take two rounds, the second 73% full.
+constexpr int MIN_PIECE = 2;
+
 struct Item {
-    int rows, row0;        // query rows of the sequence; first of the CTA's
-    int lo, hi, tiles;
-    int first;             // first key that any of the rows sees
-    int need0, need1;
+    int rows, row0;     // query rows of the sequence; first of the unit's
+    int start;          // the sequence's first token
+    int n, nq;          // its positions, its new tokens
+    int b, h;
+    int lo, hi, tiles;  // keys [lo, hi) of this piece in `tiles` tiles of 128
+    int first;          // first key that any row of the unit sees
+    int need0, need1;   // tiles that row tile 0 / 1 needs (rows of the first stop earlier if causal)
+    int slot;           // where partial results go: -1 (the whole unit), 0 (a later piece), 1 (the first)
     __device__ __forceinline__ int need(int x) const { return x ? need1 : need0; }
 };
 
-__device__ __forceinline__ Item umma_item(const AttendParams &p, int n, int nq, int tile, int split) {
-    Item w;
-    w.rows = nq * p.group;
-    w.row0 = tile * 256;
-    const RowRange a = row_range(p, n, nq, w.row0), z = row_range(p, n, nq, min(w.row0 + 256, w.rows) - 1);
-    const RowRange mid = row_range(p, n, nq, min(w.row0 + 128, w.rows) - 1);
-    const int lo = a.lo & ~127, hi = max(z.hi, 0);
-    const int all = (max(hi - lo, 0) + 127) >> 7, per = (all + p.splits - 1) / p.splits;
-    w.first = a.lo;
-    w.lo = lo + split * per * 128;
-    w.hi = min(hi, w.lo + per * 128);
-    w.tiles = w.hi > w.lo ? (w.hi - w.lo + 127) >> 7 : 0;
-    w.need0 = min(w.tiles, (max(mid.hi - w.lo, 0) + 127) >> 7);
-    w.need1 = w.rows - w.row0 > 128 ? w.tiles : 0;
-    return w;
+struct Walk {
+    int h, b, t;  // unit
+    int skip;     // its tiles before this CTA's stretch
+    int left;     // tiles left of the stretch
+    int share;    // tiles of a whole stretch
+    int start, nq, n;  // sequence b: first token, new tokens, positions
+};
+
+__device__ __forceinline__ void load_sequence(const AttendParams &p, int b, int &start, int &nq, int &n) {
+    start = __ldg(p.batch.q_starts + b);
+    nq = __ldg(p.batch.q_starts + b + 1) - start;
+    n = min(__ldg(p.batch.kv_lens + b), p.max_positions);
+}
+
+// Keys [lo, hi) that rows [256 t, 256 t + 256) see, lo rounded down to a tile; the unit's length.
+__device__ __forceinline__ int unit_length(const AttendParams &p, int n, int nq, int t, int &first, int &lo, int &hi) {
+    const int rows = nq * p.group, row0 = t * 256;
+    const RowRange a = row_range(p, n, nq, row0), z = row_range(p, n, nq, min(row0 + 256, rows) - 1);
+    first = a.lo;
+    lo = a.lo & ~127;
+    hi = max(z.hi, 0);
+    return hi > lo ? (hi - lo + 127) >> 7 : 1;
+}
+
+// The next piece of the stretch; false at its end. Advances the walk.
+__device__ __forceinline__ bool next_item(const AttendParams &p, Walk &k, Item &w) {
+    while (k.left > 0 && k.h < p.kv_heads) {
+        w.start = k.start;
+        w.nq = k.nq;
+        w.n = k.n;
+        w.rows = w.nq * p.group;
+        w.row0 = k.t * 256;
+        if (w.row0 >= w.rows) {  // past the sequence: the next one
+            k.t = 0;
+            if (++k.b == p.batch.batch) {
+                k.b = 0;
+                ++k.h;
+            }
+            load_sequence(p, k.b, k.start, k.nq, k.n);
+            continue;
+        }
+        int lo, hi;
+        const int length = unit_length(p, w.n, w.nq, k.t, w.first, lo, hi);
+        int take = length - k.skip;
+        if (take > k.left) {
+            const int at = k.skip + k.left;  // where the stretch ends in the unit
+            if (at < MIN_PIECE) break;
+            if (length - at >= MIN_PIECE) take = k.left;
+        }
+        w.b = k.b;
+        w.h = k.h;
+        w.lo = lo + k.skip * 128;
+        w.hi = min(hi, w.lo + take * 128);
+        w.tiles = w.hi > w.lo ? (w.hi - w.lo + 127) >> 7 : 0;
+        const RowRange mid = row_range(p, w.n, w.nq, min(w.row0 + 128, w.rows) - 1);
+        w.need0 = min(w.tiles, (max(mid.hi - w.lo, 0) + 127) >> 7);
+        w.need1 = w.rows - w.row0 > 128 ? w.tiles : 0;
+        w.slot = take == length ? -1 : k.skip > 0 ? 0 : 1;
+        k.left -= take;
+        if (k.skip + take == length) {
+            k.skip = 0;
+            ++k.t;
+        } else {
+            k.skip += take;
+        }
+        return true;
+    }
+    return false;
+}
+
+// Start of CTA c's stretch (one warp). Units are looked at 32 at a time; their lengths are the same
+// for every key head. Also leaves, for a unit cut at the stretch's end, what adding its pieces needs.
+__device__ __forceinline__ Walk find_stretch(const AttendParams &p, int c, int ctas, int lane) {
+    int most = 0;  // row tiles of the longest sequence
+    for (int b = lane; b < p.batch.batch; b += 32) {
+        int start, nq, n;
+        load_sequence(p, b, start, nq, n);
+        if (n != __ldg(p.batch.kv_lens + b) && nq > 0 && p.batch.status) *p.batch.status = MGC_CUDA_GATHER_OOB;
+        most = max(most, (nq * p.group + 255) >> 8);
+    }
+    most = __reduce_max_sync(0xFFFFFFFFu, most);
+    const unsigned count = (unsigned)p.batch.batch * (unsigned)most;
+    auto length_of = [&](unsigned i) {
+        if (i >= count) return 0;
+        int start, nq, n, first, lo, hi;
+        const unsigned b = i / (unsigned)most;
+        load_sequence(p, (int)b, start, nq, n);
+        const int t = (int)(i - b * (unsigned)most);
+        return t * 256 < nq * p.group ? unit_length(p, n, nq, t, first, lo, hi) : 0;
+    };
+    // the lanes' lengths summed up to and including each; the first 32 units' are kept
+    auto scan = [&](int v) {
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int u = __shfl_up_sync(0xFFFFFFFFu, v, d);
+            if (lane >= d) v += u;
+        }
+        return v;
+    };
+    const int mine0 = length_of(lane), upto0 = scan(mine0);
+    long long head = __shfl_sync(0xFFFFFFFFu, upto0, 31);  // tiles of one key head
+    for (unsigned i = 32; i < count; i += 32) head += __reduce_add_sync(0xFFFFFFFFu, length_of(i + lane));
+    Walk k{p.kv_heads, 0, 0, 0, 0, 0, 0, 0, 0};
+    const long long all = head * p.kv_heads;
+    long long share, x0;
+    if (all < 0x7FFFFFFF) {
+        share = ((unsigned)all + ctas - 1) / (unsigned)ctas;
+        share = max(share, (long long)MIN_PIECE);
+        x0 = c * share;
+        if (x0 >= all) return k;
+        k.h = (int)((unsigned)x0 / (unsigned)head);
+    } else {
+        share = (all + ctas - 1) / ctas;
+        x0 = c * share;
+        if (x0 >= all) return k;
+        k.h = (int)(x0 / head);
+    }
+    long long at = x0 - k.h * head;
+    for (unsigned i = 0; i < count; i += 32) {
+        const int mine = i ? length_of(i + lane) : mine0, upto = i ? scan(mine) : upto0;
+        const unsigned past = __ballot_sync(0xFFFFFFFFu, upto > at);
+        if (past) {
+            const int who = __ffs(past) - 1;
+            const int length = __shfl_sync(0xFFFFFFFFu, mine, who);
+            const int off = (int)at - (__shfl_sync(0xFFFFFFFFu, upto, who) - length);
+            k.b = (int)((i + who) / (unsigned)most);
+            k.t = (int)((i + who) % (unsigned)most);
+            load_sequence(p, k.b, k.start, k.nq, k.n);
+            k.left = k.share = (int)share;
+            if (off < MIN_PIECE) {
+                k.left += off;
+            } else if (length - off < MIN_PIECE) {
+                k.left -= length - off;
+                ++k.t;
+            } else {
+                k.skip = off;
+            }
+            break;
+        }
+        at -= __shfl_sync(0xFFFFFFFFu, upto, 31);
+    }
+    return k;
 }
 
 template <typename T, int DP>
@@ -240,20 +377,10 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
     __shared__ __align__(8) uint64_t full[C::STAGES], empty[C::STAGES], q_full[2], s_full[2], p_half[2], p_full[2], o_full[2];
     __shared__ __align__(8) uint64_t z_ask, z_done;
     __shared__ uint32_t tslot;
+    __shared__ Walk stretch;
     uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *sQ = base, *ring = base + 2 * C::TILE;
     const int tid = (int)threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
-    unsigned u = blockIdx.x;
-    const int split = (int)blockIdx.y;
-    const int kh = (int)(u % (unsigned)p.kv_heads);
-    u /= (unsigned)p.kv_heads;
-    const int tile0 = p.row_tiles - 1 - (int)(u % (unsigned)p.row_tiles);  // longest rows first
-    const int b = (int)(u / (unsigned)p.row_tiles);
-    const int start = __ldg(p.batch.q_starts + b), nq = __ldg(p.batch.q_starts + b + 1) - start;
-    const int n = min(__ldg(p.batch.kv_lens + b), p.max_positions);
-    if (n != __ldg(p.batch.kv_lens + b) && tid == 0 && p.batch.status) *p.batch.status = MGC_CUDA_GATHER_OOB;
-    if (tile0 * 256 >= nq * p.group) return;
-
     if (tid == 0) {
         for (int s = 0; s < C::STAGES; ++s) {
             mbar_init(&full[s], 1);
@@ -273,10 +400,16 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
         umma::prefetch_tmap(&maps.v);
     }
     if (warp == 8) umma::tmem_alloc(&tslot, 512);
+    if (warp == 11) {
+        const Walk k = find_stretch(p, (int)blockIdx.x, (int)gridDim.x, lane);
+        if (lane == 0) stretch = k;
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tbase = tslot;
+    Walk walk = stretch;
+    Item w;
     // A wait that runs out ends its role, and every role that waits for it.
     const uint32_t e = elect_one();
     auto wait = [&](uint64_t *bar, uint32_t parity) {
@@ -293,14 +426,13 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
             const int boxes = (128 / maps.box_rows) * C::HALVES;  // of a tile: at most 32
             const int part = lane / C::HALVES, half = lane % C::HALVES;
             bool ok = true;
-            for (int tile = tile0; ok && tile * 256 < nq * p.group; tile += p.row_tiles) {
-                const Item w = umma_item(p, n, nq, tile, split);
+            while (ok && next_item(p, walk, w)) {
                 // this lane's box of key tile j: page and first row in it; -1 if no row sees its keys
                 auto box = [&](int j, int &row) {
                     const int at = w.lo + j * 128 + part * maps.box_rows;
                     row = at % p.batch.page_size;
                     if (lane >= boxes || j >= w.tiles || at >= w.hi || at + maps.box_rows <= w.first) return -1;
-                    return page_of(p.batch, b, at / p.batch.page_size);
+                    return page_of(p.batch, w.b, at / p.batch.page_size);
                 };
                 int row, page = box(0, row);
                 for (int j = 0; ok && j < w.tiles; ++j) {
@@ -314,7 +446,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                         __syncwarp();
                         if (page >= 0)
                             umma::tma_load_4d(ring + slot * C::TILE + half * C::HALF + part * maps.box_rows * 128,
-                                              kv ? &maps.v : &maps.k, &full[slot], half * 64, row, kh, page);
+                                              kv ? &maps.v : &maps.k, &full[slot], half * 64, row, w.h, page);
                         ++issued;
                         if (++slot == C::STAGES) {
                             slot = 0;
@@ -357,8 +489,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                 }
                 commit_if(e, &s_full[x]);
             };
-            for (int tile = tile0; ok && tile * 256 < nq * p.group; tile += p.row_tiles) {
-                const Item w = umma_item(p, n, nq, tile, split);
+            while (ok && next_item(p, walk, w)) {
                 ok = wait(&q_full[0], q_phase) && wait(&q_full[1], q_phase);
                 q_phase ^= 1u;
                 if (ok && w.tiles > 0) {
@@ -420,8 +551,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
             int slot = 0;
             uint32_t phase = 0;
             bool ok = true;
-            for (int tile = tile0; ok && tile * 256 < nq * p.group; tile += p.row_tiles) {
-                const Item w = umma_item(p, n, nq, tile, split);
+            while (ok && next_item(p, walk, w)) {
                 for (int j = 0; ok && j < w.tiles; ++j) {
                     const int vs = (slot + 2 * j + 1) % C::STAGES, key0 = w.lo + j * 128;
                     if (key0 >= w.first && key0 + 128 <= w.hi) continue;
@@ -441,6 +571,21 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                 }
                 slot = (slot + 2 * w.tiles) % C::STAGES;
             }
+        } else {
+            // ---------------- warp 11: how many pieces has the unit cut at the stretch's end? ----------------
+            CutUnit cut{0, 0, 0, 0};
+            while (next_item(p, walk, w)) {
+                if (w.slot != 1) continue;
+                int first, lo, hi;
+                cut.h = w.h;
+                cut.b = w.b;
+                cut.t = w.row0 >> 8;
+                const int length = unit_length(p, w.n, w.nq, cut.t, first, lo, hi);
+                cut.pieces = 1;
+                // the next stretches' ends in this unit
+                for (int at = w.tiles; length - at >= MIN_PIECE; at += walk.share) ++cut.pieces;
+            }
+            if (lane == 0) p.cut[blockIdx.x] = cut;
         }
     } else {
         // ---------------- softmax: one row per thread ----------------
@@ -450,26 +595,36 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
         const uint32_t ts = tbase + lanes + C::S_COL + x * 128, to = tbase + lanes + C::O_COL + x * DP;
         uint32_t s_phase = 0, o_phase = 0;
         bool ok = true;
-        for (int tile = tile0; ok && tile * 256 < nq * p.group; tile += p.row_tiles) {
-            const Item w = umma_item(p, n, nq, tile, split);
+        while (ok && next_item(p, walk, w)) {
             const int row = w.row0 + x * 128 + r;
             const bool live = row < w.rows;
-            const int head = kh * p.group + row % p.group;
-            const long long token = start + row / p.group;
+            // element offsets of this thread's row of q and of out; a warp moves its 32 rows together,
+            // 16 bytes a lane along the rows (a row per thread touches 32 lines an instruction)
+            const int head = w.h * p.group + row % p.group;
+            const long long token = w.start + row / p.group;
+            const long long q_off = token * p.q_ts + (long long)head * p.q_hs, o_off = token * p.o_ts + (long long)head * p.o_hs;
+            constexpr int CHUNKS = DP / 8;               // 16-byte chunks of a 16-bit row
+            uint8_t *rows32 = sQ + x * C::TILE + (r & 96) * 128;  // the warp's 32 rows of the Q tile
+            auto chunk = [&](int rr, int c) { return rows32 + (c >> 3) * C::HALF + rr * 128 + (((c & 7) ^ (rr & 7)) << 4); };
+            const int lives = min(32, w.rows - (w.row0 + x * 128 + (r & 96)));  // rows of the warp that exist
             {
-                uint8_t *q = sQ + x * C::TILE + r * 128;
-                const T *src = static_cast<const T *>(p.q) + token * p.q_ts + (long long)head * p.q_hs;
+                uint4 v[CHUNKS];  // every load in flight before the first store
 #pragma unroll
-                for (int c = 0; c < DP / 8; ++c) {
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (live && c * 8 < p.head_dim) v = *reinterpret_cast<const uint4 *>(src + c * 8);
-                    *reinterpret_cast<uint4 *>(q + (c >> 3) * C::HALF + (((c & 7) ^ (r & 7)) << 4)) = v;
+                for (int i = 0; i < CHUNKS; ++i) {
+                    const int rr = (i * 32 + lane) / CHUNKS, c = (i * 32 + lane) % CHUNKS;
+                    const long long off = __shfl_sync(0xFFFFFFFFu, q_off, rr);
+                    v[i] = make_uint4(0, 0, 0, 0);
+                    if (rr < lives && c * 8 < p.head_dim)
+                        v[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q) + off + c * 8));
                 }
+#pragma unroll
+                for (int i = 0; i < CHUNKS; ++i)
+                    *reinterpret_cast<uint4 *>(chunk((i * 32 + lane) / CHUNKS, (i * 32 + lane) % CHUNKS)) = v[i];
                 umma::fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_full[x]);
             }
-            const RowRange see = row_range(p, n, nq, row);
+            const RowRange see = row_range(p, w.n, w.nq, row);
             float m = -INFINITY, l = 0.0f;  // m: the (lazy) reference of the weights, scaled
             const int need = w.need(x);
             for (int j = 0; j < need; ++j) {
@@ -556,40 +711,54 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                 tc_fence_after();
             }
             if (!ok) break;
-            // ---- the row of O ----
-            const long long at = ((long long)split * p.tokens + token) * p.q_heads + head;
-            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-            T *out = static_cast<T *>(p.out) + token * p.o_ts + (long long)head * p.o_hs;
-            if (p.splits > 1 && live) p.part_ml[at] = make_float2(m, l);
+            // ---- O: through the warp's rows of the Q tile (no longer read) to whole rows of memory ----
+            const bool whole = w.slot < 0;
+            const long long at = ((long long)blockIdx.x * 2 + w.slot) * 256 + x * 128 + (r & 96);  // a piece's first row
+            const float inv = whole ? (l > 0.0f ? 1.0f / l : 0.0f) : 1.0f;
+            if (!whole && live) p.part_ml[at + lane] = make_float2(m, l);
 #pragma unroll
-            for (int c = 0; c < DP / 32; ++c) {
+            for (int pass = 0; pass < 2; ++pass) {  // half of the channels at a time
                 uint32_t t[32];
-                if (need > 0) {
-                    umma::tmem_ld32(to + c * 32, t);
-                    umma::tmem_wait_ld();
-                } else {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) t[i] = 0u;
-                }
-                if (!live) continue;
-                if (p.splits > 1) {
+                for (int c = 0; c < DP / 64; ++c) {
+                    if (need > 0) {
+                        umma::tmem_ld32(to + pass * (DP / 2) + c * 32, t);
+                        umma::tmem_wait_ld();
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (c * 32 + i * 4 < p.head_dim)
-                            *reinterpret_cast<uint4 *>(p.part + at * p.head_dim + c * 32 + i * 4) =
-                                make_uint4(t[4 * i], t[4 * i + 1], t[4 * i + 2], t[4 * i + 3]);
-                } else {
+                        for (int i = 0; i < 32; ++i) t[i] = 0u;
+                    }
+                    if (whole) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (c * 32 + i * 8 < p.head_dim) {
-                            uint4 v;
-                            uint32_t *q = reinterpret_cast<uint32_t *>(&v);
+                        for (int i = 0; i < 4; ++i) {
+                            uint32_t q[4];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                q[e] = pack2<T>(__uint_as_float(t[8 * i + 2 * e]) * inv, __uint_as_float(t[8 * i + 2 * e + 1]) * inv);
-                            *reinterpret_cast<uint4 *>(out + c * 32 + i * 8) = v;
+                            for (int u = 0; u < 4; ++u)
+                                q[u] = pack2<T>(__uint_as_float(t[8 * i + 2 * u]) * inv, __uint_as_float(t[8 * i + 2 * u + 1]) * inv);
+                            *reinterpret_cast<uint4 *>(chunk(lane, pass * (DP / 16) + c * 4 + i)) = make_uint4(q[0], q[1], q[2], q[3]);
                         }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            *reinterpret_cast<uint4 *>(chunk(lane, c * 8 + i)) =
+                                make_uint4(t[4 * i], t[4 * i + 1], t[4 * i + 2], t[4 * i + 3]);
+                    }
                 }
+                if (whole && pass == 0) continue;
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < CHUNKS; ++i) {
+                    const int rr = (i * 32 + lane) / CHUNKS, c = (i * 32 + lane) % CHUNKS;
+                    const long long off = __shfl_sync(0xFFFFFFFFu, o_off, rr);
+                    if (rr >= lives) continue;
+                    const uint4 v = *reinterpret_cast<const uint4 *>(chunk(rr, c));
+                    if (whole) {
+                        if (c * 8 < p.head_dim) *reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + off + c * 8) = v;
+                    } else if (pass * (DP / 2) + c * 4 < p.head_dim) {
+                        *reinterpret_cast<uint4 *>(p.part + (at + rr) * p.head_dim + pass * (DP / 2) + c * 4) = v;
+                    }
+                }
+                __syncwarp();
             }
             tc_fence_before();
         }
@@ -600,6 +769,50 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
     if (warp == 8) {
         tc_fence_after();
         umma::tmem_dealloc(tbase, 512);
+    }
+}
+
+// out of the rows of units that were cut: one warp per row at a time, the pieces in order.
+template <typename T>
+__global__ void __launch_bounds__(128) paged_combine_units_kernel(const __grid_constant__ AttendParams p) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int c = (int)blockIdx.x, lane = (int)(threadIdx.x & 31);
+    const CutUnit cut = p.cut[c];
+    if (cut.pieces < 2) return;
+    int start, nq, n;
+    load_sequence(p, cut.b, start, nq, n);
+    const int rows = nq * p.group;
+    for (int r = (int)blockIdx.y * 4 + (int)(threadIdx.x >> 5); r < 256; r += (int)gridDim.y * 4) {
+        const int row = cut.t * 256 + r;
+        if (row >= rows) break;
+        auto at = [&](int i) { return ((long long)(c + i) * 2 + (i == 0 ? 1 : 0)) * 256 + r; };
+        float m = -INFINITY, l = 0.0f;
+        for (int i = lane; i < cut.pieces; i += 32) m = fmaxf(m, p.part_ml[at(i)].x);
+#pragma unroll
+        for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));
+        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (lane * 4 < p.head_dim) {
+#pragma unroll 4
+            for (int i = 0; i < cut.pieces; ++i) {
+                const float2 ml = p.part_ml[at(i)];
+                const float4 v = *reinterpret_cast<const float4 *>(p.part + at(i) * p.head_dim + lane * 4);
+                const float f = ml.y == 0.0f ? 0.0f : ex2(ml.x - m);
+                l += f * ml.y;
+                a.x += f * v.x;
+                a.y += f * v.y;
+                a.z += f * v.z;
+                a.w += f * v.w;
+            }
+            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            T *out = static_cast<T *>(p.out) + (long long)(start + row / p.group) * p.o_ts +
+                     (long long)(cut.h * p.group + row % p.group) * p.o_hs + lane * 4;
+            Pack<4, T> v;
+            v.e[0] = from_f<T>(a.x * inv);
+            v.e[1] = from_f<T>(a.y * inv);
+            v.e[2] = from_f<T>(a.z * inv);
+            v.e[3] = from_f<T>(a.w * inv);
+            v.store(out);
+        }
     }
 }
 
