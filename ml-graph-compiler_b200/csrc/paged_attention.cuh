@@ -4,6 +4,9 @@
 
 #include "paged_umma.cuh"
 
+#ifndef MGC_WAVES
+#define MGC_WAVES 3
+#endif
 namespace mgc {
 namespace paged {
 
@@ -118,12 +121,12 @@ inline Plan plan_of(const mgc_cuda_paged_attention_args &a) {
     s.row_tiles = (int)ceil_div(rows, 16 * s.wm);
     const int64_t units = c.batch * c.kv_heads * s.row_tiles;
     // enough parts for two blocks per SM; three times that for batches, whose sequences differ
-    const int64_t target = 2ll * sm_count() * (c.batch > 1 ? 3 : 1);
+    const int64_t target = 2ll * sm_count() * (c.batch > 1 ? MGC_WAVES : 1);
     int64_t most = a.max_kv;
     if (a.window > 0 && a.window + max_q < most) most = a.window + max_q;
     int64_t splits = units >= target ? 1 : ceil_div(target, units);
     if (splits > most / MIN_SPLIT_KEYS) splits = most / MIN_SPLIT_KEYS;
-    if (splits > 128) splits = 128;
+    if (splits > MAX_SPLITS) splits = MAX_SPLITS;
     if (splits < 1) splits = 1;
     if (splits > MAX_CLUSTER && c.batch > 1) splits = MAX_CLUSTER;
     s.splits = (int)splits;
@@ -184,7 +187,7 @@ template <typename T, int DP, int WM, int WN> inline int launch_mma(const Attend
     cfg.numAttrs = p.clustered ? 1 : 0;
     MGC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
     if (p.splits == 1 || p.clustered) return MGC_CUDA_OK;
-    return launch_after(paged_combine_kernel<T>, dim3((unsigned)ceil_div((int64_t)p.tokens * p.q_heads, 4)), p, stream);
+    return launch_after(paged_combine_kernel<T>, dim3((unsigned)((int64_t)p.tokens * p.q_heads)), p, stream);
 }
 
 template <typename T, int DP> inline int launch_mma_rows(const AttendParams &p, int wm, int64_t blocks, cudaStream_t stream) {

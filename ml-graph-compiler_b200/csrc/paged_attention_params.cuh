@@ -17,6 +17,8 @@ struct CutUnit {
     int h, b, t, pieces;
 };
 
+constexpr int MAX_HEAD_DIM = 256;
+
 struct AttendParams {
     Batch batch;
     const void *k_pages, *v_pages;
@@ -37,8 +39,6 @@ struct AttendParams {
     // the tcgen05 kernel: part and part_ml are [CTA][2][256] rows of pieces, and
     CutUnit *cut;       // [CTA]
 };
-
-constexpr int MAX_HEAD_DIM = 256;
 
 // Visible positions [lo, hi) of a token at position pos of a sequence of n positions.
 __device__ __forceinline__ void visible(const AttendParams &p, int n, int pos, int &lo, int &hi) {

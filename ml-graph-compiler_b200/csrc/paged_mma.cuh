@@ -573,43 +573,60 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
     }
 }
 
-// out[t][h] from the splits' partial sums: one warp per row of (token, head).
+// out[t][h] from the splits' partial sums: one block per row of (token, head), its warps taking every
+// fourth split. The splits' factors first (their loads together), then the rows: a loop that loaded
+// each split's maximum before its row took 15 us for 37 splits.
+constexpr int MAX_SPLITS = 128;
+
 template <typename T>
 __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constant__ AttendParams p) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int lane = (int)(threadIdx.x & 31);
-    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5), all = (long long)p.tokens * p.q_heads;
-    if (row >= all) return;
+    __shared__ float factor[MAX_SPLITS];
+    __shared__ float4 sum[4][MAX_HEAD_DIM / 4];
+    const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const long long row = blockIdx.x, all = (long long)p.tokens * p.q_heads;
     // rows past the last sequence have no partial sums
     const int t = (int)(row / p.q_heads);
     if (t >= __ldg(p.batch.q_starts + p.batch.batch) || t < __ldg(p.batch.q_starts)) return;
-    float m = -INFINITY, l = 0.0f;
-    for (int s = lane; s < p.splits; s += 32) m = fmaxf(m, p.part_ml[s * all + row].x);
+    const float2 ml = tid < p.splits ? p.part_ml[tid * all + row] : make_float2(-INFINITY, 0.0f);
+    __shared__ float warp_max[4], warp_sum[4];
+    float m = ml.x;
 #pragma unroll
     for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));
-    T *out = static_cast<T *>(p.out) + (long long)t * p.o_ts + (row % p.q_heads) * p.o_hs;
+    if (lane == 0) warp_max[warp] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(warp_max[0], warp_max[1]), fmaxf(warp_max[2], warp_max[3]));
+    const float f = ml.y > 0.0f ? ex2(ml.x - m) : 0.0f;
+    factor[tid] = f;
+    float l = f * ml.y;
+#pragma unroll
+    for (int x = 16; x; x >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, x);
+    if (lane == 0) warp_sum[warp] = l;
+    __syncthreads();
+    l = (warp_sum[0] + warp_sum[1]) + (warp_sum[2] + warp_sum[3]);
     for (int c = lane * 4; c < p.head_dim; c += 128) {
         float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        l = 0.0f;
-        for (int s = 0; s < p.splits; ++s) {
-            const float2 ml = p.part_ml[s * all + row];
-            if (ml.y == 0.0f) continue;
-            const float f = ex2(ml.x - m);
+#pragma unroll 8
+        for (int s = warp; s < p.splits; s += 4) {
             const float4 x = *reinterpret_cast<const float4 *>(p.part + (s * all + row) * p.head_dim + c);
-            l += f * ml.y;
-            a.x += f * x.x;
-            a.y += f * x.y;
-            a.z += f * x.z;
-            a.w += f * x.w;
+            const float g = factor[s];
+            a.x += g * x.x;
+            a.y += g * x.y;
+            a.z += g * x.z;
+            a.w += g * x.w;
         }
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-        Pack<4, T> v;
-        v.e[0] = from_f<T>(a.x * inv);
-        v.e[1] = from_f<T>(a.y * inv);
-        v.e[2] = from_f<T>(a.z * inv);
-        v.e[3] = from_f<T>(a.w * inv);
-        v.store(out + c);
+        sum[warp][c / 4] = a;
     }
+    __syncthreads();
+    if (tid * 4 >= p.head_dim) return;
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const float4 a = sum[0][tid], b = sum[1][tid], c = sum[2][tid], d = sum[3][tid];
+    Pack<4, T> v;
+    v.e[0] = from_f<T>(((a.x + b.x) + (c.x + d.x)) * inv);
+    v.e[1] = from_f<T>(((a.y + b.y) + (c.y + d.y)) * inv);
+    v.e[2] = from_f<T>(((a.z + b.z) + (c.z + d.z)) * inv);
+    v.e[3] = from_f<T>(((a.w + b.w) + (c.w + d.w)) * inv);
+    v.store(static_cast<T *>(p.out) + (long long)t * p.o_ts + (row % p.q_heads) * p.o_hs + tid * 4);
 }
 
 }  // namespace paged

@@ -559,11 +559,14 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                     phase ^= 1u;
                     if (!ok) break;
                     const int r0 = max(w.first - key0, 0), r1 = min(w.hi - key0, 128);
-                    for (int i = lane; i < 128 * C::HALVES * 8; i += 32) {
-                        const int r = (i >> 3) & 127;
-                        if (r < r0 || r >= r1)
-                            *reinterpret_cast<uint4 *>(ring + vs * C::TILE + (i >> 10) * C::HALF + r * 128 + (i & 7) * 16) =
-                                make_uint4(0, 0, 0, 0);
+                    const int out = r0 + 128 - r1;  // rows outside
+#pragma unroll 1
+                    for (int i = lane; i < out * C::HALVES * 8; i += 32) {
+                        int r = i / (C::HALVES * 8);
+                        const int c = i % (C::HALVES * 8);
+                        if (r >= r0) r += r1 - r0;
+                        *reinterpret_cast<uint4 *>(ring + vs * C::TILE + (c >> 3) * C::HALF + r * 128 + (c & 7) * 16) =
+                            make_uint4(0, 0, 0, 0);
                     }
                     umma::fence_proxy_async_smem();
                     __syncwarp();
