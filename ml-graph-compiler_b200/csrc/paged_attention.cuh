@@ -4,9 +4,6 @@
 
 #include "paged_umma.cuh"
 
-#ifndef MGC_WAVES
-#define MGC_WAVES 3
-#endif
 namespace mgc {
 namespace paged {
 
@@ -84,17 +81,27 @@ inline int check_attend(const mgc_cuda_paged_attention_args &a, const char *what
     return MGC_CUDA_OK;
 }
 
-// How a call runs: which kernel, its row tile and how its keys are split.
+// How a call runs: which kernel, its row tile and how its keys are shared out.
 struct Plan {
-    bool mma = false, umma = false;
+    bool mma = false, umma = false, even = false;
     int wm = 1;         // 16-row warps of a row tile
     int row_tiles = 1, splits = 1;
-    int ctas = 0;       // of the tcgen05 kernel
-    bool clustered = false;
+    int unit_rows = 0, ctas = 0;  // even shares: rows of a unit, CTAs
+    bool interleaved = false;
     int64_t workspace = 0;
 };
 
 constexpr int MIN_SPLIT_KEYS = 128;  // below this a split's start and merge outweigh its loads
+
+// CTAs of the tiled kernel that an SM holds (of 128 threads, by shared memory; 2 at 256 registers).
+inline int ctas_per_sm(int64_t dtype, int64_t head_dim, int wm) {
+    const int dp = head_dim <= 32 ? 32 : head_dim <= 64 ? 64 : head_dim <= 96 ? 96 : head_dim <= 128 ? 128 : 256;
+    const bool f32 = dtype == MGC_F32;
+    const int row = dp * (f32 ? 4 : 2) + 16, ring = (dp > 128 ? 2 : 3) * 2 * (f32 ? 32 : 64) * row;
+    const int bytes = ring + (!f32 && dp <= 128 ? 0 : 16 * wm * row) + 3 * 64 * 8 + 1024;
+    const int fit = 232448 / bytes;
+    return fit < 1 ? 1 : fit > 4 ? 4 : fit;
+}
 
 inline Plan plan_of(const mgc_cuda_paged_attention_args &a) {
     const mgc_cuda_paged &c = a.paged;
@@ -111,28 +118,36 @@ inline Plan plan_of(const mgc_cuda_paged_attention_args &a) {
     const int64_t group = a.q_heads / c.kv_heads;
     int64_t max_q = a.max_q < 1 ? 1 : a.max_q > c.tokens ? c.tokens : a.max_q;
     const int64_t rows = max_q * group;
+    auto even_shares = [&](int unit_rows, int ctas) {
+        s.even = true;
+        s.unit_rows = unit_rows;
+        s.ctas = ctas;
+        if (!s.umma && ctas >= c.kv_heads && ctas / c.kv_heads * c.kv_heads * 20 >= ctas * 19) {
+            s.interleaved = true;
+            s.ctas = (int)(ctas / c.kv_heads * c.kv_heads);
+        }
+        s.workspace = (int64_t)s.ctas * (2 * unit_rows * (c.head_dim * 4 + 8) + (int64_t)sizeof(CutUnit));
+    };
     if (rows > 64 && umma_fits(c) && c.batch * ceil_div(rows, 256) < 0x7FFFFFFF) {
         s.umma = true;
-        s.ctas = sm_count();
-        s.workspace = (int64_t)s.ctas * (2 * 256 * (c.head_dim * 4 + 8) + sizeof(CutUnit));
+        even_shares(256, sm_count());
         return s;
     }
     s.wm = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
     s.row_tiles = (int)ceil_div(rows, 16 * s.wm);
     const int64_t units = c.batch * c.kv_heads * s.row_tiles;
-    // enough parts for two blocks per SM; three times that for batches, whose sequences differ
-    const int64_t target = 2ll * sm_count() * (c.batch > 1 ? MGC_WAVES : 1);
     int64_t most = a.max_kv;
     if (a.window > 0 && a.window + max_q < most) most = a.window + max_q;
-    int64_t splits = units >= target ? 1 : ceil_div(target, units);
+    // CTAs that fit the GPU at once: shared memory and registers allow this many per SM
+    const int64_t slots = (int64_t)sm_count() * ctas_per_sm(c.dtype, c.head_dim, s.wm);
+    int64_t splits = slots / units;
     if (splits > most / MIN_SPLIT_KEYS) splits = most / MIN_SPLIT_KEYS;
-    if (splits > MAX_SPLITS) splits = MAX_SPLITS;
     if (splits < 1) splits = 1;
-    if (splits > MAX_CLUSTER && c.batch > 1) splits = MAX_CLUSTER;
+    if (splits > MAX_CLUSTER || (units * 2 > slots && c.batch > 1)) {
+        even_shares(16 * s.wm, (int)slots);
+        return s;
+    }
     s.splits = (int)splits;
-    s.clustered = splits > 1 && splits <= MAX_CLUSTER;
-    if (splits > 1 && !s.clustered)
-        s.workspace = splits * c.tokens * a.q_heads * (c.head_dim * 4 + 8);
     return s;
 }
 
@@ -142,7 +157,7 @@ inline int64_t attend_workspace(const mgc_cuda_paged_attention_args &a) {
 }
 
 // A combine kernel's blocks may be set up while the kernel before finishes; they wait for it themselves.
-template <typename K> inline int launch_after(K kernel, dim3 grid, const AttendParams &p, cudaStream_t stream) {
+template <typename K> inline int launch_after(K kernel, dim3 grid, const AttendParams &p, int next, cudaStream_t stream) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(128);
@@ -152,7 +167,7 @@ template <typename K> inline int launch_after(K kernel, dim3 grid, const AttendP
     dep[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = dep;
     cfg.numAttrs = 1;
-    MGC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+    MGC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, p, next));
     return MGC_CUDA_OK;
 }
 
@@ -167,42 +182,49 @@ template <typename T> inline int launch_umma(const AttendParams &p, const mgc_cu
     };
     MGC_CHECK(p.head_dim <= 64 ? go(paged_attention_umma_kernel<T, 64>, UmmaConfig<64>::SMEM, UmmaConfig<64>::THREADS)
                                : go(paged_attention_umma_kernel<T, 128>, UmmaConfig<128>::SMEM, UmmaConfig<128>::THREADS));
-    return launch_after(paged_combine_units_kernel<T>, dim3((unsigned)ctas, 32), p, stream);
+    return launch_after(paged_combine_units_kernel<T, 256>, dim3((unsigned)ctas, 32), p, 1, stream);
 }
 
-template <typename T, int DP, int WM, int WN> inline int launch_mma(const AttendParams &p, int64_t blocks, cudaStream_t stream) {
+template <typename T, int DP, int WM, int WN> inline int launch_mma(const AttendParams &p, const Plan &s, cudaStream_t stream) {
     using C = MmaConfig<T, DP, WM, WN>;
-    auto kernel = paged_attention_mma_kernel<T, DP, WM, WN>;
-    MGC_CHECK(raise_smem_ceiling((const void *)kernel));
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)blocks, (unsigned)p.splits);
     cfg.blockDim = dim3(C::THREADS);
     cfg.dynamicSmemBytes = C::SMEM;
     cfg.stream = stream;
+    if (s.even) {
+        auto kernel = paged_attention_mma_kernel<T, DP, WM, WN, true>;
+        MGC_CHECK(raise_smem_ceiling((const void *)kernel));
+        cfg.gridDim = dim3((unsigned)s.ctas);
+        MGC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+        return launch_after(paged_combine_units_kernel<T, C::R>, dim3((unsigned)s.ctas, C::R / 16), p, s.interleaved ? p.kv_heads : 1,
+                            stream);
+    }
+    auto kernel = paged_attention_mma_kernel<T, DP, WM, WN, false>;
+    MGC_CHECK(raise_smem_ceiling((const void *)kernel));
+    cfg.gridDim = dim3((unsigned)(p.batch.batch * p.kv_heads * p.row_tiles), (unsigned)p.splits);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = attr[0].val.clusterDim.z = 1;
     attr[0].val.clusterDim.y = (unsigned)p.splits;
     cfg.attrs = attr;
-    cfg.numAttrs = p.clustered ? 1 : 0;
+    cfg.numAttrs = p.splits > 1 ? 1 : 0;
     MGC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
-    if (p.splits == 1 || p.clustered) return MGC_CUDA_OK;
-    return launch_after(paged_combine_kernel<T>, dim3((unsigned)((int64_t)p.tokens * p.q_heads)), p, stream);
+    return MGC_CUDA_OK;
 }
 
-template <typename T, int DP> inline int launch_mma_rows(const AttendParams &p, int wm, int64_t blocks, cudaStream_t stream) {
-    if (wm == 1) return launch_mma<T, DP, 1, 4>(p, blocks, stream);
-    if (wm == 2) return launch_mma<T, DP, 2, 2>(p, blocks, stream);
-    return launch_mma<T, DP, 4, 1>(p, blocks, stream);
+template <typename T, int DP> inline int launch_mma_rows(const AttendParams &p, const Plan &s, cudaStream_t stream) {
+    if (s.wm == 1) return launch_mma<T, DP, 1, 4>(p, s, stream);
+    if (s.wm == 2) return launch_mma<T, DP, 2, 2>(p, s, stream);
+    return launch_mma<T, DP, 4, 1>(p, s, stream);
 }
 
 // Head widths are padded to the next of these (zero channels).
-template <typename T> inline int launch_mma_width(const AttendParams &p, int wm, int64_t blocks, cudaStream_t stream) {
-    if (p.head_dim <= 32) return launch_mma_rows<T, 32>(p, wm, blocks, stream);
-    if (p.head_dim <= 64) return launch_mma_rows<T, 64>(p, wm, blocks, stream);
-    if (p.head_dim <= 96) return launch_mma_rows<T, 96>(p, wm, blocks, stream);
-    if (p.head_dim <= 128) return launch_mma_rows<T, 128>(p, wm, blocks, stream);
-    return launch_mma_rows<T, 256>(p, wm, blocks, stream);
+template <typename T> inline int launch_mma_width(const AttendParams &p, const Plan &s, cudaStream_t stream) {
+    if (p.head_dim <= 32) return launch_mma_rows<T, 32>(p, s, stream);
+    if (p.head_dim <= 64) return launch_mma_rows<T, 64>(p, s, stream);
+    if (p.head_dim <= 96) return launch_mma_rows<T, 96>(p, s, stream);
+    if (p.head_dim <= 128) return launch_mma_rows<T, 128>(p, s, stream);
+    return launch_mma_rows<T, 256>(p, s, stream);
 }
 
 inline int attend(const mgc_cuda_paged_attention_args &a, cudaStream_t stream) {
@@ -223,25 +245,25 @@ inline int attend(const mgc_cuda_paged_attention_args &a, cudaStream_t stream) {
     p.scale_log2 = (float)(a.scale * 1.4426950408889634074);
     p.max_positions = (int)(c.table_pages * c.page_size);
     const Plan s = plan_of(a);
-    p.row_tiles = s.row_tiles; p.splits = s.splits; p.clustered = s.clustered;
+    p.row_tiles = s.row_tiles; p.splits = s.splits; p.interleaved = s.interleaved;
     p.part = nullptr; p.part_ml = nullptr; p.cut = nullptr;
     if (s.workspace) {
         if (!a.workspace || a.workspace_bytes < s.workspace || !aligned(a.workspace, 16))
             return fail(MGC_CUDA_NEEDS_WORKSPACE, "%s: needs %lld bytes of workspace (16-byte aligned), got %lld", what,
                         (long long)s.workspace, (long long)(a.workspace ? a.workspace_bytes : 0));
         p.part = static_cast<float *>(a.workspace);
-        const int64_t rows = s.umma ? (int64_t)s.ctas * 2 * 256 : (int64_t)s.splits * p.tokens * p.q_heads;
+        const int64_t rows = (int64_t)s.ctas * 2 * s.unit_rows;
         p.part_ml = reinterpret_cast<float2 *>(p.part + rows * p.head_dim);
         p.cut = reinterpret_cast<CutUnit *>(p.part_ml + rows);
     }
     if (s.mma) {
-        const int64_t blocks = c.batch * c.kv_heads * s.row_tiles;
-        if (blocks > 0x7FFFFFFF) return fail(MGC_CUDA_UNSUPPORTED, "%s: %lld blocks", what, (long long)blocks);
+        const int64_t units = c.batch * c.kv_heads * s.row_tiles;
+        if (units > 0x7FFFFFFF) return fail(MGC_CUDA_UNSUPPORTED, "%s: %lld row tiles", what, (long long)units);
         if (s.umma)
             return c.dtype == MGC_F16 ? launch_umma<__half>(p, c, s.ctas, stream) : launch_umma<__nv_bfloat16>(p, c, s.ctas, stream);
-        if (c.dtype == MGC_F32) return launch_mma_width<float>(p, s.wm, blocks, stream);
-        if (c.dtype == MGC_F16) return launch_mma_width<__half>(p, s.wm, blocks, stream);
-        return launch_mma_width<__nv_bfloat16>(p, s.wm, blocks, stream);
+        if (c.dtype == MGC_F32) return launch_mma_width<float>(p, s, stream);
+        if (c.dtype == MGC_F16) return launch_mma_width<__half>(p, s, stream);
+        return launch_mma_width<__nv_bfloat16>(p, s, stream);
     }
     const dim3 grid((unsigned)p.tokens, (unsigned)ceil_div(p.q_heads, 4));
     if (c.dtype == MGC_F32) paged_attention_row_kernel<float><<<grid, 128, 0, stream>>>(p);

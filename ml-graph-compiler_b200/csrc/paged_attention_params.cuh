@@ -30,13 +30,13 @@ struct AttendParams {
     int causal, window;
     float scale_log2;  // scale * log2 e
     int max_positions;  // positions a row of the block table can hold
-    // kernels that tile rows and split keys
-    int row_tiles;      // row tiles per (sequence, key head) in the grid
-    int splits;         // parts of a tile's keys
-    int clustered;      // the parts are one cluster; else their partial results go to part, part_ml
-    float *part;        // [splits][tokens][q_heads][head_dim], relative to the part's maximum
-    float2 *part_ml;    // [splits][tokens][q_heads]: maximum, sum
-    // the tcgen05 kernel: part and part_ml are [CTA][2][256] rows of pieces, and
+    // clusters: row tiles per (sequence, key head) in the grid, CTAs that share a tile's keys
+    int row_tiles, splits;
+    // even shares: a stretch of every key head's units side by side (CTA c: key head c % kv_heads), or
+    // the stretches key head by key head; partial results of the pieces
+    int interleaved;
+    float *part;        // [CTA][2][rows of a unit][head_dim], relative to the row's maximum
+    float2 *part_ml;    // [CTA][2][rows of a unit]: maximum (scaled, base 2), sum
     CutUnit *cut;       // [CTA]
 };
 

@@ -2,8 +2,8 @@
 // tiles of rows of any head width and page size.
 //
 // A CTA takes one (sequence, key head), a tile of R = 16 WM query rows (row = token * group + head
-// of the group, so the heads that share a key head share its K and V loads) and one of the splits
-// of the tile's visible keys. WM x WN warps: warp (wm, wn) owns rows 16 wm .. 16 wm + 15 and the
+// of the group, so the heads that share a key head share its K and V loads) and a part of the
+// tile's visible keys. WM x WN warps: warp (wm, wn) owns rows 16 wm .. 16 wm + 15 and the
 // wn-th slice of every stage's BN keys, with its own running maximum, sum and output, so warps
 // meet only at the end. K and V rows arrive by cp.async (16 bytes per thread, zero fill for keys
 // that no row sees, so nothing there can reach a sum) into a ring of STAGES stages; rows are padded
@@ -16,12 +16,14 @@
 // fresh fp32 accumulator per tile that is added to the running one in fp32: the instruction
 // truncates its sums, and a chain over the whole context would shrink the output by ~1e-8 per step.
 //
-// Splits: up to 8 CTAs of a cluster take equal parts of the visible keys and add their partial
-// results through distributed shared memory; more splits go through a workspace and
-// paged_combine_kernel. Partial sums are added in a fixed order, so a call repeats its bits.
+// When there are fewer units (row tiles of a sequence and key head) than the SMs hold CTAs, up to 8
+// CTAs of a cluster take equal parts of a unit's keys and add their partial results through
+// distributed shared memory. Else, or when 8 are not enough, every CTA takes an even share of all
+// units' keys and pieces go through a workspace (paged_work.cuh). Partial sums are added in a fixed
+// order, so a call repeats its bits.
 #pragma once
 
-#include "paged_attention_params.cuh"
+#include "paged_work.cuh"
 
 namespace mgc {
 namespace paged {
@@ -59,11 +61,6 @@ __device__ __forceinline__ void mma8(float (&c)[4], const uint32_t (&a)[4], uint
     asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 // x = hi + lo, hi the nearest TF32 value; the instruction reads the upper 19 bits of lo.
 __device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo) {
@@ -120,17 +117,9 @@ template <typename T, int DP, int WM, int WN> struct MmaConfig {
     static constexpr int SMEM = Q_BYTES + (RING > RED ? RING : RED) + STAGES * BN * 8;
 };
 
-// Position of row (token i of nq, sequence of n positions) -> its visible keys; rows past the last
-// see nothing.
-struct RowRange { int lo, hi; };
-__device__ __forceinline__ RowRange row_range(const AttendParams &p, int n, int nq, int row) {
-    RowRange r{0, 0};
-    const int i = row / p.group;
-    if (i < nq) visible(p, n, n - nq + i, r.lo, r.hi);
-    return r;
-}
-
-template <typename T, int DP, int WM, int WN>
+// EVEN: the CTA takes an even share of all units' keys (paged_work.cuh); else one row tile's keys, or
+// the part of them that its rank in a cluster names.
+template <typename T, int DP, int WM, int WN, bool EVEN>
 __global__ void __launch_bounds__(MmaConfig<T, DP, WM, WN>::THREADS)
 paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
     using C = MmaConfig<T, DP, WM, WN>;
@@ -143,40 +132,17 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
     const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int wm = warp % WM, wn = warp / WM;
     const int g4 = lane >> 2, t4 = lane & 3;
-    // block -> (sequence, key head, row tile, split); the key heads of a token row, which lie side
-    // by side in memory, run side by side
-    unsigned u = blockIdx.x;
-    const int split = (int)blockIdx.y;
-    const int kh = (int)(u % (unsigned)p.kv_heads);
-    u /= (unsigned)p.kv_heads;
-    const int tile0 = p.row_tiles - 1 - (int)(u % (unsigned)p.row_tiles);  // longest rows first
-    const int b = (int)(u / (unsigned)p.row_tiles);
-    const int start = __ldg(p.batch.q_starts + b), nq = __ldg(p.batch.q_starts + b + 1) - start;
-    const int n = min(__ldg(p.batch.kv_lens + b), p.max_positions);
-    if (n != __ldg(p.batch.kv_lens + b) && tid == 0 && p.batch.status) *p.batch.status = MGC_CUDA_GATHER_OOB;
-    const int rows = nq * p.group;
-    const T *kp = static_cast<const T *>(p.k_pages) + kh * p.head_stride;
-    const T *vp = static_cast<const T *>(p.v_pages) + kh * p.head_stride;
     const int chunks = p.head_dim / C::CH;
 
-    // channels past the head width: zero in every stage, never loaded over
-    if (chunks < CPR) {
-        const int pad = CPR - chunks;
-        for (int x = tid; x < C::STAGES * 2 * BN * pad; x += C::THREADS) {
-            const int r = x / pad, c = chunks + x % pad;
-            *reinterpret_cast<uint4 *>(ring + (size_t)r * ROW + c * 16) = make_uint4(0, 0, 0, 0);
-        }
-    }
-
-    for (int tile = tile0; tile * R < rows; tile += p.row_tiles) {
-        const int row0 = tile * R;
-        // keys that some row of the tile sees, this split's part of them, and the keys that all see
+    const int split = EVEN ? 0 : (int)blockIdx.y;
+    // one piece: rows row0 .. of (sequence b, key head kh) over keys [k_lo, k_hi)
+    auto piece = [&](int b, int kh, int start, int nq, int n, int row0, int k_lo, int k_hi, int slot) {
+        const int rows = nq * p.group, tiles = k_hi > k_lo ? (k_hi - k_lo + BN - 1) / BN : 0;
+        const T *kp = static_cast<const T *>(p.k_pages) + kh * p.head_stride;
+        const T *vp = static_cast<const T *>(p.v_pages) + kh * p.head_stride;
+        // keys below first.lo no row sees; all rows see [all_lo, all_hi)
         const RowRange first = row_range(p, n, nq, row0), last = row_range(p, n, nq, min(row0 + R, rows) - 1);
-        int lo = first.lo & ~15, hi = max(last.hi, 0);
         const int all_lo = last.lo, all_hi = first.hi;
-        const int per = (max(hi - lo, 0) + p.splits * 16 - 1) / (p.splits * 16) * 16;
-        const int k_lo = lo + split * per, k_hi = min(hi, k_lo + per);
-        const int tiles = k_hi > k_lo ? (k_hi - k_lo + BN - 1) / BN : 0;
 
         // byte offset (of K and V alike) of key j of this thread's stage row, or -1: not loaded
         auto offset_of = [&](int j) -> long long {
@@ -493,22 +459,18 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
             v.e[3] = from_f<T>(a.w * inv);
             v.store(out);
         };
-        if (p.splits == 1) {
+        if (EVEN || p.splits == 1) {
             for (int x = tid; x < live * quads; x += C::THREADS) {
                 const int r = x / quads, c = x - r * quads;
                 float m, l;
                 const float4 a = warps_sum(r, c, m, l);
-                put(r, c, a, l);
-            }
-        } else if (!p.clustered) {
-            for (int x = tid; x < live * quads; x += C::THREADS) {
-                const int r = x / quads, c = x - r * quads;
-                const int row = row0 + r, i = row / p.group, h = kh * p.group + row % p.group;
-                float m, l;
-                const float4 a = warps_sum(r, c, m, l);
-                const long long at = ((long long)split * p.tokens + start + i) * p.q_heads + h;
-                *reinterpret_cast<float4 *>(p.part + at * p.head_dim + c * 4) = a;
-                if (c == 0) p.part_ml[at] = make_float2(m, l);
+                if (!EVEN || slot < 0) {
+                    put(r, c, a, l);
+                } else {
+                    const long long at = ((long long)blockIdx.x * 2 + slot) * R + r;
+                    *reinterpret_cast<float4 *>(p.part + at * p.head_dim + c * 4) = a;
+                    if (c == 0) p.part_ml[at] = make_float2(m, l);
+                }
             }
         } else {
             // this CTA's sum over its first warp slice's rows (each quad read and written by one thread)
@@ -561,72 +523,57 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
             cluster_barrier();  // every partial read before the next tile or the exit reuses it
         }
         __syncthreads();
-        // the reduction wrote over the padding channels
-        if (chunks < CPR && (tile + p.row_tiles) * R < rows) {
-            const int pad = CPR - chunks;
-            for (int x = tid; x < C::STAGES * 2 * BN * pad; x += C::THREADS) {
-                const int r = x / pad, c = chunks + x % pad;
-                *reinterpret_cast<uint4 *>(ring + (size_t)r * ROW + c * 16) = make_uint4(0, 0, 0, 0);
-            }
-            __syncthreads();
+    };
+    // channels past the head width: zero in every stage, never loaded over; the reduction at a piece's
+    // end does write over them
+    auto zero_padding = [&]() {
+        if (chunks == CPR) return;
+        const int pad = CPR - chunks;
+        for (int x = tid; x < C::STAGES * 2 * BN * pad; x += C::THREADS) {
+            const int r = x / pad, c = chunks + x % pad;
+            *reinterpret_cast<uint4 *>(ring + (size_t)r * ROW + c * 16) = make_uint4(0, 0, 0, 0);
+        }
+    };
+
+    if constexpr (EVEN) {
+        __shared__ Walk stretch;
+        const int heads = p.interleaved ? p.kv_heads : 1, h0 = (int)blockIdx.x % heads;
+        if (warp == 0) {
+            const Walk k = find_stretch<R, BN>(p, (int)blockIdx.x / heads, (int)gridDim.x / heads, h0,
+                                               p.interleaved ? h0 + 1 : p.kv_heads, lane);
+            if (lane == 0) stretch = k;
+        }
+        __syncthreads();
+        Walk walk = stretch;
+        Item w;
+        CutUnit cut{0, 0, 0, 0};
+        while (next_item<R, BN>(p, walk, w)) {
+            zero_padding();
+            if (w.slot == 1) cut = cut_of<R, BN>(p, walk, w);
+            piece(w.b, w.h, w.start, w.nq, w.n, w.row0, w.lo, w.hi, w.slot);
+        }
+        if (tid == 0) p.cut[blockIdx.x] = cut;
+    } else {
+        // block -> (sequence, key head, row tile, split); the key heads of a token row, which lie side
+        // by side in memory, run side by side
+        unsigned u = blockIdx.x;
+        const int kh = (int)(u % (unsigned)p.kv_heads);
+        u /= (unsigned)p.kv_heads;
+        const int tile0 = p.row_tiles - 1 - (int)(u % (unsigned)p.row_tiles);  // longest rows first
+        const int b = (int)(u / (unsigned)p.row_tiles);
+        int start, nq, n;
+        load_sequence(p, b, start, nq, n);
+        if (tid == 0 && nq > 0 && n != __ldg(p.batch.kv_lens + b) && p.batch.status) *p.batch.status = MGC_CUDA_GATHER_OOB;
+        for (int tile = tile0; tile * R < nq * p.group; tile += p.row_tiles) {
+            const RowRange z = row_range(p, n, nq, min(tile * R + R, nq * p.group) - 1);
+            const int lo = row_range(p, n, nq, tile * R).lo & ~15, hi = max(z.hi, 0);
+            // this split's part of the keys that some row of the tile sees
+            const int per = (max(hi - lo, 0) + p.splits * 16 - 1) / (p.splits * 16) * 16;
+            const int k_lo = lo + split * per;
+            zero_padding();
+            piece(b, kh, start, nq, n, tile * R, k_lo, min(hi, k_lo + per), -1);
         }
     }
-}
-
-// out[t][h] from the splits' partial sums: one block per row of (token, head), its warps taking every
-// fourth split. The splits' factors first (their loads together), then the rows: a loop that loaded
-// each split's maximum before its row took 15 us for 37 splits.
-constexpr int MAX_SPLITS = 128;
-
-template <typename T>
-__global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constant__ AttendParams p) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    __shared__ float factor[MAX_SPLITS];
-    __shared__ float4 sum[4][MAX_HEAD_DIM / 4];
-    const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const long long row = blockIdx.x, all = (long long)p.tokens * p.q_heads;
-    // rows past the last sequence have no partial sums
-    const int t = (int)(row / p.q_heads);
-    if (t >= __ldg(p.batch.q_starts + p.batch.batch) || t < __ldg(p.batch.q_starts)) return;
-    const float2 ml = tid < p.splits ? p.part_ml[tid * all + row] : make_float2(-INFINITY, 0.0f);
-    __shared__ float warp_max[4], warp_sum[4];
-    float m = ml.x;
-#pragma unroll
-    for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));
-    if (lane == 0) warp_max[warp] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(warp_max[0], warp_max[1]), fmaxf(warp_max[2], warp_max[3]));
-    const float f = ml.y > 0.0f ? ex2(ml.x - m) : 0.0f;
-    factor[tid] = f;
-    float l = f * ml.y;
-#pragma unroll
-    for (int x = 16; x; x >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, x);
-    if (lane == 0) warp_sum[warp] = l;
-    __syncthreads();
-    l = (warp_sum[0] + warp_sum[1]) + (warp_sum[2] + warp_sum[3]);
-    for (int c = lane * 4; c < p.head_dim; c += 128) {
-        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-        for (int s = warp; s < p.splits; s += 4) {
-            const float4 x = *reinterpret_cast<const float4 *>(p.part + (s * all + row) * p.head_dim + c);
-            const float g = factor[s];
-            a.x += g * x.x;
-            a.y += g * x.y;
-            a.z += g * x.z;
-            a.w += g * x.w;
-        }
-        sum[warp][c / 4] = a;
-    }
-    __syncthreads();
-    if (tid * 4 >= p.head_dim) return;
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    const float4 a = sum[0][tid], b = sum[1][tid], c = sum[2][tid], d = sum[3][tid];
-    Pack<4, T> v;
-    v.e[0] = from_f<T>(((a.x + b.x) + (c.x + d.x)) * inv);
-    v.e[1] = from_f<T>(((a.y + b.y) + (c.y + d.y)) * inv);
-    v.e[2] = from_f<T>(((a.z + b.z) + (c.z + d.z)) * inv);
-    v.e[3] = from_f<T>(((a.w + b.w) + (c.w + d.w)) * inv);
-    v.store(static_cast<T *>(p.out) + (long long)t * p.o_ts + (row % p.q_heads) * p.o_hs + tid * 4);
 }
 
 }  // namespace paged

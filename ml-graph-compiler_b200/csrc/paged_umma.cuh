@@ -204,168 +204,11 @@ inline bool umma_fits(const mgc_cuda_paged &c) {
            c.page_stride < most;
 }
 
-// ---- work: 256-row units in a fixed order, cut evenly over the CTAs ---------------------------------
-// A unit is (key head, sequence, 256 query rows) and is as long as it has key tiles (at least 1). All
-// units lie end to end, key head by key head; CTA c takes the c-th of gridDim.x equal stretches. A
-// stretch that ends inside a unit cuts it (unless a piece would be below MIN_PIECE tiles): each piece
-// leaves its rows' partial results, and paged_combine_units_kernel adds them in order. 256 equal
-// units on 148 SMs would otherwise take two rounds, the second 73% full.
-constexpr int MIN_PIECE = 2;
-
-struct Item {
-    int rows, row0;     // query rows of the sequence; first of the unit's
-    int start;          // the sequence's first token
-    int n, nq;          // its positions, its new tokens
-    int b, h;
-    int lo, hi, tiles;  // keys [lo, hi) of this piece in `tiles` tiles of 128
-    int first;          // first key that any row of the unit sees
-    int need0, need1;   // tiles that row tile 0 / 1 needs (rows of the first stop earlier if causal)
-    int slot;           // where partial results go: -1 (the whole unit), 0 (a later piece), 1 (the first)
-    __device__ __forceinline__ int need(int x) const { return x ? need1 : need0; }
-};
-
-struct Walk {
-    int h, b, t;  // unit
-    int skip;     // its tiles before this CTA's stretch
-    int left;     // tiles left of the stretch
-    int share;    // tiles of a whole stretch
-    int start, nq, n;  // sequence b: first token, new tokens, positions
-};
-
-__device__ __forceinline__ void load_sequence(const AttendParams &p, int b, int &start, int &nq, int &n) {
-    start = __ldg(p.batch.q_starts + b);
-    nq = __ldg(p.batch.q_starts + b + 1) - start;
-    n = min(__ldg(p.batch.kv_lens + b), p.max_positions);
-}
-
-// Keys [lo, hi) that rows [256 t, 256 t + 256) see, lo rounded down to a tile; the unit's length.
-__device__ __forceinline__ int unit_length(const AttendParams &p, int n, int nq, int t, int &first, int &lo, int &hi) {
-    const int rows = nq * p.group, row0 = t * 256;
-    const RowRange a = row_range(p, n, nq, row0), z = row_range(p, n, nq, min(row0 + 256, rows) - 1);
-    first = a.lo;
-    lo = a.lo & ~127;
-    hi = max(z.hi, 0);
-    return hi > lo ? (hi - lo + 127) >> 7 : 1;
-}
-
-// The next piece of the stretch; false at its end. Advances the walk.
-__device__ __forceinline__ bool next_item(const AttendParams &p, Walk &k, Item &w) {
-    while (k.left > 0 && k.h < p.kv_heads) {
-        w.start = k.start;
-        w.nq = k.nq;
-        w.n = k.n;
-        w.rows = w.nq * p.group;
-        w.row0 = k.t * 256;
-        if (w.row0 >= w.rows) {  // past the sequence: the next one
-            k.t = 0;
-            if (++k.b == p.batch.batch) {
-                k.b = 0;
-                ++k.h;
-            }
-            load_sequence(p, k.b, k.start, k.nq, k.n);
-            continue;
-        }
-        int lo, hi;
-        const int length = unit_length(p, w.n, w.nq, k.t, w.first, lo, hi);
-        int take = length - k.skip;
-        if (take > k.left) {
-            const int at = k.skip + k.left;  // where the stretch ends in the unit
-            if (at < MIN_PIECE) break;
-            if (length - at >= MIN_PIECE) take = k.left;
-        }
-        w.b = k.b;
-        w.h = k.h;
-        w.lo = lo + k.skip * 128;
-        w.hi = min(hi, w.lo + take * 128);
-        w.tiles = w.hi > w.lo ? (w.hi - w.lo + 127) >> 7 : 0;
-        const RowRange mid = row_range(p, w.n, w.nq, min(w.row0 + 128, w.rows) - 1);
-        w.need0 = min(w.tiles, (max(mid.hi - w.lo, 0) + 127) >> 7);
-        w.need1 = w.rows - w.row0 > 128 ? w.tiles : 0;
-        w.slot = take == length ? -1 : k.skip > 0 ? 0 : 1;
-        k.left -= take;
-        if (k.skip + take == length) {
-            k.skip = 0;
-            ++k.t;
-        } else {
-            k.skip += take;
-        }
-        return true;
-    }
-    return false;
-}
-
-// Start of CTA c's stretch (one warp). Units are looked at 32 at a time; their lengths are the same
-// for every key head. Also leaves, for a unit cut at the stretch's end, what adding its pieces needs.
-__device__ __forceinline__ Walk find_stretch(const AttendParams &p, int c, int ctas, int lane) {
-    int most = 0;  // row tiles of the longest sequence
-    for (int b = lane; b < p.batch.batch; b += 32) {
-        int start, nq, n;
-        load_sequence(p, b, start, nq, n);
-        if (n != __ldg(p.batch.kv_lens + b) && nq > 0 && p.batch.status) *p.batch.status = MGC_CUDA_GATHER_OOB;
-        most = max(most, (nq * p.group + 255) >> 8);
-    }
-    most = __reduce_max_sync(0xFFFFFFFFu, most);
-    const unsigned count = (unsigned)p.batch.batch * (unsigned)most;
-    auto length_of = [&](unsigned i) {
-        if (i >= count) return 0;
-        int start, nq, n, first, lo, hi;
-        const unsigned b = i / (unsigned)most;
-        load_sequence(p, (int)b, start, nq, n);
-        const int t = (int)(i - b * (unsigned)most);
-        return t * 256 < nq * p.group ? unit_length(p, n, nq, t, first, lo, hi) : 0;
-    };
-    // the lanes' lengths summed up to and including each; the first 32 units' are kept
-    auto scan = [&](int v) {
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int u = __shfl_up_sync(0xFFFFFFFFu, v, d);
-            if (lane >= d) v += u;
-        }
-        return v;
-    };
-    const int mine0 = length_of(lane), upto0 = scan(mine0);
-    long long head = __shfl_sync(0xFFFFFFFFu, upto0, 31);  // tiles of one key head
-    for (unsigned i = 32; i < count; i += 32) head += __reduce_add_sync(0xFFFFFFFFu, length_of(i + lane));
-    Walk k{p.kv_heads, 0, 0, 0, 0, 0, 0, 0, 0};
-    const long long all = head * p.kv_heads;
-    long long share, x0;
-    if (all < 0x7FFFFFFF) {
-        share = ((unsigned)all + ctas - 1) / (unsigned)ctas;
-        share = max(share, (long long)MIN_PIECE);
-        x0 = c * share;
-        if (x0 >= all) return k;
-        k.h = (int)((unsigned)x0 / (unsigned)head);
-    } else {
-        share = (all + ctas - 1) / ctas;
-        x0 = c * share;
-        if (x0 >= all) return k;
-        k.h = (int)(x0 / head);
-    }
-    long long at = x0 - k.h * head;
-    for (unsigned i = 0; i < count; i += 32) {
-        const int mine = i ? length_of(i + lane) : mine0, upto = i ? scan(mine) : upto0;
-        const unsigned past = __ballot_sync(0xFFFFFFFFu, upto > at);
-        if (past) {
-            const int who = __ffs(past) - 1;
-            const int length = __shfl_sync(0xFFFFFFFFu, mine, who);
-            const int off = (int)at - (__shfl_sync(0xFFFFFFFFu, upto, who) - length);
-            k.b = (int)((i + who) / (unsigned)most);
-            k.t = (int)((i + who) % (unsigned)most);
-            load_sequence(p, k.b, k.start, k.nq, k.n);
-            k.left = k.share = (int)share;
-            if (off < MIN_PIECE) {
-                k.left += off;
-            } else if (length - off < MIN_PIECE) {
-                k.left -= length - off;
-                ++k.t;
-            } else {
-                k.skip = off;
-            }
-            break;
-        }
-        at -= __shfl_sync(0xFFFFFFFFu, upto, 31);
-    }
-    return k;
+// Key tiles that row tile x of a unit's piece needs (the rows of tile 0 stop earlier if causal).
+__device__ __forceinline__ int tiles_needed(const AttendParams &p, const Item &w, int x) {
+    if (x) return w.rows - w.row0 > 128 ? w.tiles : 0;
+    const RowRange mid = row_range(p, w.n, w.nq, min(w.row0 + 128, w.rows) - 1);
+    return min(w.tiles, (max(mid.hi - w.lo, 0) + 127) >> 7);
 }
 
 template <typename T, int DP>
@@ -401,7 +244,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
     }
     if (warp == 8) umma::tmem_alloc(&tslot, 512);
     if (warp == 11) {
-        const Walk k = find_stretch(p, (int)blockIdx.x, (int)gridDim.x, lane);
+        const Walk k = find_stretch<256, 128>(p, (int)blockIdx.x, (int)gridDim.x, 0, p.kv_heads, lane);
         if (lane == 0) stretch = k;
     }
     tc_fence_before();
@@ -426,7 +269,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
             const int boxes = (128 / maps.box_rows) * C::HALVES;  // of a tile: at most 32
             const int part = lane / C::HALVES, half = lane % C::HALVES;
             bool ok = true;
-            while (ok && next_item(p, walk, w)) {
+            while (ok && next_item<256, 128>(p, walk, w)) {
                 // this lane's box of key tile j: page and first row in it; -1 if no row sees its keys
                 auto box = [&](int j, int &row) {
                     const int at = w.lo + j * 128 + part * maps.box_rows;
@@ -489,15 +332,16 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                 }
                 commit_if(e, &s_full[x]);
             };
-            while (ok && next_item(p, walk, w)) {
+            while (ok && next_item<256, 128>(p, walk, w)) {
+                const int need0 = tiles_needed(p, w, 0), need1 = tiles_needed(p, w, 1);
                 ok = wait(&q_full[0], q_phase) && wait(&q_full[1], q_phase);
                 q_phase ^= 1u;
                 if (ok && w.tiles > 0) {
                     ok = wait(&full[slot], lap);
                     tc_fence_after();
                     if (ok) {
-                        if (w.need0 > 0) scores(0, slot);
-                        if (w.need1 > 0) scores(1, slot);
+                        if (need0 > 0) scores(0, slot);
+                        if (need1 > 0) scores(1, slot);
                         commit_if(e, &empty[slot]);
                     }
                     step();
@@ -523,7 +367,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                     const uint64_t v = mn128_desc(smem_addr(ring) + vs * C::TILE, C::HALF);
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        if (!ok || j >= w.need(x)) continue;
+                        if (!ok || j >= (x ? need1 : need0)) continue;
                         const uint32_t o = tb + C::O_COL + x * DP, w16 = tb + C::S_COL + x * 128;
                         uint32_t &phase = x ? phase1 : phase0;
                         ok = wait(&p_half[x], phase);
@@ -537,7 +381,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                         tc_fence_after();
 #pragma unroll
                         for (int kk = 4; kk < 8; ++kk) mma_f16_ts(e, o, w16 + kk * 8, v + kk * (2048 >> 4), id_o, 1);
-                        if (j + 1 < w.need(x)) scores(x, ks);
+                        if (j + 1 < (x ? need1 : need0)) scores(x, ks);
                         else commit_if(e, &o_full[x]);
                     }
                     if (ok) {
@@ -551,7 +395,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
             int slot = 0;
             uint32_t phase = 0;
             bool ok = true;
-            while (ok && next_item(p, walk, w)) {
+            while (ok && next_item<256, 128>(p, walk, w)) {
                 for (int j = 0; ok && j < w.tiles; ++j) {
                     const int vs = (slot + 2 * j + 1) % C::STAGES, key0 = w.lo + j * 128;
                     if (key0 >= w.first && key0 + 128 <= w.hi) continue;
@@ -577,17 +421,8 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
         } else {
             // ---------------- warp 11: how many pieces has the unit cut at the stretch's end? ----------------
             CutUnit cut{0, 0, 0, 0};
-            while (next_item(p, walk, w)) {
-                if (w.slot != 1) continue;
-                int first, lo, hi;
-                cut.h = w.h;
-                cut.b = w.b;
-                cut.t = w.row0 >> 8;
-                const int length = unit_length(p, w.n, w.nq, cut.t, first, lo, hi);
-                cut.pieces = 1;
-                // the next stretches' ends in this unit
-                for (int at = w.tiles; length - at >= MIN_PIECE; at += walk.share) ++cut.pieces;
-            }
+            while (next_item<256, 128>(p, walk, w))
+                if (w.slot == 1) cut = cut_of<256, 128>(p, walk, w);
             if (lane == 0) p.cut[blockIdx.x] = cut;
         }
     } else {
@@ -598,7 +433,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
         const uint32_t ts = tbase + lanes + C::S_COL + x * 128, to = tbase + lanes + C::O_COL + x * DP;
         uint32_t s_phase = 0, o_phase = 0;
         bool ok = true;
-        while (ok && next_item(p, walk, w)) {
+        while (ok && next_item<256, 128>(p, walk, w)) {
             const int row = w.row0 + x * 128 + r;
             const bool live = row < w.rows;
             // element offsets of this thread's row of q and of out; a warp moves its 32 rows together,
@@ -629,7 +464,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
             }
             const RowRange see = row_range(p, w.n, w.nq, row);
             float m = -INFINITY, l = 0.0f;  // m: the (lazy) reference of the weights, scaled
-            const int need = w.need(x);
+            const int need = tiles_needed(p, w, x);
             for (int j = 0; j < need; ++j) {
                 ok = ok && wait(&s_full[x], s_phase);
                 s_phase ^= 1u;
@@ -772,50 +607,6 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
     if (warp == 8) {
         tc_fence_after();
         umma::tmem_dealloc(tbase, 512);
-    }
-}
-
-// out of the rows of units that were cut: one warp per row at a time, the pieces in order.
-template <typename T>
-__global__ void __launch_bounds__(128) paged_combine_units_kernel(const __grid_constant__ AttendParams p) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int c = (int)blockIdx.x, lane = (int)(threadIdx.x & 31);
-    const CutUnit cut = p.cut[c];
-    if (cut.pieces < 2) return;
-    int start, nq, n;
-    load_sequence(p, cut.b, start, nq, n);
-    const int rows = nq * p.group;
-    for (int r = (int)blockIdx.y * 4 + (int)(threadIdx.x >> 5); r < 256; r += (int)gridDim.y * 4) {
-        const int row = cut.t * 256 + r;
-        if (row >= rows) break;
-        auto at = [&](int i) { return ((long long)(c + i) * 2 + (i == 0 ? 1 : 0)) * 256 + r; };
-        float m = -INFINITY, l = 0.0f;
-        for (int i = lane; i < cut.pieces; i += 32) m = fmaxf(m, p.part_ml[at(i)].x);
-#pragma unroll
-        for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));
-        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (lane * 4 < p.head_dim) {
-#pragma unroll 4
-            for (int i = 0; i < cut.pieces; ++i) {
-                const float2 ml = p.part_ml[at(i)];
-                const float4 v = *reinterpret_cast<const float4 *>(p.part + at(i) * p.head_dim + lane * 4);
-                const float f = ml.y == 0.0f ? 0.0f : ex2(ml.x - m);
-                l += f * ml.y;
-                a.x += f * v.x;
-                a.y += f * v.y;
-                a.z += f * v.z;
-                a.w += f * v.w;
-            }
-            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-            T *out = static_cast<T *>(p.out) + (long long)(start + row / p.group) * p.o_ts +
-                     (long long)(cut.h * p.group + row % p.group) * p.o_hs + lane * 4;
-            Pack<4, T> v;
-            v.e[0] = from_f<T>(a.x * inv);
-            v.e[1] = from_f<T>(a.y * inv);
-            v.e[2] = from_f<T>(a.z * inv);
-            v.e[3] = from_f<T>(a.w * inv);
-            v.store(out);
-        }
     }
 }
 

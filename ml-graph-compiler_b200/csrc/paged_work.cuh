@@ -1,0 +1,246 @@
+// How the work of an attention call is cut evenly over its CTAs, and the kernel that adds the pieces.
+#pragma once
+
+#include "paged_attention_params.cuh"
+
+namespace mgc {
+namespace paged {
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Position of row (token i of nq, sequence of n positions) -> its visible keys; rows past the last
+// see nothing.
+struct RowRange { int lo, hi; };
+__device__ __forceinline__ RowRange row_range(const AttendParams &p, int n, int nq, int row) {
+    RowRange r{0, 0};
+    const int i = row / p.group;
+    if (i < nq) visible(p, n, n - nq + i, r.lo, r.hi);
+    return r;
+}
+
+// A unit is (key head, sequence, ROWS query rows) and is as long as it has tiles of KEYS keys (at
+// least 1). All units lie end to end, key head by key head; CTA c takes the c-th of `ctas` equal
+// stretches. A stretch that ends inside a unit cuts it (unless a piece would be below MIN_PIECE
+// tiles): each piece leaves its rows' partial results, and paged_combine_units_kernel adds them in
+// order. Whole units on whole SMs would leave the last round part empty: 256 equal units on 148 SMs
+// take two rounds, the second 73% full, and sequences of mixed lengths do worse.
+constexpr int MIN_PIECE = 2;
+
+struct Item {
+    int rows, row0;     // query rows of the sequence; first of the unit's
+    int start;          // the sequence's first token
+    int n, nq;          // its positions, its new tokens
+    int b, h;
+    int lo, hi, tiles;  // keys [lo, hi) of this piece in `tiles` tiles
+    int first;          // first key that any row of the unit sees
+    int slot;           // where partial results go: -1 (the whole unit), 0 (a later piece), 1 (the first)
+};
+
+struct Walk {
+    int h, b, t;  // unit
+    int skip;     // its tiles before this CTA's stretch
+    int left;     // tiles left of the stretch
+    int share;    // tiles of a whole stretch
+    int heads;    // end of the key heads of these stretches
+    int start, nq, n;  // sequence b: first token, new tokens, positions
+};
+
+__device__ __forceinline__ void load_sequence(const AttendParams &p, int b, int &start, int &nq, int &n) {
+    start = __ldg(p.batch.q_starts + b);
+    nq = __ldg(p.batch.q_starts + b + 1) - start;
+    n = min(__ldg(p.batch.kv_lens + b), p.max_positions);
+}
+
+// Keys [lo, hi) that rows [ROWS t, ROWS t + ROWS) see, lo rounded down to a tile; the unit's length.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ int unit_length(const AttendParams &p, int n, int nq, int t, int &first, int &lo, int &hi) {
+    const int rows = nq * p.group, row0 = t * ROWS;
+    const RowRange a = row_range(p, n, nq, row0), z = row_range(p, n, nq, min(row0 + ROWS, rows) - 1);
+    first = a.lo;
+    lo = a.lo & ~(KEYS - 1);
+    hi = max(z.hi, 0);
+    return hi > lo ? (hi - lo + KEYS - 1) / KEYS : 1;
+}
+
+// The next piece of the stretch; false at its end. Advances the walk.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ bool next_item(const AttendParams &p, Walk &k, Item &w) {
+    while (k.left > 0 && k.h < k.heads) {
+        w.start = k.start;
+        w.nq = k.nq;
+        w.n = k.n;
+        w.rows = w.nq * p.group;
+        w.row0 = k.t * ROWS;
+        if (w.row0 >= w.rows) {  // past the sequence: the next one
+            k.t = 0;
+            if (++k.b == p.batch.batch) {
+                k.b = 0;
+                ++k.h;
+            }
+            load_sequence(p, k.b, k.start, k.nq, k.n);
+            continue;
+        }
+        int lo, hi;
+        const int length = unit_length<ROWS, KEYS>(p, w.n, w.nq, k.t, w.first, lo, hi);
+        int take = length - k.skip;
+        if (take > k.left) {
+            const int at = k.skip + k.left;  // where the stretch ends in the unit
+            if (at < MIN_PIECE) break;
+            if (length - at >= MIN_PIECE) take = k.left;
+        }
+        w.b = k.b;
+        w.h = k.h;
+        w.lo = lo + k.skip * KEYS;
+        w.hi = min(hi, w.lo + take * KEYS);
+        w.tiles = w.hi > w.lo ? (w.hi - w.lo + KEYS - 1) / KEYS : 0;
+        w.slot = take == length ? -1 : k.skip > 0 ? 0 : 1;
+        k.left -= take;
+        if (k.skip + take == length) {
+            k.skip = 0;
+            ++k.t;
+        } else {
+            k.skip += take;
+        }
+        return true;
+    }
+    return false;
+}
+
+// Start of stretch c of `ctas` over the units of key heads [h0, h1) (one warp). Units are looked at
+// 32 at a time; their lengths are the same for every key head.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ Walk find_stretch(const AttendParams &p, int c, int ctas, int h0, int h1, int lane) {
+    int most = 0;  // row tiles of the longest sequence
+    for (int b = lane; b < p.batch.batch; b += 32) {
+        int start, nq, n;
+        load_sequence(p, b, start, nq, n);
+        if (n != __ldg(p.batch.kv_lens + b) && nq > 0 && p.batch.status) *p.batch.status = MGC_CUDA_GATHER_OOB;
+        most = max(most, (nq * p.group + ROWS - 1) / ROWS);
+    }
+    most = __reduce_max_sync(0xFFFFFFFFu, most);
+    const unsigned count = (unsigned)p.batch.batch * (unsigned)most;
+    auto length_of = [&](unsigned i) {
+        if (i >= count) return 0;
+        int start, nq, n, first, lo, hi;
+        const unsigned b = i / (unsigned)most;
+        load_sequence(p, (int)b, start, nq, n);
+        const int t = (int)(i - b * (unsigned)most);
+        return t * ROWS < nq * p.group ? unit_length<ROWS, KEYS>(p, n, nq, t, first, lo, hi) : 0;
+    };
+    // the lanes' lengths summed up to and including each; the first 32 units' are kept
+    auto scan = [&](int v) {
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int u = __shfl_up_sync(0xFFFFFFFFu, v, d);
+            if (lane >= d) v += u;
+        }
+        return v;
+    };
+    const int mine0 = length_of(lane), upto0 = scan(mine0);
+    long long head = __shfl_sync(0xFFFFFFFFu, upto0, 31);  // tiles of one key head
+    for (unsigned i = 32; i < count; i += 32) head += __reduce_add_sync(0xFFFFFFFFu, length_of(i + lane));
+    Walk k{h1, 0, 0, 0, 0, 0, h1, 0, 0, 0};
+    const long long all = head * (h1 - h0);
+    long long share, x0;
+    if (all < 0x7FFFFFFF) {
+        share = ((unsigned)all + ctas - 1) / (unsigned)ctas;
+        share = max(share, (long long)MIN_PIECE);
+        x0 = c * share;
+        if (x0 >= all) return k;
+        k.h = (int)((unsigned)x0 / (unsigned)head);
+    } else {
+        share = (all + ctas - 1) / ctas;
+        x0 = c * share;
+        if (x0 >= all) return k;
+        k.h = (int)(x0 / head);
+    }
+    long long at = x0 - k.h * head;
+    k.h += h0;
+    for (unsigned i = 0; i < count; i += 32) {
+        const int mine = i ? length_of(i + lane) : mine0, upto = i ? scan(mine) : upto0;
+        const unsigned past = __ballot_sync(0xFFFFFFFFu, upto > at);
+        if (past) {
+            const int who = __ffs(past) - 1;
+            const int length = __shfl_sync(0xFFFFFFFFu, mine, who);
+            const int off = (int)at - (__shfl_sync(0xFFFFFFFFu, upto, who) - length);
+            k.b = (int)((i + who) / (unsigned)most);
+            k.t = (int)((i + who) % (unsigned)most);
+            load_sequence(p, k.b, k.start, k.nq, k.n);
+            k.left = k.share = (int)share;
+            if (off < MIN_PIECE) {
+                k.left += off;
+            } else if (length - off < MIN_PIECE) {
+                k.left -= length - off;
+                ++k.t;
+            } else {
+                k.skip = off;
+            }
+            break;
+        }
+        at -= __shfl_sync(0xFFFFFFFFu, upto, 31);
+    }
+    return k;
+}
+
+// What adding up the unit cut at the stretch's end (piece w, slot 1) needs: the later stretches that
+// end in it are one share apart.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ CutUnit cut_of(const AttendParams &p, const Walk &k, const Item &w) {
+    int first, lo, hi;
+    CutUnit cut{w.h, w.b, w.row0 / ROWS, 1};
+    const int length = unit_length<ROWS, KEYS>(p, w.n, w.nq, cut.t, first, lo, hi);
+    for (int at = w.tiles; length - at >= MIN_PIECE; at += k.share) ++cut.pieces;
+    return cut;
+}
+
+// out of the rows of units that were cut: one warp per row at a time, the pieces in order.
+// `next` CTAs lie between a stretch and the one after it.
+template <typename T, int ROWS>
+__global__ void __launch_bounds__(128) paged_combine_units_kernel(const __grid_constant__ AttendParams p, const int next) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int c = (int)blockIdx.x, lane = (int)(threadIdx.x & 31);
+    const CutUnit cut = p.cut[c];
+    if (cut.pieces < 2) return;
+    int start, nq, n;
+    load_sequence(p, cut.b, start, nq, n);
+    const int rows = nq * p.group;
+    for (int r = (int)blockIdx.y * 4 + (int)(threadIdx.x >> 5); r < ROWS; r += (int)gridDim.y * 4) {
+        const int row = cut.t * ROWS + r;
+        if (row >= rows) break;
+        auto at = [&](int i) { return ((long long)(c + i * next) * 2 + (i == 0 ? 1 : 0)) * ROWS + r; };
+        float m = -INFINITY, l = 0.0f;
+        for (int i = lane; i < cut.pieces; i += 32) m = fmaxf(m, p.part_ml[at(i)].x);
+#pragma unroll
+        for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));
+        for (int d = lane * 4; d < p.head_dim; d += 128) {
+            float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            l = 0.0f;
+#pragma unroll 4
+            for (int i = 0; i < cut.pieces; ++i) {
+                const float2 ml = p.part_ml[at(i)];
+                const float4 v = *reinterpret_cast<const float4 *>(p.part + at(i) * p.head_dim + d);
+                const float f = ml.y == 0.0f ? 0.0f : ex2(ml.x - m);
+                l += f * ml.y;
+                a.x += f * v.x;
+                a.y += f * v.y;
+                a.z += f * v.z;
+                a.w += f * v.w;
+            }
+            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            T *out = static_cast<T *>(p.out) + (long long)(start + row / p.group) * p.o_ts +
+                     (long long)(cut.h * p.group + row % p.group) * p.o_hs + d;
+            Pack<4, T> v;
+            v.e[0] = from_f<T>(a.x * inv);
+            v.e[1] = from_f<T>(a.y * inv);
+            v.e[2] = from_f<T>(a.z * inv);
+            v.e[3] = from_f<T>(a.w * inv);
+            v.store(out);
+        }
+    }
+}
+
+}  // namespace paged
+}  // namespace mgc
