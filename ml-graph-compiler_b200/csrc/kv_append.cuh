@@ -8,7 +8,9 @@
 // value, so memory bounds it (latency for a few tokens). A block takes one token: its warps find
 // the sequence with one ballot per 32 sequences, then each thread moves units of V channels of a
 // head (16 bytes), a rotated unit being the two chunks whose channels pair up, so that each pair
-// is read and written by one thread and q may be rotated in place.
+// is read and written by one thread and q may be rotated in place. A thread's units are the same
+// channels of several heads, so it reads its angles once; its first sources load while the block
+// looks up the token's place.
 #pragma once
 
 #include "paged_common.cuh"
@@ -27,7 +29,8 @@ struct AppendParams {
     long long table_row;
     int positions, rot, interleaved;
     int q_heads, kv_heads, head_dim;
-    int units;  // per head: rot / 2V rotated pairs of chunks, then (head_dim - rot) / V plain chunks
+    int threads;  // that work: a multiple of units
+    int units;    // per head: rot / 2V rotated pairs of chunks, then (head_dim - rot) / V plain chunks
 };
 
 // V values of the tables, which the vector forms read 16 bytes at a time.
@@ -38,13 +41,46 @@ template <int V> __device__ __forceinline__ void load_angles(const float *p, flo
     for (int i = 0; i < V; ++i) x[i] = a.e[i];
 }
 
+// One unit of a head on its way.
+template <typename S, typename T, int V> struct Unit {
+    Pack<V, S> x, y;
+};
+
 template <typename S, typename T, int V>
 __global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ AppendParams p) {
+    constexpr int BATCH = 2;
     const int t = (int)blockIdx.x;
+    // thread (w, h0) takes unit w of heads h0, h0 + step, ...: its angles are the same for all of them
+    const int h0 = (int)threadIdx.x / p.units, w = (int)threadIdx.x - h0 * p.units, step = p.threads / p.units;
+    const int heads = p.q_heads + 2 * p.kv_heads, pairs = p.rot / (2 * V);
+    const bool pair = w < pairs;
+    const int c0 = !pair ? p.rot + (w - pairs) * V : p.interleaved ? w * 2 * V : w * V;
+    const int c1 = p.interleaved ? c0 + V : c0 + p.rot / 2;
+    Unit<S, T, V> u[BATCH];
+    // the sources' addresses need no lookup: their loads overlap the search for the token's place
+    auto load = [&](Unit<S, T, V> &z, int h) {
+        if (h >= heads) return;
+        const S *src;
+        if (h < p.q_heads) {
+            src = static_cast<const S *>(p.q) + t * p.q_ts + h * p.q_hs;
+        } else if (h < p.q_heads + p.kv_heads) {
+            src = static_cast<const S *>(p.k) + t * p.k_ts + (h - p.q_heads) * p.k_hs;
+        } else {
+            src = static_cast<const S *>(p.v) + t * p.v_ts + (h - p.q_heads - p.kv_heads) * p.v_hs;
+        }
+        z.x.load(src + c0);
+        if (pair) z.y.load(src + c1);
+    };
+    const bool active = (int)threadIdx.x < p.threads;
+    if (active) {
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) load(u[i], h0 + i * step);
+    }
+
     const int b = sequence_of(p.batch, t);
     if (b < 0) return;
     const int end = __ldg(p.batch.q_starts + b + 1);
-    if (t >= end) return;  // past the last sequence
+    if (t >= end || !active) return;  // past the last sequence
     const int pos = __ldg(p.batch.kv_lens + b) - (end - t);
     int page = -1;
     if (pos >= 0) page = page_of(p.batch, b, pos / p.batch.page_size);
@@ -55,74 +91,78 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ 
         page = -1;
     }
     const long long slot = page < 0 ? 0 : (long long)page * p.page_stride + (long long)(pos % p.batch.page_size) * p.token_stride;
-    const int pairs = p.rot / (2 * V);
-    const int total = (p.q_heads + 2 * p.kv_heads) * p.units;
-    for (int u = (int)threadIdx.x; u < total; u += (int)blockDim.x) {
-        int h = u / p.units;
-        const int w = u - h * p.units;
-        const S *src;
+    float c[V], s[V];
+    if (turn && pair) {
+        load_angles<V>(p.cos + (long long)pos * p.table_row + w * V, c);
+        load_angles<V>(p.sin + (long long)pos * p.table_row + w * V, s);
+    }
+    auto finish = [&](Unit<S, T, V> &z, int h) {
+        if (h >= heads) return;
         T *dst;
         bool rotate = turn;
         if (h < p.q_heads) {
-            src = static_cast<const S *>(p.q) + t * p.q_ts + h * p.q_hs;
             dst = static_cast<T *>(p.q_out) + t * p.qo_ts + h * p.qo_hs;
         } else {
-            if (page < 0) continue;
+            if (page < 0) return;
             h -= p.q_heads;
-            const bool key = h < p.kv_heads;
-            if (!key) h -= p.kv_heads;
-            src = key ? static_cast<const S *>(p.k) + t * p.k_ts + h * p.k_hs
-                      : static_cast<const S *>(p.v) + t * p.v_ts + h * p.v_hs;
-            dst = static_cast<T *>(key ? p.k_pages : p.v_pages) + slot + h * p.head_stride;
-            rotate = rotate && key;
+            rotate = rotate && h < p.kv_heads;
+            dst = static_cast<T *>(h < p.kv_heads ? p.k_pages : p.v_pages) + slot + (h < p.kv_heads ? h : h - p.kv_heads) * p.head_stride;
         }
-        Pack<V, S> x, y;
         Pack<V, T> ox, oy;
-        if (w >= pairs) {
-            const int c = p.rot + (w - pairs) * V;
-            x.load(src + c);
+        if (!pair) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) ox.e[i] = from_f<T>(to_f(x.e[i]));
-            ox.store(dst + c);
-            continue;
+            for (int i = 0; i < V; ++i) ox.e[i] = from_f<T>(to_f(z.x.e[i]));
+            ox.store(dst + c0);
+            return;
         }
-        const int c0 = p.interleaved ? w * 2 * V : w * V;
-        const int c1 = p.interleaved ? c0 + V : c0 + p.rot / 2;
-        x.load(src + c0);
-        y.load(src + c1);
-        float z[2 * V];
+        float v[2 * V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            z[i] = to_f(x.e[i]);
-            z[V + i] = to_f(y.e[i]);
+            v[i] = to_f(z.x.e[i]);
+            v[V + i] = to_f(z.y.e[i]);
         }
         if (rotate) {
-            float c[V], s[V];
-            load_angles<V>(p.cos + (long long)pos * p.table_row + w * V, c);
-            load_angles<V>(p.sin + (long long)pos * p.table_row + w * V, s);
+            if (p.interleaved) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const int i1 = p.interleaved ? 2 * i : i, i2 = p.interleaved ? 2 * i + 1 : V + i;
-                const float x1 = z[i1], x2 = z[i2];
-                z[i1] = x1 * c[i] - x2 * s[i];
-                z[i2] = x2 * c[i] + x1 * s[i];
+                for (int i = 0; i < V; ++i) {
+                    const float x1 = v[2 * i], x2 = v[2 * i + 1];
+                    v[2 * i] = x1 * c[i] - x2 * s[i];
+                    v[2 * i + 1] = x2 * c[i] + x1 * s[i];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float x1 = v[i], x2 = v[V + i];
+                    v[i] = x1 * c[i] - x2 * s[i];
+                    v[V + i] = x2 * c[i] + x1 * s[i];
+                }
             }
         }
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            ox.e[i] = from_f<T>(z[i]);
-            oy.e[i] = from_f<T>(z[V + i]);
+            ox.e[i] = from_f<T>(v[i]);
+            oy.e[i] = from_f<T>(v[V + i]);
         }
         ox.store(dst + c0);
         oy.store(dst + c1);
+    };
+    for (int h = h0;;) {
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) finish(u[i], h + i * step);
+        h += BATCH * step;
+        if (h >= heads) break;
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) load(u[i], h + i * step);
     }
 }
 
 template <typename S, typename T, int V> inline int run_append(AppendParams &p, int tokens, cudaStream_t stream) {
     p.units = p.rot / (2 * V) + (p.head_dim - p.rot) / V;
-    const int64_t total = (int64_t)(p.q_heads + 2 * p.kv_heads) * p.units;
-    const int threads = (int)(total >= 256 ? 256 : ceil_div(total, 32) * 32);
-    kv_append_kernel<S, T, V><<<(unsigned)tokens, threads, 0, stream>>>(p);
+    const int heads = p.q_heads + 2 * p.kv_heads;
+    if (p.units > 256) return fail(MGC_CUDA_UNSUPPORTED, "mgc_cuda_kv_append: %d channels in units of %d", p.head_dim, V);
+    // whole heads of units, at most 256 threads
+    p.threads = (heads < 256 / p.units ? heads : 256 / p.units) * p.units;
+    kv_append_kernel<S, T, V><<<(unsigned)tokens, (unsigned)ceil_div(p.threads, 32) * 32, 0, stream>>>(p);
     return check_launch("kv_append_kernel");
 }
 
@@ -162,7 +202,7 @@ inline int append(const mgc_cuda_kv_append_args &a, cudaStream_t stream) {
         (a.src_dtype != c.dtype || a.q_token_stride != a.qo_token_stride || a.q_head_stride != a.qo_head_stride))
         return fail(MGC_CUDA_BAD_ARGUMENT, "%s: q rotated in place keeps its type and strides", what);
     const int64_t heads = (a.q ? a.q_heads : 0) + 2 * c.kv_heads;
-    if (c.head_dim > 65536 || heads > 1 << 20 || heads * c.head_dim > 0x7FFFFFFF)
+    if (c.head_dim > 256 || heads > 1 << 20 || heads * c.head_dim > 0x7FFFFFFF)
         return fail(MGC_CUDA_UNSUPPORTED, "%s: %lld heads of %lld channels", what, (long long)heads, (long long)c.head_dim);
     AppendParams p;
     p.batch = batch_of(c);
