@@ -85,6 +85,7 @@ inline int check_attend(const mgc_cuda_paged_attention_args &a, const char *what
 struct Plan {
     bool mma = false, umma = false, even = false;
     int wm = 1;         // 16-row warps of a row tile
+    int simt = 0;       // rows of the plain fp32 form (0: matrix instructions)
     int row_tiles = 1, splits = 1;
     int unit_rows = 0, ctas = 0;  // even shares: rows of a unit, CTAs
     bool interleaved = false;
@@ -94,11 +95,12 @@ struct Plan {
 constexpr int MIN_SPLIT_KEYS = 128;  // below this a split's start and merge outweigh its loads
 
 // CTAs of the tiled kernel that an SM holds (of 128 threads, by shared memory; 2 at 256 registers).
-inline int ctas_per_sm(int64_t dtype, int64_t head_dim, int wm) {
+inline int ctas_per_sm(int64_t dtype, int64_t head_dim, int wm, int simt) {
     const int dp = head_dim <= 32 ? 32 : head_dim <= 64 ? 64 : head_dim <= 96 ? 96 : head_dim <= 128 ? 128 : 256;
     const bool f32 = dtype == MGC_F32;
-    const int row = dp * (f32 ? 4 : 2) + 16, ring = (dp > 128 ? 2 : 3) * 2 * (f32 ? 32 : 64) * row;
-    const int bytes = ring + (!f32 && dp <= 128 ? 0 : 16 * wm * row) + 3 * 64 * 8 + 1024;
+    const int keys = !f32 ? 64 : !simt ? 32 : dp <= 32 ? 128 : dp <= 64 ? 64 : 32;
+    const int row = dp * (f32 ? 4 : 2) + 16, ring = (dp > 128 ? 2 : 3) * 2 * keys * row;
+    const int bytes = ring + (!f32 && dp <= 128 ? 0 : (simt ? simt : 16 * wm) * row) + 3 * keys * 8 + 1024;
     const int fit = 232448 / bytes;
     return fit < 1 ? 1 : fit > 4 ? 4 : fit;
 }
@@ -134,19 +136,27 @@ inline Plan plan_of(const mgc_cuda_paged_attention_args &a) {
         return s;
     }
     s.wm = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    s.row_tiles = (int)ceil_div(rows, 16 * s.wm);
+    // fp32 rows cost the FMA units ~200 instructions per 32 keys each; the split products cost ~3300
+    // for 16 rows, used or not
+    if (c.dtype == MGC_F32 && rows <= 8 && c.head_dim <= 128) s.simt = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8;
+    s.unit_rows = s.simt ? s.simt : 16 * s.wm;
+    s.row_tiles = (int)ceil_div(rows, s.unit_rows);
     const int64_t units = c.batch * c.kv_heads * s.row_tiles;
     int64_t most = a.max_kv;
     if (a.window > 0 && a.window + max_q < most) most = a.window + max_q;
     // CTAs that fit the GPU at once: shared memory and registers allow this many per SM
-    const int64_t slots = (int64_t)sm_count() * ctas_per_sm(c.dtype, c.head_dim, s.wm);
+    const int64_t slots = (int64_t)sm_count() * ctas_per_sm(c.dtype, c.head_dim, s.wm, s.simt);
     int64_t splits = slots / units;
     if (splits > most / MIN_SPLIT_KEYS) splits = most / MIN_SPLIT_KEYS;
     if (splits < 1) splits = 1;
-    if (splits > MAX_CLUSTER || (units * 2 > slots && c.batch > 1)) {
-        even_shares(16 * s.wm, (int)slots);
+    // A cluster needs no second kernel (~1000 keys' worth of time); even shares leave no SM idle when
+    // sequences differ or 8 parts are too few.
+    const int64_t in_cluster = most / (splits < MAX_CLUSTER ? splits : MAX_CLUSTER), even = most * units / slots;
+    if (in_cluster > even + 1024 || (units * 2 > slots && c.batch > 1)) {
+        even_shares(s.unit_rows, (int)slots);
         return s;
     }
+    if (splits > MAX_CLUSTER) splits = MAX_CLUSTER;
     s.splits = (int)splits;
     return s;
 }
@@ -185,21 +195,21 @@ template <typename T> inline int launch_umma(const AttendParams &p, const mgc_cu
     return launch_after(paged_combine_units_kernel<T, 256>, dim3((unsigned)ctas, 32), p, 1, stream);
 }
 
-template <typename T, int DP, int WM, int WN> inline int launch_mma(const AttendParams &p, const Plan &s, cudaStream_t stream) {
-    using C = MmaConfig<T, DP, WM, WN>;
+template <typename T, int DP, int WM, int WN, int SIMT> inline int launch_mma(const AttendParams &p, const Plan &s, cudaStream_t stream) {
+    using C = MmaConfig<T, DP, WM, WN, SIMT>;
     cudaLaunchConfig_t cfg{};
     cfg.blockDim = dim3(C::THREADS);
     cfg.dynamicSmemBytes = C::SMEM;
     cfg.stream = stream;
     if (s.even) {
-        auto kernel = paged_attention_mma_kernel<T, DP, WM, WN, true>;
+        auto kernel = paged_attention_mma_kernel<T, DP, WM, WN, SIMT, true>;
         MGC_CHECK(raise_smem_ceiling((const void *)kernel));
         cfg.gridDim = dim3((unsigned)s.ctas);
         MGC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
-        return launch_after(paged_combine_units_kernel<T, C::R>, dim3((unsigned)s.ctas, C::R / 16), p, s.interleaved ? p.kv_heads : 1,
+        return launch_after(paged_combine_units_kernel<T, C::R>, dim3((unsigned)s.ctas, (C::R + 15) / 16), p, s.interleaved ? p.kv_heads : 1,
                             stream);
     }
-    auto kernel = paged_attention_mma_kernel<T, DP, WM, WN, false>;
+    auto kernel = paged_attention_mma_kernel<T, DP, WM, WN, SIMT, false>;
     MGC_CHECK(raise_smem_ceiling((const void *)kernel));
     cfg.gridDim = dim3((unsigned)(p.batch.batch * p.kv_heads * p.row_tiles), (unsigned)p.splits);
     cudaLaunchAttribute attr[1];
@@ -213,9 +223,15 @@ template <typename T, int DP, int WM, int WN> inline int launch_mma(const Attend
 }
 
 template <typename T, int DP> inline int launch_mma_rows(const AttendParams &p, const Plan &s, cudaStream_t stream) {
-    if (s.wm == 1) return launch_mma<T, DP, 1, 4>(p, s, stream);
-    if (s.wm == 2) return launch_mma<T, DP, 2, 2>(p, s, stream);
-    return launch_mma<T, DP, 4, 1>(p, s, stream);
+    if constexpr (sizeof(T) == 4 && DP <= 128) {
+        if (s.simt == 1) return launch_mma<T, DP, 1, 4, 1>(p, s, stream);
+        if (s.simt == 2) return launch_mma<T, DP, 1, 4, 2>(p, s, stream);
+        if (s.simt == 4) return launch_mma<T, DP, 1, 4, 4>(p, s, stream);
+        if (s.simt == 8) return launch_mma<T, DP, 1, 4, 8>(p, s, stream);
+    }
+    if (s.wm == 1) return launch_mma<T, DP, 1, 4, 0>(p, s, stream);
+    if (s.wm == 2) return launch_mma<T, DP, 2, 2, 0>(p, s, stream);
+    return launch_mma<T, DP, 4, 1, 0>(p, s, stream);
 }
 
 // Head widths are padded to the next of these (zero channels).

@@ -98,11 +98,14 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
 
 constexpr int MAX_CLUSTER = 8;  // portable cluster size
 
-template <typename T, int DP, int WM, int WN> struct MmaConfig {
+// SIMT > 0: that many rows (fp32, at most 128 channels) on the FMA units, all four warps along the keys.
+template <typename T, int DP, int WM, int WN, int SIMT> struct MmaConfig {
     static constexpr bool F32 = sizeof(T) == 4;
+    // lanes that share a key of the plain form, each a part of its channels
+    static constexpr int PARTS = DP <= 32 ? 1 : DP <= 64 ? 2 : 4;
     static constexpr int THREADS = 32 * WM * WN;
-    static constexpr int R = 16 * WM;
-    static constexpr int BN = F32 ? 32 : 64;         // keys per stage
+    static constexpr int R = SIMT ? SIMT : 16 * WM;
+    static constexpr int BN = SIMT ? WN * 32 / PARTS : F32 ? 32 : 64;  // keys per stage
     static constexpr int KW = BN / WN;               // of them, a warp's
     static constexpr int KG = DP > 128 && KW > 32 ? 32 : KW;  // keys per softmax step (registers)
     static constexpr int STAGES = DP > 128 ? 2 : 3;
@@ -114,21 +117,21 @@ template <typename T, int DP, int WM, int WN> struct MmaConfig {
     static constexpr int ORED = DP + 4;              // floats of a row of the final reduction
     static constexpr int RED = WN * R * (ORED + 2) * 4;
     static constexpr int RING = STAGES * STAGE;
-    static constexpr int SMEM = Q_BYTES + (RING > RED ? RING : RED) + STAGES * BN * 8;
+    static constexpr int SMEM = Q_BYTES + (RING > RED ? RING : RED) + STAGES * BN * 8 + (SIMT ? WN * R * KW * 4 : 0);
 };
 
 // EVEN: the CTA takes an even share of all units' keys (paged_work.cuh); else one row tile's keys, or
 // the part of them that its rank in a cluster names.
-template <typename T, int DP, int WM, int WN, bool EVEN>
-__global__ void __launch_bounds__(MmaConfig<T, DP, WM, WN>::THREADS)
+template <typename T, int DP, int WM, int WN, int SIMT, bool EVEN>
+__global__ void __launch_bounds__(MmaConfig<T, DP, WM, WN, SIMT>::THREADS)
 paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
-    using C = MmaConfig<T, DP, WM, WN>;
-    constexpr int R = C::R, BN = C::BN, KW = C::KW, KG = C::KG, ROW = C::ROW, NB = KG / 8, DB = DP / 8;
+    using C = MmaConfig<T, DP, WM, WN, SIMT>;
+    constexpr int R = C::R, BN = C::BN, KW = C::KW, KG = C::KG, ROW = C::ROW, NB = KG / 8 ? KG / 8 : 1, DB = SIMT ? 1 : DP / 8;
     constexpr int CPR = DP / C::CH;  // 16-byte chunks of a padded row
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *sQ = smem;
     uint8_t *ring = smem + C::Q_BYTES;
-    long long *sOff = reinterpret_cast<long long *>(smem + C::SMEM - C::STAGES * BN * 8);
+    long long *sOff = reinterpret_cast<long long *>(smem + C::SMEM - C::STAGES * BN * 8 - (SIMT ? WN * R * KW * 4 : 0));
     const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int wm = warp % WM, wn = warp / WM;
     const int g4 = lane >> 2, t4 = lane & 3;
@@ -197,6 +200,20 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
 #pragma unroll
         for (int d = 0; d < DB; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.0f;
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+        // plain form: every row's maximum, this lane's part of its sum, and CL channels of its output
+        constexpr int SR = SIMT ? SIMT : 1, CL = DP / 32;
+        float so[SR][CL], sm_[SR], sl_[SR];
+        RowRange sr[SR];
+        if constexpr (SIMT > 0) {
+#pragma unroll
+            for (int r = 0; r < SR; ++r) {
+                sr[r] = row_range(p, n, nq, row0 + r);
+                sm_[r] = -INFINITY;
+                sl_[r] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < CL; ++i) so[r][i] = 0.0f;
+            }
+        }
 
         // the first stages; a stage's offsets are looked up well before its loads
         for (int x = tid; x < C::STAGES * BN; x += C::THREADS) sOff[x] = offset_of(k_lo + x);
@@ -216,6 +233,79 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
             if (tid < BN) next = offset_of(k_lo + (it + C::STAGES) * BN + tid);
 
             const uint8_t *st = ring + (it % C::STAGES) * C::STAGE;
+            if constexpr (SIMT > 0) {
+                // scores: lane (key, part) sums its part's channels of its key, the parts meet by
+                // shuffles; output: lane owns channels CL lane .., weights broadcast from shared memory
+                constexpr int PC = DP / C::PARTS / 4;  // 16-byte chunks of a part
+                const int key = lane % KW, part = lane / KW;
+                const int j0 = k_lo + it * BN + wn * KW, j = j0 + key;
+                if (j0 < k_hi) {
+                    float *sP = reinterpret_cast<float *>(smem + C::SMEM) - (wn + 1) * R * KW;
+                    const float4 *kr = reinterpret_cast<const float4 *>(st + (wn * KW + key) * ROW) + part * PC;
+                    float x[SR];
+#pragma unroll
+                    for (int r = 0; r < SR; ++r) x[r] = 0.0f;
+#pragma unroll
+                    for (int c = 0; c < PC; ++c) {
+                        const float4 kv = kr[c];
+#pragma unroll
+                        for (int r = 0; r < SR; ++r) {
+                            const float4 qv = reinterpret_cast<const float4 *>(sQ + r * ROW)[part * PC + c];
+                            x[r] = fmaf(qv.x, kv.x, fmaf(qv.y, kv.y, fmaf(qv.z, kv.z, fmaf(qv.w, kv.w, x[r]))));
+                        }
+                    }
+#pragma unroll
+                    for (int r = 0; r < SR; ++r) {
+#pragma unroll
+                        for (int d = KW; d < 32; d <<= 1) x[r] += __shfl_xor_sync(0xFFFFFFFFu, x[r], d);
+                        if (j < sr[r].lo || j >= sr[r].hi || j >= k_hi) x[r] = -INFINITY;
+                        float top = x[r];
+#pragma unroll
+                        for (int d = 1; d < KW; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+                        top = fmaxf(top, sm_[r]);
+                        const float y = top == -INFINITY ? 0.0f : __fmul_rn(top, p.scale_log2);
+                        const float f = ex2(__fmul_rn(sm_[r], p.scale_log2) - y), wgt = ex2(fmaf(x[r], p.scale_log2, -y));
+                        sm_[r] = top;
+                        sl_[r] = sl_[r] * f + wgt;
+#pragma unroll
+                        for (int i = 0; i < CL; ++i) so[r][i] *= f;
+                        if (part == 0) sP[r * KW + key] = wgt;
+                    }
+                    __syncwarp();
+                    const float *vr = reinterpret_cast<const float *>(st + (BN + wn * KW) * ROW) + lane * CL;
+#pragma unroll
+                    for (int k4 = 0; k4 < KW; k4 += 4) {
+                        float4 pw[SR];
+#pragma unroll
+                        for (int r = 0; r < SR; ++r) pw[r] = *reinterpret_cast<const float4 *>(sP + r * KW + k4);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            float v[CL];
+                            if constexpr (CL == 2) {
+                                const float2 t = *reinterpret_cast<const float2 *>(vr + (k4 + k) * (ROW / 4));
+                                v[0] = t.x;
+                                v[1] = t.y;
+                            } else if constexpr (CL == 4) {
+                                const float4 t = *reinterpret_cast<const float4 *>(vr + (k4 + k) * (ROW / 4));
+                                v[0] = t.x;
+                                v[1] = t.y;
+                                v[2] = t.z;
+                                v[3] = t.w;
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < CL; ++i) v[i] = vr[(k4 + k) * (ROW / 4) + i];
+                            }
+#pragma unroll
+                            for (int r = 0; r < SR; ++r) {
+                                const float wgt = k == 0 ? pw[r].x : k == 1 ? pw[r].y : k == 2 ? pw[r].z : pw[r].w;
+#pragma unroll
+                                for (int i = 0; i < CL; ++i) so[r][i] = fmaf(wgt, v[i], so[r][i]);
+                            }
+                        }
+                    }
+                    __syncwarp();  // the weights are read before the next stage's are written
+                }
+            } else {
 #pragma unroll
             for (int kg = 0; kg < KW / KG; ++kg) {
                 const int kw = wn * KW + kg * KG;  // first of the warp's keys in the stage
@@ -403,6 +493,7 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
                     }
                 }
             }
+            }
             if (tid < BN) sOff[(it % C::STAGES) * BN + tid] = next;
         }
         cp_async_wait<0>();
@@ -411,23 +502,38 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
         // ---- the warps' partial results, then the splits' ----
         float *red = reinterpret_cast<float *>(ring);
         float *sm = red + WN * R * C::ORED, *sl = sm + WN * R;
-        l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, 1);
-        l1 += __shfl_xor_sync(0xFFFFFFFFu, l1, 1);
-        l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, 2);
-        l1 += __shfl_xor_sync(0xFFFFFFFFu, l1, 2);
-        const int ra = wn * R + 16 * wm + g4;
+        if constexpr (SIMT > 0) {
 #pragma unroll
-        for (int d = 0; d < DB; ++d) {
-            *reinterpret_cast<float2 *>(red + ra * C::ORED + d * 8 + t4 * 2) = make_float2(o[d][0], o[d][1]);
-            *reinterpret_cast<float2 *>(red + (ra + 8) * C::ORED + d * 8 + t4 * 2) = make_float2(o[d][2], o[d][3]);
+            for (int r = 0; r < SR; ++r) {
+#pragma unroll
+                for (int d = 1; d < KW; d <<= 1) sl_[r] += __shfl_xor_sync(0xFFFFFFFFu, sl_[r], d);
+#pragma unroll
+                for (int i = 0; i < CL; ++i) red[(wn * R + r) * C::ORED + lane * CL + i] = so[r][i];
+                if (lane == 0) {
+                    sm[wn * R + r] = __fmul_rn(sm_[r], p.scale_log2);
+                    sl[wn * R + r] = sl_[r];
+                }
+            }
+            __syncthreads();
+        } else {
+            l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, 1);
+            l1 += __shfl_xor_sync(0xFFFFFFFFu, l1, 1);
+            l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, 2);
+            l1 += __shfl_xor_sync(0xFFFFFFFFu, l1, 2);
+            const int ra = wn * R + 16 * wm + g4;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                *reinterpret_cast<float2 *>(red + ra * C::ORED + d * 8 + t4 * 2) = make_float2(o[d][0], o[d][1]);
+                *reinterpret_cast<float2 *>(red + (ra + 8) * C::ORED + d * 8 + t4 * 2) = make_float2(o[d][2], o[d][3]);
+            }
+            if (t4 == 0) {
+                sm[ra] = m0 * p.scale_log2;
+                sm[ra + 8] = m1 * p.scale_log2;
+                sl[ra] = l0;
+                sl[ra + 8] = l1;
+            }
+            __syncthreads();
         }
-        if (t4 == 0) {
-            sm[ra] = m0 * p.scale_log2;
-            sm[ra + 8] = m1 * p.scale_log2;
-            sl[ra] = l0;
-            sl[ra + 8] = l1;
-        }
-        __syncthreads();
         const int quads = p.head_dim / 4;
         const int live = min(R, rows - row0);
         auto warps_sum = [&](int r, int c, float &m, float &l) {
