@@ -89,6 +89,7 @@ struct Plan {
     int row_tiles = 1, splits = 1;
     int unit_rows = 0, ctas = 0;  // even shares: rows of a unit, CTAs
     bool interleaved = false;
+    int live_rows = 1;  // of a unit, going by max_q
     int64_t workspace = 0;
 };
 
@@ -123,6 +124,7 @@ inline Plan plan_of(const mgc_cuda_paged_attention_args &a) {
     auto even_shares = [&](int unit_rows, int ctas) {
         s.even = true;
         s.unit_rows = unit_rows;
+        s.live_rows = (int)(rows < unit_rows ? rows : unit_rows);
         s.ctas = ctas;
         if (!s.umma && ctas >= c.kv_heads && ctas / c.kv_heads * c.kv_heads * 20 >= ctas * 19) {
             s.interleaved = true;
@@ -206,7 +208,7 @@ template <typename T, int DP, int WM, int WN, int SIMT> inline int launch_mma(co
         MGC_CHECK(raise_smem_ceiling((const void *)kernel));
         cfg.gridDim = dim3((unsigned)s.ctas);
         MGC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
-        return launch_after(paged_combine_units_kernel<T, C::R>, dim3((unsigned)s.ctas, (C::R + 15) / 16), p, s.interleaved ? p.kv_heads : 1,
+        return launch_after(paged_combine_units_kernel<T, C::R>, dim3((unsigned)s.ctas, (unsigned)s.live_rows), p, s.interleaved ? p.kv_heads : 1,
                             stream);
     }
     auto kernel = paged_attention_mma_kernel<T, DP, WM, WN, SIMT, false>;

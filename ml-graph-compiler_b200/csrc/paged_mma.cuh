@@ -650,6 +650,7 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
             if (lane == 0) stretch = k;
         }
         __syncthreads();
+        asm volatile("griddepcontrol.launch_dependents;");  // the kernel that adds the pieces waits on its own
         Walk walk = stretch;
         Item w;
         CutUnit cut{0, 0, 0, 0};

@@ -196,18 +196,26 @@ __device__ __forceinline__ CutUnit cut_of(const AttendParams &p, const Walk &k, 
     return cut;
 }
 
-// out of the rows of units that were cut: one warp per row at a time, the pieces in order.
-// `next` CTAs lie between a stretch and the one after it.
+// out of the rows of units that were cut, the pieces in order; `next` CTAs lie between a stretch and
+// the one after it. Units of many rows are cut into few pieces: a warp per row. Units of few rows can
+// be cut into many (a long context on all SMs): a block per row, its warps taking every fourth piece.
+// The factors come first, their loads together: a loop that loaded each piece's maximum before its
+// row took 26 us for 37 pieces.
 template <typename T, int ROWS>
 __global__ void __launch_bounds__(128) paged_combine_units_kernel(const __grid_constant__ AttendParams p, const int next) {
+    constexpr int WARPS = ROWS > 64 ? 1 : 4;  // that share a row
+    __shared__ float4 sum[WARPS][32];
+    __shared__ float warp_l[WARPS];
+    const int c = (int)blockIdx.x, lane = (int)(threadIdx.x & 31), warp = (int)(threadIdx.x >> 5);
+    const int share = WARPS > 1 ? warp : 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int c = (int)blockIdx.x, lane = (int)(threadIdx.x & 31);
     const CutUnit cut = p.cut[c];
     if (cut.pieces < 2) return;
     int start, nq, n;
     load_sequence(p, cut.b, start, nq, n);
     const int rows = nq * p.group;
-    for (int r = (int)blockIdx.y * 4 + (int)(threadIdx.x >> 5); r < ROWS; r += (int)gridDim.y * 4) {
+    const int r0 = WARPS > 1 ? (int)blockIdx.y : (int)blockIdx.y * 4 + warp, step = (int)gridDim.y * (4 / WARPS);
+    for (int r = r0; r < ROWS; r += step) {
         const int row = cut.t * ROWS + r;
         if (row >= rows) break;
         auto at = [&](int i) { return ((long long)(c + i * next) * 2 + (i == 0 ? 1 : 0)) * ROWS + r; };
@@ -215,29 +223,53 @@ __global__ void __launch_bounds__(128) paged_combine_units_kernel(const __grid_c
         for (int i = lane; i < cut.pieces; i += 32) m = fmaxf(m, p.part_ml[at(i)].x);
 #pragma unroll
         for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));
-        for (int d = lane * 4; d < p.head_dim; d += 128) {
+        T *out = static_cast<T *>(p.out) + (long long)(start + row / p.group) * p.o_ts +
+                 (long long)(cut.h * p.group + row % p.group) * p.o_hs;
+        for (int d0 = 0; d0 < p.head_dim; d0 += 128) {
+            const int d = d0 + lane * 4;
+            const bool mine = d < p.head_dim;
             float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             l = 0.0f;
-#pragma unroll 4
-            for (int i = 0; i < cut.pieces; ++i) {
-                const float2 ml = p.part_ml[at(i)];
-                const float4 v = *reinterpret_cast<const float4 *>(p.part + at(i) * p.head_dim + d);
-                const float f = ml.y == 0.0f ? 0.0f : ex2(ml.x - m);
+            for (int i0 = 0; i0 < cut.pieces; i0 += 32 * WARPS) {
+                // lane k holds the factor of this warp's k-th piece of the batch
+                const int i = i0 + lane * WARPS + share;
+                const float2 ml = i < cut.pieces ? p.part_ml[at(i)] : make_float2(0.0f, 0.0f);
+                const float f = ml.y > 0.0f ? ex2(ml.x - m) : 0.0f;
                 l += f * ml.y;
-                a.x += f * v.x;
-                a.y += f * v.y;
-                a.z += f * v.z;
-                a.w += f * v.w;
+                const int count = min(32, (cut.pieces - i0 - share + WARPS - 1) / WARPS);
+#pragma unroll 8
+                for (int k = 0; k < count; ++k) {
+                    const float g = __shfl_sync(0xFFFFFFFFu, f, k);
+                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (mine) v = *reinterpret_cast<const float4 *>(p.part + at(i0 + k * WARPS + share) * p.head_dim + d);
+                    a.x += g * v.x;
+                    a.y += g * v.y;
+                    a.z += g * v.z;
+                    a.w += g * v.w;
+                }
             }
+#pragma unroll
+            for (int x = 16; x; x >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, x);
+            if constexpr (WARPS > 1) {
+                sum[warp][lane] = a;
+                if (lane == 0) warp_l[warp] = l;
+                __syncthreads();
+                if (warp == 0) {
+                    l = (warp_l[0] + warp_l[1]) + (warp_l[2] + warp_l[3]);
+                    const float4 x = sum[1][lane], y = sum[2][lane], z = sum[3][lane];
+                    a = make_float4((a.x + x.x) + (y.x + z.x), (a.y + x.y) + (y.y + z.y), (a.z + x.z) + (y.z + z.z),
+                                    (a.w + x.w) + (y.w + z.w));
+                }
+                __syncthreads();
+            }
+            if (!mine || (WARPS > 1 && warp)) continue;
             const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-            T *out = static_cast<T *>(p.out) + (long long)(start + row / p.group) * p.o_ts +
-                     (long long)(cut.h * p.group + row % p.group) * p.o_hs + d;
             Pack<4, T> v;
             v.e[0] = from_f<T>(a.x * inv);
             v.e[1] = from_f<T>(a.y * inv);
             v.e[2] = from_f<T>(a.z * inv);
             v.e[3] = from_f<T>(a.w * inv);
-            v.store(out);
+            v.store(out + d);
         }
     }
 }

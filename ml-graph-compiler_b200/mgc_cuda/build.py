@@ -4,7 +4,8 @@ The counterpart of the reference's C build driver (``codegen/build.py:129-209``)
 ``$MGC_NVCC``, else ``nvcc`` on the PATH, else ``/usr/local/cuda/bin/nvcc``; the library is
 rebuilt only when the hash of the sources and flags changes (the key is stored next to the
 library), and written atomically. Unlike the C backend there is one library for every model:
-a model is data (a launch list and a weights blob), not generated source.
+a model is data (a launch list and a weights blob), not generated source. The paged-cache operators'
+torch binding is a second, small module (``build_binding``).
 """
 
 from __future__ import annotations
@@ -53,6 +54,11 @@ def sources() -> list[Path]:
     return sorted([*SRC_DIR.glob("*.cu"), *SRC_DIR.glob("*.cuh"), *INCLUDE_DIR.glob("*.h")])
 
 
+def binding_path() -> Path:
+    """The torch binding of the paged-cache operators, a Python extension module."""
+    return LIB_DIR / "_mgc_paged.so"
+
+
 def source_key(flags: list[str]) -> str:
     h = hashlib.sha256()
     for path in sources():
@@ -89,7 +95,7 @@ def _run(cmd: list[str], verbose: bool) -> None:
         print(" ".join(cmd))
     proc = subprocess.run(cmd, capture_output=True, text=True, check=False)
     if proc.returncode != 0:
-        raise CodegenError(f"nvcc failed:\n{' '.join(cmd)}\n{proc.stderr[-6000:]}")
+        raise CodegenError(f"{Path(cmd[0]).name} failed:\n{' '.join(cmd)}\n{proc.stderr[-6000:]}")
     if verbose and proc.stderr:
         print(proc.stderr[-6000:])
 
@@ -127,5 +133,33 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     return lib
 
 
+def build_binding(force: bool = False, verbose: bool = False) -> Path:
+    """Compile the torch binding (csrc/paged_torch.cpp, host code) if it, the header or torch changed."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    source, out = SRC_DIR / "paged_torch.cpp", binding_path()
+    stamp = out.with_suffix(".key")
+    include = [*cpp_extension.include_paths(), sysconfig.get_path("include"), str(INCLUDE_DIR),
+               str(Path(find_nvcc()).resolve().parents[1] / "include")]
+    libs = cpp_extension.library_paths()
+    flags = ["-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+             *(f"-I{p}" for p in include)]
+    key = _object_key(source, [*flags, torch.__version__, sysconfig.get_python_version()])
+    if not force and out.exists() and stamp.exists() and stamp.read_text().strip() == key:
+        return out
+    LIB_DIR.mkdir(parents=True, exist_ok=True)
+    tmp = out.with_name(f"{out.name}.tmp{os.getpid()}")
+    cxx = os.environ.get("MGC_CXX") or shutil.which("g++") or "g++"
+    _run([cxx, *flags, str(source), "-o", str(tmp), *(f"-L{p}" for p in libs), *(f"-Wl,-rpath,{p}" for p in libs),
+          "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"], verbose)
+    tmp.replace(out)
+    stamp.write_text(key + "\n")
+    return out
+
+
 if __name__ == "__main__":
     print(build(force=True, verbose=True))
+    print(build_binding(force=True, verbose=True))
