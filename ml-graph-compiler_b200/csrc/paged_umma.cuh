@@ -30,12 +30,6 @@
 #include "paged_mma.cuh"
 #include "umma_ptx.cuh"
 
-#ifndef MGC_POLY
-#define MGC_POLY 0
-#endif
-#ifndef MGC_WAITK
-#define MGC_WAITK "try_wait"
-#endif
 namespace mgc {
 namespace paged {
 
@@ -65,7 +59,11 @@ template <int DP> struct UmmaConfig {
     // 256 x 224 + 128 x 56
     static constexpr int THREADS = 384;
     static constexpr int SOFTMAX_REGS = 224, OTHER_REGS = 56;
-    static constexpr uint32_t S_COL = 0, O_COL = 256; // TMEM columns: S0 S1 O0 O1
+    // TMEM columns: S0 S1 O0 O1, the weights of a tile over its scores; with 64 channels there is room
+    // for weights of their own (S0 S1 P0 P1 O0 O1), so the next tile's scores are made while this
+    // one's weights are
+    static constexpr bool APART = DP == 64;
+    static constexpr uint32_t S_COL = 0, P_COL = APART ? 256 : 0, P_STEP = APART ? 64 : 128, O_COL = APART ? 384 : 256;
 };
 
 // D = A B with A in TMEM (16-bit values packed in pairs along K) or shared memory.
@@ -129,30 +127,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
-// 2^x for x <= 2^7 on the FMA pipe: x = n + f, n the nearest whole number (taken from the low bits of
-// x + 1.5 * 2^23), 2^f by the polynomial of least largest relative error on [-1/2, 1/2] (found by
-// exchange: 7.5e-5 of degree 3, 2.7e-6 of degree 4, below the rounding of the weights to bf16 and
-// f16), n added to the exponent field. Below 2^-126 it stays at 2^-126.
-template <typename T> __device__ __forceinline__ float2 exp2_poly(float2 x) {
-    constexpr float MAGIC = 12582912.0f;
-    x.x = fmaxf(x.x, -126.0f);
-    x.y = fmaxf(x.y, -126.0f);
-    const float2 t = add2(x, make_float2(MAGIC, MAGIC)), n = add2(t, make_float2(-MAGIC, -MAGIC));
-    const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
-    float2 e;
-    if (std::is_same<T, __nv_bfloat16>::value) {
-        e = fma2(f, make_float2(5.517166853e-02f, 5.517166853e-02f), make_float2(2.426111251e-01f, 2.426111251e-01f));
-        e = fma2(e, f, make_float2(6.932609677e-01f, 6.932609677e-01f));
-        e = fma2(e, f, make_float2(9.999280572e-01f, 9.999280572e-01f));
-    } else {
-        e = fma2(f, make_float2(9.570102207e-03f, 9.570102207e-03f), make_float2(5.591785908e-02f, 5.591785908e-02f));
-        e = fma2(e, f, make_float2(2.402474433e-01f, 2.402474433e-01f));
-        e = fma2(e, f, make_float2(6.931217909e-01f, 6.931217909e-01f));
-        e = fma2(e, f, make_float2(9.999992847e-01f, 9.999992847e-01f));
-    }
-    return make_float2(__int_as_float(__float_as_int(e.x) + (__float_as_int(t.x) << 23)),
-                       __int_as_float(__float_as_int(e.y) + (__float_as_int(t.y) << 23)));
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -165,7 +139,7 @@ __device__ __forceinline__ bool poll(uint32_t e, uint64_t *bar, uint32_t parity)
     uint32_t done;
     asm volatile(
         "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %3, 0;\n\tsetp.ne.b32 p, 0, 0;\n\t"
-        "@q mbarrier." MGC_WAITK ".parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+        "@q mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
         : "=r"(done) : "r"(smem_addr(bar)), "r"(parity), "r"(e) : "memory");
     return __any_sync(0xFFFFFFFFu, done != 0);
 }
@@ -215,9 +189,8 @@ template <typename T, int DP>
 __global__ void __launch_bounds__(UmmaConfig<DP>::THREADS, 1)
 paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid_constant__ UmmaMaps maps) {
     using C = UmmaConfig<DP>;
-    constexpr int POLY = MGC_POLY;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t full[C::STAGES], empty[C::STAGES], q_full[2], s_full[2], p_half[2], p_full[2], o_full[2];
+    __shared__ __align__(8) uint64_t full[C::STAGES], empty[C::STAGES], q_full[2], s_full[2], s_free[2], p_half[2], p_full[2], p_free[2], o_full[2];
     __shared__ __align__(8) uint64_t z_ask, z_done;
     __shared__ uint32_t tslot;
     __shared__ Walk stretch;
@@ -232,6 +205,8 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
         for (int x = 0; x < 2; ++x) {
             mbar_init(&q_full[x], 4);
             mbar_init(&s_full[x], 1);
+            mbar_init(&s_free[x], 4);
+            mbar_init(&p_free[x], 1);
             mbar_init(&p_half[x], 4);
             mbar_init(&p_full[x], 4);
             mbar_init(&o_full[x], 1);
@@ -368,8 +343,14 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         if (!ok || j >= (x ? need1 : need0)) continue;
-                        const uint32_t o = tb + C::O_COL + x * DP, w16 = tb + C::S_COL + x * 128;
+                        const uint32_t o = tb + C::O_COL + x * DP, w16 = tb + C::P_COL + x * C::P_STEP;
                         uint32_t &phase = x ? phase1 : phase0;
+                        if (C::APART && j + 1 < (x ? need1 : need0)) {
+                            ok = wait(&s_free[x], phase);
+                            if (!ok) continue;
+                            tc_fence_after();
+                            scores(x, ks);
+                        }
                         ok = wait(&p_half[x], phase);
                         if (!ok) continue;
                         tc_fence_after();
@@ -381,8 +362,9 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                         tc_fence_after();
 #pragma unroll
                         for (int kk = 4; kk < 8; ++kk) mma_f16_ts(e, o, w16 + kk * 8, v + kk * (2048 >> 4), id_o, 1);
-                        if (j + 1 < (x ? need1 : need0)) scores(x, ks);
-                        else commit_if(e, &o_full[x]);
+                        if (j + 1 >= (x ? need1 : need0)) commit_if(e, &o_full[x]);
+                        else if (C::APART) commit_if(e, &p_free[x]);
+                        else scores(x, ks);
                     }
                     if (ok) {
                         commit_if(e, &empty[vs]);
@@ -431,7 +413,8 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
         const int x = warp >> 2, r = tid & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tbase + lanes + C::S_COL + x * 128, to = tbase + lanes + C::O_COL + x * DP;
-        uint32_t s_phase = 0, o_phase = 0;
+        const uint32_t tp = tbase + lanes + C::P_COL + x * C::P_STEP;
+        uint32_t s_phase = 0, o_phase = 0, free_phase = 0;
         bool ok = true;
         while (ok && next_item<256, 128>(p, walk, w)) {
             const int row = w.row0 + x * 128 + r;
@@ -479,6 +462,11 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                     for (int i = 0; i < 32; ++i) s[c * 32 + i] = __uint_as_float(t[i]);
                 }
                 umma::tmem_wait_ld();
+                if (C::APART) {  // the next tile's scores may take this one's place
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&s_free[x]);
+                }
                 const int key0 = w.lo + j * 128;
                 const bool edge = __any_sync(0xFFFFFFFFu, live && (key0 < see.lo || key0 + 128 > see.hi));
                 if (edge) {
@@ -498,6 +486,12 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                 const float mt = __fmul_rn(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), p.scale_log2);
                 // grown by more than 2^8 (or the first finite maximum): move the reference
                 const bool grow = mt > m + 8.0f;
+                if (C::APART && j > 0) {  // the products with the last tile's weights are done
+                    ok = wait(&p_free[x], free_phase);
+                    free_phase ^= 1u;
+                    if (!ok) break;
+                    tc_fence_after();
+                }
                 if (j > 0 && __any_sync(0xFFFFFFFFu, grow)) {
                     const float f = grow ? ex2(m - mt) : 1.0f;
                     l *= f;
@@ -515,31 +509,22 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                 const float y = m == -INFINITY ? 0.0f : m;
                 const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), y2 = make_float2(-y, -y);
                 float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-                // POLY of every 8 pairs by the polynomial: the exponential unit alone would bound the tile
-                auto weights = [&](auto poly) {
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {  // the first 64 keys' products start while the others' weights are made
+                for (int c = 0; c < 2; ++c) {  // the first 64 keys' products start while the others' weights are made
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            float2 z = fma2(make_float2(s[c * 64 + 2 * i], s[c * 64 + 2 * i + 1]), scale2, y2);
-                            if ((i & 7) < decltype(poly)::value) {
-                                z = exp2_poly<T>(z);
-                            } else {
-                                z.x = ex2(z.x);
-                                z.y = ex2(z.y);
-                            }
-                            sum[i & 1] = add2(sum[i & 1], z);
-                            t[i] = pack2<T>(z.x, z.y);
-                        }
-                        tmem_st32(ts + c * 32, t);
-                        tmem_wait_st();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(c ? &p_full[x] : &p_half[x]);
+                    for (int i = 0; i < 32; ++i) {
+                        float2 z = fma2(make_float2(s[c * 64 + 2 * i], s[c * 64 + 2 * i + 1]), scale2, y2);
+                        z.x = ex2(z.x);
+                        z.y = ex2(z.y);
+                        sum[i & 1] = add2(sum[i & 1], z);
+                        t[i] = pack2<T>(z.x, z.y);
                     }
-                };
-                if (edge) weights(std::integral_constant<int, 0>{});  // masked scores: exact zeros
-                else weights(std::integral_constant<int, POLY>{});
+                    tmem_st32(tp + c * 32, t);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(c ? &p_full[x] : &p_half[x]);
+                }
                 sum[0] = add2(sum[0], sum[1]);
                 l += sum[0].x + sum[0].y;
             }
