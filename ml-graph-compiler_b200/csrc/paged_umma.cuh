@@ -309,16 +309,21 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
             };
             while (ok && next_item<256, 128>(p, walk, w)) {
                 const int need0 = tiles_needed(p, w, 0), need1 = tiles_needed(p, w, 1);
-                ok = wait(&q_full[0], q_phase) && wait(&q_full[1], q_phase);
+                // the first scores of each row tile as soon as its queries are there
+                if (w.tiles > 0) ok = wait(&full[slot], lap);
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    ok = ok && wait(&q_full[x], q_phase);
+                    tc_fence_after();
+                    if (ok && (x ? need1 : need0) > 0) scores(x, slot);
+                    // a warpgroup whose rows see nothing here waits all the same: it must not be two
+                    // items ahead, where q_full's parity would say the opposite
+                    else if (ok && lane == 0) mbar_arrive(&o_full[x]);
+                    __syncwarp();
+                }
                 q_phase ^= 1u;
                 if (ok && w.tiles > 0) {
-                    ok = wait(&full[slot], lap);
-                    tc_fence_after();
-                    if (ok) {
-                        if (need0 > 0) scores(0, slot);
-                        if (need1 > 0) scores(1, slot);
-                        commit_if(e, &empty[slot]);
-                    }
+                    commit_if(e, &empty[slot]);
                     step();
                 }
                 for (int j = 0; ok && j < w.tiles; ++j) {
@@ -468,12 +473,22 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                     if (lane == 0) mbar_arrive(&s_free[x]);
                 }
                 const int key0 = w.lo + j * 128;
-                const bool edge = __any_sync(0xFFFFFFFFu, live && (key0 < see.lo || key0 + 128 > see.hi));
-                if (edge) {
-                    const int from = see.lo - key0, to_ = see.hi - key0;
+                if (__any_sync(0xFFFFFFFFu, live && (key0 < see.lo || key0 + 128 > see.hi))) {
+                    // only the 32-key slices that some row of the warp does not see whole
+                    const int from = live ? see.lo - key0 : 0, to_ = live ? see.hi - key0 : 128;
 #pragma unroll
-                    for (int i = 0; i < 128; ++i)
-                        if (i < from || i >= to_) s[i] = -INFINITY;
+                    for (int c = 0; c < 4; ++c) {
+                        if (__any_sync(0xFFFFFFFFu, to_ < c * 32 + 32)) {
+#pragma unroll
+                            for (int i = c * 32; i < c * 32 + 32; ++i)
+                                if (i >= to_) s[i] = -INFINITY;
+                        }
+                        if (__any_sync(0xFFFFFFFFu, from > c * 32)) {
+#pragma unroll
+                            for (int i = c * 32; i < c * 32 + 32; ++i)
+                                if (i < from) s[i] = -INFINITY;
+                        }
+                    }
                 }
                 float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
@@ -528,11 +543,9 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                 sum[0] = add2(sum[0], sum[1]);
                 l += sum[0].x + sum[0].y;
             }
-            if (need > 0) {
-                ok = ok && wait(&o_full[x], o_phase);
-                o_phase ^= 1u;
-                tc_fence_after();
-            }
+            ok = ok && wait(&o_full[x], o_phase);
+            o_phase ^= 1u;
+            tc_fence_after();
             if (!ok) break;
             // ---- O: through the warp's rows of the Q tile (no longer read) to whole rows of memory ----
             const bool whole = w.slot < 0;

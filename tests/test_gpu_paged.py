@@ -90,6 +90,16 @@ def test_ragged_batches(dtype: str, qs: list[int], ks: list[int], causal: bool) 
         agree(PagedBatch(qs, ks, heads=4, kv_heads=kv_heads, dim=dim, page=16, dtype=dtype), causal=causal)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_short_sequences_beside_a_chunk(dtype: str, dim: int) -> None:
+    """One chunk and hundreds of single tokens: a block of the tcgen05 kernel walks many units whose
+    second row tile is empty, so its second warpgroup has nothing to wait for but the next unit."""
+    qs = [300, *[1] * 500, 0, 129, *[2] * 100]
+    ks = [400, *[1 + (37 * b) % 290 for b in range(500)], 5, 129, *[2 + (11 * b) % 40 for b in range(100)]]
+    agree(PagedBatch(qs, ks, heads=2, kv_heads=2, dim=dim, page=16, dtype=dtype))
+
+
 @pytest.mark.parametrize("dtype", ALL)
 @pytest.mark.parametrize("window", [1, 2, 16, 100, 128, 1000, 5000])
 def test_windows(dtype: str, window: int) -> None:
