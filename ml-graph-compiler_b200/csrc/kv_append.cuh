@@ -5,12 +5,12 @@
 // are row p of the tables: x1' = x1 c - x2 s, x2' = x2 c + x1 s, in fp32, rounded once.
 //
 // Every value is read once and written once and the arithmetic is three operations per rotated
-// value, so memory bounds it (latency for a few tokens). A block takes one token: its warps find
-// the sequence with one ballot per 32 sequences, then each thread moves units of V channels of a
-// head (16 bytes), a rotated unit being the two chunks whose channels pair up, so that each pair
-// is read and written by one thread and q may be rotated in place. A thread's units are the same
-// channels of several heads, so it reads its angles once; its first sources load while the block
-// looks up the token's place.
+// value, so memory bounds it (latency for a few tokens). A block takes a run of consecutive tokens:
+// its warps find a sequence with one ballot per 32 sequences and count on from there, looking up a
+// page where one begins. Each thread moves units of V channels of a head (16 bytes), a rotated unit
+// being the two chunks whose channels pair up, so that each pair is read and written by one thread
+// and q may be rotated in place. A thread's units are the same channels of several heads, so it
+// reads a token's angles once.
 #pragma once
 
 #include "paged_common.cuh"
@@ -30,6 +30,7 @@ struct AppendParams {
     int positions, rot, interleaved;
     int q_heads, kv_heads, head_dim;
     int threads;  // that work: a multiple of units
+    int tokens, per_block;
     int units;    // per head: rot / 2V rotated pairs of chunks, then (head_dim - rot) / V plain chunks
 };
 
@@ -46,20 +47,22 @@ template <typename S, typename T, int V> struct Unit {
     Pack<V, S> x, y;
 };
 
+// Blocks an SM holds, by registers: 4 (64 registers) ran 19466 tokens of 48 heads x 128 bf16 in 84 us,
+// 5 to 8 (spills) in 124 to 247 us, unbounded (85 registers) in 138 us. The wide fp32 units need more.
+template <typename S, int V> constexpr int RESIDENT = V * (int)sizeof(S) > 16 ? 2 : 4;
+
 template <typename S, typename T, int V>
-__global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(256, RESIDENT<S, V>) kv_append_kernel(const __grid_constant__ AppendParams p) {
     constexpr int BATCH = 2;
-    const int t = (int)blockIdx.x;
-    // thread (w, h0) takes unit w of heads h0, h0 + step, ...: its angles are the same for all of them
+    const int t0 = (int)blockIdx.x * p.per_block, t1 = min(t0 + p.per_block, p.tokens);
+    // thread (w, h0) takes unit w of heads h0, h0 + step, ...
     const int h0 = (int)threadIdx.x / p.units, w = (int)threadIdx.x - h0 * p.units, step = p.threads / p.units;
     const int heads = p.q_heads + 2 * p.kv_heads, pairs = p.rot / (2 * V);
-    const bool pair = w < pairs;
+    const bool pair = w < pairs, active = (int)threadIdx.x < p.threads;
     const int c0 = !pair ? p.rot + (w - pairs) * V : p.interleaved ? w * 2 * V : w * V;
     const int c1 = p.interleaved ? c0 + V : c0 + p.rot / 2;
-    Unit<S, T, V> u[BATCH];
-    // the sources' addresses need no lookup: their loads overlap the search for the token's place
-    auto load = [&](Unit<S, T, V> &z, int h) {
-        if (h >= heads) return;
+    auto load = [&](Unit<S, T, V> &z, int t, int h) {
+        if (h >= heads || !active) return;
         const S *src;
         if (h < p.q_heads) {
             src = static_cast<const S *>(p.q) + t * p.q_ts + h * p.q_hs;
@@ -71,39 +74,17 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ 
         z.x.load(src + c0);
         if (pair) z.y.load(src + c1);
     };
-    const bool active = (int)threadIdx.x < p.threads;
-    if (active) {
-#pragma unroll
-        for (int i = 0; i < BATCH; ++i) load(u[i], h0 + i * step);
-    }
-
-    const int b = sequence_of(p.batch, t);
-    if (b < 0) return;
-    const int end = __ldg(p.batch.q_starts + b + 1);
-    if (t >= end || !active) return;  // past the last sequence
-    const int pos = __ldg(p.batch.kv_lens + b) - (end - t);
-    int page = -1;
-    if (pos >= 0) page = page_of(p.batch, b, pos / p.batch.page_size);
-    bool turn = pos >= 0 && p.rot > 0;
-    if (turn && pos >= p.positions) {
-        if (p.batch.status) *p.batch.status = MGC_CUDA_GATHER_OOB;
-        turn = false;
-        page = -1;
-    }
-    const long long slot = page < 0 ? 0 : (long long)page * p.page_stride + (long long)(pos % p.batch.page_size) * p.token_stride;
+    // the place of token t: looked up where a sequence or a page begins, counted on in between
+    int b = -1, end = t0, n = 0, page = -1, held = -1;
     float c[V], s[V];
-    if (turn && pair) {
-        load_angles<V>(p.cos + (long long)pos * p.table_row + w * V, c);
-        load_angles<V>(p.sin + (long long)pos * p.table_row + w * V, s);
-    }
-    auto finish = [&](Unit<S, T, V> &z, int h) {
-        if (h >= heads) return;
+    auto finish = [&](Unit<S, T, V> &z, int t, int h, bool turn, long long slot) {
+        if (h >= heads || !active) return;
         T *dst;
         bool rotate = turn;
         if (h < p.q_heads) {
             dst = static_cast<T *>(p.q_out) + t * p.qo_ts + h * p.qo_hs;
         } else {
-            if (page < 0) return;
+            if (slot < 0) return;
             h -= p.q_heads;
             rotate = rotate && h < p.kv_heads;
             dst = static_cast<T *>(h < p.kv_heads ? p.k_pages : p.v_pages) + slot + (h < p.kv_heads ? h : h - p.kv_heads) * p.head_stride;
@@ -146,13 +127,49 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ 
         ox.store(dst + c0);
         oy.store(dst + c1);
     };
-    for (int h = h0;;) {
+    auto place = [&](Unit<S, T, V> (&u)[BATCH], int t) {
+        if (t >= end) {
+            b = sequence_of(p.batch, t);
+            if (b < 0) return;
+            end = __ldg(p.batch.q_starts + b + 1);
+            n = __ldg(p.batch.kv_lens + b);
+            held = -1;
+        }
+        if (b < 0 || t >= end) return;  // outside every sequence
+        const int pos = n - (end - t);
+        if (pos >= 0 && (held < 0 || pos / p.batch.page_size != held)) {
+            held = pos / p.batch.page_size;
+            page = page_of(p.batch, b, held);
+        }
+        bool turn = pos >= 0 && p.rot > 0;
+        long long slot = pos < 0 || page < 0
+                             ? -1
+                             : (long long)page * p.page_stride + (long long)(pos - held * p.batch.page_size) * p.token_stride;
+        if (turn && pos >= p.positions) {
+            if (p.batch.status) *p.batch.status = MGC_CUDA_GATHER_OOB;
+            turn = false;
+            slot = -1;
+        }
+        if (turn && pair) {
+            load_angles<V>(p.cos + (long long)pos * p.table_row + w * V, c);
+            load_angles<V>(p.sin + (long long)pos * p.table_row + w * V, s);
+        }
+        for (int h = h0;;) {
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) finish(u[i], h + i * step);
-        h += BATCH * step;
-        if (h >= heads) break;
+            for (int i = 0; i < BATCH; ++i) finish(u[i], t, h + i * step, turn, slot);
+            h += BATCH * step;
+            if (h >= heads) break;
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) load(u[i], h + i * step);
+            for (int i = 0; i < BATCH; ++i) load(u[i], t, h + i * step);
+        }
+    };
+    // a token's sources load while its place is found (the next token's in a second set of registers
+    // left fewer blocks on an SM: 144 us)
+    Unit<S, T, V> u[BATCH];
+    for (int t = t0; t < t1; ++t) {
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) load(u[i], t, h0 + i * step);
+        place(u, t);
     }
 }
 
@@ -162,7 +179,10 @@ template <typename S, typename T, int V> inline int run_append(AppendParams &p, 
     if (p.units > 256) return fail(MGC_CUDA_UNSUPPORTED, "mgc_cuda_kv_append: %d channels in units of %d", p.head_dim, V);
     // whole heads of units, at most 256 threads
     p.threads = (heads < 256 / p.units ? heads : 256 / p.units) * p.units;
-    kv_append_kernel<S, T, V><<<(unsigned)tokens, (unsigned)ceil_div(p.threads, 32) * 32, 0, stream>>>(p);
+    // runs of consecutive tokens, as many as the GPU holds blocks
+    p.tokens = tokens;
+    p.per_block = (int)ceil_div(tokens, (int64_t)sm_count() * RESIDENT<S, V>);
+    kv_append_kernel<S, T, V><<<(unsigned)ceil_div(tokens, p.per_block), (unsigned)ceil_div(p.threads, 32) * 32, 0, stream>>>(p);
     return check_launch("kv_append_kernel");
 }
 
