@@ -16,11 +16,19 @@
 // fresh fp32 accumulator per tile that is added to the running one in fp32: the instruction
 // truncates its sums, and a chain over the whole context would shrink the output by ~1e-8 per step.
 //
+// fp32 with few rows per key head (SIMT): the split products would cost the same for 1 row as for 16;
+// up to 8 rows go through the FMA units instead, a key per lane for the scores and channels per lane
+// for the output.
+//
 // When there are fewer units (row tiles of a sequence and key head) than the SMs hold CTAs, up to 8
 // CTAs of a cluster take equal parts of a unit's keys and add their partial results through
 // distributed shared memory. Else, or when 8 are not enough, every CTA takes an even share of all
 // units' keys and pieces go through a workspace (paged_work.cuh). Partial sums are added in a fixed
 // order, so a call repeats its bits.
+//
+// Decoding is bound by memory: 64 sequences of 8 key heads x 128 up to 8192 positions, bf16, 1.32 GB
+// in ~240 us (5.5 TB/s, 85 % of the copy bandwidth); one of 131071 positions 98 us (5.5 TB/s); 16 GPT-2
+// sequences up to 1024 positions, fp32, 22 us (3.2 TB/s: two launches and the blocks' start are half).
 #pragma once
 
 #include "paged_work.cuh"
