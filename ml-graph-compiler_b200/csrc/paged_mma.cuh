@@ -155,12 +155,21 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
         const RowRange first = row_range(p, n, nq, row0), last = row_range(p, n, nq, min(row0 + R, rows) - 1);
         const int all_lo = last.lo, all_hi = first.hi;
 
-        // byte offset (of K and V alike) of key j of this thread's stage row, or -1: not loaded
-        auto offset_of = [&](int j) -> long long {
+        // Byte offset (of K and V alike) of key j of this thread's stage row, or -1: not loaded. In two
+        // halves, the table's entry fetched a stage's work before it is looked at.
+        const int ps = p.batch.page_size;
+        auto fetch_page = [&](int j) {
+            const int at = j / ps;
+            return j < k_hi && j >= first.lo && at < p.batch.table_pages
+                       ? __ldg(p.batch.table + (long long)b * p.batch.table_stride + at) : -1;
+        };
+        auto offset_of = [&](int j, int page) -> long long {
             if (j >= k_hi || j < first.lo) return -1;
-            const int page = page_of(p.batch, b, j / p.batch.page_size);
-            if (page < 0) return -1;
-            return ((long long)page * p.page_stride + (long long)(j % p.batch.page_size) * p.token_stride) * (long long)sizeof(T);
+            if (page < 0 || page >= p.batch.pages) {
+                if (p.batch.status) *p.batch.status = MGC_CUDA_GATHER_OOB;
+                return -1;
+            }
+            return ((long long)page * p.page_stride + (long long)(j % ps) * p.token_stride) * (long long)sizeof(T);
         };
         auto load_stage = [&](int it) {
             uint8_t *st = ring + (it % C::STAGES) * C::STAGE;
@@ -224,7 +233,7 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
         }
 
         // the first stages; a stage's offsets are looked up well before its loads
-        for (int x = tid; x < C::STAGES * BN; x += C::THREADS) sOff[x] = offset_of(k_lo + x);
+        for (int x = tid; x < C::STAGES * BN; x += C::THREADS) sOff[x] = offset_of(k_lo + x, fetch_page(k_lo + x));
         __syncthreads();
 #pragma unroll
         for (int it = 0; it < C::STAGES - 1; ++it) {
@@ -237,8 +246,8 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
             __syncthreads();
             if (it + C::STAGES - 1 < tiles) load_stage(it + C::STAGES - 1);
             cp_async_commit();
-            long long next = -1;  // the slot of this stage's own offsets is free
-            if (tid < BN) next = offset_of(k_lo + (it + C::STAGES) * BN + tid);
+            const int j_next = k_lo + (it + C::STAGES) * BN + tid;
+            const int page_next = tid < BN ? fetch_page(j_next) : -1;
 
             const uint8_t *st = ring + (it % C::STAGES) * C::STAGE;
             if constexpr (SIMT > 0) {
@@ -502,7 +511,8 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
                 }
             }
             }
-            if (tid < BN) sOff[(it % C::STAGES) * BN + tid] = next;
+            // the slot of this stage's own offsets is free
+            if (tid < BN) sOff[(it % C::STAGES) * BN + tid] = offset_of(j_next, page_next);
         }
         cp_async_wait<0>();
         __syncthreads();
