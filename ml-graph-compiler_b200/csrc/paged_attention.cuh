@@ -100,7 +100,7 @@ inline int ctas_per_sm(int64_t dtype, int64_t head_dim, int wm, int simt) {
     const int dp = head_dim <= 32 ? 32 : head_dim <= 64 ? 64 : head_dim <= 96 ? 96 : head_dim <= 128 ? 128 : 256;
     const bool f32 = dtype == MGC_F32;
     const int keys = !f32 ? 64 : !simt ? 32 : dp <= 32 ? 128 : dp <= 64 ? 64 : 32;
-    const int row = dp * (f32 ? 4 : 2) + 16, ring = (dp > 128 ? 2 : 3) * 2 * keys * row;
+    const int row = dp * (f32 ? 4 : 2) + 16, ring = (dp > 128 || simt ? 2 : 3) * 2 * keys * row;
     const int bytes = ring + (!f32 && dp <= 128 ? 0 : (simt ? simt : 16 * wm) * row) + 3 * keys * 8 + 1024;
     const int fit = 232448 / bytes;
     return fit < 1 ? 1 : fit > 4 ? 4 : fit;

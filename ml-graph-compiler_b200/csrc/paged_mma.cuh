@@ -27,8 +27,8 @@
 // order, so a call repeats its bits.
 //
 // Decoding is bound by memory: 64 sequences of 8 key heads x 128 up to 8192 positions, bf16, 1.32 GB
-// in ~240 us (5.5 TB/s, 85 % of the copy bandwidth); one of 131071 positions 98 us (5.5 TB/s); 16 GPT-2
-// sequences up to 1024 positions, fp32, 22 us (3.2 TB/s: two launches and the blocks' start are half).
+// in ~227 us (5.8 TB/s, 90 % of the copy bandwidth); one of 131071 positions 98 us (5.5 TB/s); 16 GPT-2
+// sequences up to 1024 positions, fp32, 21 us (3.4 TB/s: two launches and the blocks' start are half).
 #pragma once
 
 #include "paged_work.cuh"
@@ -116,7 +116,8 @@ template <typename T, int DP, int WM, int WN, int SIMT> struct MmaConfig {
     static constexpr int BN = SIMT ? WN * 32 / PARTS : F32 ? 32 : 64;  // keys per stage
     static constexpr int KW = BN / WN;               // of them, a warp's
     static constexpr int KG = DP > 128 && KW > 32 ? 32 : KW;  // keys per softmax step (registers)
-    static constexpr int STAGES = DP > 128 ? 2 : 3;
+    // two for the plain form: more blocks an SM beat more stages a block (16 x 1024 fp32 24.8 -> 22.6 us)
+    static constexpr int STAGES = DP > 128 || SIMT ? 2 : 3;
     static constexpr int CH = 16 / (int)sizeof(T);   // elements of a 16-byte chunk
     static constexpr int ROW = DP * (int)sizeof(T) + 16;  // bytes of a padded K / V row
     static constexpr int STAGE = 2 * BN * ROW;
