@@ -27,7 +27,7 @@
 // order, so a call repeats its bits.
 //
 // Decoding is bound by memory: 64 sequences of 8 key heads x 128 up to 8192 positions, bf16, 1.32 GB
-// in ~227 us (5.8 TB/s, 90 % of the copy bandwidth); one of 131071 positions 98 us (5.5 TB/s); 16 GPT-2
+// in ~231 us (5.7 TB/s, 88 % of the copy bandwidth); one of 131071 positions 102 us (5.3 TB/s); 16 GPT-2
 // sequences up to 1024 positions, fp32, 21 us (3.4 TB/s: two launches and the blocks' start are half).
 #pragma once
 
