@@ -42,14 +42,16 @@ class Pages:
         self.device = device
 
     def extend(self, new: list[int]) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-        """Room for ``new[b]`` more tokens of every sequence: (block_table, kv_lens, q_starts)."""
+        """Room for ``new[b]`` more tokens of every sequence: (block_table, kv_lens, q_starts). When there
+        are too few free pages it raises and nothing changes, so a caller can release a sequence and
+        try again."""
+        need = [-(-(n + old) // self.page_size) - len(own) for n, old, own in zip(new, self.lens, self.owned)]
+        if sum(need) > len(self.free):
+            raise RuntimeError("the cache has no free page")
         starts = [0]
         for b, n in enumerate(new):
             self.lens[b] += n
-            while len(self.owned[b]) * self.page_size < self.lens[b]:
-                if not self.free:
-                    raise RuntimeError("the cache has no free page")
-                self.owned[b].append(self.free.pop())
+            self.owned[b] += [self.free.pop() for _ in range(need[b])]
             starts.append(starts[-1] + n)
         width = max(1, max(len(p) for p in self.owned))
         table = [p + [0] * (width - len(p)) for p in self.owned]
