@@ -161,7 +161,10 @@ class Gpt2:
 
 def generate(model: Gpt2, prompts: list[list[int]], tokens: int, *, page_size: int = 16, chunk: int = 256) -> tuple[list[list[int]], list[float], torch.Tensor]:
     """Greedy continuation of every prompt by ``tokens`` tokens: (sequences, seconds of each step, the
-    last logits). Prompts are cached in chunks of at most ``chunk`` tokens a sequence."""
+    last logits). Prompts, of at least one token each, are cached in chunks of at most ``chunk`` tokens a
+    sequence."""
+    if not prompts or not all(prompts):
+        raise ValueError("every prompt needs a token")
     batch, dev = len(prompts), model.device
     need = sum(-(-(len(p) + tokens) // page_size) for p in prompts)
     pages, cache = Pages(need, page_size, batch, dev), model.cache(need, page_size)

@@ -22,3 +22,15 @@ def test_a_failed_extend_changes_nothing() -> None:
     assert lens.tolist() == [0, 17, 3] and starts.tolist() == [0, 0, 12, 15]
     used = [table[b, : -(-n // 16)].tolist() for b, n in enumerate(lens.tolist())]
     assert len(sum(used, [])) == len(set(sum(used, []))) == 3
+
+
+def test_empty_prompts_are_refused() -> None:
+    """A sequence without a token has no logits to go on from."""
+
+    class Untouched:
+        def __getattribute__(self, name: str):
+            raise AssertionError(f"{name} was used")
+
+    for prompts in ([[1, 2], []], [[]], []):
+        with pytest.raises(ValueError, match="prompt"):
+            generate.generate(Untouched(), prompts, 4)
