@@ -96,6 +96,7 @@ class Gpt2:
         return torch.cuda.current_stream(self.device).cuda_stream
 
     def _norm(self, x: torch.Tensor, ln: tuple[torch.Tensor, torch.Tensor]) -> torch.Tensor:
+        x = x.contiguous()  # a product's rows may be padded
         y = torch.empty_like(x)
         check(self.lib.mgc_cuda_layer_norm(x.shape[0], x.shape[1], x.data_ptr(), ln[0].data_ptr(), ln[1].data_ptr(), 1e-5,
                                            y.data_ptr(), self._stream()), "mgc_cuda_layer_norm", self.lib)
@@ -105,14 +106,15 @@ class Gpt2:
                  res: torch.Tensor | None = None) -> torch.Tensor:
         m, k = x.shape
         n = w.shape[0]
-        # TF32 rows are 16-byte aligned: the odd vocabulary's logits get padded rows
+        # rows of a multiple of 16 bytes, what TF32 takes: odd widths (the vocabulary's) get padded ones
         ldc = -(-n // 4) * 4
         y = torch.empty(m, ldc, device=x.device)
         precision = self.precision if n % 4 == 0 and k % 4 == 0 else FP32
-        check(self.lib.mgc_cuda_gemm(m, n, k, 1, x.data_ptr(), k, 1, 0, w.data_ptr(), 1, k, 0, y.data_ptr(), ldc, 0, 1.0,
+        check(self.lib.mgc_cuda_gemm(m, n, k, 1, x.data_ptr(), max(x.stride(0), k), 1, 0, w.data_ptr(), 1, k, 0,
+                                     y.data_ptr(), ldc, 0, 1.0,
                                      bias.data_ptr() if bias is not None else None, 1 if bias is not None else 0,
-                                     res.data_ptr() if res is not None else None, n, 0, 1.0, act, 0.0, 0.0, precision,
-                                     self._stream()), "mgc_cuda_gemm", self.lib)
+                                     res.data_ptr() if res is not None else None, res.stride(0) if res is not None else n, 0,
+                                     1.0, act, 0.0, 0.0, precision, self._stream()), "mgc_cuda_gemm", self.lib)
         return y[:, :n]
 
     def step(self, ids: torch.Tensor, new: list[int], pages: Pages, cache: list[tuple[torch.Tensor, torch.Tensor]],

@@ -40,3 +40,13 @@ def test_pages_are_reused_and_run_out() -> None:
 
 def test_the_command_checks_itself() -> None:
     assert generate.main(["--batch", "2", "--prompt", "40", "--tokens", "5", "--layers", "2", "--check"]) == 0
+
+
+@pytest.mark.parametrize("d,heads,vocab", [(66, 2, 101), (65, 5, 64), (60, 3, 99)])
+@pytest.mark.parametrize("precision,tol", [(generate.FP32, 1e-4), (generate.TF32, 2e-2)])
+def test_widths_that_are_no_multiple_of_four(d: int, heads: int, vocab: int, precision: int, tol: float) -> None:
+    model = generate.Gpt2(layers=2, d=d, heads=heads, vocab=vocab, max_pos=64, precision=precision)
+    out, _, logits = generate.generate(model, [list(range(1, 31)), [7]], 4, chunk=16)
+    for b, seq in enumerate(out):
+        want = model.plain(torch.tensor(seq[:-1], device="cuda"))[0]
+        assert float((logits[b].double() - want).abs().max()) <= tol
