@@ -20,8 +20,9 @@ __global__ void __launch_bounds__(128) paged_attention_row_kernel(const __grid_c
     const int end = __ldg(p.batch.q_starts + b + 1);
     if (t >= end) return;
     const int n = __ldg(p.batch.kv_lens + b);
+    if (n > p.max_positions && p.batch.status) *p.batch.status = MGC_CUDA_GATHER_OOB;
     int lo, hi;
-    visible(p, n, n - (end - t), lo, hi);
+    visible(p, min(n, p.max_positions), n - (end - t), lo, hi);
     const T *q = static_cast<const T *>(p.q) + t * p.q_ts + h * p.q_hs;
     const long long head = (h / p.group) * p.head_stride;
     float qv[C], o[C], m = -INFINITY, l = 0.0f;

@@ -40,10 +40,10 @@ struct AttendParams {
     CutUnit *cut;       // [CTA]
 };
 
-// Visible positions [lo, hi) of a token at position pos of a sequence of n positions.
+// Visible positions [lo, hi) of a token at position pos, of the n positions that can be read.
 __device__ __forceinline__ void visible(const AttendParams &p, int n, int pos, int &lo, int &hi) {
     hi = p.causal ? min(n, pos + 1) : n;
-    lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+    lo = p.window > 0 ? max(0, min(n, pos - p.window + 1)) : 0;
 }
 
 }  // namespace paged

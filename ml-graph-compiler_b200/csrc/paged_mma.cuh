@@ -148,12 +148,12 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
 
     const int split = EVEN ? 0 : (int)blockIdx.y;
     // one piece: rows row0 .. of (sequence b, key head kh) over keys [k_lo, k_hi)
-    auto piece = [&](int b, int kh, int start, int nq, int n, int row0, int k_lo, int k_hi, int slot) {
-        const int rows = nq * p.group, tiles = k_hi > k_lo ? (k_hi - k_lo + BN - 1) / BN : 0;
+    auto piece = [&](int b, int kh, const Sequence &seq, int row0, int k_lo, int k_hi, int slot) {
+        const int rows = seq.nq * p.group, tiles = k_hi > k_lo ? (k_hi - k_lo + BN - 1) / BN : 0;
         const T *kp = static_cast<const T *>(p.k_pages) + kh * p.head_stride;
         const T *vp = static_cast<const T *>(p.v_pages) + kh * p.head_stride;
         // keys below first.lo no row sees; all rows see [all_lo, all_hi)
-        const RowRange first = row_range(p, n, nq, row0), last = row_range(p, n, nq, min(row0 + R, rows) - 1);
+        const RowRange first = row_range(p, seq, row0), last = row_range(p, seq, min(row0 + R, rows) - 1);
         const int all_lo = last.lo, all_hi = first.hi;
 
         // Byte offset (of K and V alike) of key j of this thread's stage row, or -1: not loaded. In two
@@ -190,7 +190,7 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
         // Q: fragments in registers, or rows in shared memory
         auto q_ptr = [&](int row) {
             const int i = row / p.group, h = kh * p.group + row % p.group;
-            return static_cast<const T *>(p.q) + (long long)(start + i) * p.q_ts + (long long)h * p.q_hs;
+            return static_cast<const T *>(p.q) + (long long)(seq.start + i) * p.q_ts + (long long)h * p.q_hs;
         };
         uint32_t qf[C::Q_REGS ? DP / 16 : 1][4];
         if constexpr (C::Q_REGS) {
@@ -213,7 +213,7 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
             }
         }
 
-        const RowRange r0 = row_range(p, n, nq, row0 + 16 * wm + g4), r1 = row_range(p, n, nq, row0 + 16 * wm + g4 + 8);
+        const RowRange r0 = row_range(p, seq, row0 + 16 * wm + g4), r1 = row_range(p, seq, row0 + 16 * wm + g4 + 8);
         float o[DB][4];
 #pragma unroll
         for (int d = 0; d < DB; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.0f;
@@ -225,7 +225,7 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
         if constexpr (SIMT > 0) {
 #pragma unroll
             for (int r = 0; r < SR; ++r) {
-                sr[r] = row_range(p, n, nq, row0 + r);
+                sr[r] = row_range(p, seq, row0 + r);
                 sm_[r] = -INFINITY;
                 sl_[r] = 0.0f;
 #pragma unroll
@@ -576,7 +576,7 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
         auto put = [&](int r, int c, float4 a, float l) {
             const float inv = l > 0.0f ? 1.0f / l : 0.0f;
             const int row = row0 + r, i = row / p.group, h = kh * p.group + row % p.group;
-            T *out = static_cast<T *>(p.out) + (long long)(start + i) * p.o_ts + (long long)h * p.o_hs + c * 4;
+            T *out = static_cast<T *>(p.out) + (long long)(seq.start + i) * p.o_ts + (long long)h * p.o_hs + c * 4;
             Pack<4, T> v;
             v.e[0] = from_f<T>(a.x * inv);
             v.e[1] = from_f<T>(a.y * inv);
@@ -676,7 +676,7 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
         while (next_item<R, BN>(p, walk, w)) {
             zero_padding();
             if (w.slot == 1) cut = cut_of<R, BN>(p, walk, w);
-            piece(w.b, w.h, w.start, w.nq, w.n, w.row0, w.lo, w.hi, w.slot);
+            piece(w.b, w.h, w.seq, w.row0, w.lo, w.hi, w.slot);
         }
         if (tid == 0) p.cut[blockIdx.x] = cut;
     } else {
@@ -687,17 +687,16 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
         u /= (unsigned)p.kv_heads;
         const int tile0 = p.row_tiles - 1 - (int)(u % (unsigned)p.row_tiles);  // longest rows first
         const int b = (int)(u / (unsigned)p.row_tiles);
-        int start, nq, n;
-        load_sequence(p, b, start, nq, n);
-        if (tid == 0 && nq > 0 && n != __ldg(p.batch.kv_lens + b) && p.batch.status) *p.batch.status = MGC_CUDA_GATHER_OOB;
-        for (int tile = tile0; tile * R < nq * p.group; tile += p.row_tiles) {
-            const RowRange z = row_range(p, n, nq, min(tile * R + R, nq * p.group) - 1);
-            const int lo = row_range(p, n, nq, tile * R).lo & ~15, hi = max(z.hi, 0);
+        const Sequence seq = load_sequence(p, b);
+        if (tid == 0 && past_table(p, seq) && p.batch.status) *p.batch.status = MGC_CUDA_GATHER_OOB;
+        for (int tile = tile0; tile * R < seq.nq * p.group; tile += p.row_tiles) {
+            const RowRange z = row_range(p, seq, min(tile * R + R, seq.nq * p.group) - 1);
+            const int lo = row_range(p, seq, tile * R).lo & ~15, hi = max(z.hi, 0);
             // this split's part of the keys that some row of the tile sees
             const int per = (max(hi - lo, 0) + p.splits * 16 - 1) / (p.splits * 16) * 16;
             const int k_lo = lo + split * per;
             zero_padding();
-            piece(b, kh, start, nq, n, tile * R, k_lo, min(hi, k_lo + per), -1);
+            piece(b, kh, seq, tile * R, k_lo, min(hi, k_lo + per), -1);
         }
     }
 }

@@ -188,7 +188,7 @@ inline bool umma_fits(const mgc_cuda_paged &c) {
 // Key tiles that row tile x of a unit's piece needs (the rows of tile 0 stop earlier if causal).
 __device__ __forceinline__ int tiles_needed(const AttendParams &p, const Item &w, int x) {
     if (x) return w.rows - w.row0 > 128 ? w.tiles : 0;
-    const RowRange mid = row_range(p, w.n, w.nq, min(w.row0 + 128, w.rows) - 1);
+    const RowRange mid = row_range(p, w.seq, min(w.row0 + 128, w.rows) - 1);
     return min(w.tiles, (max(mid.hi - w.lo, 0) + 127) >> 7);
 }
 
@@ -434,7 +434,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
             // element offsets of this thread's row of q and of out; a warp moves its 32 rows together,
             // 16 bytes a lane along the rows (a row per thread touches 32 lines an instruction)
             const int head = w.h * p.group + row % p.group;
-            const long long token = w.start + row / p.group;
+            const long long token = w.seq.start + row / p.group;
             const long long q_off = token * p.q_ts + (long long)head * p.q_hs, o_off = token * p.o_ts + (long long)head * p.o_hs;
             constexpr int CHUNKS = DP / 8;               // 16-byte chunks of a 16-bit row
             uint8_t *rows32 = sQ + x * C::TILE + (r & 96) * 128;  // the warp's 32 rows of the Q tile
@@ -457,7 +457,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_full[x]);
             }
-            const RowRange see = row_range(p, w.n, w.nq, row);
+            const RowRange see = row_range(p, w.seq, row);
             float m = -INFINITY, l = 0.0f;  // m: the (lazy) reference of the weights, scaled
             const int need = tiles_needed(p, w, x);
             for (int j = 0; j < need; ++j) {

@@ -11,13 +11,26 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Position of row (token i of nq, sequence of n positions) -> its visible keys; rows past the last
-// see nothing.
+// A sequence: its first new token's row and position, its new tokens, and the positions that can be
+// read (its length, cut off where the block table ends; the new tokens stay where they are).
+struct Sequence { int start, base, nq, n; };
+__device__ __forceinline__ Sequence load_sequence(const AttendParams &p, int b) {
+    Sequence s;
+    s.start = __ldg(p.batch.q_starts + b);
+    s.nq = __ldg(p.batch.q_starts + b + 1) - s.start;
+    s.n = __ldg(p.batch.kv_lens + b);
+    s.base = s.n - s.nq;
+    s.n = min(s.n, p.max_positions);
+    return s;
+}
+__device__ __forceinline__ bool past_table(const AttendParams &p, const Sequence &s) { return s.nq > 0 && s.base + s.nq > p.max_positions; }
+
+// Visible keys of a row (a token and a head); rows past the last see nothing.
 struct RowRange { int lo, hi; };
-__device__ __forceinline__ RowRange row_range(const AttendParams &p, int n, int nq, int row) {
+__device__ __forceinline__ RowRange row_range(const AttendParams &p, const Sequence &s, int row) {
     RowRange r{0, 0};
     const int i = row / p.group;
-    if (i < nq) visible(p, n, n - nq + i, r.lo, r.hi);
+    if (i < s.nq) visible(p, s.n, s.base + i, r.lo, r.hi);
     return r;
 }
 
@@ -31,8 +44,7 @@ constexpr int MIN_PIECE = 2;
 
 struct Item {
     int rows, row0;     // query rows of the sequence; first of the unit's
-    int start;          // the sequence's first token
-    int n, nq;          // its positions, its new tokens
+    Sequence seq;
     int b, h;
     int lo, hi, tiles;  // keys [lo, hi) of this piece in `tiles` tiles
     int first;          // first key that any row of the unit sees
@@ -45,20 +57,14 @@ struct Walk {
     int left;     // tiles left of the stretch
     int share;    // tiles of a whole stretch
     int heads;    // end of the key heads of these stretches
-    int start, nq, n;  // sequence b: first token, new tokens, positions
+    Sequence seq;  // sequence b
 };
-
-__device__ __forceinline__ void load_sequence(const AttendParams &p, int b, int &start, int &nq, int &n) {
-    start = __ldg(p.batch.q_starts + b);
-    nq = __ldg(p.batch.q_starts + b + 1) - start;
-    n = min(__ldg(p.batch.kv_lens + b), p.max_positions);
-}
 
 // Keys [lo, hi) that rows [ROWS t, ROWS t + ROWS) see, lo rounded down to a tile; the unit's length.
 template <int ROWS, int KEYS>
-__device__ __forceinline__ int unit_length(const AttendParams &p, int n, int nq, int t, int &first, int &lo, int &hi) {
-    const int rows = nq * p.group, row0 = t * ROWS;
-    const RowRange a = row_range(p, n, nq, row0), z = row_range(p, n, nq, min(row0 + ROWS, rows) - 1);
+__device__ __forceinline__ int unit_length(const AttendParams &p, const Sequence &s, int t, int &first, int &lo, int &hi) {
+    const int rows = s.nq * p.group, row0 = t * ROWS;
+    const RowRange a = row_range(p, s, row0), z = row_range(p, s, min(row0 + ROWS, rows) - 1);
     first = a.lo;
     lo = a.lo & ~(KEYS - 1);
     hi = max(z.hi, 0);
@@ -69,10 +75,8 @@ __device__ __forceinline__ int unit_length(const AttendParams &p, int n, int nq,
 template <int ROWS, int KEYS>
 __device__ __forceinline__ bool next_item(const AttendParams &p, Walk &k, Item &w) {
     while (k.left > 0 && k.h < k.heads) {
-        w.start = k.start;
-        w.nq = k.nq;
-        w.n = k.n;
-        w.rows = w.nq * p.group;
+        w.seq = k.seq;
+        w.rows = w.seq.nq * p.group;
         w.row0 = k.t * ROWS;
         if (w.row0 >= w.rows) {  // past the sequence: the next one
             k.t = 0;
@@ -80,11 +84,11 @@ __device__ __forceinline__ bool next_item(const AttendParams &p, Walk &k, Item &
                 k.b = 0;
                 ++k.h;
             }
-            load_sequence(p, k.b, k.start, k.nq, k.n);
+            k.seq = load_sequence(p, k.b);
             continue;
         }
         int lo, hi;
-        const int length = unit_length<ROWS, KEYS>(p, w.n, w.nq, k.t, w.first, lo, hi);
+        const int length = unit_length<ROWS, KEYS>(p, w.seq, k.t, w.first, lo, hi);
         int take = length - k.skip;
         if (take > k.left) {
             const int at = k.skip + k.left;  // where the stretch ends in the unit
@@ -115,20 +119,19 @@ template <int ROWS, int KEYS>
 __device__ __forceinline__ Walk find_stretch(const AttendParams &p, int c, int ctas, int h0, int h1, int lane) {
     int most = 0;  // row tiles of the longest sequence
     for (int b = lane; b < p.batch.batch; b += 32) {
-        int start, nq, n;
-        load_sequence(p, b, start, nq, n);
-        if (n != __ldg(p.batch.kv_lens + b) && nq > 0 && p.batch.status) *p.batch.status = MGC_CUDA_GATHER_OOB;
-        most = max(most, (nq * p.group + ROWS - 1) / ROWS);
+        const Sequence s = load_sequence(p, b);
+        if (past_table(p, s) && p.batch.status) *p.batch.status = MGC_CUDA_GATHER_OOB;
+        most = max(most, (s.nq * p.group + ROWS - 1) / ROWS);
     }
     most = __reduce_max_sync(0xFFFFFFFFu, most);
     const unsigned count = (unsigned)p.batch.batch * (unsigned)most;
     auto length_of = [&](unsigned i) {
         if (i >= count) return 0;
-        int start, nq, n, first, lo, hi;
+        int first, lo, hi;
         const unsigned b = i / (unsigned)most;
-        load_sequence(p, (int)b, start, nq, n);
+        const Sequence s = load_sequence(p, (int)b);
         const int t = (int)(i - b * (unsigned)most);
-        return t * ROWS < nq * p.group ? unit_length<ROWS, KEYS>(p, n, nq, t, first, lo, hi) : 0;
+        return t * ROWS < s.nq * p.group ? unit_length<ROWS, KEYS>(p, s, t, first, lo, hi) : 0;
     };
     // the lanes' lengths summed up to and including each; the first 32 units' are kept
     auto scan = [&](int v) {
@@ -142,7 +145,7 @@ __device__ __forceinline__ Walk find_stretch(const AttendParams &p, int c, int c
     const int mine0 = length_of(lane), upto0 = scan(mine0);
     long long head = __shfl_sync(0xFFFFFFFFu, upto0, 31);  // tiles of one key head
     for (unsigned i = 32; i < count; i += 32) head += __reduce_add_sync(0xFFFFFFFFu, length_of(i + lane));
-    Walk k{h1, 0, 0, 0, 0, 0, h1, 0, 0, 0};
+    Walk k{h1, 0, 0, 0, 0, 0, h1, {0, 0, 0, 0}};
     const long long all = head * (h1 - h0);
     long long share, x0;
     if (all < 0x7FFFFFFF) {
@@ -168,7 +171,7 @@ __device__ __forceinline__ Walk find_stretch(const AttendParams &p, int c, int c
             const int off = (int)at - (__shfl_sync(0xFFFFFFFFu, upto, who) - length);
             k.b = (int)((i + who) / (unsigned)most);
             k.t = (int)((i + who) % (unsigned)most);
-            load_sequence(p, k.b, k.start, k.nq, k.n);
+            k.seq = load_sequence(p, k.b);
             k.left = k.share = (int)share;
             if (off < MIN_PIECE) {
                 k.left += off;
@@ -191,7 +194,7 @@ template <int ROWS, int KEYS>
 __device__ __forceinline__ CutUnit cut_of(const AttendParams &p, const Walk &k, const Item &w) {
     int first, lo, hi;
     CutUnit cut{w.h, w.b, w.row0 / ROWS, 1};
-    const int length = unit_length<ROWS, KEYS>(p, w.n, w.nq, cut.t, first, lo, hi);
+    const int length = unit_length<ROWS, KEYS>(p, w.seq, cut.t, first, lo, hi);
     for (int at = w.tiles; length - at >= MIN_PIECE; at += k.share) ++cut.pieces;
     return cut;
 }
@@ -211,9 +214,8 @@ __global__ void __launch_bounds__(128) paged_combine_units_kernel(const __grid_c
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const CutUnit cut = p.cut[c];
     if (cut.pieces < 2) return;
-    int start, nq, n;
-    load_sequence(p, cut.b, start, nq, n);
-    const int rows = nq * p.group;
+    const Sequence s = load_sequence(p, cut.b);
+    const int rows = s.nq * p.group;
     const int r0 = WARPS > 1 ? (int)blockIdx.y : (int)blockIdx.y * 4 + warp, step = (int)gridDim.y * (4 / WARPS);
     for (int r = r0; r < ROWS; r += step) {
         const int row = cut.t * ROWS + r;
@@ -223,7 +225,7 @@ __global__ void __launch_bounds__(128) paged_combine_units_kernel(const __grid_c
         for (int i = lane; i < cut.pieces; i += 32) m = fmaxf(m, p.part_ml[at(i)].x);
 #pragma unroll
         for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));
-        T *out = static_cast<T *>(p.out) + (long long)(start + row / p.group) * p.o_ts +
+        T *out = static_cast<T *>(p.out) + (long long)(s.start + row / p.group) * p.o_ts +
                  (long long)(cut.h * p.group + row % p.group) * p.o_hs;
         for (int d0 = 0; d0 < p.head_dim; d0 += 128) {
             const int d = d0 + lane * 4;
