@@ -315,8 +315,9 @@ int mgc_cuda_layer_norm(int64_t rows, int64_t cols, const float *x, const float 
  * positions, position p in row p % page_size of page block_table[b * table_stride + p / page_size].
  * Its i-th new token is at position kv_lens[b] - (q_starts[b + 1] - q_starts[b]) + i. block_table,
  * kv_lens and q_starts are device arrays that only the kernels read. A page number outside
- * [0, pages), a position past table_pages pages or one past the rotation table sets *status_dev (when
- * not NULL) to MGC_CUDA_GATHER_OOB; nothing is read or written there. All fields are 8 bytes wide. */
+ * [0, pages), a position past table_pages pages, one past the rotation table or a row outside
+ * [0, tokens) sets *status_dev (when not NULL) to MGC_CUDA_GATHER_OOB; nothing is read or written
+ * there, and what remains of the sequence keeps its positions. All fields are 8 bytes wide. */
 typedef struct {
     void *k, *v;
     int64_t pages, page_stride, token_stride, head_stride;

@@ -166,6 +166,8 @@ __global__ void __launch_bounds__(256, RESIDENT<S, V>) kv_append_kernel(const __
     };
     // a token's sources load while its place is found (the next token's in a second set of registers
     // left fewer blocks on an SM: 144 us)
+    if (blockIdx.x == 0 && threadIdx.x == 0 && p.batch.status && __ldg(p.batch.q_starts + p.batch.batch) > p.tokens)
+        *p.batch.status = MGC_CUDA_GATHER_OOB;
     Unit<S, T, V> u[BATCH];
     for (int t = t0; t < t1; ++t) {
 #pragma unroll

@@ -15,12 +15,13 @@ __global__ void __launch_bounds__(128) paged_attention_row_kernel(const __grid_c
     const int lane = (int)(threadIdx.x & 31);
     const int t = (int)blockIdx.x;
     const int h = (int)blockIdx.y * 4 + (int)(threadIdx.x >> 5);
+    if (t == 0 && h == 0)
+        for (int i = lane; i < p.batch.batch; i += 32) check_sequence(p, i);
     const int b = sequence_of(p.batch, t);
     if (b < 0 || h >= p.q_heads) return;
     const int end = __ldg(p.batch.q_starts + b + 1);
     if (t >= end) return;
     const int n = __ldg(p.batch.kv_lens + b);
-    if (n > p.max_positions && p.batch.status) *p.batch.status = MGC_CUDA_GATHER_OOB;
     int lo, hi;
     visible(p, min(n, p.max_positions), n - (end - t), lo, hi);
     const T *q = static_cast<const T *>(p.q) + t * p.q_ts + h * p.q_hs;

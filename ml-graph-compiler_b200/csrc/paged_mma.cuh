@@ -688,7 +688,7 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
         const int tile0 = p.row_tiles - 1 - (int)(u % (unsigned)p.row_tiles);  // longest rows first
         const int b = (int)(u / (unsigned)p.row_tiles);
         const Sequence seq = load_sequence(p, b);
-        if (tid == 0 && past_table(p, seq) && p.batch.status) *p.batch.status = MGC_CUDA_GATHER_OOB;
+        if (tid == 0) check_sequence(p, b);
         for (int tile = tile0; tile * R < seq.nq * p.group; tile += p.row_tiles) {
             const RowRange z = row_range(p, seq, min(tile * R + R, seq.nq * p.group) - 1);
             const int lo = row_range(p, seq, tile * R).lo & ~15, hi = max(z.hi, 0);

@@ -11,19 +11,25 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// A sequence: its first new token's row and position, its new tokens, and the positions that can be
-// read (its length, cut off where the block table ends; the new tokens stay where they are).
+// A sequence: its first new token's row and position, its new tokens (rows of q outside it do not
+// exist and are left out), and the positions that can be read (its length, cut off where the block
+// table ends). Neither cut moves the tokens that are left.
 struct Sequence { int start, base, nq, n; };
 __device__ __forceinline__ Sequence load_sequence(const AttendParams &p, int b) {
+    const int start = __ldg(p.batch.q_starts + b), end = __ldg(p.batch.q_starts + b + 1), length = __ldg(p.batch.kv_lens + b);
     Sequence s;
-    s.start = __ldg(p.batch.q_starts + b);
-    s.nq = __ldg(p.batch.q_starts + b + 1) - s.start;
-    s.n = __ldg(p.batch.kv_lens + b);
-    s.base = s.n - s.nq;
-    s.n = min(s.n, p.max_positions);
+    s.start = max(start, 0);
+    s.nq = max(min(end, p.tokens) - s.start, 0);
+    s.base = length - (end - s.start);
+    s.n = min(length, p.max_positions);
     return s;
 }
-__device__ __forceinline__ bool past_table(const AttendParams &p, const Sequence &s) { return s.nq > 0 && s.base + s.nq > p.max_positions; }
+// Sets the status word if something of sequence b was cut off.
+__device__ __forceinline__ void check_sequence(const AttendParams &p, int b) {
+    const int start = __ldg(p.batch.q_starts + b), end = __ldg(p.batch.q_starts + b + 1);
+    if (p.batch.status && (start < 0 || end < start || end > p.tokens || (end > start && __ldg(p.batch.kv_lens + b) > p.max_positions)))
+        *p.batch.status = MGC_CUDA_GATHER_OOB;
+}
 
 // Visible keys of a row (a token and a head); rows past the last see nothing.
 struct RowRange { int lo, hi; };
@@ -120,7 +126,7 @@ __device__ __forceinline__ Walk find_stretch(const AttendParams &p, int c, int c
     int most = 0;  // row tiles of the longest sequence
     for (int b = lane; b < p.batch.batch; b += 32) {
         const Sequence s = load_sequence(p, b);
-        if (past_table(p, s) && p.batch.status) *p.batch.status = MGC_CUDA_GATHER_OOB;
+        check_sequence(p, b);
         most = max(most, (s.nq * p.group + ROWS - 1) / ROWS);
     }
     most = __reduce_max_sync(0xFFFFFFFFu, most);

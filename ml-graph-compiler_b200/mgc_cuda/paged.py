@@ -17,7 +17,7 @@ a call can be captured into a CUDA graph. There is no autograd. The C entry poin
 take raises ``GraphError`` or ``CodegenError`` and nothing runs.
 
 What a kernel cannot accept (a page number outside the cache, a position past the block table or
-past the rotation table) is skipped and recorded in ``status``, an int32 tensor of one element that
+past the rotation table, a row of q_starts that the operands do not have) is skipped and recorded in ``status``, an int32 tensor of one element that
 the caller may pass and hand to ``check_status`` when it next synchronises.
 """
 

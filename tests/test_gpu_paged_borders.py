@@ -54,3 +54,76 @@ def test_lengths_past_the_block_table_keep_their_positions(dtype: str, layout: s
     with pytest.raises(GraphError, match="out of range"):
         paged.check_status(status)
     compare(got, *reference(x, 64**-0.5, window=window, lens=lens))
+
+
+# ---- rows that the operands do not have ----------------------------------------------------------
+def inside(x: PagedBatch):
+    """x.q, its out and its cache-sized operands as views of larger buffers whose other rows must stay as
+    they are: what a kernel reads or writes past the views shows there."""
+    room = torch.full((x.q.shape[0] + 600, *x.q.shape[1:]), math.nan, dtype=x.q.dtype, device="cuda")
+    room[300:-300] = x.q
+    out = torch.full_like(room, 7.0)
+    x.q = room[300:-300]
+    return out
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("layout", ["tokens", "odd"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("shift", [-2, 3, 200])
+@pytest.mark.parametrize("qs,ks", BATCHES)
+def test_rows_past_the_operands_are_left_out(dtype: str, layout: str, dim: int, shift: int, qs, ks) -> None:
+    """q_starts that begin before the first row or end after the last: the rows that exist keep their
+    positions, nothing else is read or written, and the status says so."""
+    x = PagedBatch(qs, ks, heads=4, kv_heads=2, dim=dim, page=16, dtype=dtype, layout=layout)
+    out = inside(x)
+    tokens = x.q.shape[0]
+    starts = [0]
+    for n in qs:
+        starts.append(starts[-1] + n)
+    if shift < 0:
+        starts[0] = shift
+    else:
+        starts[-1] += shift
+    x.q_starts = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    # the sequence that is too long has its other tokens before the first row or after the last
+    lens = list(x.ks)
+    if shift > 0:
+        lens[-1] -= shift
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = out[300:-300]
+    paged.paged_attention(x.q, *x.operands, out=got, max_q=max(qs) + abs(shift), max_kv=max(ks), status=status)
+    with pytest.raises(GraphError, match="out of range"):
+        paged.check_status(status)
+    compare(got, *reference(x, dim**-0.5, lens=lens))
+    assert bool((out[:300] == 7.0).all()) and bool((out[300 + tokens :] == 7.0).all())
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("layout", ["tokens", "odd"])
+@pytest.mark.parametrize("starts", [[0, 0x7FFFFFFF], [-0x7FFFFFFF, 0x7FFFFFFF], [5, 3], [100, 400], [-9, -2], [0, -5]])
+@pytest.mark.parametrize("tokens", [1, 3, 150])
+def test_any_starts_stay_inside_the_operands(dtype: str, layout: str, starts, tokens: int) -> None:
+    x = PagedBatch([tokens, 1], [200, 9], heads=4, kv_heads=2, dim=64, page=16, dtype=dtype, layout=layout)
+    out = inside(x)
+    x.q_starts = torch.tensor([*starts, starts[-1]], dtype=torch.int32, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    paged.paged_attention(x.q, *x.operands, out=out[300:-300], max_q=tokens, max_kv=200, status=status)
+    with pytest.raises(GraphError, match="out of range"):
+        paged.check_status(status)
+    assert bool((out[:300] == 7.0).all()) and bool((out[-300:] == 7.0).all())
+
+
+def test_append_with_rows_past_the_operands() -> None:
+    x = PagedBatch([3, 4], [40, 9], heads=4, kv_heads=2, dim=64, page=16, dtype="bf16")
+    k = torch.randn(7, 2, 64, device="cuda").to(torch.bfloat16)
+    x.q_starts = torch.tensor([0, 3, 9], dtype=torch.int32, device="cuda")
+    before = x.k.clone()
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    paged.kv_append(k, k, *x.operands, status=status)
+    with pytest.raises(GraphError, match="out of range"):
+        paged.check_status(status)
+    for b, rows, at in ((0, slice(0, 3), slice(37, 40)), (1, slice(3, 7), slice(3, 7))):
+        page, row = x.slots[b]
+        before[page[at], row[at]] = k[rows]
+    assert torch.equal(before.nan_to_num(7.0), x.k.nan_to_num(7.0))
