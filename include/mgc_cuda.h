@@ -337,8 +337,9 @@ typedef struct {
  * cos and sin fp32 tables of `positions` rows of rot/2 values, table_row elements apart. rot 0:
  * no rotation. The sources are of src_dtype, the pages' type or MGC_F32; q_out is of the pages'
  * type and may be q itself (same strides, src_dtype the pages' type). Arithmetic in fp32, rounded
- * once. A token at a negative position (more new tokens than cached positions) is not cached, and
- * its query is copied unrotated. */
+ * once. A token at a negative position (more new tokens than cached positions) or in no sequence
+ * (before q_starts[0], from q_starts[batch] on) is not cached, and its query is copied unrotated.
+ * A call with batch 0 does nothing. */
 typedef struct {
     mgc_cuda_paged paged;
     int64_t src_dtype;
@@ -359,7 +360,7 @@ int mgc_cuda_kv_append(const mgc_cuda_kv_append_args *args, void *stream);
 /* mgc_cuda_paged_attention: out[t][h] = sum_j w_j v_j, w the softmax over the visible positions j of
  * scale * q[t][h] . k_j, key head h / (q_heads / kv_heads). Visible to a token at position p:
  * j < kv_lens[b]; with `causal`, j <= p; with window > 0 (causal only), j > p - window. A token
- * with no visible position gets zeros. q and out are of the pages' type. Cache rows that no token of
+ * with no visible position, or in no sequence, gets zeros (a call with batch 0 does nothing). q and out are of the pages' type. Cache rows that no token of
  * their sequence may see are not used, whatever they hold. max_q and max_kv, the longest sequence's
  * new tokens and positions, are host values that size the launch: longer sequences are computed
  * too, by fewer blocks than they could use. `workspace` (16-byte aligned) holds partial results when

@@ -131,13 +131,11 @@ __global__ void __launch_bounds__(256, RESIDENT<S, V>) kv_append_kernel(const __
     auto place = [&](Unit<S, T, V> (&u)[BATCH], int t) {
         if (t >= end) {
             b = sequence_of(p.batch, t);
-            if (b < 0) return;
-            end = __ldg(p.batch.q_starts + b + 1);
-            n = __ldg(p.batch.kv_lens + b);
+            end = b < 0 ? t : __ldg(p.batch.q_starts + b + 1);
+            n = b < 0 ? 0 : __ldg(p.batch.kv_lens + b);
             held = -1;
         }
-        if (b < 0 || t >= end) return;  // outside every sequence
-        const int pos = n - (end - t);
+        const int pos = t >= end ? -1 : n - (end - t);  // in no sequence: nowhere to cache, nothing to rotate by
         if (pos >= 0 && (held < 0 || pos / p.batch.page_size != held)) {
             held = pos / p.batch.page_size;
             page = page_of(p.batch, b, held);

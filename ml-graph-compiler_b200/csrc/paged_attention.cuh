@@ -18,9 +18,13 @@ __global__ void __launch_bounds__(128) paged_attention_row_kernel(const __grid_c
     if (t == 0 && h == 0)
         for (int i = lane; i < p.batch.batch; i += 32) check_sequence(p, i);
     const int b = sequence_of(p.batch, t);
-    if (b < 0 || h >= p.q_heads) return;
-    const int end = __ldg(p.batch.q_starts + b + 1);
-    if (t >= end) return;
+    if (h >= p.q_heads) return;
+    T *out = static_cast<T *>(p.out) + t * p.o_ts + h * p.o_hs;
+    const int end = b < 0 ? t : __ldg(p.batch.q_starts + b + 1);
+    if (t >= end) {  // in no sequence
+        for (int d = lane; d < p.head_dim; d += 32) out[d] = from_f<T>(0.0f);
+        return;
+    }
     const int n = __ldg(p.batch.kv_lens + b);
     int lo, hi;
     visible(p, min(n, p.max_positions), n - (end - t), lo, hi);
@@ -56,7 +60,6 @@ __global__ void __launch_bounds__(128) paged_attention_row_kernel(const __grid_c
             if (d < p.head_dim) o[c] = o[c] * scale + w * to_f(v[d]);
         }
     }
-    T *out = static_cast<T *>(p.out) + t * p.o_ts + h * p.o_hs;
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {

@@ -699,6 +699,7 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
             piece(b, kh, seq, tile * R, k_lo, min(hi, k_lo + per), -1);
         }
     }
+    zero_outside<T>(p, (int)(blockIdx.y * gridDim.x + blockIdx.x), (int)(gridDim.x * gridDim.y), warp, WM * WN, lane);
 }
 
 }  // namespace paged

@@ -176,6 +176,7 @@ PyObject *kv_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
             x.interleaved = PyObject_IsTrue(a[10]) == 1;
         }
         const c10::cuda::CUDAGuard guard(device);
+        if (q && x.paged.batch == 0) out.copy_(*q);  // no sequence: the call itself does nothing
         void *stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
         int status;
         Py_BEGIN_ALLOW_THREADS;
@@ -229,6 +230,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
         x.causal = PyObject_IsTrue(a[9]) == 1;
         x.window = whole(a[10], 0);
         const c10::cuda::CUDAGuard guard(device);
+        if (x.paged.batch == 0) out.zero_();  // no sequence: the call itself does nothing
         void *stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
         // partial results of keys that are shared out, from torch's stream-ordered allocator: the
         // block returns to this stream's pool after the call

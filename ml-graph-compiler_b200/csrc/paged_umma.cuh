@@ -413,11 +413,12 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                 slot = (slot + 2 * w.tiles) % C::STAGES;
             }
         } else {
-            // ---------------- warp 11: how many pieces has the unit cut at the stretch's end? ----------------
+            // ---------------- warp 11: how many pieces has the unit cut at the stretch's end? Rows of no sequence ----------------
             CutUnit cut{0, 0, 0, 0};
             while (next_item<256, 128>(p, walk, w))
                 if (w.slot == 1) cut = cut_of<256, 128>(p, walk, w);
             if (lane == 0) p.cut[blockIdx.x] = cut;
+            zero_outside<T>(p, (int)blockIdx.x, (int)gridDim.x, 0, 1, lane);
         }
     } else {
         // ---------------- softmax: one row per thread ----------------

@@ -31,6 +31,21 @@ __device__ __forceinline__ void check_sequence(const AttendParams &p, int b) {
         *p.batch.status = MGC_CUDA_GATHER_OOB;
 }
 
+// Zeros in the rows of out that no sequence has (a batch padded to a fixed number of rows): this warp
+// takes heads h0, h0 + step, ... of tokens t0, t0 + t_step, ... For kernels whose rows are 16-byte
+// chunks.
+template <typename T> __device__ __forceinline__ void zero_outside(const AttendParams &p, int t0, int t_step, int h0, int h_step, int lane) {
+    const int first = min(max(__ldg(p.batch.q_starts), 0), p.tokens);
+    const int last = min(max(__ldg(p.batch.q_starts + p.batch.batch), first), p.tokens);
+    if (first == 0 && last == p.tokens) return;
+    for (long long i = t0; i < first + p.tokens - last; i += t_step) {
+        T *row = static_cast<T *>(p.out) + (i < first ? i : i - first + last) * p.o_ts;
+        for (int h = h0; h < p.q_heads; h += h_step)
+            for (int d = lane * (16 / (int)sizeof(T)); d < p.head_dim; d += 32 * (16 / (int)sizeof(T)))
+                *reinterpret_cast<uint4 *>(row + h * p.o_hs + d) = make_uint4(0, 0, 0, 0);
+    }
+}
+
 // Visible keys of a row (a token and a head); rows past the last see nothing.
 struct RowRange { int lo, hi; };
 __device__ __forceinline__ RowRange row_range(const AttendParams &p, const Sequence &s, int row) {

@@ -80,7 +80,8 @@ def kv_append(
     With ``cos`` and ``sin`` (float32 [positions, rot / 2], rot <= head_dim) the first rot channels
     of every key are rotated by the token's position on the way, pair i being channels (i, i + rot/2),
     or (2i, 2i + 1) when ``interleaved``. With ``q`` [tokens, heads, head_dim] the queries are rotated
-    too: the result (``q_out`` if given, which may be ``q`` itself) is returned in the cache's type.
+    too: the result (``q_out`` if given, which may be ``q`` itself) is returned in the cache's type;
+    rows that no sequence has are copied as they are.
     ``q``, ``k`` and ``v`` are of the cache's type or float32, strided views of a fused projection
     included; the arithmetic is fp32, rounded once."""
     return (_EXT or _binding()).kv_append(k, v, k_cache, v_cache, block_table, kv_lens, q_starts, q, cos, sin, interleaved,
@@ -107,7 +108,7 @@ def paged_attention(
     positions, head h reading key head h // (heads // kv_heads); returns ``out`` of q's shape.
 
     A token at position p sees positions j < kv_len, j <= p if ``causal``, and j > p - window if
-    ``window`` is positive; a token that sees nothing gets zeros. ``scale`` defaults to
+    ``window`` is positive; a token that sees nothing, or that no sequence has, gets zeros. ``scale`` defaults to
     head_dim ** -0.5. ``max_q`` and ``max_kv``, the longest sequence's new tokens and positions,
     size the launch; without them it is sized by the packed tokens and the block table."""
     return (_EXT or _binding()).paged_attention(q, k_cache, v_cache, block_table, kv_lens, q_starts, max_q, max_kv, scale,

@@ -127,3 +127,52 @@ def test_append_with_rows_past_the_operands() -> None:
         page, row = x.slots[b]
         before[page[at], row[at]] = k[rows]
     assert torch.equal(before.nan_to_num(7.0), x.k.nan_to_num(7.0))
+
+
+# ---- rows of q that no sequence has --------------------------------------------------------------
+def padded(qs, ks, before: int, after: int, **kw) -> PagedBatch:
+    """A batch with rows of q in front of the first sequence's and behind the last one's."""
+    x = PagedBatch([before, *qs, after], [before, *ks, after], **kw)
+    x.qs, x.ks, x.slots = x.qs[1:-1], x.ks[1:-1], x.slots[1:-1]
+    x.block_table, x.kv_lens, x.q_starts = x.block_table[1:-1], x.kv_lens[1:-1], x.q_starts[1:-1]
+    x.before = before
+    x.rows = lambda b: slice(before + sum(x.qs[:b]), before + sum(x.qs[: b + 1]))
+    return x
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("layout", ["tokens", "odd"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("before,after", [(0, 5), (3, 0), (2, 300)])
+@pytest.mark.parametrize("qs,ks", BATCHES)
+def test_rows_of_no_sequence_get_zeros(dtype: str, layout: str, dim: int, before: int, after: int, qs, ks) -> None:
+    """A batch padded to a fixed number of rows, as a captured graph runs it."""
+    x = padded(qs, ks, before, after, heads=4, kv_heads=2, dim=dim, page=16, dtype=dtype, layout=layout)
+    compare(attend(x), *reference(x, dim**-0.5))
+
+
+@pytest.mark.parametrize("dtype", ALL)
+def test_queries_of_no_sequence_are_copied(dtype: str) -> None:
+    """kv_append returns them as they are, and caches nothing for them."""
+    x = padded([3, 40], [20, 40], 2, 70, heads=4, kv_heads=2, dim=64, page=16, dtype=dtype)
+    a = torch.arange(64, device="cuda")[:, None] * torch.linspace(0.1, 1.0, 32, device="cuda")
+    k = x.q[:, :2]
+    before = [x.k.clone(), x.v.clone()]
+    out = torch.full(x.q.shape, math.nan, dtype=x.q.dtype, device="cuda")
+    paged.kv_append(k, k, *x.operands, q=x.q, q_out=out, cos=a.cos(), sin=a.sin())
+    assert torch.equal(out[:2], x.q[:2]) and torch.equal(out[-70:], x.q[-70:])
+    for b in range(2):
+        page, row = x.slots[b]
+        at = torch.arange(x.ks[b] - x.qs[b], x.ks[b], device="cuda")
+        for was, now in zip(before, (x.k, x.v)):
+            was[page[at], row[at]] = now[page[at], row[at]]
+    for was, now in zip(before, (x.k, x.v)):
+        assert torch.equal(was.nan_to_num(7.0), now.nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("dtype", ALL)
+def test_rows_without_any_sequence(dtype: str) -> None:
+    x = padded([], [], 3, 4, heads=4, kv_heads=2, dim=64, page=16, dtype=dtype)
+    out = torch.full(x.q.shape, math.nan, dtype=x.q.dtype, device="cuda")
+    assert not paged.paged_attention(x.q, *x.operands, out=out).any()
+    assert torch.equal(paged.kv_append(x.q[:, :2], x.q[:, :2], *x.operands, q=x.q), x.q)
