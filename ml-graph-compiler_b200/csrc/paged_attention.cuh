@@ -118,12 +118,13 @@ inline Plan plan_of(const mgc_cuda_paged_attention_args &a) {
     auto rows16 = [&](const void *q, int64_t x, int64_t y, int64_t z) {
         return aligned(q, 16) && x * es % 16 == 0 && y * es % 16 == 0 && z * es % 16 == 0;
     };
-    // 16-byte rows everywhere; anything else takes the row kernel
-    s.mma = c.head_dim % chunk == 0 && rows16(c.k, c.page_stride, c.token_stride, c.head_stride) &&
+    const int64_t group = a.q_heads / c.kv_heads;
+    // 16-byte rows everywhere, and a sequence's rows (with those of its last tile) counted in 32 bits;
+    // anything else takes the row kernel
+    s.mma = c.head_dim % chunk == 0 && c.tokens * group < 0x80000000ll - 256 && rows16(c.k, c.page_stride, c.token_stride, c.head_stride) &&
             rows16(c.v, 0, 0, 0) && rows16(a.q, a.q_token_stride, a.q_head_stride, 0) &&
             rows16(a.out, a.o_token_stride, a.o_head_stride, 0);
     if (!s.mma) return s;
-    const int64_t group = a.q_heads / c.kv_heads;
     int64_t max_q = a.max_q < 1 ? 1 : a.max_q > c.tokens ? c.tokens : a.max_q;
     const int64_t rows = max_q * group;
     auto even_shares = [&](int unit_rows, int ctas) {
