@@ -147,6 +147,9 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
     const int chunks = p.head_dim / C::CH;
 
     const int split = EVEN ? 0 : (int)blockIdx.y;
+    __shared__ int bad_pages;  // set once a page number was out of range
+    if (tid == 0) bad_pages = 0;
+    if constexpr (!EVEN) __syncthreads();  // else below
     // one piece: rows row0 .. of (sequence b, key head kh) over keys [k_lo, k_hi)
     auto piece = [&](int b, int kh, const Sequence &seq, int row0, int k_lo, int k_hi, int slot) {
         const int rows = seq.nq * p.group, tiles = k_hi > k_lo ? (k_hi - k_lo + BN - 1) / BN : 0;
@@ -168,9 +171,15 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
             if (j >= k_hi || j < first.lo) return -1;
             if (page < 0 || page >= p.batch.pages) {
                 if (p.batch.status) *p.batch.status = MGC_CUDA_GATHER_OOB;
+                bad_pages = 1;
                 return -1;
             }
             return ((long long)page * p.page_stride + (long long)(j % ps) * p.token_stride) * (long long)sizeof(T);
+        };
+        // once the CTA has met such a page, every key's is looked up again before its score counts
+        auto on_page = [&](int j) {
+            const int page = fetch_page(j);
+            return page >= 0 && page < p.batch.pages;
         };
         auto load_stage = [&](int it) {
             uint8_t *st = ring + (it % C::STAGES) * C::STAGE;
@@ -249,6 +258,7 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
             cp_async_commit();
             const int j_next = k_lo + (it + C::STAGES) * BN + tid;
             const int page_next = tid < BN ? fetch_page(j_next) : -1;
+            const bool check_pages = *static_cast<volatile int *>(&bad_pages) != 0;
 
             const uint8_t *st = ring + (it % C::STAGES) * C::STAGE;
             if constexpr (SIMT > 0) {
@@ -260,6 +270,7 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
                 if (j0 < k_hi) {
                     float *sP = reinterpret_cast<float *>(smem + C::SMEM) - (wn + 1) * R * KW;
                     const float4 *kr = reinterpret_cast<const float4 *>(st + (wn * KW + key) * ROW) + part * PC;
+                    const bool key_there = j < k_hi && (!check_pages || on_page(j));
                     float x[SR];
 #pragma unroll
                     for (int r = 0; r < SR; ++r) x[r] = 0.0f;
@@ -276,7 +287,7 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
                     for (int r = 0; r < SR; ++r) {
 #pragma unroll
                         for (int d = KW; d < 32; d <<= 1) x[r] += __shfl_xor_sync(0xFFFFFFFFu, x[r], d);
-                        if (j < sr[r].lo || j >= sr[r].hi || j >= k_hi) x[r] = -INFINITY;
+                        if (j < sr[r].lo || j >= sr[r].hi || !key_there) x[r] = -INFINITY;
                         float top = x[r];
 #pragma unroll
                         for (int d = 1; d < KW; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
@@ -419,7 +430,7 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
                     }
                 }
                 // mask where some row of the tile does not see some key
-                const bool whole = j0 >= all_lo && j0 + KG <= all_hi && j0 + KG <= k_hi;
+                const bool whole = j0 >= all_lo && j0 + KG <= all_hi && j0 + KG <= k_hi && !check_pages;
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
@@ -427,7 +438,7 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
                         if (!whole) {
                             const int j = j0 + nb * 8 + t4 * 2 + (e & 1);
                             const RowRange &r = e < 2 ? r0 : r1;
-                            if (j < r.lo || j >= r.hi || j >= k_hi) s[nb][e] = -INFINITY;
+                            if (j < r.lo || j >= r.hi || j >= k_hi || (check_pages && !on_page(j))) s[nb][e] = -INFINITY;
                         }
                     }
                 }

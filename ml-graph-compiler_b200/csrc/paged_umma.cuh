@@ -18,6 +18,8 @@
 //   rescale needs no wait: S of tile j is committed after P V of tile j - 1.
 // * 64 channels leave TMEM for weights apart from the scores: the next tile's scores are made
 //   while this one's weights are.
+// * A page number out of range: the loading warp writes zeros where its keys and values would be and
+//   names the boxes (wrong_boxes), whose scores the softmax warps mask.
 // * Rows of V that no row sees (past the last visible key, before the first) are zeroed in shared
 //   memory before they are used: a page's unused rows hold anything, and 0 * NaN is NaN.
 //
@@ -201,6 +203,10 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
     __shared__ __align__(8) uint64_t z_ask, z_done;
     __shared__ uint32_t tslot;
     __shared__ Walk stretch;
+    // bit l of entry t % 8: lane l's box of the CTA's t-th key tile has no page. An entry is written before
+    // its K tile is announced; by then the weights of the fifth tile before it, at the latest, are done, so
+    // eight entries outlast their readers.
+    __shared__ uint32_t wrong_boxes[8];
     uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *sQ = base, *ring = base + 2 * C::TILE;
     const int tid = (int)threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
@@ -247,27 +253,40 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::OTHER_REGS));
         if (warp == 9) {
             // ---------------- loads ----------------
-            int slot = 0, laps = 0, issued = 0;
+            int slot = 0, laps = 0, issued = 0, tile = 0;
             const int boxes = (128 / maps.box_rows) * C::HALVES;  // of a tile: at most 32
             const int part = lane / C::HALVES, half = lane % C::HALVES;
             bool ok = true;
             while (ok && next_item<256, 128>(p, walk, w)) {
-                // this lane's box of key tile j: page and first row in it; -1 if no row sees its keys
+                // this lane's box of key tile j: page and first row in it; -1 if no row sees its keys, -2
+                // if it should have a page
                 auto box = [&](int j, int &row) {
                     const int at = w.lo + j * 128 + part * maps.box_rows;
                     row = at % p.batch.page_size;
                     if (lane >= boxes || j >= w.tiles || at >= w.hi || at + maps.box_rows <= w.first) return -1;
-                    return page_of(p.batch, w.b, at / p.batch.page_size);
+                    const int page = page_of(p.batch, w.b, at / p.batch.page_size);
+                    return page < 0 ? -2 : page;
                 };
                 int row, page = box(0, row);
                 for (int j = 0; ok && j < w.tiles; ++j) {
                     int next_row, next = box(j + 1, next_row);  // looked up one tile ahead
                     const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xFFFFFFFFu, page >= 0)) * (uint32_t)maps.box_rows * 128u;
+                    const uint32_t wrong = __ballot_sync(0xFFFFFFFFu, page == -2);
 #pragma unroll
                     for (int kv = 0; kv < 2; ++kv) {
                         if (laps > 0) ok = ok && wait(&empty[slot], (uint32_t)(laps - 1) & 1u);
                         if (!ok) break;
-                        if (lane == 0) mbar_expect_tx(&full[slot], bytes);
+                        if (wrong) {
+                            uint4 *z = reinterpret_cast<uint4 *>(ring + slot * C::TILE + half * C::HALF + part * maps.box_rows * 128);
+                            if (page == -2)
+                                for (int i = 0; i < maps.box_rows * 8; ++i) z[i] = make_uint4(0, 0, 0, 0);
+                            umma::fence_proxy_async_smem();
+                            __syncwarp();
+                        }
+                        if (lane == 0) {
+                            if (kv == 0) *static_cast<volatile uint32_t *>(&wrong_boxes[tile & 7]) = wrong;
+                            mbar_expect_tx(&full[slot], bytes);
+                        }
                         __syncwarp();
                         if (page >= 0)
                             umma::tma_load_4d(ring + slot * C::TILE + half * C::HALF + part * maps.box_rows * 128,
@@ -280,6 +299,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                     }
                     page = next;
                     row = next_row;
+                    ++tile;
                 }
             }
             // after a timeout, the copies still in flight
@@ -428,6 +448,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
         const uint32_t ts = tbase + lanes + C::S_COL + x * 128, to = tbase + lanes + C::O_COL + x * DP;
         const uint32_t tp = tbase + lanes + C::P_COL + x * C::P_STEP;
         uint32_t s_phase = 0, o_phase = 0, free_phase = 0;
+        int tile0 = 0;  // the CTA's key tiles before this piece
         bool ok = true;
         while (ok && next_item<256, 128>(p, walk, w)) {
             const int row = w.row0 + x * 128 + r;
@@ -498,6 +519,12 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                         }
                     }
                 }
+                if (const uint32_t wrong = *static_cast<volatile uint32_t *>(&wrong_boxes[(tile0 + j) & 7])) {
+                    const int shift = 31 - __clz(maps.box_rows);  // box sizes are powers of two
+#pragma unroll
+                    for (int i = 0; i < 128; ++i)
+                        if (wrong >> ((i >> shift) * C::HALVES) & 1u) s[i] = -INFINITY;
+                }
                 float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
                 for (int i = 4; i < 124; i += 8) {
@@ -551,6 +578,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                 sum[0] = add2(sum[0], sum[1]);
                 l += sum[0].x + sum[0].y;
             }
+            tile0 += w.tiles;
             ok = ok && wait(&o_full[x], o_phase);
             o_phase ^= 1u;
             tc_fence_after();

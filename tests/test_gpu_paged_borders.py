@@ -37,6 +37,29 @@ BATCHES = [
 
 @pytest.mark.parametrize("dtype", ALL)
 @pytest.mark.parametrize("layout", ["tokens", "odd"])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (64, 128), (128, 8), (96, 24)])
+@pytest.mark.parametrize("qs,ks", BATCHES)
+def test_keys_of_bad_pages_are_left_out(dtype: str, layout: str, dim: int, page: int, qs, ks) -> None:
+    """A page number outside the cache: its keys weigh nothing, in every kernel; other sequences and the
+    rest of its own are untouched. A sequence of bad pages only gets zeros."""
+    x = PagedBatch(qs, ks, heads=4, kv_heads=2, dim=dim, page=page, dtype=dtype, layout=layout)
+    present = [torch.ones(n, dtype=torch.bool, device="cuda") for n in ks]
+    bad = [-1, x.k.shape[0], 1 << 30]
+    pages = -(-ks[0] // page)
+    for i, slot in enumerate(sorted({0, pages // 2, pages - 1})):
+        x.block_table[0, slot] = bad[i]
+        present[0][slot * page : (slot + 1) * page] = False
+    x.block_table[2] = -1
+    present[2][:] = False
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = attend(x, status)
+    with pytest.raises(GraphError, match="out of range"):
+        paged.check_status(status)
+    compare(got, *reference(x, dim**-0.5, present=present))
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("layout", ["tokens", "odd"])
 @pytest.mark.parametrize("window", [0, 70])
 @pytest.mark.parametrize("length", [37, 0x7FFFFFFF])
 @pytest.mark.parametrize("qs,ks", BATCHES)
