@@ -133,9 +133,13 @@ __global__ void __launch_bounds__(256, RESIDENT<S, V>) kv_append_kernel(const __
             b = sequence_of(p.batch, t);
             end = b < 0 ? t : __ldg(p.batch.q_starts + b + 1);
             n = b < 0 ? 0 : __ldg(p.batch.kv_lens + b);
+            if (t >= end) {  // in no sequence: position -1, nowhere to cache, nothing to rotate by
+                end = t + 1;
+                n = 0;
+            }
             held = -1;
         }
-        const int pos = t >= end ? -1 : n - (end - t);  // in no sequence: nowhere to cache, nothing to rotate by
+        const int pos = n - (end - t);
         if (pos >= 0 && (held < 0 || pos / p.batch.page_size != held)) {
             held = pos / p.batch.page_size;
             page = page_of(p.batch, b, held);

@@ -147,9 +147,6 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
     const int chunks = p.head_dim / C::CH;
 
     const int split = EVEN ? 0 : (int)blockIdx.y;
-    __shared__ int bad_pages;  // set once a page number was out of range
-    if (tid == 0) bad_pages = 0;
-    if constexpr (!EVEN) __syncthreads();  // else below
     // one piece: rows row0 .. of (sequence b, key head kh) over keys [k_lo, k_hi)
     auto piece = [&](int b, int kh, const Sequence &seq, int row0, int k_lo, int k_hi, int slot) {
         const int rows = seq.nq * p.group, tiles = k_hi > k_lo ? (k_hi - k_lo + BN - 1) / BN : 0;
@@ -162,6 +159,7 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
         // Byte offset (of K and V alike) of key j of this thread's stage row, or -1: not loaded. In two
         // halves, the table's entry fetched a stage's work before it is looked at.
         const int ps = p.batch.page_size;
+        bool bad_page = false;  // met by this thread
         auto fetch_page = [&](int j) {
             const int at = j / ps;
             return j < k_hi && j >= first.lo && at < p.batch.table_pages
@@ -171,12 +169,11 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
             if (j >= k_hi || j < first.lo) return -1;
             if (page < 0 || page >= p.batch.pages) {
                 if (p.batch.status) *p.batch.status = MGC_CUDA_GATHER_OOB;
-                bad_pages = 1;
+                bad_page = true;
                 return -1;
             }
             return ((long long)page * p.page_stride + (long long)(j % ps) * p.token_stride) * (long long)sizeof(T);
         };
-        // once the CTA has met such a page, every key's is looked up again before its score counts
         auto on_page = [&](int j) {
             const int page = fetch_page(j);
             return page >= 0 && page < p.batch.pages;
@@ -222,15 +219,19 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
             }
         }
 
+        // A piece that meets a page number out of range is computed once more, `careful`: then every key's
+        // page is looked up again before its score counts. (A check of each stage cost 2 % of 64 x 8192.)
         const RowRange r0 = row_range(p, seq, row0 + 16 * wm + g4), r1 = row_range(p, seq, row0 + 16 * wm + g4 + 8);
-        float o[DB][4];
-#pragma unroll
-        for (int d = 0; d < DB; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.0f;
-        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+        float o[DB][4], m0, m1, l0, l1;
         // plain form: every row's maximum, this lane's part of its sum, and CL channels of its output
         constexpr int SR = SIMT ? SIMT : 1, CL = DP / 32;
         float so[SR][CL], sm_[SR], sl_[SR];
         RowRange sr[SR];
+        for (bool careful = false;; careful = true) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.0f;
+        m0 = m1 = -INFINITY;
+        l0 = l1 = 0.0f;
         if constexpr (SIMT > 0) {
 #pragma unroll
             for (int r = 0; r < SR; ++r) {
@@ -258,7 +259,6 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
             cp_async_commit();
             const int j_next = k_lo + (it + C::STAGES) * BN + tid;
             const int page_next = tid < BN ? fetch_page(j_next) : -1;
-            const bool check_pages = *static_cast<volatile int *>(&bad_pages) != 0;
 
             const uint8_t *st = ring + (it % C::STAGES) * C::STAGE;
             if constexpr (SIMT > 0) {
@@ -270,7 +270,7 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
                 if (j0 < k_hi) {
                     float *sP = reinterpret_cast<float *>(smem + C::SMEM) - (wn + 1) * R * KW;
                     const float4 *kr = reinterpret_cast<const float4 *>(st + (wn * KW + key) * ROW) + part * PC;
-                    const bool key_there = j < k_hi && (!check_pages || on_page(j));
+                    const bool key_there = j < k_hi && (!careful || on_page(j));
                     float x[SR];
 #pragma unroll
                     for (int r = 0; r < SR; ++r) x[r] = 0.0f;
@@ -430,7 +430,7 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
                     }
                 }
                 // mask where some row of the tile does not see some key
-                const bool whole = j0 >= all_lo && j0 + KG <= all_hi && j0 + KG <= k_hi && !check_pages;
+                const bool whole = j0 >= all_lo && j0 + KG <= all_hi && j0 + KG <= k_hi;
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
@@ -438,8 +438,19 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
                         if (!whole) {
                             const int j = j0 + nb * 8 + t4 * 2 + (e & 1);
                             const RowRange &r = e < 2 ? r0 : r1;
-                            if (j < r.lo || j >= r.hi || j >= k_hi || (check_pages && !on_page(j))) s[nb][e] = -INFINITY;
+                            if (j < r.lo || j >= r.hi || j >= k_hi) s[nb][e] = -INFINITY;
                         }
+                    }
+                }
+                if (careful) {  // a lane looks up two keys, or one
+                    uint32_t gone[2];
+                    gone[0] = __ballot_sync(0xFFFFFFFFu, lane < KG && !on_page(j0 + lane));
+                    gone[1] = __ballot_sync(0xFFFFFFFFu, lane + 32 < KG && !on_page(j0 + 32 + lane));
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (gone[nb / 4] >> (nb % 4 * 8 + t4 * 2 + (e & 1)) & 1u) s[nb][e] = -INFINITY;
                     }
                 }
                 float x0 = m0, x1 = m1;
@@ -527,7 +538,8 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
             if (tid < BN) sOff[(it % C::STAGES) * BN + tid] = offset_of(j_next, page_next);
         }
         cp_async_wait<0>();
-        __syncthreads();
+        if (!__syncthreads_or(bad_page) || careful) break;
+        }
 
         // ---- the warps' partial results, then the splits' ----
         float *red = reinterpret_cast<float *>(ring);
@@ -678,6 +690,8 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
             const Walk k = find_stretch<R, BN>(p, (int)blockIdx.x / heads, (int)gridDim.x / heads, h0,
                                                p.interleaved ? h0 + 1 : p.kv_heads, lane);
             if (lane == 0) stretch = k;
+        } else {
+            zero_outside<T>(p, (int)blockIdx.x, (int)gridDim.x, warp - 1, WM * WN - 1, lane);
         }
         __syncthreads();
         asm volatile("griddepcontrol.launch_dependents;");  // the kernel that adds the pieces waits on its own
@@ -700,6 +714,7 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
         const int b = (int)(u / (unsigned)p.row_tiles);
         const Sequence seq = load_sequence(p, b);
         if (tid == 0) check_sequence(p, b);
+        zero_outside<T>(p, (int)(blockIdx.y * gridDim.x + blockIdx.x), (int)(gridDim.x * gridDim.y), warp, WM * WN, lane);
         for (int tile = tile0; tile * R < seq.nq * p.group; tile += p.row_tiles) {
             const RowRange z = row_range(p, seq, min(tile * R + R, seq.nq * p.group) - 1);
             const int lo = row_range(p, seq, tile * R).lo & ~15, hi = max(z.hi, 0);
@@ -710,7 +725,6 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
             piece(b, kh, seq, tile * R, k_lo, min(hi, k_lo + per), -1);
         }
     }
-    zero_outside<T>(p, (int)(blockIdx.y * gridDim.x + blockIdx.x), (int)(gridDim.x * gridDim.y), warp, WM * WN, lane);
 }
 
 }  // namespace paged

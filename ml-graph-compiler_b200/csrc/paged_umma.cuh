@@ -18,8 +18,8 @@
 //   rescale needs no wait: S of tile j is committed after P V of tile j - 1.
 // * 64 channels leave TMEM for weights apart from the scores: the next tile's scores are made
 //   while this one's weights are.
-// * A page number out of range: the loading warp writes zeros where its keys and values would be and
-//   names the boxes (wrong_boxes), whose scores the softmax warps mask.
+// * A page number out of range: its keys are not loaded, the products use whatever the stage held, and
+//   at the unit's end its rows are computed again one per thread, without those keys (row_again).
 // * Rows of V that no row sees (past the last visible key, before the first) are zeroed in shared
 //   memory before they are used: a page's unused rows hold anything, and 0 * NaN is NaN.
 //
@@ -194,6 +194,72 @@ __device__ __forceinline__ int tiles_needed(const AttendParams &p, const Item &w
     return min(w.tiles, (max(mid.hi - w.lo, 0) + 127) >> 7);
 }
 
+// The slow way round for rows whose tiles held something that they do not see: this thread's row over
+// the keys of piece w that it sees, on the FMA units. Maximum and sum first, then the output, 32
+// channels at a time, into TMEM where the products would have left it. The whole warp calls.
+template <typename T, int DP>
+__device__ __forceinline__ void row_again(const AttendParams &p, const Item &w, int row, uint32_t to, float &m, float &l) {
+    const RowRange see = row_range(p, w.seq, row);
+    const int lo = max(see.lo, w.lo), hi = min(see.hi, w.hi);
+    const T *q = static_cast<const T *>(p.q) + (long long)(w.seq.start + row / p.group) * p.q_ts +
+                 (long long)(w.h * p.group + row % p.group) * p.q_hs;
+    const long long head = (long long)w.h * p.head_stride;
+    auto at = [&](int j) -> long long {
+        const int page = page_of(p.batch, w.b, j / p.batch.page_size);
+        return page < 0 ? -1 : (long long)page * p.page_stride + (long long)(j % p.batch.page_size) * p.token_stride + head;
+    };
+    auto score = [&](long long off) {
+        const T *k = static_cast<const T *>(p.k_pages) + off;
+        float s = 0.0f;
+#pragma unroll 1
+        for (int c = 0; c < p.head_dim; c += 8) {
+            Pack<8, T> x, y;
+            x.load(q + c);
+            y.load(k + c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s = fmaf(to_f(x.e[i]), to_f(y.e[i]), s);
+        }
+        return s * p.scale_log2;
+    };
+    m = -INFINITY;
+    l = 0.0f;
+#pragma unroll 1
+    for (int j = lo; j < hi; ++j) {
+        const long long off = at(j);
+        if (off < 0) continue;
+        const float s = score(off), top = fmaxf(m, s);
+        if (s == -INFINITY) continue;
+        l = l * (top == -INFINITY ? 1.0f : ex2(m - top)) + ex2(s - top);
+        m = top;
+    }
+#pragma unroll 1
+    for (int c0 = 0; c0 < DP; c0 += 32) {
+        float o[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+#pragma unroll 1
+        for (int j = lo; j < hi; ++j) {
+            const long long off = at(j);
+            if (off < 0) continue;
+            const float s = score(off), wgt = s == -INFINITY ? 0.0f : ex2(s - m);
+#pragma unroll
+            for (int c = 0; c < 32; c += 8) {
+                if (c0 + c >= p.head_dim) continue;
+                Pack<8, T> v;
+                v.load(static_cast<const T *>(p.v_pages) + off + c0 + c);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[c + i] = fmaf(wgt, to_f(v.e[i]), o[c + i]);
+            }
+        }
+        uint32_t t[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) t[i] = __float_as_uint(o[i]);
+        __syncwarp();
+        tmem_st32(to + c0, t);
+    }
+    tmem_wait_st();
+}
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(UmmaConfig<DP>::THREADS, 1)
 paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid_constant__ UmmaMaps maps) {
@@ -203,14 +269,12 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
     __shared__ __align__(8) uint64_t z_ask, z_done;
     __shared__ uint32_t tslot;
     __shared__ Walk stretch;
-    // bit l of entry t % 8: lane l's box of the CTA's t-th key tile has no page. An entry is written before
-    // its K tile is announced; by then the weights of the fifth tile before it, at the latest, are done, so
-    // eight entries outlast their readers.
-    __shared__ uint32_t wrong_boxes[8];
+    __shared__ int bad_page;  // a page number was out of range
     uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *sQ = base, *ring = base + 2 * C::TILE;
     const int tid = (int)threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
     if (tid == 0) {
+        bad_page = 0;
         for (int s = 0; s < C::STAGES; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
@@ -235,6 +299,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
         const Walk k = find_stretch<256, 128>(p, (int)blockIdx.x, (int)gridDim.x, 0, p.kv_heads, lane);
         if (lane == 0) stretch = k;
     }
+    if (warp == 10) zero_outside<T>(p, (int)blockIdx.x, (int)gridDim.x, 0, 1, lane);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -253,40 +318,29 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::OTHER_REGS));
         if (warp == 9) {
             // ---------------- loads ----------------
-            int slot = 0, laps = 0, issued = 0, tile = 0;
+            int slot = 0, laps = 0, issued = 0;
             const int boxes = (128 / maps.box_rows) * C::HALVES;  // of a tile: at most 32
             const int part = lane / C::HALVES, half = lane % C::HALVES;
             bool ok = true;
             while (ok && next_item<256, 128>(p, walk, w)) {
-                // this lane's box of key tile j: page and first row in it; -1 if no row sees its keys, -2
-                // if it should have a page
+                // this lane's box of key tile j: page and first row in it; -1 if no row sees its keys
                 auto box = [&](int j, int &row) {
                     const int at = w.lo + j * 128 + part * maps.box_rows;
                     row = at % p.batch.page_size;
                     if (lane >= boxes || j >= w.tiles || at >= w.hi || at + maps.box_rows <= w.first) return -1;
                     const int page = page_of(p.batch, w.b, at / p.batch.page_size);
-                    return page < 0 ? -2 : page;
+                    if (page < 0) *static_cast<volatile int *>(&bad_page) = 1;
+                    return page;
                 };
                 int row, page = box(0, row);
                 for (int j = 0; ok && j < w.tiles; ++j) {
                     int next_row, next = box(j + 1, next_row);  // looked up one tile ahead
                     const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xFFFFFFFFu, page >= 0)) * (uint32_t)maps.box_rows * 128u;
-                    const uint32_t wrong = __ballot_sync(0xFFFFFFFFu, page == -2);
 #pragma unroll
                     for (int kv = 0; kv < 2; ++kv) {
                         if (laps > 0) ok = ok && wait(&empty[slot], (uint32_t)(laps - 1) & 1u);
                         if (!ok) break;
-                        if (wrong) {
-                            uint4 *z = reinterpret_cast<uint4 *>(ring + slot * C::TILE + half * C::HALF + part * maps.box_rows * 128);
-                            if (page == -2)
-                                for (int i = 0; i < maps.box_rows * 8; ++i) z[i] = make_uint4(0, 0, 0, 0);
-                            umma::fence_proxy_async_smem();
-                            __syncwarp();
-                        }
-                        if (lane == 0) {
-                            if (kv == 0) *static_cast<volatile uint32_t *>(&wrong_boxes[tile & 7]) = wrong;
-                            mbar_expect_tx(&full[slot], bytes);
-                        }
+                        if (lane == 0) mbar_expect_tx(&full[slot], bytes);
                         __syncwarp();
                         if (page >= 0)
                             umma::tma_load_4d(ring + slot * C::TILE + half * C::HALF + part * maps.box_rows * 128,
@@ -299,7 +353,6 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                     }
                     page = next;
                     row = next_row;
-                    ++tile;
                 }
             }
             // after a timeout, the copies still in flight
@@ -433,12 +486,11 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                 slot = (slot + 2 * w.tiles) % C::STAGES;
             }
         } else {
-            // ---------------- warp 11: how many pieces has the unit cut at the stretch's end? Rows of no sequence ----------------
+            // ---------------- warp 11: how many pieces has the unit cut at the stretch's end? ----------------
             CutUnit cut{0, 0, 0, 0};
             while (next_item<256, 128>(p, walk, w))
                 if (w.slot == 1) cut = cut_of<256, 128>(p, walk, w);
             if (lane == 0) p.cut[blockIdx.x] = cut;
-            zero_outside<T>(p, (int)blockIdx.x, (int)gridDim.x, 0, 1, lane);
         }
     } else {
         // ---------------- softmax: one row per thread ----------------
@@ -448,7 +500,6 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
         const uint32_t ts = tbase + lanes + C::S_COL + x * 128, to = tbase + lanes + C::O_COL + x * DP;
         const uint32_t tp = tbase + lanes + C::P_COL + x * C::P_STEP;
         uint32_t s_phase = 0, o_phase = 0, free_phase = 0;
-        int tile0 = 0;  // the CTA's key tiles before this piece
         bool ok = true;
         while (ok && next_item<256, 128>(p, walk, w)) {
             const int row = w.row0 + x * 128 + r;
@@ -519,12 +570,6 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                         }
                     }
                 }
-                if (const uint32_t wrong = *static_cast<volatile uint32_t *>(&wrong_boxes[(tile0 + j) & 7])) {
-                    const int shift = 31 - __clz(maps.box_rows);  // box sizes are powers of two
-#pragma unroll
-                    for (int i = 0; i < 128; ++i)
-                        if (wrong >> ((i >> shift) * C::HALVES) & 1u) s[i] = -INFINITY;
-                }
                 float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
                 for (int i = 4; i < 124; i += 8) {
@@ -578,11 +623,17 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                 sum[0] = add2(sum[0], sum[1]);
                 l += sum[0].x + sum[0].y;
             }
-            tile0 += w.tiles;
             ok = ok && wait(&o_full[x], o_phase);
             o_phase ^= 1u;
             tc_fence_after();
             if (!ok) break;
+            if (*static_cast<volatile int *>(&bad_page) && need > 0) {  // of this piece?
+                bool bad = false;
+                for (int at = max(w.lo, w.first) / p.batch.page_size + lane; at <= (w.hi - 1) / p.batch.page_size; at += 32)
+                    bad = bad || page_of(p.batch, w.b, at) < 0;
+                if (__any_sync(0xFFFFFFFFu, bad))
+                    row_again<T, DP>(p, w, w.row0 + x * 128 + r, to, m, l);
+            }
             // ---- O: through the warp's rows of the Q tile (no longer read) to whole rows of memory ----
             const bool whole = w.slot < 0;
             const long long at = ((long long)blockIdx.x * 2 + w.slot) * 256 + x * 128 + (r & 96);  // a piece's first row
