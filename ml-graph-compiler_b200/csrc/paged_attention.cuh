@@ -28,43 +28,13 @@ __global__ void __launch_bounds__(128) paged_attention_row_kernel(const __grid_c
     const int n = __ldg(p.batch.kv_lens + b);
     int lo, hi;
     visible(p, min(n, p.max_positions), n - (end - t), lo, hi);
-    const T *q = static_cast<const T *>(p.q) + t * p.q_ts + h * p.q_hs;
-    const long long head = (h / p.group) * p.head_stride;
-    float qv[C], o[C], m = -INFINITY, l = 0.0f;
+    RowSum<C> x;
+    x.over_keys<T>(p, b, h / p.group, static_cast<const T *>(p.q) + t * p.q_ts + h * p.q_hs, lo, hi, lane);
+    const float inv = x.l > 0.0f ? 1.0f / x.l : 0.0f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const int d = lane + 32 * c;
-        qv[c] = d < p.head_dim ? to_f(q[d]) * p.scale_log2 : 0.0f;
-        o[c] = 0.0f;
-    }
-    for (int j = lo; j < hi; ++j) {
-        const int page = page_of(p.batch, b, j / p.batch.page_size);
-        if (page < 0) continue;
-        const long long at = page * p.page_stride + (j % p.batch.page_size) * p.token_stride + head;
-        const T *k = static_cast<const T *>(p.k_pages) + at, *v = static_cast<const T *>(p.v_pages) + at;
-        float s = 0.0f;
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int d = lane + 32 * c;
-            if (d < p.head_dim) s += qv[c] * to_f(k[d]);
-        }
-#pragma unroll
-        for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, x);
-        if (s == -INFINITY) continue;  // weighs nothing (and would leave -inf - -inf at the start)
-        const float m2 = fmaxf(m, s), scale = exp2f(m - m2), w = exp2f(s - m2);
-        l = l * scale + w;
-        m = m2;
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int d = lane + 32 * c;
-            if (d < p.head_dim) o[c] = o[c] * scale + w * to_f(v[d]);
-        }
-    }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-        const int d = lane + 32 * c;
-        if (d < p.head_dim) out[d] = from_f<T>(o[c] * inv);
+        if (d < p.head_dim) out[d] = from_f<T>(x.o[c] * inv);
     }
 }
 

@@ -174,10 +174,6 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
             }
             return ((long long)page * p.page_stride + (long long)(j % ps) * p.token_stride) * (long long)sizeof(T);
         };
-        auto on_page = [&](int j) {
-            const int page = fetch_page(j);
-            return page >= 0 && page < p.batch.pages;
-        };
         auto load_stage = [&](int it) {
             uint8_t *st = ring + (it % C::STAGES) * C::STAGE;
             const long long *off = sOff + (it % C::STAGES) * BN;
@@ -219,15 +215,12 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
             }
         }
 
-        // A piece that meets a page number out of range is computed once more, `careful`: then every key's
-        // page is looked up again before its score counts. (A check of each stage cost 2 % of 64 x 8192.)
         const RowRange r0 = row_range(p, seq, row0 + 16 * wm + g4), r1 = row_range(p, seq, row0 + 16 * wm + g4 + 8);
         float o[DB][4], m0, m1, l0, l1;
         // plain form: every row's maximum, this lane's part of its sum, and CL channels of its output
         constexpr int SR = SIMT ? SIMT : 1, CL = DP / 32;
         float so[SR][CL], sm_[SR], sl_[SR];
         RowRange sr[SR];
-        for (bool careful = false;; careful = true) {
 #pragma unroll
         for (int d = 0; d < DB; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.0f;
         m0 = m1 = -INFINITY;
@@ -270,7 +263,6 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
                 if (j0 < k_hi) {
                     float *sP = reinterpret_cast<float *>(smem + C::SMEM) - (wn + 1) * R * KW;
                     const float4 *kr = reinterpret_cast<const float4 *>(st + (wn * KW + key) * ROW) + part * PC;
-                    const bool key_there = j < k_hi && (!careful || on_page(j));
                     float x[SR];
 #pragma unroll
                     for (int r = 0; r < SR; ++r) x[r] = 0.0f;
@@ -287,7 +279,7 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
                     for (int r = 0; r < SR; ++r) {
 #pragma unroll
                         for (int d = KW; d < 32; d <<= 1) x[r] += __shfl_xor_sync(0xFFFFFFFFu, x[r], d);
-                        if (j < sr[r].lo || j >= sr[r].hi || !key_there) x[r] = -INFINITY;
+                        if (j < sr[r].lo || j >= sr[r].hi || j >= k_hi) x[r] = -INFINITY;
                         float top = x[r];
 #pragma unroll
                         for (int d = 1; d < KW; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
@@ -442,17 +434,6 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
                         }
                     }
                 }
-                if (careful) {  // a lane looks up two keys, or one
-                    uint32_t gone[2];
-                    gone[0] = __ballot_sync(0xFFFFFFFFu, lane < KG && !on_page(j0 + lane));
-                    gone[1] = __ballot_sync(0xFFFFFFFFu, lane + 32 < KG && !on_page(j0 + 32 + lane));
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (gone[nb / 4] >> (nb % 4 * 8 + t4 * 2 + (e & 1)) & 1u) s[nb][e] = -INFINITY;
-                    }
-                }
                 float x0 = m0, x1 = m1;
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
@@ -538,13 +519,50 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
             if (tid < BN) sOff[(it % C::STAGES) * BN + tid] = offset_of(j_next, page_next);
         }
         cp_async_wait<0>();
-        if (!__syncthreads_or(bad_page) || careful) break;
+        // The piece is computed again, row by row and only with the keys that a row sees, if it met a page
+        // number out of range or if NaN came out that need not belong there (the row's sum is none): a
+        // weight 0 of a key that a row does not see times a value that is not finite, or the split of an
+        // infinite value. Where every row sees every key the 16-bit and the plain form cannot have made
+        // one. (Looking at each stage cost 2 % of 64 x 8192 in bf16.)
+        bool again = bad_page;
+        const bool partly = all_lo > first.lo || all_hi < last.hi;
+        if constexpr (SIMT > 0) {
+            if (partly) {
+#pragma unroll
+                for (int r = 0; r < SR; ++r) {
+#pragma unroll
+                    for (int i = 0; i < CL; ++i) again = again || (so[r][i] != so[r][i] && sl_[r] == sl_[r]);
+                }
+            }
+        } else if (C::F32 || partly) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                again = again || (l0 == l0 && (o[d][0] != o[d][0] || o[d][1] != o[d][1]));
+                again = again || (l1 == l1 && (o[d][2] != o[d][2] || o[d][3] != o[d][3]));
+            }
         }
+        again = __syncthreads_or(again);
 
         // ---- the warps' partial results, then the splits' ----
         float *red = reinterpret_cast<float *>(ring);
         float *sm = red + WN * R * C::ORED, *sl = sm + WN * R;
-        if constexpr (SIMT > 0) {
+        if (again) {  // as the first slice's result, the others empty
+            for (int r = warp; r < R; r += WM * WN) {
+                RowSum<DP / 32> x;
+                const RowRange see = row_range(p, seq, row0 + r);
+                x.template over_keys<T>(p, b, kh, row0 + r < rows ? q_ptr(row0 + r) : nullptr, max(see.lo, k_lo), min(see.hi, k_hi), lane);
+#pragma unroll 1
+                for (int s = 0; s < WN; ++s) {
+#pragma unroll
+                    for (int c = 0; c < DP / 32; ++c) red[(s * R + r) * C::ORED + lane + 32 * c] = s ? 0.0f : x.o[c];
+                    if (lane == 0) {
+                        sm[s * R + r] = s ? -INFINITY : x.m;
+                        sl[s * R + r] = s ? 0.0f : x.l;
+                    }
+                }
+            }
+            __syncthreads();
+        } else if constexpr (SIMT > 0) {
 #pragma unroll
             for (int r = 0; r < SR; ++r) {
 #pragma unroll

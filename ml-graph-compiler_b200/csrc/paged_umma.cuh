@@ -20,6 +20,9 @@
 //   while this one's weights are.
 // * A page number out of range: its keys are not loaded, the products use whatever the stage held, and
 //   at the unit's end its rows are computed again one per thread, without those keys (row_again).
+// * A value that is not finite, at a key that some rows of a tile see and others do not: 0 * inf is NaN.
+//   Rows that come out with NaN or infinities and do not see such a key of their tiles are computed
+//   again too.
 // * Rows of V that no row sees (past the last visible key, before the first) are zeroed in shared
 //   memory before they are used: a page's unused rows hold anything, and 0 * NaN is NaN.
 //
@@ -196,9 +199,10 @@ __device__ __forceinline__ int tiles_needed(const AttendParams &p, const Item &w
 
 // The slow way round for rows whose tiles held something that they do not see: this thread's row over
 // the keys of piece w that it sees, on the FMA units. Maximum and sum first, then the output, 32
-// channels at a time, into TMEM where the products would have left it. The whole warp calls.
+// channels at a time, into TMEM where the products would have left it. The whole warp calls; threads
+// without `all` compute their row only if a key that it does not see has a value that is not finite.
 template <typename T, int DP>
-__device__ __forceinline__ void row_again(const AttendParams &p, const Item &w, int row, uint32_t to, float &m, float &l) {
+__device__ __forceinline__ void row_again(const AttendParams &p, const Item &w, int row, bool all, bool maybe, uint32_t to, float &m, float &l) {
     const RowRange see = row_range(p, w.seq, row);
     const int lo = max(see.lo, w.lo), hi = min(see.hi, w.hi);
     const T *q = static_cast<const T *>(p.q) + (long long)(w.seq.start + row / p.group) * p.q_ts +
@@ -221,10 +225,31 @@ __device__ __forceinline__ void row_again(const AttendParams &p, const Item &w, 
         }
         return s * p.scale_log2;
     };
-    m = -INFINITY;
-    l = 0.0f;
+    if (!all && maybe) {
 #pragma unroll 1
-    for (int j = lo; j < hi; ++j) {
+        for (int j = max(w.lo, w.first); j < w.hi && !all; ++j) {
+            if (j == lo && lo < hi) j = hi;  // those it sees
+            if (j >= w.hi) break;
+            const long long off = at(j);
+            if (off < 0) continue;
+            float z = 0.0f;
+#pragma unroll 1
+            for (int c = 0; c < p.head_dim; c += 8) {
+                Pack<8, T> v;
+                v.load(static_cast<const T *>(p.v_pages) + off + c);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) z = fmaf(to_f(v.e[i]), 0.0f, z);
+            }
+            all = z != z;
+        }
+    }
+    if (!__any_sync(0xFFFFFFFFu, all)) return;
+    if (all) {
+        m = -INFINITY;
+        l = 0.0f;
+    }
+#pragma unroll 1
+    for (int j = all ? lo : hi; j < hi; ++j) {
         const long long off = at(j);
         if (off < 0) continue;
         const float s = score(off), top = fmaxf(m, s);
@@ -235,10 +260,14 @@ __device__ __forceinline__ void row_again(const AttendParams &p, const Item &w, 
 #pragma unroll 1
     for (int c0 = 0; c0 < DP; c0 += 32) {
         float o[32];
+        uint32_t t[32];
+        __syncwarp();
+        umma::tmem_ld32(to + c0, t);
+        umma::tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+        for (int i = 0; i < 32; ++i) o[i] = all ? 0.0f : __uint_as_float(t[i]);
 #pragma unroll 1
-        for (int j = lo; j < hi; ++j) {
+        for (int j = all ? lo : hi; j < hi; ++j) {
             const long long off = at(j);
             if (off < 0) continue;
             const float s = score(off), wgt = s == -INFINITY ? 0.0f : ex2(s - m);
@@ -251,7 +280,6 @@ __device__ __forceinline__ void row_again(const AttendParams &p, const Item &w, 
                 for (int i = 0; i < 8; ++i) o[c + i] = fmaf(wgt, to_f(v.e[i]), o[c + i]);
             }
         }
-        uint32_t t[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) t[i] = __float_as_uint(o[i]);
         __syncwarp();
@@ -627,12 +655,28 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
             o_phase ^= 1u;
             tc_fence_after();
             if (!ok) break;
-            if (*static_cast<volatile int *>(&bad_page) && need > 0) {  // of this piece?
-                bool bad = false;
-                for (int at = max(w.lo, w.first) / p.batch.page_size + lane; at <= (w.hi - 1) / p.batch.page_size; at += 32)
-                    bad = bad || page_of(p.batch, w.b, at) < 0;
-                if (__any_sync(0xFFFFFFFFu, bad))
-                    row_again<T, DP>(p, w, w.row0 + x * 128 + r, to, m, l);
+            if (need > 0) {
+                bool bad = false;  // a page of this piece
+                if (*static_cast<volatile int *>(&bad_page)) {
+                    for (int at = max(w.lo, w.first) / p.batch.page_size + lane; at <= (w.hi - 1) / p.batch.page_size; at += 32)
+                        bad = bad || page_of(p.batch, w.b, at) < 0;
+                    bad = __any_sync(0xFFFFFFFFu, bad);
+                }
+                // a row that is not finite, although its scores are, and that does not see all of the piece
+                bool maybe = live && l == l && (see.lo > max(w.lo, w.first) || see.hi < w.hi);
+                if (__any_sync(0xFFFFFFFFu, maybe)) {
+                    float odd[2] = {0.0f, 0.0f};  // NaN once a channel is not finite
+#pragma unroll
+                    for (int c = 0; c < DP / 32; ++c) {
+                        uint32_t t[32];
+                        umma::tmem_ld32(to + c * 32, t);
+                        umma::tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) odd[i & 1] = fmaf(__uint_as_float(t[i]), 0.0f, odd[i & 1]);
+                    }
+                    maybe = maybe && odd[0] + odd[1] != 0.0f;
+                }
+                if (bad || __any_sync(0xFFFFFFFFu, maybe)) row_again<T, DP>(p, w, w.row0 + x * 128 + r, bad, maybe, to, m, l);
             }
             // ---- O: through the warp's rows of the Q tile (no longer read) to whole rows of memory ----
             const bool whole = w.slot < 0;

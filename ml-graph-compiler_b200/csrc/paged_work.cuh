@@ -55,6 +55,49 @@ __device__ __forceinline__ RowRange row_range(const AttendParams &p, const Seque
     return r;
 }
 
+// One query row by the definition, a key at a time, lane l holding channels l, l + 32, ...: maximum
+// (scaled, base 2), sum, output. What the kernels for unaligned operands and the pieces with missing
+// pages or values that are not finite take.
+template <int C> struct RowSum {
+    float o[C], m, l;
+    template <typename T>
+    __device__ __forceinline__ void over_keys(const AttendParams &p, int b, int kh, const T *q, int lo, int hi, int lane) {
+        const long long head = kh * p.head_stride;
+        float qv[C];
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int d = lane + 32 * c;
+            qv[c] = lo < hi && d < p.head_dim ? to_f(q[d]) * p.scale_log2 : 0.0f;
+            o[c] = 0.0f;
+        }
+        for (int j = lo; j < hi; ++j) {
+            const int page = page_of(p.batch, b, j / p.batch.page_size);
+            if (page < 0) continue;
+            const long long at = page * p.page_stride + (j % p.batch.page_size) * p.token_stride + head;
+            const T *k = static_cast<const T *>(p.k_pages) + at, *v = static_cast<const T *>(p.v_pages) + at;
+            float s = 0.0f;
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const int d = lane + 32 * c;
+                if (d < p.head_dim) s += qv[c] * to_f(k[d]);
+            }
+#pragma unroll
+            for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, x);
+            if (s == -INFINITY) continue;  // weighs nothing (and would leave -inf - -inf at the start)
+            const float m2 = fmaxf(m, s), scale = exp2f(m - m2), w = exp2f(s - m2);
+            l = l * scale + w;
+            m = m2;
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const int d = lane + 32 * c;
+                if (d < p.head_dim) o[c] = o[c] * scale + w * to_f(v[d]);
+            }
+        }
+    }
+};
+
 // A unit is (key head, sequence, ROWS query rows) and is as long as it has tiles of KEYS keys (at
 // least 1). All units lie end to end, key head by key head; CTA c takes the c-th of `ctas` equal
 // stretches. A stretch that ends inside a unit cuts it (unless a piece would be below MIN_PIECE

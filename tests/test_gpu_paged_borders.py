@@ -199,3 +199,44 @@ def test_rows_without_any_sequence(dtype: str) -> None:
     out = torch.full(x.q.shape, math.nan, dtype=x.q.dtype, device="cuda")
     assert not paged.paged_attention(x.q, *x.operands, out=out).any()
     assert torch.equal(paged.kv_append(x.q[:, :2], x.q[:, :2], *x.operands, q=x.q), x.q)
+
+
+# ---- values that are not finite ------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("layout", ["tokens", "odd"])
+@pytest.mark.parametrize("qs,ks", [([1], [300]), ([1, 1], [9000, 40]), ([2], [90]), ([4, 1], [300, 33]), ([9], [100]), ([30], [200])])
+def test_infinite_and_nan_values_that_are_seen(dtype: str, layout: str, qs, ks) -> None:
+    """A value's infinity or NaN reaches its channel and no other."""
+    x = PagedBatch(qs, ks, heads=2, kv_heads=2, dim=64, page=16, dtype=dtype, layout=layout)
+    page, row = x.slots[0]
+    x.v[page[5], row[5], 0, 3] = math.inf
+    x.v[page[6], row[6], 0, 4] = -math.inf
+    x.v[page[7], row[7], 1, 5] = math.nan
+    x.v[page[8], row[8], 1, 6] = math.inf
+    x.v[page[9], row[9], 1, 6] = -math.inf
+    if dtype == "f32":
+        x.v[page[10], row[10], 0, 7] = 3.4028e38
+    compare(attend(x), *reference(x, 64**-0.5))
+
+
+HIDDEN = [([3], [40], 0), ([2, 1], [300, 40], 0), ([4], [40], 8), ([24], [300], 0), ([24], [300], 50), ([60], [700], 300),
+          ([150], [400], 0), ([300], [400], 0), ([300, 40], [1500, 90], 100), ([600], [600], 70)]
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("layout", ["tokens", "odd"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("qs,ks,window", HIDDEN)
+def test_values_that_a_row_does_not_see_do_not_reach_it(dtype: str, layout: str, dim: int, qs, ks, window: int) -> None:
+    """Infinities and NaN at positions that some new tokens see and others, earlier or later ones, do not."""
+    x = PagedBatch(qs, ks, heads=4, kv_heads=2, dim=dim, page=16, dtype=dtype, layout=layout)
+    page, row = x.slots[0]
+    n, first = ks[0], ks[0] - qs[0]
+    for i, at in enumerate(sorted({n - 1, n - 2, first + qs[0] // 2, first + 1, max(0, first - window), max(0, first - window + 1)})):
+        x.v[page[at], row[at], :, 2 * i] = (math.inf, math.nan, -math.inf)[i % 3]
+        x.k[page[at], row[at], 1, 0] = (math.nan, math.inf)[i % 2] if at == n - 1 else x.k[page[at], row[at], 1, 0]
+    want, bound = reference(x, dim**-0.5, window=window)
+    got = attend(x, window=window)
+    # the last token sees a key that is not finite: what its second head group gets is undefined
+    want[x.rows(0).stop - 1, 2:], got[x.rows(0).stop - 1, 2:], bound[x.rows(0).stop - 1, 2:] = 0.0, 0.0, 1.0
+    compare(got, want, bound)
