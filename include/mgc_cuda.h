@@ -360,12 +360,13 @@ int mgc_cuda_kv_append(const mgc_cuda_kv_append_args *args, void *stream);
 /* mgc_cuda_paged_attention: out[t][h] = sum_j w_j v_j, w the softmax over the visible positions j of
  * scale * q[t][h] . k_j, key head h / (q_heads / kv_heads). Visible to a token at position p:
  * j < kv_lens[b]; with `causal`, j <= p; with window > 0 (causal only), j > p - window. A token
- * with no visible position, or in no sequence, gets zeros (a call with batch 0 does nothing). q and out are of the pages' type. Cache rows that a token
- * does not see do not reach it, whatever they hold. max_q and max_kv, the longest sequence's
- * new tokens and positions, are host values that size the launch: longer sequences are computed
- * too, by fewer blocks than they could use. `workspace` (16-byte aligned) holds partial results when
- * a row's keys are split over many blocks; when it is smaller than
- * mgc_cuda_paged_attention_workspace says (0 for most calls), the call returns
+ * with no visible position, or in no sequence, gets zeros (a call with batch 0 does nothing). q and
+ * out are of the pages' type. Cache rows that a token does not see do not reach it, whatever they
+ * hold. max_q and max_kv, the longest sequence's new tokens and positions, are host values that size
+ * the launch: longer sequences are computed too, by fewer blocks than they could use. `workspace`
+ * (16-byte aligned) holds partial results when units of rows are cut and shared out over all SMs, as
+ * in 16-bit chunks (39 MB at 128 channels on 148 SMs) and in large batches; when it is smaller than
+ * mgc_cuda_paged_attention_workspace says (0 for single tokens of a few sequences), the call returns
  * MGC_CUDA_NEEDS_WORKSPACE and nothing runs. A wait that runs out sets *status_dev to
  * MGC_CUDA_TIMEOUT. */
 typedef struct {

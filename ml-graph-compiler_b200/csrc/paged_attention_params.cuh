@@ -19,6 +19,14 @@ struct CutUnit {
 
 constexpr int MAX_HEAD_DIM = 256;
 
+// Half has five exponent bits: a weight below 2^-14 of the largest would lose bits and one below 2^-25
+// vanish from the products (not from the sum), and a long context can hold much of its mass there. So
+// f16 weights are made 2^LIFT times as large; output and sum carry the factor and it cancels. The tcgen05
+// kernel lets weights grow to 2^LAZY before it moves their reference: 2^15 at most in either kernel.
+// What is left of the range: steps of 2^-38 of the largest weight, 2^-35 at least in the tcgen05 kernel.
+template <typename T> struct Weight { static constexpr float LIFT = 0.0f, LAZY = 8.0f, LAZY_LIFT = 0.0f; };
+template <> struct Weight<__half> { static constexpr float LIFT = 14.0f, LAZY = 4.0f, LAZY_LIFT = 11.0f; };
+
 struct AttendParams {
     Batch batch;
     const void *k_pages, *v_pages;

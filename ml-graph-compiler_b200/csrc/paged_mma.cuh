@@ -448,16 +448,17 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
                 // nothing yet has the maximum -inf: subtract 0 instead
                 const float y0 = x0 == -INFINITY ? 0.0f : x0 * p.scale_log2, y1 = x1 == -INFINITY ? 0.0f : x1 * p.scale_log2;
                 const float a0 = ex2(m0 * p.scale_log2 - y0), a1 = ex2(m1 * p.scale_log2 - y1);
+                const float z0 = Weight<T>::LIFT - y0, z1 = Weight<T>::LIFT - y1;
                 m0 = x0;
                 m1 = x1;
                 l0 *= a0;
                 l1 *= a1;
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
-                    s[nb][0] = ex2(fmaf(s[nb][0], p.scale_log2, -y0));
-                    s[nb][1] = ex2(fmaf(s[nb][1], p.scale_log2, -y0));
-                    s[nb][2] = ex2(fmaf(s[nb][2], p.scale_log2, -y1));
-                    s[nb][3] = ex2(fmaf(s[nb][3], p.scale_log2, -y1));
+                    s[nb][0] = ex2(fmaf(s[nb][0], p.scale_log2, z0));
+                    s[nb][1] = ex2(fmaf(s[nb][1], p.scale_log2, z0));
+                    s[nb][2] = ex2(fmaf(s[nb][2], p.scale_log2, z1));
+                    s[nb][3] = ex2(fmaf(s[nb][3], p.scale_log2, z1));
                     l0 += s[nb][0] + s[nb][1];
                     l1 += s[nb][2] + s[nb][3];
                 }

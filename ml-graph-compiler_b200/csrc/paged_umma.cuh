@@ -13,8 +13,8 @@
 //   K and V tiles in the order K0 V0 K1 V1 ... K is a K-major operand, V (channels contiguous) an
 //   MN-major one. Channels past the head width are the tensor map's zero fill.
 // * The maximum is lazy: O (in TMEM) is rescaled only when a row's maximum has grown by more than
-//   2^8 since the last time; the weights then stay below 2^8, far from overflow in either type,
-//   and the row sum carries the same reference, so the result is unchanged. With 128 channels a
+//   2^8 (f16: 2^4) since the last time; the weights then stay below 2^8 (f16: 2^15, Weight), far from
+//   overflow, and the row sum carries the same reference, so the result is unchanged. With 128 channels a
 //   rescale needs no wait: S of tile j is committed after P V of tile j - 1.
 // * 64 channels leave TMEM for weights apart from the scores: the next tile's scores are made
 //   while this one's weights are.
@@ -254,7 +254,7 @@ __device__ __forceinline__ void row_again(const AttendParams &p, const Item &w, 
         if (off < 0) continue;
         const float s = score(off), top = fmaxf(m, s);
         if (s == -INFINITY) continue;
-        l = l * (top == -INFINITY ? 1.0f : ex2(m - top)) + ex2(s - top);
+        l = l * (top == -INFINITY ? 1.0f : ex2(m - top)) + ex2(s - top + Weight<T>::LAZY_LIFT);
         m = top;
     }
 #pragma unroll 1
@@ -270,7 +270,7 @@ __device__ __forceinline__ void row_again(const AttendParams &p, const Item &w, 
         for (int j = all ? lo : hi; j < hi; ++j) {
             const long long off = at(j);
             if (off < 0) continue;
-            const float s = score(off), wgt = s == -INFINITY ? 0.0f : ex2(s - m);
+            const float s = score(off), wgt = s == -INFINITY ? 0.0f : ex2(s - m + Weight<T>::LAZY_LIFT);
 #pragma unroll
             for (int c = 0; c < 32; c += 8) {
                 if (c0 + c >= p.head_dim) continue;
@@ -607,8 +607,8 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
 #pragma unroll
                 for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], s[124 + e]);
                 const float mt = __fmul_rn(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), p.scale_log2);
-                // grown by more than 2^8 (or the first finite maximum): move the reference
-                const bool grow = mt > m + 8.0f;
+                // grown by more than 2^LAZY (or the first finite maximum): move the reference
+                const bool grow = mt > m + Weight<T>::LAZY;
                 if (C::APART && j > 0) {  // the products with the last tile's weights are done
                     ok = wait(&p_free[x], free_phase);
                     free_phase ^= 1u;
@@ -630,7 +630,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                 }
                 if (grow) m = mt;
                 const float y = m == -INFINITY ? 0.0f : m;
-                const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), y2 = make_float2(-y, -y);
+                const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), y2 = make_float2(Weight<T>::LAZY_LIFT - y, Weight<T>::LAZY_LIFT - y);
                 float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {  // the first 64 keys' products start while the others' weights are made

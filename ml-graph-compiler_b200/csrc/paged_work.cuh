@@ -86,7 +86,7 @@ template <int C> struct RowSum {
 #pragma unroll
             for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, x);
             if (s == -INFINITY) continue;  // weighs nothing (and would leave -inf - -inf at the start)
-            const float m2 = fmaxf(m, s), scale = exp2f(m - m2), w = exp2f(s - m2);
+            const float m2 = fmaxf(m, s), scale = exp2f(m - m2), w = exp2f(s - m2 + Weight<T>::LIFT);
             l = l * scale + w;
             m = m2;
 #pragma unroll

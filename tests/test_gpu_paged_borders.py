@@ -201,6 +201,25 @@ def test_rows_without_any_sequence(dtype: str) -> None:
     assert torch.equal(paged.kv_append(x.q[:, :2], x.q[:, :2], *x.operands, q=x.q), x.q)
 
 
+# ---- weights far below the largest ---------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("below", [10.0, 17.0, 17.4])
+@pytest.mark.parametrize("qs,n", [([1], 131072), ([1], 16384), ([24], 16384), ([150], 16384)])
+def test_one_key_above_a_long_flat_tail(dtype: str, dim: int, below: float, qs, n: int) -> None:
+    """The first key's score is `below` above all others', whose weights together still count: below half
+    precision's range, 131071 of them hold 3.6e-3 of the mass at 17.4."""
+    x = PagedBatch(qs, [n], heads=2, kv_heads=1, dim=dim, page=16, dtype=dtype)
+    x.q.zero_()
+    x.q[..., 0] = 8.0
+    page, row = x.slots[0]
+    x.k[page, row, :, 0] = 0.0
+    x.k[page[0], row[0], :, 0] = below
+    x.v[page, row] = x.v[page, row].abs()
+    x.v[page[0], row[0]] = 0.0
+    compare(attend(x, scale=0.125), *reference(x, 0.125))
+
+
 # ---- values that are not finite ------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", ALL)
 @pytest.mark.parametrize("layout", ["tokens", "odd"])
