@@ -52,6 +52,16 @@ int64_t dtype_of(at::ScalarType t) {
     }
 }
 
+// A truth value.
+bool truth(PyObject *o, const char *what, const char *name) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) {
+        PyErr_Clear();
+        refuse(what, std::string(name) + " has no truth value");
+    }
+    return v != 0;
+}
+
 // The first six operands of every call and the status word.
 void fill(mgc_cuda_paged &p, const char *what, PyObject *const *a, PyObject *status, int64_t tokens) {
     const at::Tensor &k = *tensor(a[0], what, "k_cache"), &v = *tensor(a[1], what, "v_cache"),
@@ -161,6 +171,7 @@ PyObject *kv_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
             rows(what, "q_out", out, tokens, x.q_heads, dim, device, x.qo_token_stride, x.qo_head_stride);
             x.q_out = out.data_ptr();
         }
+        const bool interleaved = truth(a[10], what, "interleaved");
         if (!cos != !sin) refuse(what, "cos and sin come together");
         if (cos) {
             if (cos->dim() != 2 || sin->sizes() != cos->sizes() || cos->scalar_type() != at::kFloat ||
@@ -173,7 +184,7 @@ PyObject *kv_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
             x.table_row = cos->stride(0);
             x.positions = cos->size(0);
             x.rot = 2 * cos->size(1);
-            x.interleaved = PyObject_IsTrue(a[10]) == 1;
+            x.interleaved = interleaved;
         }
         const c10::cuda::CUDAGuard guard(device);
         if (q && x.paged.batch == 0) out.copy_(*q);  // no sequence: the call itself does nothing
@@ -227,7 +238,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
             PyErr_Clear();
             refuse(what, "scale is a number");
         }
-        x.causal = PyObject_IsTrue(a[9]) == 1;
+        x.causal = truth(a[9], what, "causal");
         x.window = whole(a[10], 0);
         const c10::cuda::CUDAGuard guard(device);
         if (x.paged.batch == 0) out.zero_();  // no sequence: the call itself does nothing
