@@ -6,11 +6,13 @@
 // links against torch only.
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_strided.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <initializer_list>
 #include <sstream>
 #include <string>
 
@@ -50,6 +52,18 @@ int64_t dtype_of(at::ScalarType t) {
     case at::kBFloat16: return MGC_BF16;
     default: return -1;
     }
+}
+
+// There is no backward pass: an operand that a gradient is recorded for is refused.
+void no_gradient(const char *what, std::initializer_list<const at::Tensor *> operands) {
+    if (!at::GradMode::is_enabled()) return;
+    for (const at::Tensor *t : operands)
+        if (t && t->defined() && t->requires_grad()) refuse(what, "an operand requires a gradient, which the call cannot record (torch.no_grad(), or detach it)");
+}
+
+// The kernels wrote t: autograd's saved copies of it are out of date.
+void written(const at::Tensor &t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 // A truth value.
@@ -186,6 +200,7 @@ PyObject *kv_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
             x.rot = 2 * cos->size(1);
             x.interleaved = interleaved;
         }
+        no_gradient(what, {&k, &v, &cache, tensor(a[3], what, "v_cache"), q, cos, sin, &out});
         const c10::cuda::CUDAGuard guard(device);
         if (q && x.paged.batch == 0) out.copy_(*q);  // no sequence: the call itself does nothing
         void *stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
@@ -194,7 +209,10 @@ PyObject *kv_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
         status = append_fn(&x, stream);
         Py_END_ALLOW_THREADS;
         check(status, what);
+        written(cache);
+        written(*tensor(a[3], what, "v_cache"));
         if (!q) Py_RETURN_NONE;
+        if (a[11] != Py_None) written(out);
         return THPVariable_Wrap(std::move(out));
     });
 }
@@ -240,6 +258,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
         }
         x.causal = truth(a[9], what, "causal");
         x.window = whole(a[10], 0);
+        no_gradient(what, {&q, &cache, tensor(a[2], what, "v_cache"), &out});
         const c10::cuda::CUDAGuard guard(device);
         if (x.paged.batch == 0) out.zero_();  // no sequence: the call itself does nothing
         void *stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
@@ -257,6 +276,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
         status = attend_fn(&x, stream);
         Py_END_ALLOW_THREADS;
         check(status, what);
+        if (a[11] != Py_None) written(out);
         return THPVariable_Wrap(std::move(out));
     });
 }

@@ -12,7 +12,8 @@ batch of sequences with any number of new tokens each, packed along one axis:
 
 These three stay on the device: nothing is copied to the host and no call synchronises. All tensors
 are torch CUDA tensors on one device; the kernels run on torch's current stream of that device, so
-a call can be captured into a CUDA graph. There is no autograd. The C entry points are
+a call can be captured into a CUDA graph. There is no backward pass: where gradients are recorded, an
+operand that requires one raises ``GraphError``. The C entry points are
 ``mgc_cuda_kv_append`` and ``mgc_cuda_paged_attention`` (include/mgc_cuda.h); an operand they cannot
 take raises ``GraphError`` or ``CodegenError`` and nothing runs.
 
