@@ -59,7 +59,13 @@ def binding_path() -> Path:
     return LIB_DIR / "_mgc_paged.so"
 
 
+def _placeless(flags: list[str]) -> list[str]:
+    """The flags without include paths: a tree that moved, sources unchanged, is still built."""
+    return [f for f in flags if not f.startswith("-I")]
+
+
 def source_key(flags: list[str]) -> str:
+    flags = _placeless(flags)
     h = hashlib.sha256()
     for path in sources():
         h.update(path.name.encode())
@@ -84,7 +90,7 @@ def _object_key(source: Path, flags: list[str]) -> str:
         seen[path] = path.read_bytes()
         for name in re.findall(rb'^\s*#include\s+"([^"]+)"', seen[path], flags=re.M):
             todo += [d / name.decode() for d in (SRC_DIR, INCLUDE_DIR) if (d / name.decode()).exists()]
-    h = hashlib.sha256(" ".join(flags).encode())
+    h = hashlib.sha256(" ".join(_placeless(flags)).encode())
     for path in sorted(seen):
         h.update(path.name.encode() + seen[path])
     return h.hexdigest()[:20]
@@ -133,23 +139,35 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     return lib
 
 
-def build_binding(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the torch binding (csrc/paged_torch.cpp, host code) if it, the header or torch changed."""
+def _binding_flags() -> list[str]:
+    import torch
+
+    return ["-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+
+
+def binding_key() -> str:
+    """Key of the torch binding: its source and the header, the flags, torch's and Python's versions."""
     import sysconfig
 
     import torch
+
+    return _object_key(SRC_DIR / "paged_torch.cpp", [*_binding_flags(), torch.__version__, sysconfig.get_python_version()])
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> Path:
+    """Compile the torch binding (csrc/paged_torch.cpp, host code) if it, the header or torch changed."""
+    source, out = SRC_DIR / "paged_torch.cpp", binding_path()
+    stamp, key = out.with_suffix(".key"), binding_key()
+    if not force and out.exists() and stamp.exists() and stamp.read_text().strip() == key:
+        return out
+    import sysconfig
+
     from torch.utils import cpp_extension
 
-    source, out = SRC_DIR / "paged_torch.cpp", binding_path()
-    stamp = out.with_suffix(".key")
     include = [*cpp_extension.include_paths(), sysconfig.get_path("include"), str(INCLUDE_DIR),
                str(Path(find_nvcc()).resolve().parents[1] / "include")]
     libs = cpp_extension.library_paths()
-    flags = ["-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-             *(f"-I{p}" for p in include)]
-    key = _object_key(source, [*flags, torch.__version__, sysconfig.get_python_version()])
-    if not force and out.exists() and stamp.exists() and stamp.read_text().strip() == key:
-        return out
+    flags = [*_binding_flags(), *(f"-I{p}" for p in include)]
     LIB_DIR.mkdir(parents=True, exist_ok=True)
     tmp = out.with_name(f"{out.name}.tmp{os.getpid()}")
     cxx = os.environ.get("MGC_CXX") or shutil.which("g++") or "g++"

@@ -65,9 +65,7 @@ def library(path: str | Path | None = None) -> ctypes.CDLL:
     with _LIB_LOCK:
         if _LIB is not None and path is None:
             return _LIB
-        lib_path = Path(path) if path is not None else _build.library_path()
-        if path is None and not lib_path.exists():
-            lib_path = _build.build()
+        lib_path = Path(path) if path is not None else _build.build()
         lib = ctypes.CDLL(str(lib_path))
         for name, (res, args) in SIGNATURES.items():
             fn = getattr(lib, name)

@@ -40,14 +40,13 @@ _EXT_LOCK = threading.Lock()
 
 
 def _binding() -> ModuleType:
-    """The torch binding (csrc/paged_torch.cpp) with the C entry points handed to it, loaded once."""
+    """The torch binding (csrc/paged_torch.cpp) with the C entry points handed to it, loaded once (built
+    first if its sources, torch or Python changed)."""
     global _EXT
     with _EXT_LOCK:
         if _EXT is None:
             lib = library()
-            path = _build.binding_path()
-            if not path.exists():
-                _build.build_binding()
+            path = _build.build_binding()
             spec = importlib.util.spec_from_file_location("_mgc_paged", path)
             if spec is None or spec.loader is None:
                 raise CodegenError(f"cannot load {path}")
