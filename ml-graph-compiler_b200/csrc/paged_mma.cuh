@@ -445,9 +445,11 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
                 x0 = fmaxf(x0, __shfl_xor_sync(0xFFFFFFFFu, x0, 2));
                 x1 = fmaxf(x1, __shfl_xor_sync(0xFFFFFFFFu, x1, 2));
                 // weights 2^(scale s - scale m), one rounding in the exponent; a row that has seen
-                // nothing yet has the maximum -inf: subtract 0 instead
-                const float y0 = x0 == -INFINITY ? 0.0f : x0 * p.scale_log2, y1 = x1 == -INFINITY ? 0.0f : x1 * p.scale_log2;
-                const float a0 = ex2(m0 * p.scale_log2 - y0), a1 = ex2(m1 * p.scale_log2 - y1);
+                // nothing yet has the maximum -inf: subtract 0 instead. The products are rounded on their own:
+                // contracted with the difference, a maximum that stays would rescale the row by its product's
+                // rounding, 2^-24 of the exponent a tile, which adds up along a long context
+                const float y0 = x0 == -INFINITY ? 0.0f : __fmul_rn(x0, p.scale_log2), y1 = x1 == -INFINITY ? 0.0f : __fmul_rn(x1, p.scale_log2);
+                const float a0 = ex2(__fmul_rn(m0, p.scale_log2) - y0), a1 = ex2(__fmul_rn(m1, p.scale_log2) - y1);
                 const float z0 = Weight<T>::LIFT - y0, z1 = Weight<T>::LIFT - y1;
                 m0 = x0;
                 m1 = x1;
@@ -588,8 +590,8 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
                 *reinterpret_cast<float2 *>(red + (ra + 8) * C::ORED + d * 8 + t4 * 2) = make_float2(o[d][2], o[d][3]);
             }
             if (t4 == 0) {
-                sm[ra] = m0 * p.scale_log2;
-                sm[ra + 8] = m1 * p.scale_log2;
+                sm[ra] = __fmul_rn(m0, p.scale_log2);
+                sm[ra + 8] = __fmul_rn(m1, p.scale_log2);
                 sl[ra] = l0;
                 sl[ra + 8] = l1;
             }
