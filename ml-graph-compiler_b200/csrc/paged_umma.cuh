@@ -155,11 +155,12 @@ __device__ __forceinline__ bool poll(uint32_t e, uint64_t *bar, uint32_t parity)
         : "=r"(done) : "r"(smem_addr(bar)), "r"(parity), "r"(e) : "memory");
     return __any_sync(0xFFFFFFFFu, done != 0);
 }
+constexpr long long WAIT_LIMIT = 4 * umma::WAIT_LIMIT_CYCLES;  // what row_again may take
 __device__ __forceinline__ bool warp_wait(uint32_t e, uint64_t *bar, uint32_t parity) {
     if (poll(e, bar, parity)) return true;
     const long long t0 = clock64();
     while (!poll(e, bar, parity))
-        if (__any_sync(0xFFFFFFFFu, clock64() - t0 > umma::WAIT_LIMIT_CYCLES)) return false;
+        if (__any_sync(0xFFFFFFFFu, clock64() - t0 > WAIT_LIMIT)) return false;
     return true;
 }
 
@@ -198,92 +199,94 @@ __device__ __forceinline__ int tiles_needed(const AttendParams &p, const Item &w
 }
 
 // The slow way round for rows whose tiles held something that they do not see: this thread's row over
-// the keys of piece w that it sees, on the FMA units. Maximum and sum first, then the output, 32
-// channels at a time, into TMEM where the products would have left it. The whole warp calls; threads
-// without `all` compute their row only if a key that it does not see has a value that is not finite.
-template <typename T, int DP>
-__device__ __forceinline__ void row_again(const AttendParams &p, const Item &w, int row, bool all, bool maybe, uint32_t to, float &m, float &l) {
+// the keys of piece w that it sees, on the FMA units, into TMEM where the products would have left it.
+// `q` names the row's 16-byte chunks in shared memory. The whole warp calls; threads without `all` compute
+// their row only if a key that it does not see has a value that is not finite. A piece of 16384 keys of 128
+// channels takes about 40 ms while the other roles wait: WAIT_LIMIT, 4.5 s, covers pieces of 1.7 million.
+template <typename T, int DP, typename Q>
+__device__ __forceinline__ void row_again(const AttendParams &p, const Item &w, int row, Q q, bool all, bool maybe, uint32_t to, float &m, float &l) {
     const RowRange see = row_range(p, w.seq, row);
-    const int lo = max(see.lo, w.lo), hi = min(see.hi, w.hi);
-    const T *q = static_cast<const T *>(p.q) + (long long)(w.seq.start + row / p.group) * p.q_ts +
-                 (long long)(w.h * p.group + row % p.group) * p.q_hs;
+    const int lo = max(see.lo, w.lo), hi = min(see.hi, w.hi), ps = p.batch.page_size;
     const long long head = (long long)w.h * p.head_stride;
-    auto at = [&](int j) -> long long {
-        const int page = page_of(p.batch, w.b, j / p.batch.page_size);
-        return page < 0 ? -1 : (long long)page * p.page_stride + (long long)(j % p.batch.page_size) * p.token_stride + head;
-    };
-    auto score = [&](long long off) {
-        const T *k = static_cast<const T *>(p.k_pages) + off;
-        float s = 0.0f;
+    // calls f with the offset of each key of [from, to) that has a page, until it returns false
+    auto keys = [&](int from, int to, auto f) {
+        for (int j = from; j < to;) {
+            const int at = j / ps, end = to - at * ps < ps ? to : (at + 1) * ps, page = page_of(p.batch, w.b, at);
+            long long off = (long long)page * p.page_stride + (long long)(j - at * ps) * p.token_stride + head;
+            if (page >= 0) {
 #pragma unroll 1
-        for (int c = 0; c < p.head_dim; c += 8) {
-            Pack<8, T> x, y;
-            x.load(q + c);
-            y.load(k + c);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s = fmaf(to_f(x.e[i]), to_f(y.e[i]), s);
+                for (; j < end; ++j, off += p.token_stride)
+                    if (!f(off)) return;
+            }
+            j = end;
         }
-        return s * p.scale_log2;
     };
     if (!all && maybe) {
-#pragma unroll 1
-        for (int j = max(w.lo, w.first); j < w.hi && !all; ++j) {
-            if (j == lo && lo < hi) j = hi;  // those it sees
-            if (j >= w.hi) break;
-            const long long off = at(j);
-            if (off < 0) continue;
+        auto finite = [&](long long off) {
             float z = 0.0f;
-#pragma unroll 1
-            for (int c = 0; c < p.head_dim; c += 8) {
+#pragma unroll
+            for (int c = 0; c < DP / 8; ++c) {
+                if (c * 8 >= p.head_dim) continue;
                 Pack<8, T> v;
-                v.load(static_cast<const T *>(p.v_pages) + off + c);
+                v.load(static_cast<const T *>(p.v_pages) + off + c * 8);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) z = fmaf(to_f(v.e[i]), 0.0f, z);
             }
             all = z != z;
-        }
+            return !all;
+        };
+        keys(max(w.lo, w.first), min(lo, w.hi), finite);
+        if (!all) keys(max(max(hi, w.lo), w.first), w.hi, finite);
     }
     if (!__any_sync(0xFFFFFFFFu, all)) return;
+    float o[DP];
+#pragma unroll
+    for (int i = 0; i < DP; ++i) o[i] = 0.0f;
     if (all) {
         m = -INFINITY;
         l = 0.0f;
+        keys(lo, hi, [&](long long off) {
+            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < DP / 8; ++c) {
+                if (c * 8 >= p.head_dim) continue;
+                Pack<8, T> x, y;
+                x.load(q(c));
+                y.load(static_cast<const T *>(p.k_pages) + off + c * 8);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) part[i & 3] = fmaf(to_f(x.e[i]), to_f(y.e[i]), part[i & 3]);
+            }
+            const float s = __fmul_rn((part[0] + part[1]) + (part[2] + part[3]), p.scale_log2);
+            if (s == -INFINITY) return true;
+            if (s > m) {
+                const float f = ex2(m - s);
+                m = s;
+                l *= f;
+#pragma unroll
+                for (int i = 0; i < DP; ++i) o[i] *= f;
+            }
+            const float wgt = ex2(s - m + Weight<T>::LAZY_LIFT);
+            l += wgt;
+#pragma unroll
+            for (int c = 0; c < DP / 8; ++c) {
+                if (c * 8 >= p.head_dim) continue;
+                Pack<8, T> v;
+                v.load(static_cast<const T *>(p.v_pages) + off + c * 8);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[c * 8 + i] = fmaf(wgt, to_f(v.e[i]), o[c * 8 + i]);
+            }
+            return true;
+        });
     }
-#pragma unroll 1
-    for (int j = all ? lo : hi; j < hi; ++j) {
-        const long long off = at(j);
-        if (off < 0) continue;
-        const float s = score(off), top = fmaxf(m, s);
-        if (s == -INFINITY) continue;
-        l = l * (top == -INFINITY ? 1.0f : ex2(m - top)) + ex2(s - top + Weight<T>::LAZY_LIFT);
-        m = top;
-    }
-#pragma unroll 1
-    for (int c0 = 0; c0 < DP; c0 += 32) {
-        float o[32];
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c) {
         uint32_t t[32];
-        __syncwarp();
-        umma::tmem_ld32(to + c0, t);
+        umma::tmem_ld32(to + c * 32, t);
         umma::tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = all ? 0.0f : __uint_as_float(t[i]);
-#pragma unroll 1
-        for (int j = all ? lo : hi; j < hi; ++j) {
-            const long long off = at(j);
-            if (off < 0) continue;
-            const float s = score(off), wgt = s == -INFINITY ? 0.0f : ex2(s - m + Weight<T>::LAZY_LIFT);
-#pragma unroll
-            for (int c = 0; c < 32; c += 8) {
-                if (c0 + c >= p.head_dim) continue;
-                Pack<8, T> v;
-                v.load(static_cast<const T *>(p.v_pages) + off + c0 + c);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) o[c + i] = fmaf(wgt, to_f(v.e[i]), o[c + i]);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 32; ++i) t[i] = __float_as_uint(o[i]);
-        __syncwarp();
-        tmem_st32(to + c0, t);
+        for (int i = 0; i < 32; ++i) t[i] = all ? __float_as_uint(o[c * 32 + i]) : t[i];
+        tmem_st32(to + c * 32, t);
     }
     tmem_wait_st();
 }
@@ -676,7 +679,10 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                     }
                     maybe = maybe && odd[0] + odd[1] != 0.0f;
                 }
-                if (bad || __any_sync(0xFFFFFFFFu, maybe)) row_again<T, DP>(p, w, w.row0 + x * 128 + r, bad, maybe, to, m, l);
+                if (bad || __any_sync(0xFFFFFFFFu, maybe)) {
+                    auto q = [&](int c) { return reinterpret_cast<const T *>(chunk(lane, c)); };
+                    row_again<T, DP>(p, w, w.row0 + x * 128 + r, q, bad, maybe, to, m, l);
+                }
             }
             // ---- O: through the warp's rows of the Q tile (no longer read) to whole rows of memory ----
             const bool whole = w.slot < 0;

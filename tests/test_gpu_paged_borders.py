@@ -259,3 +259,17 @@ def test_values_that_a_row_does_not_see_do_not_reach_it(dtype: str, layout: str,
     # the last token sees a key that is not finite: what its second head group gets is undefined
     want[x.rows(0).stop - 1, 2:], got[x.rows(0).stop - 1, 2:], bound[x.rows(0).stop - 1, 2:] = 0.0, 0.0, 1.0
     compare(got, want, bound)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("qs", [[300], [30]])
+def test_rows_computed_again_over_a_long_context(dtype: str, dim: int, qs) -> None:
+    """No wait of the other warps runs out meanwhile."""
+    x = PagedBatch(qs, [30000], heads=8, kv_heads=2, dim=dim, page=16, dtype=dtype)
+    page, row = x.slots[0]
+    x.v[page[-1], row[-1], :, 5] = math.nan
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = attend(x, status)
+    paged.check_status(status)
+    compare(got, *reference(x, dim**-0.5))
