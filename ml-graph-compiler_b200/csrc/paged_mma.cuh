@@ -118,6 +118,9 @@ template <typename T, int DP, int WM, int WN, int SIMT> struct MmaConfig {
     static constexpr int KG = DP > 128 && KW > 32 ? 32 : KW;  // keys per softmax step (registers)
     // two for the plain form: more blocks an SM beat more stages a block (16 x 1024 fp32 24.8 -> 22.6 us)
     static constexpr int STAGES = DP > 128 || SIMT ? 2 : 3;
+    // blocks that an SM is to hold (0: as it comes): even shares are cut for 4, and at 148 registers 3 fit, so
+    // that a second round ran (64 x 4096, 16-bit, 8 key heads x 64: 116 us, at 128 registers 80 us)
+    static constexpr int RESIDENT = !F32 && DP == 64 && WM == 1 ? 4 : 0;
     static constexpr int CH = 16 / (int)sizeof(T);   // elements of a 16-byte chunk
     static constexpr int ROW = DP * (int)sizeof(T) + 16;  // bytes of a padded K / V row
     static constexpr int STAGE = 2 * BN * ROW;
@@ -132,7 +135,7 @@ template <typename T, int DP, int WM, int WN, int SIMT> struct MmaConfig {
 // EVEN: the CTA takes an even share of all units' keys (paged_work.cuh); else one row tile's keys, or
 // the part of them that its rank in a cluster names.
 template <typename T, int DP, int WM, int WN, int SIMT, bool EVEN>
-__global__ void __launch_bounds__(MmaConfig<T, DP, WM, WN, SIMT>::THREADS)
+__global__ void __launch_bounds__(MmaConfig<T, DP, WM, WN, SIMT>::THREADS, MmaConfig<T, DP, WM, WN, SIMT>::RESIDENT * EVEN)
 paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
     using C = MmaConfig<T, DP, WM, WN, SIMT>;
     constexpr int R = C::R, BN = C::BN, KW = C::KW, KG = C::KG, ROW = C::ROW, NB = KG / 8 ? KG / 8 : 1, DB = SIMT ? 1 : DP / 8;

@@ -60,6 +60,7 @@ __device__ __forceinline__ RowRange row_range(const AttendParams &p, const Seque
 // pages or values that are not finite take.
 template <int C> struct RowSum {
     float o[C], m, l;
+    __device__ __forceinline__ RowSum() {}
     template <typename T>
     __device__ __forceinline__ void over_keys(const AttendParams &p, int b, int kh, const T *q, int lo, int hi, int lane) {
         const long long head = kh * p.head_stride;
