@@ -528,10 +528,10 @@ paged_attention_mma_kernel(const __grid_constant__ AttendParams p) {
         // The piece is computed again, row by row and only with the keys that a row sees, if it met a page
         // number out of range or if NaN came out that need not belong there (the row's sum is none): a
         // weight 0 of a key that a row does not see times a value that is not finite, or the split of an
-        // infinite value. Where every row sees every key the 16-bit and the plain form cannot have made
-        // one. (Looking at each stage cost 2 % of 64 x 8192 in bf16.)
+        // infinite value. A single token's rows all see the same keys: there the 16-bit and the plain form
+        // cannot have made one. (Looking at each stage cost 2 % of 64 x 8192 in bf16.)
         bool again = bad_page;
-        const bool partly = all_lo > first.lo || all_hi < last.hi;
+        const bool partly = rows > p.group;
         if constexpr (SIMT > 0) {
             if (partly) {
 #pragma unroll
