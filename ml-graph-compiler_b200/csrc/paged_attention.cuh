@@ -70,7 +70,9 @@ struct Plan {
 
 constexpr int MIN_SPLIT_KEYS = 128;  // below this a split's start and merge outweigh its loads
 
-// CTAs of the tiled kernel that an SM holds (of 128 threads, by shared memory; 2 at 256 registers).
+// CTAs of the tiled kernel (128 threads) that an SM holds by its shared memory. Registers are not counted:
+// the even-share kernels of 16-bit types with 64 channels and more than 16 rows (168 registers), and of fp32
+// with 96 channels and 8 rows, hold 3 where this says 4, so their last shares run in a second round.
 inline int ctas_per_sm(int64_t dtype, int64_t head_dim, int wm, int simt) {
     const int dp = head_dim <= 32 ? 32 : head_dim <= 64 ? 64 : head_dim <= 96 ? 96 : head_dim <= 128 ? 128 : 256;
     const bool f32 = dtype == MGC_F32;
@@ -122,7 +124,7 @@ inline Plan plan_of(const mgc_cuda_paged_attention_args &a) {
     const int64_t units = c.batch * c.kv_heads * s.row_tiles;
     int64_t most = a.max_kv;
     if (a.window > 0 && a.window + max_q < most) most = a.window + max_q;
-    // CTAs that fit the GPU at once: shared memory and registers allow this many per SM
+    // CTAs that fit the GPU at once, going by shared memory
     const int64_t slots = (int64_t)sm_count() * ctas_per_sm(c.dtype, c.head_dim, s.wm, s.simt);
     int64_t splits = slots / units;
     if (splits > most / MIN_SPLIT_KEYS) splits = most / MIN_SPLIT_KEYS;

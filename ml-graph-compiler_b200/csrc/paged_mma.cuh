@@ -27,8 +27,9 @@
 // order, so a call repeats its bits.
 //
 // Decoding is bound by memory: 64 sequences of 8 key heads x 128 up to 8192 positions, bf16, 1.32 GB
-// in ~231 us (5.7 TB/s, 88 % of the copy bandwidth); one of 131071 positions 102 us (5.3 TB/s); 16 GPT-2
-// sequences up to 1024 positions, fp32, 21 us (3.4 TB/s: two launches and the blocks' start are half).
+// in 229 to 248 us (5.8 to 5.3 TB/s, 89 to 82 % of the copy bandwidth); one of 131071 positions 101 to 110 us
+// (5.3 to 4.9 TB/s, the second kernel in it); 16 GPT-2 sequences up to 1024 positions, fp32, in clusters of
+// two, 22.5 us (3.2 TB/s: the blocks' start, the first loads and the cluster's sum are half).
 #pragma once
 
 #include "paged_work.cuh"

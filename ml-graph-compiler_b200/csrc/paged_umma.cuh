@@ -7,7 +7,7 @@
 // K = 128) with P read from TMEM. The two row tiles alternate: while one warpgroup exponentiates,
 // the tensor core works for the other.
 //
-// * Q rows: each thread copies its own row into 128B-swizzled shared memory (any strides).
+// * Q rows: a warp copies its 32 rows together into 128B-swizzled shared memory (any strides).
 // * K and V tiles arrive by TMA from the pages, one box of min(page_size, 128) rows x 64 channels
 //   per page and channel half, lane l of the loading warp issuing box l; a ring of stages holds
 //   K and V tiles in the order K0 V0 K1 V1 ... K is a K-major operand, V (channels contiguous) an
@@ -28,8 +28,9 @@
 //
 // Bound: the tensor core and the exponential unit about equally (2048 cycles each per key tile and
 // pair of row tiles at 128 channels); measured 2930 cycles a pair, the rest being the chain scores ->
-// weights -> products of each row tile. 2048 tokens x 32 heads of 128 over 16384 positions, bf16:
-// ~430 us, 1.2 PFLOP/s, at which the power cap lowers the clock.
+// weights -> products of each row tile. 2048 tokens x 32 heads of 128 over 16384 positions, bf16: 520 us
+// in calls one after the other for seconds, 0.99 PFLOP/s, with the clock at the power cap. The softmax role
+// of the 128-channel kernel spills (260 bytes written, 408 read a thread), the 64-channel one does not.
 //
 // Every mbarrier wait is bounded; on timeout the CTA sets the status word, drains its copies,
 // frees its TMEM and returns.

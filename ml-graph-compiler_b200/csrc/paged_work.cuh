@@ -264,7 +264,7 @@ __device__ __forceinline__ CutUnit cut_of(const AttendParams &p, const Walk &k, 
     return cut;
 }
 
-// out of the rows of units that were cut, the pieces in order; `next` CTAs lie between a stretch and
+// Adds up out of the rows of units that were cut, the pieces in order; `next` CTAs lie between a stretch and
 // the one after it. Units of many rows are cut into few pieces: a warp per row. Units of few rows can
 // be cut into many (a long context on all SMs): a block per row, its warps taking every fourth piece.
 // The factors come first, their loads together: a loop that loaded each piece's maximum before its

@@ -2,7 +2,7 @@
 cache, where a compiled graph computes a whole sequence of fixed length.
 
 ``Gpt2`` holds a decoder of the GPT-2 layout (pre-LayerNorm, tanh GELU, learned positions, head tied to
-the token embedding; ``zoo.gpt2``'s) with random weights or given ones, and runs one step for a batch
+the token embedding; ``zoo.gpt2``'s) with random weights, and runs one step for a batch
 of sequences with any number of new tokens each: layer norms, products and epilogues by
 ``mgc_cuda_layer_norm`` and ``mgc_cuda_gemm``, the cache and its attention by ``mgc_cuda.paged``.
 ``Pages`` hands out the pages of a cache to sequences.
