@@ -385,6 +385,62 @@ typedef struct {
 int mgc_cuda_paged_attention(const mgc_cuda_paged_attention_args *args, void *stream);
 int64_t mgc_cuda_paged_attention_workspace(const mgc_cuda_paged_attention_args *args);
 
+/* ---- quantised paged cache, head norms -----------------------------------------------------------
+ * Pages of keys and values in 4 or 8 bits: mgc_cuda_paged's k and v are bytes of codes (its strides in
+ * bytes, multiples of 16, from 16-byte aligned pages), channel c of a row the byte c (8 bits) or the
+ * nibble c % 2 of byte c / 2, the lower one first (4 bits); its dtype is that of the call's queries,
+ * outputs and sources. The scales are two arrays of pairs of halves (scale, offset), that of group g of
+ * head h of token t of page n at k_scales + 2 (n page_stride + t token_stride + h head_stride + g), and a
+ * code stands for scale * code + offset. head_dim is a multiple of 16, at most 256; group a multiple of
+ * 64 that divides it, or head_dim. */
+typedef struct {
+    int64_t bits;   /* 4 or 8; 0 (the append alone): plain pages */
+    int64_t group;  /* channels that share a pair */
+    void *k_scales, *v_scales;
+    int64_t page_stride, token_stride, head_stride;  /* of the scales, in pairs */
+} mgc_cuda_quantized;
+
+/* mgc_cuda_kv_append with what a decoder does to each head before, and to pages of either kind.
+ * q_norm, k_norm (fp32 [head_dim], NULL: none): a query or key x becomes
+ *   x fp32((sum x^2 / head_dim + eps)^-1/2) w   (the sum in fp64)
+ * before it is rotated. Quantised pages take a group x as offset = half(min x), scale = half((max x -
+ * offset) / L), L = 2^bits - 1, codes (x - offset) / scale rounded to the nearest even whole number
+ * within [0, L]; all steps in fp32, extremes held within +-65504; a group with a value that is not
+ * finite gets the pair (NaN, NaN). The sources are then of the call's dtype, else of the pages' or
+ * MGC_F32. A token that is not cached keeps its query as it is, unless only its page is missing. */
+typedef struct {
+    mgc_cuda_kv_append_args append;
+    mgc_cuda_quantized quantized;
+    const float *q_norm, *k_norm;
+    double eps;
+} mgc_cuda_kv_append_heads_args;
+
+int mgc_cuda_kv_append_heads(const mgc_cuda_kv_append_heads_args *args, void *stream);
+
+/* The inverse: row t of k_out and v_out [tokens, kv_heads, head_dim] (of paged.dtype) gets the values
+ * that the cache holds for packed token t, zeros for a token without a cached position or whose page
+ * is missing (the latter sets *status_dev). A call with batch 0 does nothing. */
+typedef struct {
+    mgc_cuda_paged paged;
+    mgc_cuda_quantized quantized;
+    void *k_out;
+    int64_t k_token_stride, k_head_stride;
+    void *v_out;
+    int64_t v_token_stride, v_head_stride;
+} mgc_cuda_kv_read_args;
+
+int mgc_cuda_kv_read(const mgc_cuda_kv_read_args *args, void *stream);
+
+/* mgc_cuda_paged_attention over quantised pages: the same definition with the values that the codes
+ * stand for. A pair (scale, offset) that is not finite makes its group's values NaN. */
+typedef struct {
+    mgc_cuda_paged_attention_args attention;
+    mgc_cuda_quantized quantized;
+} mgc_cuda_paged_attention_quantized_args;
+
+int mgc_cuda_paged_attention_quantized(const mgc_cuda_paged_attention_quantized_args *args, void *stream);
+int64_t mgc_cuda_paged_attention_quantized_workspace(const mgc_cuda_paged_attention_quantized_args *args);
+
 #ifdef __cplusplus
 }
 #endif

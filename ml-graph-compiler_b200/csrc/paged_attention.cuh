@@ -39,23 +39,6 @@ __global__ void __launch_bounds__(128) paged_attention_row_kernel(const __grid_c
 }
 
 // ---- host side ---------------------------------------------------------------------------------
-inline int check_attend(const mgc_cuda_paged_attention_args &a, const char *what) {
-    const mgc_cuda_paged &c = a.paged;
-    MGC_CHECK(check_paged(c, what));
-    if (c.tokens > 0 && c.batch > 0 && (!a.q || !a.out)) return fail(MGC_CUDA_BAD_ARGUMENT, "%s: q or out is NULL", what);
-    if (a.q_heads < 1 || a.q_heads % c.kv_heads)
-        return fail(MGC_CUDA_BAD_ARGUMENT, "%s: %lld query heads over %lld key heads", what, (long long)a.q_heads,
-                    (long long)c.kv_heads);
-    if (c.head_dim > MAX_HEAD_DIM || a.q_heads > 65535)
-        return fail(MGC_CUDA_UNSUPPORTED, "%s: %lld heads of %lld channels (at most %d channels)", what,
-                    (long long)a.q_heads, (long long)c.head_dim, MAX_HEAD_DIM);
-    if (a.window < 0 || (a.window > 0 && !a.causal))
-        return fail(MGC_CUDA_BAD_ARGUMENT, "%s: a window of %lld needs causal attention", what, (long long)a.window);
-    if (!(a.scale > 0.0) || a.scale > 1e30) return fail(MGC_CUDA_BAD_ARGUMENT, "%s: scale %g", what, a.scale);
-    if (a.max_q < 0 || a.max_kv < 0) return fail(MGC_CUDA_BAD_ARGUMENT, "%s: negative bound", what);
-    return MGC_CUDA_OK;
-}
-
 // How a call runs: which kernel, its row tile and how its keys are shared out.
 struct Plan {
     bool mma = false, umma = false, even = false;
@@ -228,21 +211,9 @@ inline int attend(const mgc_cuda_paged_attention_args &a, cudaStream_t stream) {
     const mgc_cuda_paged &c = a.paged;
     MGC_CHECK(check_attend(a, what));
     if (c.tokens == 0 || c.batch == 0) return MGC_CUDA_OK;
-    AttendParams p;
-    p.batch = batch_of(c);
-    p.k_pages = c.k; p.v_pages = c.v;
-    p.page_stride = c.page_stride; p.token_stride = c.token_stride; p.head_stride = c.head_stride;
-    p.q = a.q; p.out = a.out;
-    p.q_ts = a.q_token_stride; p.q_hs = a.q_head_stride; p.o_ts = a.o_token_stride; p.o_hs = a.o_head_stride;
-    p.tokens = (int)c.tokens; p.q_heads = (int)a.q_heads; p.kv_heads = (int)c.kv_heads;
-    p.group = p.q_heads / p.kv_heads; p.head_dim = (int)c.head_dim;
-    p.causal = a.causal != 0;
-    p.window = (int)(a.window > 0x3FFFFFFF ? 0x3FFFFFFF : a.window);
-    p.scale_log2 = (float)(a.scale * 1.4426950408889634074);
-    p.max_positions = (int)(c.table_pages * c.page_size);
+    AttendParams p = attend_params(a);
     const Plan s = plan_of(a);
     p.row_tiles = s.row_tiles; p.splits = s.splits; p.interleaved = s.interleaved;
-    p.part = nullptr; p.part_ml = nullptr; p.cut = nullptr;
     if (s.workspace) {
         if (!a.workspace || a.workspace_bytes < s.workspace || !aligned(a.workspace, 16))
             return fail(MGC_CUDA_NEEDS_WORKSPACE, "%s: needs %lld bytes of workspace (16-byte aligned), got %lld", what,

@@ -56,6 +56,10 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "mgc_cuda_kv_append": (_I, [_VP, _VP]),
     "mgc_cuda_paged_attention": (_I, [_VP, _VP]),
     "mgc_cuda_paged_attention_workspace": (_I64, [_VP]),
+    "mgc_cuda_kv_append_heads": (_I, [_VP, _VP]),
+    "mgc_cuda_kv_read": (_I, [_VP, _VP]),
+    "mgc_cuda_paged_attention_quantized": (_I, [_VP, _VP]),
+    "mgc_cuda_paged_attention_quantized_workspace": (_I64, [_VP]),
 }
 
 
