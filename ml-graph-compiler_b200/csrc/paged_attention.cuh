@@ -129,21 +129,6 @@ inline int64_t attend_workspace(const mgc_cuda_paged_attention_args &a) {
     return a.paged.tokens == 0 || a.paged.batch == 0 ? 0 : plan_of(a).workspace;
 }
 
-// A combine kernel's blocks may be set up while the kernel before finishes; they wait for it themselves.
-template <typename K> inline int launch_after(K kernel, dim3 grid, const AttendParams &p, int next, cudaStream_t stream) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(128);
-    cfg.stream = stream;
-    cudaLaunchAttribute dep[1];
-    dep[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    dep[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = dep;
-    cfg.numAttrs = 1;
-    MGC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, p, next));
-    return MGC_CUDA_OK;
-}
-
 template <typename T> inline int launch_umma(const AttendParams &p, const mgc_cuda_paged &c, int ctas, cudaStream_t stream) {
     UmmaMaps maps;
     memset(&maps, 0, sizeof maps);

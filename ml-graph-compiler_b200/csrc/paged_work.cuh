@@ -341,5 +341,20 @@ __global__ void __launch_bounds__(128) paged_combine_units_kernel(const __grid_c
     }
 }
 
+// A combine kernel's blocks may be set up while the kernel before finishes; they wait for it themselves.
+template <typename K> inline int launch_after(K kernel, dim3 grid, const AttendParams &p, int next, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(128);
+    cfg.stream = stream;
+    cudaLaunchAttribute dep[1];
+    dep[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    dep[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = dep;
+    cfg.numAttrs = 1;
+    MGC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, p, next));
+    return MGC_CUDA_OK;
+}
+
 }  // namespace paged
 }  // namespace mgc

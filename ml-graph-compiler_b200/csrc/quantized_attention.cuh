@@ -2,104 +2,128 @@
 // definition with k_j and v_j the values that the codes stand for.
 #pragma once
 
-#include "paged_work.cuh"
-#include "quantized_common.cuh"
+#include "quantized_mma.cuh"
 
 namespace mgc {
 namespace paged {
-
-// One warp per (token, query head), lane l holding channels l, l + 32, ...
-template <typename T, int BITS>
-__global__ void __launch_bounds__(128) quantized_attention_row_kernel(const __grid_constant__ AttendParams p, const Quantized z) {
-    constexpr int C = MAX_HEAD_DIM / 32;
-    const int lane = (int)(threadIdx.x & 31);
-    const int t = (int)blockIdx.x;
-    const int h = (int)blockIdx.y * 4 + (int)(threadIdx.x >> 5);
-    if (t == 0 && h == 0)
-        for (int i = lane; i < p.batch.batch; i += 32) check_sequence(p, i);
-    const int b = sequence_of(p.batch, t);
-    if (h >= p.q_heads) return;
-    T *out = static_cast<T *>(p.out) + t * p.o_ts + h * p.o_hs;
-    const int end = b < 0 ? t : __ldg(p.batch.q_starts + b + 1);
-    if (t >= end) {  // in no sequence
-        for (int d = lane; d < p.head_dim; d += 32) out[d] = from_f<T>(0.0f);
-        return;
-    }
-    const int length = __ldg(p.batch.kv_lens + b), kh = h / p.group;
-    int lo, hi;
-    visible(p, min(length, p.max_positions), length - (end - t), lo, hi);
-    const T *q = static_cast<const T *>(p.q) + t * p.q_ts + h * p.q_hs;
-    float qv[C], o[C], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-        const int d = lane + 32 * c;
-        qv[c] = lo < hi && d < p.head_dim ? to_f(q[d]) * p.scale_log2 : 0.0f;
-        o[c] = 0.0f;
-    }
-    for (int j = lo; j < hi; ++j) {
-        const int page = page_of(p.batch, b, j / p.batch.page_size);
-        if (page < 0) continue;
-        const int r = j % p.batch.page_size;
-        const long long at = page * p.page_stride + r * p.token_stride + kh * p.head_stride;
-        const long long pair = page * z.page_stride + r * z.token_stride + kh * z.head_stride;
-        auto value = [&](const void *pages, const __half2 *scales, int d) {
-            const uint8_t *row = static_cast<const uint8_t *>(pages) + at;
-            const int code = BITS == 8 ? row[d] : row[d >> 1] >> 4 * (d & 1) & 15;
-            const float2 so = __half22float2(scales[pair + d / z.group]);
-            return fmaf(so.x, (float)code, so.y);
-        };
-        float s = 0.0f;
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int d = lane + 32 * c;
-            if (d < p.head_dim) s += qv[c] * value(p.k_pages, z.k_scales, d);
-        }
-#pragma unroll
-        for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, x);
-        if (s == -INFINITY) continue;
-        const float m2 = fmaxf(m, s), scale = exp2f(m - m2), w = exp2f(s - m2);
-        l = l * scale + w;
-        m = m2;
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int d = lane + 32 * c;
-            if (d < p.head_dim) o[c] = o[c] * scale + w * value(p.v_pages, z.v_scales, d);
-        }
-    }
-    const float inv = l > 0.0f ? 1.0f / l : l != l ? l : 0.0f;
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-        const int d = lane + 32 * c;
-        if (d < p.head_dim) out[d] = from_f<T>(o[c] * inv);
-    }
-}
 
 inline int check_attend_quantized(const mgc_cuda_paged_attention_quantized_args &a, const char *what) {
     MGC_CHECK(check_attend(a.attention, what));
     return check_quantized(a.quantized, a.attention.paged, what);
 }
 
+// How a call runs.
+struct QuantPlan {
+    int nb = 1;          // eights of query rows of a unit
+    int row_tiles = 1;
+    bool even = false, interleaved = false;
+    int ctas = 0, live_rows = 1;
+    int64_t workspace = 0;
+};
+
+inline int width_of(int64_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
+
+// Calls `go` with the configuration of a type, width and row tile.
+template <typename F> inline auto with_config(int64_t dtype, int64_t bits, int64_t head_dim, int nb, F go) {
+    auto widths = [&](auto type, auto b) {
+        using T = decltype(type);
+        constexpr int BITS = decltype(b)::value;
+        const int dp = width_of(head_dim);
+        if (dp == 64) return nb > 1 ? go(QuantConfig<T, BITS, 64, 2>()) : go(QuantConfig<T, BITS, 64, 1>());
+        if (dp == 128) return nb > 1 ? go(QuantConfig<T, BITS, 128, 2>()) : go(QuantConfig<T, BITS, 128, 1>());
+        return go(QuantConfig<T, BITS, 256, 1>());
+    };
+    auto types = [&](auto b) {
+        if (dtype == MGC_F32) return widths(float(), b);
+        return dtype == MGC_F16 ? widths(__half(), b) : widths(__nv_bfloat16(), b);
+    };
+    return bits == 4 ? types(std::integral_constant<int, 4>()) : types(std::integral_constant<int, 8>());
+}
+
+inline QuantPlan quant_plan_of(const mgc_cuda_paged_attention_quantized_args &a) {
+    const mgc_cuda_paged &c = a.attention.paged;
+    QuantPlan s;
+    const int64_t group = a.attention.q_heads / c.kv_heads;
+    const int64_t max_q = a.attention.max_q < 1 ? 1 : a.attention.max_q > c.tokens ? c.tokens : a.attention.max_q;
+    const int64_t rows = max_q * group;
+    s.nb = rows <= 8 || c.head_dim > 128 ? 1 : 2;
+    const int unit_rows = 8 * s.nb;
+    s.row_tiles = (int)ceil_div(rows, unit_rows);
+    s.live_rows = (int)(rows < unit_rows ? rows : unit_rows);
+    const int64_t units = c.batch * c.kv_heads * s.row_tiles;
+    int64_t most = a.attention.max_kv;
+    if (a.attention.window > 0 && a.attention.window + max_q < most) most = a.attention.window + max_q;
+    // the kernel that adds pieces stores four elements at once
+    const int es = elem_size(c.dtype);
+    const bool wide = aligned(a.attention.out, 4 * es) && a.attention.o_token_stride % 4 == 0 && a.attention.o_head_stride % 4 == 0;
+    const int resident = with_config(c.dtype, a.quantized.bits, c.head_dim, s.nb, [](auto config) { return decltype(config)::RESIDENT; });
+    const int64_t slots = (int64_t)sm_count() * resident;
+    // Even shares cost a second kernel and the pieces' way through memory, some 500 keys' worth of time
+    if (wide && most > 512 + most * units / slots) {
+        s.even = true;
+        s.ctas = (int)slots;
+        if (slots >= c.kv_heads && slots / c.kv_heads * c.kv_heads * 20 >= slots * 19) {
+            s.interleaved = true;
+            s.ctas = (int)(slots / c.kv_heads * c.kv_heads);
+        }
+        s.workspace = (int64_t)s.ctas * (2 * unit_rows * (c.head_dim * 4 + 8) + (int64_t)sizeof(CutUnit));
+    }
+    return s;
+}
+
 inline int64_t attend_quantized_workspace(const mgc_cuda_paged_attention_quantized_args &a) {
     if (check_attend_quantized(a, "mgc_cuda_paged_attention_quantized_workspace") != MGC_CUDA_OK) return -1;
-    return 0;
+    return a.attention.paged.tokens == 0 || a.attention.paged.batch == 0 ? 0 : quant_plan_of(a).workspace;
+}
+
+template <typename T, int BITS, int DP, int NB>
+inline int launch_quantized(const QuantParams &p, const QuantPlan &s, QuantConfig<T, BITS, DP, NB>, cudaStream_t stream) {
+    using C = QuantConfig<T, BITS, DP, NB>;
+    if (s.even) {
+        auto kernel = quantized_attention_kernel<T, BITS, DP, NB, true>;
+        MGC_CHECK(raise_smem_ceiling((const void *)kernel));
+        kernel<<<(unsigned)s.ctas, C::THREADS, C::SMEM, stream>>>(p);
+        MGC_CHECK(check_launch("quantized_attention_kernel"));
+        return launch_after(paged_combine_units_kernel<T, C::R>, dim3((unsigned)s.ctas, (unsigned)s.live_rows), p.a,
+                            s.interleaved ? p.a.kv_heads : 1, stream);
+    }
+    auto kernel = quantized_attention_kernel<T, BITS, DP, NB, false>;
+    MGC_CHECK(raise_smem_ceiling((const void *)kernel));
+    kernel<<<(unsigned)(p.a.batch.batch * p.a.kv_heads * s.row_tiles), C::THREADS, C::SMEM, stream>>>(p);
+    return check_launch("quantized_attention_kernel");
 }
 
 inline int attend_quantized(const mgc_cuda_paged_attention_quantized_args &a, cudaStream_t stream) {
     const char *what = "mgc_cuda_paged_attention_quantized";
-    const mgc_cuda_paged &c = a.attention.paged;
+    const mgc_cuda_paged_attention_args &b = a.attention;
+    const mgc_cuda_paged &c = b.paged;
     MGC_CHECK(check_attend_quantized(a, what));
     if (c.tokens == 0 || c.batch == 0) return MGC_CUDA_OK;
-    const AttendParams p = attend_params(a.attention);
-    const Quantized z = quantized_of(a.quantized, c);
-    const dim3 grid((unsigned)p.tokens, (unsigned)ceil_div(p.q_heads, 4));
-    auto go = [&](auto type) {
-        using T = decltype(type);
-        if (z.bits == 4) quantized_attention_row_kernel<T, 4><<<grid, 128, 0, stream>>>(p, z);
-        else quantized_attention_row_kernel<T, 8><<<grid, 128, 0, stream>>>(p, z);
-        return check_launch("quantized_attention_row_kernel");
-    };
-    if (c.dtype == MGC_F32) return go(float());
-    return c.dtype == MGC_F16 ? go(__half()) : go(__nv_bfloat16());
+    QuantParams p;
+    p.a = attend_params(b);
+    p.z = quantized_of(a.quantized, c);
+    const QuantPlan s = quant_plan_of(a);
+    if (c.tokens * p.a.group >= 0x80000000ll - 256 || c.batch * c.kv_heads * s.row_tiles > 0x7FFFFFFF)
+        return fail(MGC_CUDA_UNSUPPORTED, "%s: %lld tokens of %d heads a key head", what, (long long)c.tokens, p.a.group);
+    p.a.row_tiles = s.row_tiles;
+    p.a.interleaved = s.interleaved;
+    if (s.workspace) {
+        if (!b.workspace || b.workspace_bytes < s.workspace || !aligned(b.workspace, 16))
+            return fail(MGC_CUDA_NEEDS_WORKSPACE, "%s: needs %lld bytes of workspace (16-byte aligned), got %lld", what,
+                        (long long)s.workspace, (long long)(b.workspace ? b.workspace_bytes : 0));
+        const int64_t rows = (int64_t)s.ctas * 16 * s.nb;
+        p.a.part = static_cast<float *>(b.workspace);
+        p.a.part_ml = reinterpret_cast<float2 *>(p.a.part + rows * p.a.head_dim);
+        p.a.cut = reinterpret_cast<CutUnit *>(p.a.part_ml + rows);
+    }
+    // pairs of a row copied at once where their addresses allow it
+    const int64_t all = 4 * p.z.groups;
+    p.pair_bytes = (all == 8 || all == 16) && aligned(p.z.k_scales, (int)all) && aligned(p.z.v_scales, (int)all) &&
+                           p.z.page_stride * 4 % all == 0 && p.z.token_stride * 4 % all == 0 && p.z.head_stride * 4 % all == 0
+                       ? (int)all : 4;
+    const int chunk = 16 / elem_size(c.dtype);
+    p.q_wide = aligned(b.q, 16) && b.q_token_stride % chunk == 0 && b.q_head_stride % chunk == 0;
+    return with_config(c.dtype, a.quantized.bits, c.head_dim, s.nb, [&](auto config) { return launch_quantized(p, s, config, stream); });
 }
 
 }  // namespace paged
