@@ -136,9 +136,10 @@ __device__ __forceinline__ int unit_length(const AttendParams &p, const Sequence
     return hi > lo ? (hi - lo + KEYS - 1) / KEYS : 1;
 }
 
-// The next piece of the stretch; false at its end. Advances the walk.
-template <int ROWS, int KEYS>
-__device__ __forceinline__ bool next_item(const AttendParams &p, Walk &k, Item &w) {
+// The next piece of the stretch; false at its end. Advances the walk. (P: AttendParams, or what adds to it and
+// has a load_sequence of its own.)
+template <int ROWS, int KEYS, typename P>
+__device__ __forceinline__ bool next_item(const P &p, Walk &k, Item &w) {
     while (k.left > 0 && k.h < k.heads) {
         w.seq = k.seq;
         w.rows = w.seq.nq * p.group;
@@ -180,8 +181,8 @@ __device__ __forceinline__ bool next_item(const AttendParams &p, Walk &k, Item &
 
 // Start of stretch c of `ctas` over the units of key heads [h0, h1) (one warp). Units are looked at
 // 32 at a time; their lengths are the same for every key head.
-template <int ROWS, int KEYS>
-__device__ __forceinline__ Walk find_stretch(const AttendParams &p, int c, int ctas, int h0, int h1, int lane) {
+template <int ROWS, int KEYS, typename P>
+__device__ __forceinline__ Walk find_stretch(const P &p, int c, int ctas, int h0, int h1, int lane) {
     int most = 0;  // row tiles of the longest sequence
     for (int b = lane; b < p.batch.batch; b += 32) {
         const Sequence s = load_sequence(p, b);

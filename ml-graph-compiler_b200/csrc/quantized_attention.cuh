@@ -1,8 +1,12 @@
 // Attention of new tokens over quantised pages (quantized_common.cuh): paged_attention_params.cuh's
-// definition with k_j and v_j the values that the codes stand for.
+// definition with k_j and v_j the values that the codes stand for. The choice of kernels and the launch.
+//
+// Sequences with few query rows a key head attend over the codes (quantized_mma.cuh). For those with many the
+// values are written to plain pages in the workspace first (quantized_expand.cuh) and the kernels for plain pages
+// attend over them; key heads some at a time where the workspace would be large.
 #pragma once
 
-#include "quantized_mma.cuh"
+#include "quantized_expand.cuh"
 
 namespace mgc {
 namespace paged {
@@ -18,8 +22,46 @@ struct QuantPlan {
     int row_tiles = 1;
     bool even = false, interleaved = false;
     int ctas = 0, live_rows = 1;
-    int64_t workspace = 0;
+    int64_t workspace = 0;  // of the part over codes
+    // the part over plain pages: 0 heads if there is none
+    int heads = 0;          // key heads at a time
+    int page = 0, slots = 0;
+    int rows_left = 0;      // sequences of more query rows a key head are its
+    int64_t pages_bytes = 0, inner = 0;  // of k or v; of the attention over them
+    bool rest = true;       // the part over codes may have sequences
+    int64_t index_bytes = 0;  // of block table and lengths
+    int64_t total() const { return heads ? 2 * pages_bytes + index_bytes + inner + workspace : workspace; }
 };
+
+// More query rows a key head than this take the way over plain pages.
+constexpr int64_t DIRECT_ROWS = 64;
+constexpr int64_t EXPANDED_BYTES = 1ll << 30;  // of plain pages at a time
+
+inline int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
+
+// The call of the attention over plain pages for key heads [h0, h0 + heads).
+inline mgc_cuda_paged_attention_args expanded_args(const mgc_cuda_paged_attention_args &a, const QuantPlan &s, int h0, int heads, char *at) {
+    mgc_cuda_paged_attention_args x = a;
+    mgc_cuda_paged &c = x.paged;
+    const int es = elem_size(c.dtype), group = (int)(a.q_heads / c.kv_heads);
+    c.k = at;
+    c.v = at + s.pages_bytes;
+    c.pages = c.batch * s.slots;
+    c.kv_heads = heads;
+    c.page_size = s.page;
+    c.token_stride = c.head_dim;
+    c.head_stride = c.head_dim * s.page;
+    c.page_stride = c.head_stride * heads;
+    c.block_table = reinterpret_cast<int32_t *>(at + 2 * s.pages_bytes);
+    c.table_stride = c.table_pages = s.slots;
+    c.kv_lens = c.block_table + c.batch * s.slots;
+    x.q = static_cast<const char *>(a.q) + (int64_t)h0 * group * a.q_head_stride * es;
+    x.out = static_cast<char *>(a.out) + (int64_t)h0 * group * a.o_head_stride * es;
+    x.q_heads = (int64_t)heads * group;
+    x.workspace = at + 2 * s.pages_bytes + s.index_bytes;
+    x.workspace_bytes = s.inner;
+    return x;
+}
 
 inline int width_of(int64_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 
@@ -68,12 +110,39 @@ inline QuantPlan quant_plan_of(const mgc_cuda_paged_attention_quantized_args &a)
         }
         s.workspace = (int64_t)s.ctas * (2 * unit_rows * (c.head_dim * 4 + 8) + (int64_t)sizeof(CutUnit));
     }
+    if (rows <= DIRECT_ROWS) return s;
+    // Plain pages of the cache's size, or of a divisor that the tcgen05 kernel takes (paged_umma.cuh): 128, or a power of
+    // two from 8 to 64
+    int64_t page = c.page_size;
+    if (page % 128 == 0) page = 128;
+    else if (page % 8 == 0) page &= -page;
+    const int64_t capacity = c.table_pages * c.page_size;
+    const int64_t longest = a.attention.max_kv < capacity ? (a.attention.max_kv < 1 ? 1 : a.attention.max_kv) : capacity;
+    const int64_t per_seq = ceil_div(longest, page);
+    const int64_t head_bytes = c.batch * per_seq * page * c.head_dim * es;
+    if (capacity == 0 || c.batch > 65535 || 2 * head_bytes > EXPANDED_BYTES || c.batch * per_seq > 0x7FFFFFFF) return s;
+    int64_t heads = EXPANDED_BYTES / (2 * head_bytes);
+    s.heads = (int)(heads > c.kv_heads ? c.kv_heads : heads);
+    s.page = (int)page;
+    s.slots = (int)per_seq;
+    s.rows_left = c.batch > 1 ? (int)DIRECT_ROWS : 0;
+    s.rest = c.batch > 1 || per_seq * page < capacity;
+    s.pages_bytes = up256(head_bytes * s.heads);
+    s.index_bytes = up256(4 * (c.batch * per_seq + c.batch));
+    if (!s.rest) s.workspace = 0;
+    // (the heads of the last pass may be fewer)
+    for (int h0 = 0; h0 < c.kv_heads; h0 += s.heads) {
+        const int n = (int)(c.kv_heads - h0 < s.heads ? c.kv_heads - h0 : s.heads);
+        const mgc_cuda_paged_attention_args x = expanded_args(a.attention, s, h0, n, reinterpret_cast<char *>(256));
+        const int64_t bytes = up256(mgc_cuda_paged_attention_workspace(&x));
+        if (bytes > s.inner) s.inner = bytes;
+    }
     return s;
 }
 
 inline int64_t attend_quantized_workspace(const mgc_cuda_paged_attention_quantized_args &a) {
     if (check_attend_quantized(a, "mgc_cuda_paged_attention_quantized_workspace") != MGC_CUDA_OK) return -1;
-    return a.attention.paged.tokens == 0 || a.attention.paged.batch == 0 ? 0 : quant_plan_of(a).workspace;
+    return a.attention.paged.tokens == 0 || a.attention.paged.batch == 0 ? 0 : quant_plan_of(a).total();
 }
 
 template <typename T, int BITS, int DP, int NB>
@@ -93,6 +162,36 @@ inline int launch_quantized(const QuantParams &p, const QuantPlan &s, QuantConfi
     return check_launch("quantized_attention_kernel");
 }
 
+// The sequences that are expanded: values to plain pages, attention over them, some key heads at a time.
+inline int attend_expanded(const mgc_cuda_paged_attention_args &a, const QuantParams &p, const QuantPlan &s, char *space, cudaStream_t stream) {
+    const mgc_cuda_paged &c = a.paged;
+    for (int h0 = 0; h0 < p.a.kv_heads; h0 += s.heads) {
+        const int n = p.a.kv_heads - h0 < s.heads ? p.a.kv_heads - h0 : s.heads;
+        const mgc_cuda_paged_attention_args x = expanded_args(a, s, h0, n, space);
+        ExpandParams e;
+        e.a = p.a;
+        e.z = p.z;
+        e.k = x.paged.k;
+        e.v = x.paged.v;
+        e.table = const_cast<int32_t *>(x.paged.block_table);
+        e.kv_lens = const_cast<int32_t *>(x.paged.kv_lens);
+        e.slots = s.slots;
+        e.page = s.page;
+        e.h0 = h0;
+        e.heads = n;
+        const dim3 grid((unsigned)s.slots, (unsigned)n, (unsigned)c.batch);
+        auto go = [&](auto type) {
+            using T = decltype(type);
+            if (p.z.bits == 4) quantized_expand_kernel<T, 4><<<grid, 256, 0, stream>>>(e);
+            else quantized_expand_kernel<T, 8><<<grid, 256, 0, stream>>>(e);
+            return check_launch("quantized_expand_kernel");
+        };
+        MGC_CHECK(c.dtype == MGC_F32 ? go(float()) : c.dtype == MGC_F16 ? go(__half()) : go(__nv_bfloat16()));
+        MGC_CHECK(mgc_cuda_paged_attention(&x, stream));
+    }
+    return MGC_CUDA_OK;
+}
+
 inline int attend_quantized(const mgc_cuda_paged_attention_quantized_args &a, cudaStream_t stream) {
     const char *what = "mgc_cuda_paged_attention_quantized";
     const mgc_cuda_paged_attention_args &b = a.attention;
@@ -100,19 +199,27 @@ inline int attend_quantized(const mgc_cuda_paged_attention_quantized_args &a, cu
     MGC_CHECK(check_attend_quantized(a, what));
     if (c.tokens == 0 || c.batch == 0) return MGC_CUDA_OK;
     QuantParams p;
-    p.a = attend_params(b);
+    static_cast<AttendParams &>(p.a) = attend_params(b);
     p.z = quantized_of(a.quantized, c);
     const QuantPlan s = quant_plan_of(a);
     if (c.tokens * p.a.group >= 0x80000000ll - 256 || c.batch * c.kv_heads * s.row_tiles > 0x7FFFFFFF)
         return fail(MGC_CUDA_UNSUPPORTED, "%s: %lld tokens of %d heads a key head", what, (long long)c.tokens, p.a.group);
     p.a.row_tiles = s.row_tiles;
     p.a.interleaved = s.interleaved;
+    if (s.total() && (!b.workspace || b.workspace_bytes < s.total() || !aligned(b.workspace, 16)))
+        return fail(MGC_CUDA_NEEDS_WORKSPACE, "%s: needs %lld bytes of workspace (16-byte aligned), got %lld", what,
+                    (long long)s.total(), (long long)(b.workspace ? b.workspace_bytes : 0));
+    char *space = static_cast<char *>(b.workspace);
+    p.a.rows_left = s.rows_left;
+    p.a.kv_left = s.heads ? s.slots * s.page : 0;
+    if (s.heads) {
+        MGC_CHECK(attend_expanded(b, p, s, space, stream));
+        if (!s.rest) return MGC_CUDA_OK;
+        space += s.total() - s.workspace;
+    }
     if (s.workspace) {
-        if (!b.workspace || b.workspace_bytes < s.workspace || !aligned(b.workspace, 16))
-            return fail(MGC_CUDA_NEEDS_WORKSPACE, "%s: needs %lld bytes of workspace (16-byte aligned), got %lld", what,
-                        (long long)s.workspace, (long long)(b.workspace ? b.workspace_bytes : 0));
         const int64_t rows = (int64_t)s.ctas * 16 * s.nb;
-        p.a.part = static_cast<float *>(b.workspace);
+        p.a.part = reinterpret_cast<float *>(space);
         p.a.part_ml = reinterpret_cast<float2 *>(p.a.part + rows * p.a.head_dim);
         p.a.cut = reinterpret_cast<CutUnit *>(p.a.part_ml + rows);
     }

@@ -129,8 +129,22 @@ template <typename T> __device__ __forceinline__ void zero_outside_rows(const At
     }
 }
 
+// A call in two parts: these kernels leave sequences with more than `rows_left` query rows a key head to the
+// other (quantized_attention.cuh), if they have at most `kv_left` positions. kv_left 0: all are taken here.
+struct QuantAttend : AttendParams {
+    int rows_left, kv_left;
+};
+__device__ __forceinline__ bool left_out(const QuantAttend &p, const Sequence &s) {
+    return s.n <= p.kv_left && s.nq * p.group > p.rows_left;
+}
+__device__ __forceinline__ Sequence load_sequence(const QuantAttend &p, int b) {
+    Sequence s = load_sequence(static_cast<const AttendParams &>(p), b);
+    if (p.kv_left && left_out(p, s)) s.nq = 0;
+    return s;
+}
+
 struct QuantParams {
-    AttendParams a;
+    QuantAttend a;
     Quantized z;
     int pair_bytes;  // pairs of a row copied at once: 4, or all of them (8, 16)
     int q_wide;      // rows of q allow 16-byte loads
@@ -143,7 +157,7 @@ quantized_attention_kernel(const __grid_constant__ QuantParams params) {
     using C = QuantConfig<T, BITS, DP, NB>;
     constexpr int R = C::R, BN = C::BN, KW = C::KW, ROW = C::ROW, CPR = C::CPR, SLABS = C::SLABS, STAGES = C::STAGES;
     constexpr float LIFT = Weight<__half>::LIFT;
-    const AttendParams &p = params.a;
+    const QuantAttend &p = params.a;
     const Quantized &z = params.z;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint32_t there[C::WARPS][STAGES];  // keys of a stage that were loaded
