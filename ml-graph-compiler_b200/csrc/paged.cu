@@ -13,7 +13,7 @@ int mgc_cuda_kv_append(const mgc_cuda_kv_append_args *args, void *stream) {
 int mgc_cuda_paged_attention(const mgc_cuda_paged_attention_args *args, void *stream) {
     mgc::last_error().clear();
     if (!args) return mgc::fail(MGC_CUDA_BAD_ARGUMENT, "mgc_cuda_paged_attention: args is NULL");
-    return mgc::paged::attend(*args, (cudaStream_t)stream);
+    return mgc::paged::attend(*args, args->paged.dtype, (cudaStream_t)stream);
 }
 
 int64_t mgc_cuda_paged_attention_workspace(const mgc_cuda_paged_attention_args *args) {

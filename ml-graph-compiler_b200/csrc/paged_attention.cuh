@@ -129,7 +129,7 @@ inline int64_t attend_workspace(const mgc_cuda_paged_attention_args &a) {
     return a.paged.tokens == 0 || a.paged.batch == 0 ? 0 : plan_of(a).workspace;
 }
 
-template <typename T> inline int launch_umma(const AttendParams &p, const mgc_cuda_paged &c, int ctas, cudaStream_t stream) {
+template <typename T, typename O> inline int launch_umma(const AttendParams &p, const mgc_cuda_paged &c, int ctas, cudaStream_t stream) {
     UmmaMaps maps;
     memset(&maps, 0, sizeof maps);
     if (!umma_maps(&maps, c)) return fail(MGC_CUDA_UNSUPPORTED, "mgc_cuda_paged_attention: tensor map encoding failed");
@@ -138,9 +138,9 @@ template <typename T> inline int launch_umma(const AttendParams &p, const mgc_cu
         kernel<<<(unsigned)ctas, threads, smem, stream>>>(p, maps);
         return check_launch("paged_attention_umma_kernel");
     };
-    MGC_CHECK(p.head_dim <= 64 ? go(paged_attention_umma_kernel<T, 64>, UmmaConfig<64>::SMEM, UmmaConfig<64>::THREADS)
-                               : go(paged_attention_umma_kernel<T, 128>, UmmaConfig<128>::SMEM, UmmaConfig<128>::THREADS));
-    return launch_after(paged_combine_units_kernel<T, 256>, dim3((unsigned)ctas, 32), p, 1, stream);
+    MGC_CHECK(p.head_dim <= 64 ? go(paged_attention_umma_kernel<T, 64, O>, UmmaConfig<64>::SMEM, UmmaConfig<64>::THREADS)
+                               : go(paged_attention_umma_kernel<T, 128, O>, UmmaConfig<128>::SMEM, UmmaConfig<128>::THREADS));
+    return launch_after(paged_combine_units_kernel<O, 256>, dim3((unsigned)ctas, 32), p, 1, stream);
 }
 
 template <typename T, int DP, int WM, int WN, int SIMT> inline int launch_mma(const AttendParams &p, const Plan &s, cudaStream_t stream) {
@@ -191,13 +191,15 @@ template <typename T> inline int launch_mma_width(const AttendParams &p, const P
     return launch_mma_rows<T, 256>(p, s, stream);
 }
 
-inline int attend(const mgc_cuda_paged_attention_args &a, cudaStream_t stream) {
+int attend(const mgc_cuda_paged_attention_args &a, int64_t q_dtype, cudaStream_t stream) {
     const char *what = "mgc_cuda_paged_attention";
     const mgc_cuda_paged &c = a.paged;
     MGC_CHECK(check_attend(a, what));
     if (c.tokens == 0 || c.batch == 0) return MGC_CUDA_OK;
     AttendParams p = attend_params(a);
     const Plan s = plan_of(a);
+    if (q_dtype != c.dtype && !(s.umma && c.dtype == MGC_F16 && q_dtype == MGC_BF16))
+        return fail(MGC_CUDA_UNSUPPORTED, "%s: queries of type %d over pages of type %d", what, (int)q_dtype, (int)c.dtype);
     p.row_tiles = s.row_tiles; p.splits = s.splits; p.interleaved = s.interleaved;
     if (s.workspace) {
         if (!a.workspace || a.workspace_bytes < s.workspace || !aligned(a.workspace, 16))
@@ -212,7 +214,9 @@ inline int attend(const mgc_cuda_paged_attention_args &a, cudaStream_t stream) {
         const int64_t units = c.batch * c.kv_heads * s.row_tiles;
         if (units > 0x7FFFFFFF) return fail(MGC_CUDA_UNSUPPORTED, "%s: %lld row tiles", what, (long long)units);
         if (s.umma)
-            return c.dtype == MGC_F16 ? launch_umma<__half>(p, c, s.ctas, stream) : launch_umma<__nv_bfloat16>(p, c, s.ctas, stream);
+            return c.dtype != MGC_F16      ? launch_umma<__nv_bfloat16, __nv_bfloat16>(p, c, s.ctas, stream)
+                   : q_dtype != MGC_F16 ? launch_umma<__half, __nv_bfloat16>(p, c, s.ctas, stream)
+                                        : launch_umma<__half, __half>(p, c, s.ctas, stream);
         if (c.dtype == MGC_F32) return launch_mma_width<float>(p, s, stream);
         if (c.dtype == MGC_F16) return launch_mma_width<__half>(p, s, stream);
         return launch_mma_width<__nv_bfloat16>(p, s, stream);

@@ -72,6 +72,10 @@ inline int check_attend(const mgc_cuda_paged_attention_args &a, const char *what
     return MGC_CUDA_OK;
 }
 
+// The call behind mgc_cuda_paged_attention (paged.cu). q_dtype: of q and out, where it is not the pages'
+// (bf16 over half pages, in calls that take the tcgen05 kernel).
+int attend(const mgc_cuda_paged_attention_args &a, int64_t q_dtype, cudaStream_t stream);
+
 // The parameters that a call's arguments give; its plan adds the rest.
 inline AttendParams attend_params(const mgc_cuda_paged_attention_args &a) {
     const mgc_cuda_paged &c = a.paged;

@@ -201,11 +201,11 @@ __device__ __forceinline__ int tiles_needed(const AttendParams &p, const Item &w
 
 // The slow way round for rows whose tiles held something that they do not see: this thread's row over
 // the keys of piece w that it sees, on the FMA units, into TMEM where the products would have left it.
-// `q` names the row's 16-byte chunks in shared memory. The whole warp calls; threads without `all` compute
+// `q` names the row's 16-byte chunks in shared memory, scale_log2 goes with them. The whole warp calls; threads without `all` compute
 // their row only if a key that it does not see has a value that is not finite. A piece of 16384 keys of 128
 // channels takes about 40 ms while the other roles wait: WAIT_LIMIT, 4.5 s, covers pieces of 1.7 million.
 template <typename T, int DP, typename Q>
-__device__ __forceinline__ void row_again(const AttendParams &p, const Item &w, int row, Q q, bool all, bool maybe, uint32_t to, float &m, float &l) {
+__device__ __forceinline__ void row_again(const AttendParams &p, const Item &w, int row, Q q, float scale_log2, bool all, bool maybe, uint32_t to, float &m, float &l) {
     const RowRange see = row_range(p, w.seq, row);
     const int lo = max(see.lo, w.lo), hi = min(see.hi, w.hi), ps = p.batch.page_size;
     const long long head = (long long)w.h * p.head_stride;
@@ -257,7 +257,7 @@ __device__ __forceinline__ void row_again(const AttendParams &p, const Item &w, 
 #pragma unroll
                 for (int i = 0; i < 8; ++i) part[i & 3] = fmaf(to_f(x.e[i]), to_f(y.e[i]), part[i & 3]);
             }
-            const float s = __fmul_rn((part[0] + part[1]) + (part[2] + part[3]), p.scale_log2);
+            const float s = __fmul_rn((part[0] + part[1]) + (part[2] + part[3]), scale_log2);
             if (s == -INFINITY) return true;
             if (s > m) {
                 const float f = ex2(m - s);
@@ -292,7 +292,20 @@ __device__ __forceinline__ void row_again(const AttendParams &p, const Item &w, 
     tmem_wait_st();
 }
 
-template <typename T, int DP>
+// Eight values of q's type in the pages' type, times f.
+template <typename T, typename O> __device__ __forceinline__ uint4 as_pages(uint4 v, float f) {
+    Pack<8, O> x;
+    Pack<8, T> y;
+    x.raw[0] = v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y.e[i] = from_f<T>(to_f(x.e[i]) * f);
+    return y.raw[0];
+}
+
+// T: the pages' type, O: q's and out's. Where they differ (bf16 queries over half pages: keys and values that
+// were written in 4 or 8 bits keep more of them in half's 11 bits), a row of q is scaled by a power of two so that
+// its largest value is in [1, 2).
+template <typename T, int DP, typename O = T>
 __global__ void __launch_bounds__(UmmaConfig<DP>::THREADS, 1)
 paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid_constant__ UmmaMaps maps) {
     using C = UmmaConfig<DP>;
@@ -331,7 +344,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
         const Walk k = find_stretch<256, 128>(p, (int)blockIdx.x, (int)gridDim.x, 0, p.kv_heads, lane);
         if (lane == 0) stretch = k;
     }
-    if (warp == 10) zero_outside<T>(p, (int)blockIdx.x, (int)gridDim.x, 0, 1, lane);
+    if (warp == 10) zero_outside<O>(p, (int)blockIdx.x, (int)gridDim.x, 0, 1, lane);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -545,6 +558,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
             uint8_t *rows32 = sQ + x * C::TILE + (r & 96) * 128;  // the warp's 32 rows of the Q tile
             auto chunk = [&](int rr, int c) { return rows32 + (c >> 3) * C::HALF + rr * 128 + (((c & 7) ^ (rr & 7)) << 4); };
             const int lives = min(32, w.rows - (w.row0 + x * 128 + (r & 96)));  // rows of the warp that exist
+            float scale_log2 = p.scale_log2;
             {
                 uint4 v[CHUNKS];  // every load in flight before the first store
 #pragma unroll
@@ -553,7 +567,25 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                     const long long off = __shfl_sync(0xFFFFFFFFu, q_off, rr);
                     v[i] = make_uint4(0, 0, 0, 0);
                     if (rr < lives && c * 8 < p.head_dim)
-                        v[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q) + off + c * 8));
+                        v[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const O *>(p.q) + off + c * 8));
+                }
+                if constexpr (!std::is_same<T, O>::value) {
+#pragma unroll
+                    for (int i = 0; i < CHUNKS; ++i) {
+                        Pack<8, O> e8;
+                        e8.raw[0] = v[i];
+                        float most = 0.0f;
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) most = fmaxf(most, fabsf(to_f(e8.e[u])));
+#pragma unroll
+                        for (int d = 1; d < CHUNKS; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
+                        const int ex = (int)(__float_as_uint(most) >> 23);
+                        const int up = ex == 0 || ex == 255 ? 0 : max(min(127 - ex, 126), -126);
+                        v[i] = as_pages<T, O>(v[i], __uint_as_float((uint32_t)(127 + up) << 23));
+                        // rows 32 / CHUNKS i .. of the warp are these lanes': theirs takes the scale along
+                        const int mine = __shfl_sync(0xFFFFFFFFu, up, (lane * CHUNKS) % 32);
+                        if (lane * CHUNKS / 32 == i) scale_log2 = p.scale_log2 * __uint_as_float((uint32_t)(127 - mine) << 23);
+                    }
                 }
 #pragma unroll
                 for (int i = 0; i < CHUNKS; ++i)
@@ -610,7 +642,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], s[124 + e]);
-                const float mt = __fmul_rn(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), p.scale_log2);
+                const float mt = __fmul_rn(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), scale_log2);
                 // grown by more than 2^LAZY (or the first finite maximum): move the reference
                 const bool grow = mt > m + Weight<T>::LAZY;
                 if (C::APART && j > 0) {  // the products with the last tile's weights are done
@@ -634,7 +666,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                 }
                 if (grow) m = mt;
                 const float y = m == -INFINITY ? 0.0f : m;
-                const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), y2 = make_float2(Weight<T>::LAZY_LIFT - y, Weight<T>::LAZY_LIFT - y);
+                const float2 scale2 = make_float2(scale_log2, scale_log2), y2 = make_float2(Weight<T>::LAZY_LIFT - y, Weight<T>::LAZY_LIFT - y);
                 float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {  // the first 64 keys' products start while the others' weights are made
@@ -682,7 +714,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                 }
                 if (bad || __any_sync(0xFFFFFFFFu, maybe)) {
                     auto q = [&](int c) { return reinterpret_cast<const T *>(chunk(lane, c)); };
-                    row_again<T, DP>(p, w, w.row0 + x * 128 + r, q, bad, maybe, to, m, l);
+                    row_again<T, DP>(p, w, w.row0 + x * 128 + r, q, scale_log2, bad, maybe, to, m, l);
                 }
             }
             // ---- O: through the warp's rows of the Q tile (no longer read) to whole rows of memory ----
@@ -708,7 +740,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                             uint32_t q[4];
 #pragma unroll
                             for (int u = 0; u < 4; ++u)
-                                q[u] = pack2<T>(__uint_as_float(t[8 * i + 2 * u]) * inv, __uint_as_float(t[8 * i + 2 * u + 1]) * inv);
+                                q[u] = pack2<O>(__uint_as_float(t[8 * i + 2 * u]) * inv, __uint_as_float(t[8 * i + 2 * u + 1]) * inv);
                             *reinterpret_cast<uint4 *>(chunk(lane, pass * (DP / 16) + c * 4 + i)) = make_uint4(q[0], q[1], q[2], q[3]);
                         }
                     } else {
@@ -727,7 +759,7 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                     if (rr >= lives) continue;
                     const uint4 v = *reinterpret_cast<const uint4 *>(chunk(rr, c));
                     if (whole) {
-                        if (c * 8 < p.head_dim) *reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + off + c * 8) = v;
+                        if (c * 8 < p.head_dim) *reinterpret_cast<uint4 *>(static_cast<O *>(p.out) + off + c * 8) = v;
                     } else if (pass * (DP / 2) + c * 4 < p.head_dim) {
                         *reinterpret_cast<uint4 *>(p.part + (at + rr) * p.head_dim + pass * (DP / 2) + c * 4) = v;
                     }

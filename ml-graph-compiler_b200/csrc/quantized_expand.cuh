@@ -7,8 +7,8 @@
 //
 // Pages of `page` positions (the cache's page size or a divisor), one head's rows side by side; sequence b's
 // positions from page * s on are page b * slots + s. Rows that no token sees are zero, so that whatever the cache
-// holds there is not met again; a missing page stays missing. Values are fp32, rounded once to the type, and held
-// within half's range in f16.
+// holds there is not met again; a missing page stays missing. Values are fp32, rounded once to the pages' type:
+// fp32, or half for 16-bit queries, held within its range.
 #pragma once
 
 #include "kv_read.cuh"
