@@ -12,8 +12,15 @@ namespace mgc {
 namespace paged {
 
 inline int check_attend_quantized(const mgc_cuda_paged_attention_quantized_args &a, const char *what) {
+    const mgc_cuda_paged &c = a.attention.paged;
     MGC_CHECK(check_attend(a.attention, what));
-    return check_quantized(a.quantized, a.attention.paged, what);
+    MGC_CHECK(check_quantized(a.quantized, c, what));
+    // the kernel multiplies strides by page numbers and rows in 32 bits
+    const int64_t most = 0xFFFFFFFFll;
+    auto fits = [&](int64_t page, int64_t token) { return page <= most && token <= most / c.page_size; };
+    if (!fits(c.page_stride / 16, c.token_stride / 16) || !fits(a.quantized.page_stride, a.quantized.token_stride))
+        return fail(MGC_CUDA_UNSUPPORTED, "%s: a page does not fit 32 bits", what);
+    return MGC_CUDA_OK;
 }
 
 // How a call runs.
@@ -66,21 +73,23 @@ inline mgc_cuda_paged_attention_args expanded_args(const mgc_cuda_paged_attentio
 
 inline int width_of(int64_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 
-// Calls `go` with the configuration of a type, width and row tile.
-template <typename F> inline auto with_config(int64_t dtype, int64_t bits, int64_t head_dim, int nb, F go) {
+// Calls `go` with the configuration of a type, width, row tile and grouping.
+template <typename F> inline auto with_config(int64_t dtype, const mgc_cuda_quantized &z, int64_t head_dim, int nb, F go) {
     auto widths = [&](auto type, auto b) {
         using T = decltype(type);
         constexpr int BITS = decltype(b)::value;
         const int dp = width_of(head_dim);
-        if (dp == 64) return nb > 1 ? go(QuantConfig<T, BITS, 64, 2>()) : go(QuantConfig<T, BITS, 64, 1>());
-        if (dp == 128) return nb > 1 ? go(QuantConfig<T, BITS, 128, 2>()) : go(QuantConfig<T, BITS, 128, 1>());
-        return go(QuantConfig<T, BITS, 256, 1>());
+        if (dp == 64) return nb > 1 ? go(QuantConfig<T, BITS, 64, 2, true>()) : go(QuantConfig<T, BITS, 64, 1, true>());
+        const bool one = z.group == head_dim;
+        if (dp == 256) return one ? go(QuantConfig<T, BITS, 256, 1, true>()) : go(QuantConfig<T, BITS, 256, 1, false>());
+        if (one) return nb > 1 ? go(QuantConfig<T, BITS, 128, 2, true>()) : go(QuantConfig<T, BITS, 128, 1, true>());
+        return nb > 1 ? go(QuantConfig<T, BITS, 128, 2, false>()) : go(QuantConfig<T, BITS, 128, 1, false>());
     };
     auto types = [&](auto b) {
         if (dtype == MGC_F32) return widths(float(), b);
         return dtype == MGC_F16 ? widths(__half(), b) : widths(__nv_bfloat16(), b);
     };
-    return bits == 4 ? types(std::integral_constant<int, 4>()) : types(std::integral_constant<int, 8>());
+    return z.bits == 4 ? types(std::integral_constant<int, 4>()) : types(std::integral_constant<int, 8>());
 }
 
 inline QuantPlan quant_plan_of(const mgc_cuda_paged_attention_quantized_args &a) {
@@ -99,7 +108,7 @@ inline QuantPlan quant_plan_of(const mgc_cuda_paged_attention_quantized_args &a)
     // the kernel that adds pieces stores four elements at once
     const int es = elem_size(c.dtype);
     const bool wide = aligned(a.attention.out, 4 * es) && a.attention.o_token_stride % 4 == 0 && a.attention.o_head_stride % 4 == 0;
-    const int resident = with_config(c.dtype, a.quantized.bits, c.head_dim, s.nb, [](auto config) { return decltype(config)::RESIDENT; });
+    const int resident = with_config(c.dtype, a.quantized, c.head_dim, s.nb, [](auto config) { return decltype(config)::RESIDENT; });
     const int64_t slots = (int64_t)sm_count() * resident;
     // Even shares cost a second kernel and the pieces' way through memory, some 500 keys' worth of time
     if (wide && most > 512 + most * units / slots) {
@@ -153,18 +162,16 @@ inline int64_t attend_quantized_workspace(const mgc_cuda_paged_attention_quantiz
     return a.attention.paged.tokens == 0 || a.attention.paged.batch == 0 ? 0 : quant_plan_of(a).total();
 }
 
-template <typename T, int BITS, int DP, int NB>
-inline int launch_quantized(const QuantParams &p, const QuantPlan &s, QuantConfig<T, BITS, DP, NB>, cudaStream_t stream) {
-    using C = QuantConfig<T, BITS, DP, NB>;
+template <typename C> inline int launch_quantized(const QuantParams &p, const QuantPlan &s, C, cudaStream_t stream) {
     if (s.even) {
-        auto kernel = quantized_attention_kernel<T, BITS, DP, NB, true>;
+        auto kernel = quantized_attention_kernel<C, true>;
         MGC_CHECK(raise_smem_ceiling((const void *)kernel));
         kernel<<<(unsigned)s.ctas, C::THREADS, C::SMEM, stream>>>(p);
         MGC_CHECK(check_launch("quantized_attention_kernel"));
-        return launch_after(paged_combine_units_kernel<T, C::R>, dim3((unsigned)s.ctas, (unsigned)s.live_rows), p.a,
+        return launch_after(paged_combine_units_kernel<typename C::T, C::R>, dim3((unsigned)s.ctas, (unsigned)s.live_rows), p.a,
                             s.interleaved ? p.a.kv_heads : 1, stream);
     }
-    auto kernel = quantized_attention_kernel<T, BITS, DP, NB, false>;
+    auto kernel = quantized_attention_kernel<C, false>;
     MGC_CHECK(raise_smem_ceiling((const void *)kernel));
     kernel<<<(unsigned)(p.a.batch.batch * p.a.kv_heads * s.row_tiles), C::THREADS, C::SMEM, stream>>>(p);
     return check_launch("quantized_attention_kernel");
@@ -231,14 +238,18 @@ inline int attend_quantized(const mgc_cuda_paged_attention_quantized_args &a, cu
         p.a.part_ml = reinterpret_cast<float2 *>(p.a.part + rows * p.a.head_dim);
         p.a.cut = reinterpret_cast<CutUnit *>(p.a.part_ml + rows);
     }
-    // pairs of a row copied at once where their addresses allow it
-    const int64_t all = 4 * p.z.groups;
-    p.pair_bytes = (all == 8 || all == 16) && aligned(p.z.k_scales, (int)all) && aligned(p.z.v_scales, (int)all) &&
-                           p.z.page_stride * 4 % all == 0 && p.z.token_stride * 4 % all == 0 && p.z.head_stride * 4 % all == 0
-                       ? (int)all : 4;
+    // division by the page size: with s = ceil(log2 d), ceil(2^(31 + s) / d) fits 32 bits and is exact below 2^31
+    int shift = 0;
+    while ((1ll << shift) < c.page_size) ++shift;
+    p.page_shift = 31 + shift;
+    p.page_magic = (uint32_t)(((1ull << (31 + shift)) + (uint64_t)c.page_size - 1) / (uint64_t)c.page_size);
+    p.code_page = (uint32_t)(c.page_stride / 16);
+    p.code_token = (uint32_t)(c.token_stride / 16);
+    p.pair_page = (uint32_t)a.quantized.page_stride;
+    p.pair_token = (uint32_t)a.quantized.token_stride;
     const int chunk = 16 / elem_size(c.dtype);
     p.q_wide = aligned(b.q, 16) && b.q_token_stride % chunk == 0 && b.q_head_stride % chunk == 0;
-    return with_config(c.dtype, a.quantized.bits, c.head_dim, s.nb, [&](auto config) { return launch_quantized(p, s, config, stream); });
+    return with_config(c.dtype, a.quantized, c.head_dim, s.nb, [&](auto config) { return launch_quantized(p, s, config, stream); });
 }
 
 }  // namespace paged

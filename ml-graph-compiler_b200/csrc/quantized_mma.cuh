@@ -2,10 +2,16 @@
 // rows per key head, which the bytes of the cache bound.
 //
 // Codes go into the products as halves, which hold them exactly, and what a group's channels share comes after:
-//   score:  q . k_j = sum_g scale_jg (q_g . (code_jg - c)) + (offset_jg + c scale_jg) sum(q_g)
-//   output: o_d     = sum_j (w_j scale_jg) (code_jd - c) + sum_j w_j (offset_jg + c scale_jg),  c = 2^(bits - 1)
+//   score:  q . k_j = sum_g scale_jg (q_g . code_jg) + offset_jg sum(q_g)
+//   output: o_d     = sum_j (w_j scale_jg) code_jd + sum_j w_j offset_jg
 // so a value costs its conversion and nothing else: no rounding of keys or values, fp32 queries and weights
-// in two halves each (22 bits).
+// in two halves each (22 bits). With c = 2^(bits - 1), codes become halves
+//  * exactly and centred, as 1024 + code (or 64 + code), less 1024 + c: values, whose weights are rounded, so that
+//    the error goes with |code - c| and not with the code (0.04 % of the output over 131071 keys, 0.02 % centred),
+//    and the keys of fp32 calls;
+//  * by masks alone: 16-bit calls' keys. Bits 4 to 7 of a half that is otherwise zero are the subnormal
+//    code * 2^-20, a byte is code * 2^-24, and the power of two comes off with the scales. A subnormal's products are
+//    cut off at 2^-24 of what a normal operand would have given, 2^-18 of a 4-bit step times the largest query value.
 //
 // A CTA takes a unit of R = 8 NB query rows (row = token * group + head of the group) of one key head. Keys are
 // the M = 16 side of m16n8k16 products and rows the N = 8 side: a key head's 4 to 8 query heads leave less of
@@ -13,11 +19,11 @@
 // stages (cp.async), maximum, sum and output, so warps meet only at the end of a piece.
 //  * K: both operands may take the contraction's channels in any order, so lane (g, t) of a fragment takes
 //    eight consecutive codes of key g's 32 (a 4- or 8-byte load) and Q's fragments follow that order.
-//  * V: as V^T, 16 channels by 16 keys: lane (g, t) takes eight consecutive channels of keys t and t + 4 and pairs
-//    the two keys' codes by byte permutations. Key i of a fragment is therefore position (i / 2) + 4 (i % 2)
-//    of its eight; scores are made in the same order, and movmatrix turns weights [key][row] into the second
-//    product's operand.
-//  * 16-byte chunks of a row are permuted by the row's number so that both reads are free of bank conflicts.
+//  * V: as V^T, 16 channels by 16 keys: lane (g, t) takes eight consecutive channels of two keys at a time and pairs
+//    the two keys' codes by byte permutations (first(t) and second(t) below). Scores are made in
+//    the same order of keys, and movmatrix turns weights [key][row] into the second product's operand.
+//  * rows are padded so that both reads are free of bank conflicts (QuantConfig).
+//  * scales and offsets: lane l reads key l's a step ahead and leaves them as floats in shared memory.
 //  * weights times scales are halves 2^14 times as large (paged_attention_params.cuh's reasons), relative to
 //    S_g, a power of two at or above the group's scales so far: tokens' scales may differ by far.
 //  * query rows are scaled by a power of two into half's range (bf16 and fp32 have more exponent).
@@ -31,20 +37,29 @@
 namespace mgc {
 namespace paged {
 
-template <typename T, int BITS, int DP, int NB> struct QuantConfig {
-    static constexpr bool F32 = sizeof(T) == 4;
+// ONE: a head is one group. Else every 64 channels are treated as a group of their own.
+template <typename T_, int BITS_, int DP_, int NB_, bool ONE_> struct QuantConfig {
+    using T = T_;
+    static constexpr int BITS = BITS_, DP = DP_, NB = NB_;
+    static constexpr bool ONE = ONE_, F32 = sizeof(T) == 4;
     static constexpr int WARPS = 4, THREADS = 32 * WARPS;
     static constexpr int R = 8 * NB;             // query rows of a unit
     static constexpr int KW = 32, BN = KW * WARPS;  // keys of a warp's step, of a tile
-    static constexpr int ROW = DP * BITS / 8, CPR = ROW / 16;  // bytes and chunks of a row of codes
-    static constexpr int SLABS = DP / 64;        // most groups, too
-    static constexpr int CODES = KW * ROW, PAIRS = KW * SLABS * 4;
-    static constexpr int STAGE = 2 * (CODES + PAIRS);
-    static constexpr int STAGES = STAGE > 8192 ? 2 : 3;
+    // Bytes and chunks of a row of codes, bytes between rows. A warp reads 16 bytes of each of a fragment's eight
+    // rows (keys, 4 bits), 32 of its rows 0 to 3 and 4 to 7 (8 bits), and 32 of the four rows first(t) or second(t)
+    // (values): 16 times an odd number lets eight rows' 16 bytes and four even or four odd rows' 32 bytes fall into
+    // different banks, 32 times an odd number four rows' 32 bytes if the rows differ modulo 4.
+    static constexpr int ROW = DP * BITS / 8, CPR = ROW / 16, PITCH = ROW + (BITS == 4 ? 16 : 32);
+    static __device__ __forceinline__ int first(int t) { return BITS == 4 ? 2 * t : t; }
+    static __device__ __forceinline__ int second(int t) { return BITS == 4 ? 2 * t + 1 : 4 + (t ^ 2); }
+    static constexpr int SLABS = DP / 64, GS = ONE ? 1 : SLABS;  // groups that are told apart
+    static constexpr int CODES = KW * PITCH, STAGE = 2 * CODES;
+    static constexpr int STAGES = DP > 64 || BITS > 4 ? 2 : 3;
     static constexpr int RING = WARPS * STAGES * STAGE;
+    static constexpr int PAIRS = KW * GS * 8;    // bytes of a step's scales and offsets of K or V
     static constexpr int ORED = DP + 4;
     static constexpr int RED = WARPS * R * (ORED + 2) * 4;
-    static constexpr int SMEM = RING > RED ? RING : RED;
+    static constexpr int SMEM = RING + WARPS * 2 * PAIRS > RED ? RING + WARPS * 2 * PAIRS : RED;
     // blocks of an SM, by shared memory and by registers (128 threads of 128, 168 or 255)
     static constexpr int BY_SMEM = 232448 / (SMEM + 1024 + 64);
     static constexpr int BY_REGS = (NB > 1 && DP > 64) || (F32 && DP > 128) ? 2 : DP > 128 || (F32 && DP * NB > 64) ? 3 : 4;
@@ -56,67 +71,70 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-template <int BYTES> __device__ __forceinline__ void cp_async_small(uint32_t dst, const void *src, int bytes) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ uint32_t sub_half2(uint32_t a, uint32_t b) {
     const __half2 d = __hsub2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
     return *reinterpret_cast<const uint32_t *>(&d);
 }
-// (x & mask) | bits: a code put into the mantissa of 1024 (its low bits) or 64 (bits 4 to 7 of the half).
+// (x & mask) | bits
 __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
     uint32_t y;
     asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(bits));
     return y;
 }
-constexpr uint32_t HALF2_1024 = 0x64006400u, HALF2_64 = 0x54005400u;
-constexpr uint32_t HALF2_1032 = 0x64086408u, HALF2_72 = 0x54805480u, HALF2_1152 = 0x64806480u;
 
-// Eight codes of a key, less c, as four pairs; channel(i, s) is the s-th of pair i.
-template <int BITS> struct Key;
-template <> struct Key<4> {
+// Eight codes of a row as four pairs of halves; channel(i, s) is the s-th of pair i. UNIT: the half of code
+// MID + 1. EXACT: normal halves.
+template <int BITS, bool EXACT> struct Key;
+template <bool EXACT> struct Key<4, EXACT> {
+    static constexpr float UNIT = EXACT ? 1.0f : 1.0f / 1048576.0f, MID = EXACT ? 8.0f : 0.0f;
     uint32_t w;
     __device__ __forceinline__ void load(const uint8_t *p) { w = *reinterpret_cast<const uint32_t *>(p); }
+    // a nibble in bits 0 to 3, 4 to 7 of both halves of x
+    static __device__ __forceinline__ uint32_t low(uint32_t x) {
+        return EXACT ? sub_half2(and_or(x, 0x000F000Fu, 0x64006400u), 0x64086408u) : x << 4 & 0x00F000F0u;
+    }
+    static __device__ __forceinline__ uint32_t high(uint32_t x) {
+        return EXACT ? sub_half2(and_or(x, 0x00F000F0u, 0x54005400u), 0x54805480u) : x & 0x00F000F0u;
+    }
     __device__ __forceinline__ void pairs(uint32_t (&h)[4]) const {
-        h[0] = sub_half2(and_or(w, 0x000F000Fu, HALF2_1024), HALF2_1032);
-        h[1] = sub_half2(and_or(w, 0x00F000F0u, HALF2_64), HALF2_72);
-        h[2] = sub_half2(and_or(w >> 8, 0x000F000Fu, HALF2_1024), HALF2_1032);
-        h[3] = sub_half2(and_or(w >> 8, 0x00F000F0u, HALF2_64), HALF2_72);
+        h[0] = low(w);
+        h[1] = high(w);
+        h[2] = EXACT ? low(w >> 8) : high(w >> 4);
+        h[3] = high(w >> 8);
     }
     static __device__ __forceinline__ constexpr int channel(int i, int second) { return i + 4 * second; }
+    // codes 2 J and 2 J + 1 of rows a and b: (a's, b's) pairs
+    template <int J> static __device__ __forceinline__ void two_rows(const Key &a, const Key &b, uint32_t &even, uint32_t &odd) {
+        const uint32_t x = __byte_perm(a.w, b.w, J | J << 4 | (4 + J) << 8 | (4 + J) << 12);
+        even = low(x);
+        odd = high(x);
+    }
 };
-template <> struct Key<8> {
+template <bool EXACT> struct Key<8, EXACT> {
+    static constexpr float UNIT = EXACT ? 1.0f : 1.0f / 16777216.0f, MID = EXACT ? 128.0f : 0.0f;
     uint2 w;
     __device__ __forceinline__ void load(const uint8_t *p) { w = *reinterpret_cast<const uint2 *>(p); }
+    // bytes 0 and 1, 2 and 3 of x
+    static __device__ __forceinline__ uint32_t low(uint32_t x) {
+        return EXACT ? sub_half2(__byte_perm(x, 0x64646464u, 0x4140), 0x64806480u) : __byte_perm(x, 0, 0x4140);
+    }
+    static __device__ __forceinline__ uint32_t high(uint32_t x) {
+        return EXACT ? sub_half2(__byte_perm(x, 0x64646464u, 0x4342), 0x64806480u) : __byte_perm(x, 0, 0x4342);
+    }
     __device__ __forceinline__ void pairs(uint32_t (&h)[4]) const {
-        h[0] = sub_half2(__byte_perm(w.x, 0x64646464u, 0x4140), HALF2_1152);
-        h[1] = sub_half2(__byte_perm(w.x, 0x64646464u, 0x4342), HALF2_1152);
-        h[2] = sub_half2(__byte_perm(w.y, 0x64646464u, 0x4140), HALF2_1152);
-        h[3] = sub_half2(__byte_perm(w.y, 0x64646464u, 0x4342), HALF2_1152);
+        h[0] = low(w.x);
+        h[1] = high(w.x);
+        h[2] = low(w.y);
+        h[3] = high(w.y);
     }
     static __device__ __forceinline__ constexpr int channel(int i, int second) { return 2 * i + second; }
+    template <int J> static __device__ __forceinline__ void two_rows(const Key &a, const Key &b, uint32_t &even, uint32_t &odd) {
+        constexpr int I = 2 * (J & 1);
+        const uint32_t x = __byte_perm(J < 2 ? a.w.x : a.w.y, J < 2 ? b.w.x : b.w.y, I | (4 + I) << 4 | (I + 1) << 8 | (5 + I) << 12);
+        even = low(x);
+        odd = high(x);
+    }
 };
-// Codes 2 j and 2 j + 1 of two keys a and b, less c: (a's, b's) pairs.
-template <int J> __device__ __forceinline__ void two_keys(const Key<4> &a, const Key<4> &b, uint32_t &even, uint32_t &odd) {
-    const uint32_t x = __byte_perm(a.w, b.w, J | J << 4 | (4 + J) << 8 | (4 + J) << 12);
-    even = sub_half2(and_or(x, 0x000F000Fu, HALF2_1024), HALF2_1032);
-    odd = sub_half2(and_or(x, 0x00F000F0u, HALF2_64), HALF2_72);
-}
-template <int J> __device__ __forceinline__ void two_keys(const Key<8> &a, const Key<8> &b, uint32_t &even, uint32_t &odd) {
-    constexpr int I = 2 * (J & 1);
-    const uint32_t x = __byte_perm(J < 2 ? a.w.x : a.w.y, J < 2 ? b.w.x : b.w.y, I | (4 + I) << 4 | (I + 1) << 8 | (5 + I) << 12);
-    even = sub_half2(__byte_perm(x, 0x64646464u, 0x4140), HALF2_1152);
-    odd = sub_half2(__byte_perm(x, 0x64646464u, 0x4342), HALF2_1152);
-}
-
-// What row r (0..7 of eight) exclusive-ors its chunks' numbers with. A warp reads one chunk of eight rows
-// (keys, 4 bits), two adjacent chunks of rows {0, 4, 1, 5} or {2, 6, 3, 7} (8 bits) and of rows 0..3 or 4..7
-// (values): in each the chunks land in different banks.
-template <int ROW> __device__ __forceinline__ int swizzle(int r) {
-    if constexpr (ROW == 32) return r >> 2 & 1;
-    else if constexpr (ROW == 64) return ((r >> 1 ^ r >> 2) & 1) << 1 | (r >> 2 & 1);
-    else return ((r & 3) ^ (r >> 2 & 1) << 1) << 1 | (r >> 2 & 1);
-}
 
 // Zeros in the rows of out that no sequence has, whatever their alignment (zero_outside's work).
 template <typename T> __device__ __forceinline__ void zero_outside_rows(const AttendParams &p, int t0, int t_step, int h0, int h_step, int lane) {
@@ -146,107 +164,118 @@ __device__ __forceinline__ Sequence load_sequence(const QuantAttend &p, int b) {
 struct QuantParams {
     QuantAttend a;
     Quantized z;
-    int pair_bytes;  // pairs of a row copied at once: 4, or all of them (8, 16)
-    int q_wide;      // rows of q allow 16-byte loads
+    int q_wide;             // rows of q allow 16-byte loads
+    uint32_t page_magic;    // j / page_size = j * page_magic >> page_shift for 0 <= j < 2^31
+    int page_shift;
+    // strides that fit 32 bits: of codes in 16 bytes, of scales in pairs
+    uint32_t code_page, code_token, pair_page, pair_token;
 };
 
 // EVEN: the CTA takes an even share of all units' keys (paged_work.cuh); else one unit's keys.
-template <typename T, int BITS, int DP, int NB, bool EVEN>
-__global__ void __launch_bounds__(QuantConfig<T, BITS, DP, NB>::THREADS, QuantConfig<T, BITS, DP, NB>::RESIDENT)
-quantized_attention_kernel(const __grid_constant__ QuantParams params) {
-    using C = QuantConfig<T, BITS, DP, NB>;
-    constexpr int R = C::R, BN = C::BN, KW = C::KW, ROW = C::ROW, CPR = C::CPR, SLABS = C::SLABS, STAGES = C::STAGES;
+template <typename C, bool EVEN>
+__global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_kernel(const __grid_constant__ QuantParams params) {
+    using T = typename C::T;
+    constexpr int BITS = C::BITS, DP = C::DP, NB = C::NB, R = C::R, BN = C::BN, KW = C::KW, PITCH = C::PITCH, CPR = C::CPR;
+    constexpr int SLABS = C::SLABS, GS = C::GS, STAGES = C::STAGES;
     constexpr float LIFT = Weight<__half>::LIFT;
+    using KCodes = Key<BITS, C::F32>;
+    using VCodes = Key<BITS, true>;
     const QuantAttend &p = params.a;
     const Quantized &z = params.z;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint32_t there[C::WARPS][STAGES];  // keys of a stage that were loaded
     const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g4 = lane >> 2, t4 = lane & 3;
-    const int key0 = (g4 >> 1) + 4 * (g4 & 1);  // position of fragment key g4 within its eight
+    const int key0 = g4 & 1 ? C::second(g4 >> 1) : C::first(g4 >> 1);  // row of fragment key g4 among its eight
     uint8_t *ring = smem + warp * STAGES * C::STAGE;
-    // the group of 64 channels from 64 x on, and whether it begins there
-    int group_of[SLABS];
-    bool begins[SLABS + 1];
-#pragma unroll
-    for (int x = 0; x < SLABS; ++x) {
-        group_of[x] = x == 0 ? 0 : 64 * x / z.group;
-        begins[x] = x == 0 || group_of[x] != group_of[x - 1];
-    }
-    begins[SLABS] = true;
-    const int slabs32 = (p.head_dim + 31) / 32, slabs64 = (p.head_dim + 63) / 64, row_bytes = p.head_dim * BITS / 8;
+    float2 *kpair = reinterpret_cast<float2 *>(smem + C::RING) + warp * 2 * KW * GS, *vpair = kpair + KW * GS;
+    const int row_bytes = p.head_dim * BITS / 8;
 
     // one piece: rows row0 .. of (sequence b, key head kh) over keys [k_lo, k_hi)
     auto piece = [&](int b, int kh, const Sequence &seq, int row0, int k_lo, int k_hi, int slot) {
         const int rows = seq.nq * p.group, tiles = k_hi > k_lo ? (k_hi - k_lo + BN - 1) / BN : 0;
-        const uint8_t *kp = static_cast<const uint8_t *>(p.k_pages) + kh * p.head_stride;
-        const uint8_t *vp = static_cast<const uint8_t *>(p.v_pages) + kh * p.head_stride;
+        // this lane's part of a copied row: chunk lane % CPR of row lane / CPR of those copied at once
+        constexpr int AT_ONCE = KW / CPR;
+        const int part = lane % CPR, copied = min(16, row_bytes - part * 16);
+        const uint8_t *kp = static_cast<const uint8_t *>(p.k_pages) + kh * p.head_stride + part * 16;
+        const uint8_t *vp = static_cast<const uint8_t *>(p.v_pages) + kh * p.head_stride + part * 16;
         const __half2 *ksp = z.k_scales + kh * z.head_stride, *vsp = z.v_scales + kh * z.head_stride;
         // keys below first.lo no row sees; all rows see [last.lo, first.hi)
         const RowRange first = row_range(p, seq, row0), last = row_range(p, seq, min(row0 + R, rows) - 1);
         const int ps = p.batch.page_size;
+        const int32_t *table = p.batch.table + (long long)b * p.batch.table_stride;
 
-        auto fetch_page = [&](int it) {
-            const int j = k_lo + it * BN + warp * KW + lane, at = j / ps;
-            return j < k_hi && j >= first.lo && at < p.batch.table_pages
-                       ? __ldg(p.batch.table + (long long)b * p.batch.table_stride + at) : -1;
-        };
-        auto load_stage = [&](int it, int page) {
-            uint8_t *st = ring + (it % STAGES) * C::STAGE;
+        // Lane l looks after key l of the warp's step: its page (-1: nothing to load) and row within the page,
+        // looked up a step ahead of the loads.
+        struct Place { int page, row; };
+        bool missing = false;
+        auto fetch = [&](int it) {
             const int j = k_lo + it * BN + warp * KW + lane;
-            const bool in = j < k_hi && j >= first.lo, ok = in && page >= 0 && page < p.batch.pages;
-            if (in && !ok && p.batch.status) *p.batch.status = MGC_CUDA_GATHER_OOB;
-            const unsigned mask = __ballot_sync(0xFFFFFFFFu, ok);
+            Place x{-1, 0};
+            if (j >= k_hi || j < first.lo) return x;
+            const int at = (int)((unsigned long long)(unsigned)j * params.page_magic >> params.page_shift);
+            x.row = j - at * ps;
+            if (at < p.batch.table_pages) x.page = __ldg(table + at);
+            return x;
+        };
+        // pages out of range: nothing to load
+        auto checked = [&](int it, Place x) {
+            const int j = k_lo + it * BN + warp * KW + lane;
+            if ((unsigned)x.page >= (unsigned)p.batch.pages) {
+                missing = missing || (j < k_hi && j >= first.lo);
+                x.page = -1;
+            }
+            return x;
+        };
+        auto load_stage = [&](int it, Place x) {
+            uint8_t *st = ring + (it % STAGES) * C::STAGE;
+            const unsigned mask = __ballot_sync(0xFFFFFFFFu, x.page >= 0);
             if (lane == 0) there[warp][it % STAGES] = mask;
-            const int in_page = j % ps;
-            const long long codes = ok ? page * p.page_stride + in_page * p.token_stride : -1;
-            const long long pairs = ok ? page * z.page_stride + in_page * z.token_stride : 0;
+            const uint32_t dst = smem_u32(st + (lane / CPR) * PITCH + part * 16);
 #pragma unroll
             for (int i = 0; i < CPR; ++i) {
-                const int r = i * (KW / CPR) + lane / CPR, c = lane % CPR;
-                const long long o = __shfl_sync(0xFFFFFFFFu, codes, r);
-                const long long at = o < 0 ? 0 : o + c * 16;
-                const int bytes = o < 0 ? 0 : min(16, row_bytes - c * 16);
-                if (c * 16 < row_bytes) {
-                    const uint32_t dst = smem_u32(st + r * ROW + (c ^ swizzle<ROW>(r & 7)) * 16);
-                    cp_async16(dst, kp + at, bytes);
-                    cp_async16(dst + C::CODES, vp + at, bytes);
+                const int page = __shfl_sync(0xFFFFFFFFu, x.page, i * AT_ONCE + lane / CPR);
+                const uint32_t row = (uint32_t)__shfl_sync(0xFFFFFFFFu, x.row, i * AT_ONCE + lane / CPR);
+                const int bytes = page >= 0 ? copied : 0;
+                const unsigned long long o =
+                    page >= 0 ? ((unsigned long long)(unsigned)page * params.code_page + row * params.code_token) * 16 : 0;
+                if (copied > 0) {
+                    cp_async16(dst + i * AT_ONCE * PITCH, kp + o, bytes);
+                    cp_async16(dst + i * AT_ONCE * PITCH + C::CODES, vp + o, bytes);
                 }
             }
-            const uint32_t dst = smem_u32(st + 2 * C::CODES + lane * SLABS * 4);
-            if (SLABS >= 2 && params.pair_bytes == 8) {
-                cp_async_small<8>(dst, ksp + pairs, ok ? 8 : 0);
-                cp_async_small<8>(dst + C::PAIRS, vsp + pairs, ok ? 8 : 0);
-            } else if (SLABS >= 4 && params.pair_bytes == 16) {
-                cp_async_small<16>(dst, ksp + pairs, ok ? 16 : 0);
-                cp_async_small<16>(dst + C::PAIRS, vsp + pairs, ok ? 16 : 0);
-            } else {
+        };
+        // key l's pairs of a step into registers
+        uint32_t kraw[GS], vraw[GS];
+        auto load_pairs = [&](Place x) {
+            const unsigned long long o = (unsigned long long)(unsigned)x.page * params.pair_page + (uint32_t)x.row * params.pair_token;
 #pragma unroll
-                for (int g = 0; g < SLABS; ++g) {
-                    if (g >= z.groups) break;
-                    cp_async_small<4>(dst + 4 * g, ksp + pairs + g, ok ? 4 : 0);
-                    cp_async_small<4>(dst + C::PAIRS + 4 * g, vsp + pairs + g, ok ? 4 : 0);
+            for (int s = 0; s < GS; ++s) {
+                kraw[s] = vraw[s] = 0u;
+                const int g = GS == 1 ? 0 : 64 * s / z.group;
+                if (x.page >= 0 && 64 * s < p.head_dim) {
+                    kraw[s] = __ldg(reinterpret_cast<const unsigned int *>(ksp + o + g));
+                    vraw[s] = __ldg(reinterpret_cast<const unsigned int *>(vsp + o + g));
                 }
             }
         };
 
         // the first stages' loads, Q meanwhile
-        int page_next = -1;
-        {
-            int page[STAGES];
+        Place at[STAGES];  // of steps it + 1, it + 2, ...
 #pragma unroll
-            for (int it = 0; it < STAGES; ++it) page[it] = fetch_page(it);
+        for (int it = 0; it < STAGES; ++it) at[it] = fetch(it);
 #pragma unroll
-            for (int it = 0; it < STAGES - 1; ++it) {
-                if (it < tiles) load_stage(it, page[it]);
-                cp_async_commit();
-            }
-            page_next = page[STAGES - 1];
+        for (int it = 0; it < STAGES; ++it) at[it] = checked(it, at[it]);
+#pragma unroll
+        for (int it = 0; it < STAGES - 1; ++it) {
+            if (it < tiles) load_stage(it, at[it]);
+            cp_async_commit();
         }
+        load_pairs(at[0]);
         // fragments of Q (row 8 nb + g4, channels 32 i + 8 t4 .. + 7 in Key's order), times a power of two; what
         // rows 2 t4 and 2 t4 + 1 need: that power's inverse times the scale, the groups' sums
         uint32_t qh[DP / 32][NB][4], ql[C::F32 ? DP / 32 : 1][NB][4];
-        float rs[NB][2], qs[NB][2][SLABS];
+        float rs[NB][2], qs[NB][2][GS];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             const int row = row0 + 8 * nb + g4;
@@ -272,50 +301,48 @@ quantized_attention_kernel(const __grid_constant__ QuantParams params) {
             }
             top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-            // 2^up, the row's largest then in [1, 2), in fp32 in [2^13, 2^14): its lower halves keep their bits
+            // 2^up: the row's largest then in [2^8, 2^9), in fp32 in [2^13, 2^14) (its second halves keep their bits)
             const int e = (int)(__float_as_uint(top) >> 23);
-            int up = e == 0 || e == 255 ? 0 : (C::F32 ? 13 : 0) + 127 - e;
+            int up = e == 0 || e == 255 ? 0 : (C::F32 ? 13 : 8) + 127 - e;
             up = max(min(up, 126), -126);
             const float f = __uint_as_float((uint32_t)(127 + up) << 23);
             const float scale = p.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
-            float sum[SLABS];
+            float sum[GS];
 #pragma unroll
-            for (int s = 0; s < SLABS; ++s) sum[s] = 0.0f;
+            for (int x = 0; x < GS; ++x) sum[x] = 0.0f;
 #pragma unroll
             for (int i = 0; i < DP / 32; ++i) {
-                float part = 0.0f;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const float a = to_f(raw[i].e[Key<BITS>::channel(k, 0)]) * f, c = to_f(raw[i].e[Key<BITS>::channel(k, 1)]) * f;
+                    const float a = to_f(raw[i].e[KCodes::channel(k, 0)]) * f, c = to_f(raw[i].e[KCodes::channel(k, 1)]) * f;
                     qh[i][nb][k] = pack2<__half>(a, c);
                     if constexpr (C::F32) {
                         const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&qh[i][nb][k]));
                         ql[i][nb][k] = pack2<__half>(a - h.x, c - h.y);
                     }
-                    part += a + c;
+                    sum[C::ONE ? 0 : i / 2] += a + c;
                 }
-#pragma unroll
-                for (int s = 0; s < SLABS; ++s) sum[s] += s == group_of[i / 2] ? part : 0.0f;
             }
             rs[nb][0] = __shfl_sync(0xFFFFFFFFu, scale, 8 * t4);
             rs[nb][1] = __shfl_sync(0xFFFFFFFFu, scale, 8 * t4 + 4);
 #pragma unroll
-            for (int s = 0; s < SLABS; ++s) {
-                sum[s] += __shfl_xor_sync(0xFFFFFFFFu, sum[s], 1);
-                sum[s] += __shfl_xor_sync(0xFFFFFFFFu, sum[s], 2);
-                qs[nb][0][s] = __shfl_sync(0xFFFFFFFFu, sum[s], 8 * t4);
-                qs[nb][1][s] = __shfl_sync(0xFFFFFFFFu, sum[s], 8 * t4 + 4);
+            for (int x = 0; x < GS; ++x) {
+                sum[x] += __shfl_xor_sync(0xFFFFFFFFu, sum[x], 1);
+                sum[x] += __shfl_xor_sync(0xFFFFFFFFu, sum[x], 2);
+                qs[nb][0][x] = __shfl_sync(0xFFFFFFFFu, sum[x], 8 * t4);
+                qs[nb][1][x] = __shfl_sync(0xFFFFFFFFu, sum[x], 8 * t4 + 4);
             }
         }
         RowRange see[NB][2];
-        float o[SLABS][4][NB][4], off[NB][2][SLABS], m[NB][2], l[NB][2], top_scale[SLABS];
+        float o[SLABS][4][NB][4], off[NB][2][GS], m[NB][2], l[NB][2], top_scale[GS];
 #pragma unroll
-        for (int s = 0; s < SLABS; ++s) {
-            top_scale[s] = __uint_as_float((127u - 24) << 23);  // the least scale that half has
+        for (int x = 0; x < GS; ++x) top_scale[x] = 1.0f / 16777216.0f;  // the least scale that half has
+#pragma unroll
+        for (int x = 0; x < SLABS; ++x) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) o[s][j][nb][0] = o[s][j][nb][1] = o[s][j][nb][2] = o[s][j][nb][3] = 0.0f;
+                for (int nb = 0; nb < NB; ++nb) o[x][j][nb][0] = o[x][j][nb][1] = o[x][j][nb][2] = o[x][j][nb][3] = 0.0f;
             }
         }
 #pragma unroll
@@ -326,7 +353,7 @@ quantized_attention_kernel(const __grid_constant__ QuantParams params) {
                 m[nb][e] = -INFINITY;
                 l[nb][e] = 0.0f;
 #pragma unroll
-                for (int s = 0; s < SLABS; ++s) off[nb][e][s] = 0.0f;
+                for (int x = 0; x < GS; ++x) off[nb][e][x] = 0.0f;
             }
         }
 
@@ -334,35 +361,68 @@ quantized_attention_kernel(const __grid_constant__ QuantParams params) {
             cp_async_wait<STAGES - 2>();
             __syncwarp();
             // (the slot's last readers were this warp's lanes, a step ago)
-            if (it + STAGES - 1 < tiles) load_stage(it + STAGES - 1, page_next);
+            if (it + STAGES - 1 < tiles) load_stage(it + STAGES - 1, at[STAGES - 1]);
             cp_async_commit();
-            page_next = fetch_page(it + STAGES);
             const int j0 = k_lo + it * BN + warp * KW;
+            const uint32_t loaded = there[warp][it % STAGES];
+            const Place next = fetch(it + STAGES);
+            // key l's scales: K's, and V's relative to S, a power of two at or above all so far (scales that are
+            // not finite make their own NaN)
+#pragma unroll
+            for (int x = 0; x < GS; ++x) {
+                float2 k = __half22float2(*reinterpret_cast<const __half2 *>(&kraw[x]));
+                float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&vraw[x]));
+                const uint32_t mine = __float_as_uint(v.x) & 0x7FFFFFFFu;
+                const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, mine < 0x7F800000u ? mine : 0u);
+                if (most > __float_as_uint(top_scale[x])) {
+                    const float now = __uint_as_float((most + 0x7FFFFFu) & 0xFF800000u), ratio = top_scale[x] / now;
+                    top_scale[x] = now;
+#pragma unroll
+                    for (int y = C::ONE ? 0 : x; y < (C::ONE ? SLABS : x + 1); ++y) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) o[y][j][nb][e] *= ratio;
+                            }
+                        }
+                    }
+                }
+                k.y = fmaf(KCodes::MID, k.x, k.y);
+                k.x *= 1.0f / KCodes::UNIT;
+                v.y = fmaf(VCodes::MID, v.x, v.y);
+                v.x *= __uint_as_float((254u << 23) - __float_as_uint(top_scale[x]));  // 1 / S, S from 2^-24 to 2^16
+                kpair[lane * GS + x] = k;
+                vpair[lane * GS + x] = v;
+            }
+            // the next step's, and the place of the one after the stages
+            load_pairs(at[1]);
+#pragma unroll
+            for (int x = 0; x + 1 < STAGES; ++x) at[x] = at[x + 1];
+            at[STAGES - 1] = checked(it + STAGES, next);
+            __syncwarp();
             if (j0 >= k_hi) continue;
             const uint8_t *st = ring + (it % STAGES) * C::STAGE;
-            const uint32_t loaded = there[warp][it % STAGES];
-            const __half2 *kpair = reinterpret_cast<const __half2 *>(st + 2 * C::CODES), *vpair = kpair + KW * SLABS;
+            const int k_at = key0 * PITCH + t4 * BITS;
 
             // ---- scores ----
             float s[2][NB][4];
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt) {
                 const int ra = 16 * mt + key0, rb = ra + 8;
-                const uint8_t *rowa = st + ra * ROW, *rowb = st + rb * ROW;
                 float acc[NB][4];
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[nb][e] = s[mt][nb][e] = 0.0f;
                 }
+                // (channels past the head width: whatever is there is finite and the query has zeros)
 #pragma unroll
                 for (int i = 0; i < DP / 32; ++i) {
-                    if (i >= slabs32) break;
-                    Key<BITS> a, c;
-                    // chunk of channels 32 i + 8 t4: BITS bytes a lane, 4 BITS a quad
-                    const int chunk = (i * 4 * BITS + t4 * BITS) / 16, in = (i * 4 * BITS + t4 * BITS) % 16;
-                    a.load(rowa + (chunk ^ swizzle<ROW>(ra & 7)) * 16 + in);
-                    c.load(rowb + (chunk ^ swizzle<ROW>(rb & 7)) * 16 + in);
+                    KCodes a, c;  // channels 32 i + 8 t4: BITS bytes a lane
+                    a.load(st + k_at + 16 * mt * PITCH + i * 4 * BITS);
+                    c.load(st + k_at + (16 * mt + 8) * PITCH + i * 4 * BITS);
                     uint32_t ha[4], hc[4];
                     a.pairs(ha);
                     c.pairs(hc);
@@ -377,28 +437,21 @@ quantized_attention_kernel(const __grid_constant__ QuantParams params) {
                         }
                     }
                     // a group's end (fp32: every 64 channels, the instruction truncates its sums)
-                    const bool ends = ((i & 1) && begins[i / 2 + 1]) || i + 1 == slabs32;
+                    const bool ends = i + 1 == DP / 32 || (!C::ONE && (i & 1));
                     if (ends || (C::F32 && (i & 1))) {
-                        const int gi = group_of[i / 2];
-                        const float2 pa = __half22float2(kpair[ra * SLABS + gi]), pb = __half22float2(kpair[rb * SLABS + gi]);
-                        const float oa = fmaf((float)(1 << (BITS - 1)), pa.x, pa.y), ob = fmaf((float)(1 << (BITS - 1)), pb.x, pb.y);
+                        const int x = C::ONE ? 0 : i / 2;
+                        const float2 pa = kpair[ra * GS + x], pb = kpair[rb * GS + x];
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb) {
-                            float q0 = qs[nb][0][0], q1 = qs[nb][1][0];
-#pragma unroll
-                            for (int x = 1; x < SLABS; ++x) {
-                                q0 = x == gi ? qs[nb][0][x] : q0;
-                                q1 = x == gi ? qs[nb][1][x] : q1;
-                            }
                             s[mt][nb][0] = fmaf(pa.x, acc[nb][0], s[mt][nb][0]);
                             s[mt][nb][1] = fmaf(pa.x, acc[nb][1], s[mt][nb][1]);
                             s[mt][nb][2] = fmaf(pb.x, acc[nb][2], s[mt][nb][2]);
                             s[mt][nb][3] = fmaf(pb.x, acc[nb][3], s[mt][nb][3]);
                             if (ends) {
-                                s[mt][nb][0] = fmaf(oa, q0, s[mt][nb][0]);
-                                s[mt][nb][1] = fmaf(oa, q1, s[mt][nb][1]);
-                                s[mt][nb][2] = fmaf(ob, q0, s[mt][nb][2]);
-                                s[mt][nb][3] = fmaf(ob, q1, s[mt][nb][3]);
+                                s[mt][nb][0] = fmaf(pa.y, qs[nb][0][x], s[mt][nb][0]);
+                                s[mt][nb][1] = fmaf(pa.y, qs[nb][1][x], s[mt][nb][1]);
+                                s[mt][nb][2] = fmaf(pb.y, qs[nb][0][x], s[mt][nb][2]);
+                                s[mt][nb][3] = fmaf(pb.y, qs[nb][1][x], s[mt][nb][3]);
                             }
                             acc[nb][0] = acc[nb][1] = acc[nb][2] = acc[nb][3] = 0.0f;
                         }
@@ -417,7 +470,10 @@ quantized_attention_kernel(const __grid_constant__ QuantParams params) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int r = 16 * mt + key0 + (e < 2 ? 0 : 8), j = j0 + r;
-                            if (j < see[nb][e & 1].lo || j >= see[nb][e & 1].hi || !(loaded >> r & 1)) hidden |= 1u << (8 * nb + 4 * mt + e);
+                            if (j < see[nb][e & 1].lo || j >= see[nb][e & 1].hi || !(loaded >> r & 1)) {
+                                hidden |= 1u << (8 * nb + 4 * mt + e);
+                                s[mt][nb][e] = -INFINITY;
+                            }
                         }
                     }
                 }
@@ -428,21 +484,15 @@ quantized_attention_kernel(const __grid_constant__ QuantParams params) {
             for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float x = m[nb][e];
-#pragma unroll
-                    for (int mt = 0; mt < 2; ++mt) {
-#pragma unroll
-                        for (int k = 0; k < 4; k += 2) {
-                            s[mt][nb][e + k] *= rs[nb][e];
-                            if (hidden >> (8 * nb + 4 * mt + e + k) & 1) s[mt][nb][e + k] = -INFINITY;
-                            x = fmaxf(x, s[mt][nb][e + k]);
-                        }
-                    }
+                    float x = fmaxf(fmaxf(s[0][nb][e], s[0][nb][e + 2]), fmaxf(s[1][nb][e], s[1][nb][e + 2]));
                     x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 4));
                     x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 8));
                     x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 16));
-                    const float y = x == -INFINITY ? 0.0f : x;  // nothing seen yet: subtract 0
-                    fall[nb][e] = ex2(m[nb][e] - y);
+                    x = fmaxf(x, m[nb][e]);
+                    // weights 2^(rs s - rs m); nothing seen yet: subtract 0. The products are rounded on their own, so
+                    // that a maximum that stays leaves the row as it is (paged_mma.cuh)
+                    const float y = x == -INFINITY ? 0.0f : __fmul_rn(x, rs[nb][e]);
+                    fall[nb][e] = ex2(__fmul_rn(m[nb][e], rs[nb][e]) - y);
                     moved = moved || fall[nb][e] != 1.0f;
                     m[nb][e] = x;
                     float sum = 0.0f;
@@ -450,7 +500,7 @@ quantized_attention_kernel(const __grid_constant__ QuantParams params) {
                     for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
                         for (int k = 0; k < 4; k += 2) {
-                            s[mt][nb][e + k] = ex2(s[mt][nb][e + k] - y + LIFT);
+                            s[mt][nb][e + k] = ex2(fmaf(s[mt][nb][e + k], rs[nb][e], LIFT - y));
                             sum += s[mt][nb][e + k];
                         }
                     }
@@ -461,9 +511,12 @@ quantized_attention_kernel(const __grid_constant__ QuantParams params) {
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-                    for (int x = 0; x < SLABS; ++x) {
+                    for (int x = 0; x < GS; ++x) {
                         off[nb][0][x] *= fall[nb][0];
                         off[nb][1][x] *= fall[nb][1];
+                    }
+#pragma unroll
+                    for (int x = 0; x < SLABS; ++x) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             o[x][j][nb][0] *= fall[nb][0];
@@ -478,56 +531,25 @@ quantized_attention_kernel(const __grid_constant__ QuantParams params) {
             uint32_t bh[2][NB][2], bl[C::F32 ? 2 : 1][NB][2];
 #pragma unroll
             for (int x = 0; x < SLABS; ++x) {
-                if (x >= slabs64) break;
-                const int gi = group_of[x];
-                if (begins[x]) {  // a group begins: its weights
-                    // the largest scale so far, as a power of two (scales that are not finite make their own NaN)
-                    uint32_t mine = __float_as_uint(__low2float(vpair[lane * SLABS + gi])) & 0x7FFFFFFFu;
-                    if (mine >= 0x7F800000u || !(loaded >> lane & 1)) mine = 0;
-                    const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, mine);
-                    float up = 0.0f;  // the group's S
-#pragma unroll
-                    for (int y = 0; y < SLABS; ++y) up = y == gi ? top_scale[y] : up;
-                    if (most > __float_as_uint(up)) {
-                        const float now = __uint_as_float((most + 0x7FFFFFu) & 0xFF800000u), ratio = up / now;
-                        up = now;
-#pragma unroll
-                        for (int y = 0; y < SLABS; ++y) {
-                            if (y == gi) top_scale[y] = now;
-                            if (group_of[y] != gi) continue;
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-#pragma unroll
-                                for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e) o[y][j][nb][e] *= ratio;
-                                }
-                            }
-                        }
-                    }
-                    // (S is a power of two from 2^-24 to 2^16)
-                    const float inv = __uint_as_float((254u << 23) - __float_as_uint(up));
+                if (x == 0 || !C::ONE) {  // a group's weights
+                    const int y = C::ONE ? 0 : x;
 #pragma unroll
                     for (int mt = 0; mt < 2; ++mt) {
-                        const float2 pa = __half22float2(vpair[(16 * mt + key0) * SLABS + gi]);
-                        const float2 pb = __half22float2(vpair[(16 * mt + key0 + 8) * SLABS + gi]);
-                        const float oa = fmaf((float)(1 << (BITS - 1)), pa.x, pa.y), ob = fmaf((float)(1 << (BITS - 1)), pb.x, pb.y);
-                        const float fa = pa.x * inv, fb = pb.x * inv;
+                        const float2 pa = vpair[(16 * mt + key0) * GS + y], pb = vpair[(16 * mt + key0 + 8) * GS + y];
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb) {
-                            float w[4], t[4];
+                            const float (&u)[4] = s[mt][nb];
+                            float w[4] = {u[0] * pa.x, u[1] * pa.x, u[2] * pb.x, u[3] * pb.x};
+                            if (hidden) {  // 0 times what is not finite
+                                const uint32_t hide = hidden >> (8 * nb + 4 * mt);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                w[e] = s[mt][nb][e] * (e < 2 ? fa : fb);
-                                t[e] = s[mt][nb][e] * (e < 2 ? oa : ob);
-                                if (hidden >> (8 * nb + 4 * mt + e) & 1) w[e] = t[e] = 0.0f;  // 0 times what is not finite
-                            }
-#pragma unroll
-                            for (int y = 0; y < SLABS; ++y) {
-                                if (y == gi) {
-                                    off[nb][0][y] += t[0] + t[2];
-                                    off[nb][1][y] += t[1] + t[3];
+                                for (int e = 0; e < 4; ++e) {
+                                    w[e] = hide >> e & 1 ? 0.0f : w[e];
+                                    off[nb][e & 1][y] += hide >> e & 1 ? 0.0f : u[e] * (e < 2 ? pa.y : pb.y);
                                 }
+                            } else {
+                                off[nb][0][y] = fmaf(u[0], pa.y, fmaf(u[2], pb.y, off[nb][0][y]));
+                                off[nb][1][y] = fmaf(u[1], pa.y, fmaf(u[3], pb.y, off[nb][1][y]));
                             }
                             const uint32_t h0 = pack2<__half>(w[0], w[1]), h1 = pack2<__half>(w[2], w[3]);
                             bh[mt][nb][0] = movmatrix(h0);
@@ -551,19 +573,16 @@ quantized_attention_kernel(const __grid_constant__ QuantParams params) {
                 }
 #pragma unroll
                 for (int mt = 0; mt < 2; ++mt) {
-                    // eight channels from 64 x + 8 g4 on of keys t4, t4 + 4 and eight further: BITS bytes a lane
-                    const int chunk = (x * 8 * BITS + g4 * BITS) / 16, in = (x * 8 * BITS + g4 * BITS) % 16;
-                    Key<BITS> key[4];
+                    // eight channels from 64 x + 8 g4 on of four keys: BITS bytes a lane
+                    VCodes key[4];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int r = 16 * mt + t4 + 4 * k;
-                        key[k].load(st + C::CODES + r * ROW + (chunk ^ swizzle<ROW>(r & 7)) * 16 + in);
-                    }
+                    for (int k = 0; k < 4; ++k)
+                        key[k].load(st + C::CODES + (k & 1 ? C::second(t4) : C::first(t4)) * PITCH + g4 * BITS + (16 * mt + 8 * (k >> 1)) * PITCH + x * 8 * BITS);
                     auto tile = [&](auto index) {
                         constexpr int J = decltype(index)::value;
                         uint32_t a[4];
-                        two_keys<J>(key[0], key[1], a[0], a[1]);
-                        two_keys<J>(key[2], key[3], a[2], a[3]);
+                        VCodes::template two_rows<J>(key[0], key[1], a[0], a[1]);
+                        VCodes::template two_rows<J>(key[2], key[3], a[2], a[3]);
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb) {
                             if constexpr (C::F32) {
@@ -591,6 +610,7 @@ quantized_attention_kernel(const __grid_constant__ QuantParams params) {
                 }
             }
         }
+        if (missing && p.batch.status) *p.batch.status = MGC_CUDA_GATHER_OOB;
         cp_async_wait<0>();
         __syncthreads();
 
@@ -604,27 +624,20 @@ quantized_attention_kernel(const __grid_constant__ QuantParams params) {
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) l[nb][e] += __shfl_xor_sync(0xFFFFFFFFu, l[nb][e], d);
 #pragma unroll
-                for (int x = 0; x < SLABS; ++x) {
+                for (int x = 0; x < GS; ++x) {
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) off[nb][e][x] += __shfl_xor_sync(0xFFFFFFFFu, off[nb][e][x], d);
                 }
 #pragma unroll
                 for (int x = 0; x < SLABS; ++x) {
-                    if (x >= slabs64) break;
-                    const int gi = group_of[x];
-                    float add = off[nb][e][0], up = top_scale[0];
-#pragma unroll
-                    for (int y = 1; y < SLABS; ++y) {
-                        add = y == gi ? off[nb][e][y] : add;
-                        up = y == gi ? top_scale[y] : up;
-                    }
+                    const float add = off[nb][e][C::ONE ? 0 : x], up = top_scale[C::ONE ? 0 : x] / VCodes::UNIT;
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         *reinterpret_cast<float2 *>(red + r * C::ORED + 64 * x + 8 * g4 + 2 * j) =
                             make_float2(fmaf(up, o[x][j][nb][e], add), fmaf(up, o[x][j][nb][2 + e], add));
                 }
                 if (g4 == 0) {
-                    sm[r] = m[nb][e];
+                    sm[r] = __fmul_rn(m[nb][e], rs[nb][e]);
                     sl[r] = l[nb][e];
                 }
             }
