@@ -7,11 +7,17 @@
 // contraction: a code falls on one side of its border whatever the order of the sum, so that a call
 // repeats its bits and any computation of these steps gives the same codes.
 //
-// Memory bounds it. A head takes SEG lanes (8, 16 or 32) of eight channels each, held as four pairs: pair i
-// of the rotated channels is turned by one lane, and what a head needs of all its channels (the sum, a
-// group's extremes) meets by shuffles. Pages of codes want a lane's eight channels side by side: where pairs
-// lie rot / 2 apart the values change lanes through shared memory.
+// Memory bounds it. A head takes 8, 16 or 32 lanes of eight channels each, in two fours: a lane of the rotated
+// channels holds the fours whose channels pair up, so that one lane turns a pair, and what a head needs of all
+// its channels (the sum, a group's extremes) meets by shuffles. Pages of codes want a lane's eight channels side by
+// side: where pairs lie rot / 2 apart, keys change lanes through shared memory. Each warp takes a run of consecutive
+// tokens, all heads of one after the other, the next heads' loads ahead.
+//
+// Codes: the quotient by the group's scale is taken as a product with its inverse, and only where that lies next to
+// the border between two codes (one value in some thousand) as the definition's division.
 #pragma once
+
+#include <type_traits>
 
 #include "quantized_common.cuh"
 
@@ -32,10 +38,11 @@ struct HeadsParams {
     int positions, rot, interleaved;
     int q_heads, kv_heads, head_dim;
     int seg;  // lanes of a head
-    int tokens, per_block;
+    int tokens, run, parts;
+    double inv_dim;
 };
 
-constexpr int HEADS_WARPS = 4;
+constexpr int HEADS_WARPS = 4, HEADS_RESIDENT = 8;
 
 // (mean + eps)^-1/2 as fp32. In fp32's range one Newton step from the hardware's root leaves 2^-43, so that
 // the rounding to fp32 is the exact root's but for one case in 2^18.
@@ -45,71 +52,110 @@ __device__ __forceinline__ float inverse_root(double m) {
     return (float)(r * (1.5 - 0.5 * m * r * r));
 }
 
-// Channel of slot s (0..7) of lane `sl` of a head: slots k and 4 + k are pair 4 sl + k.
-__device__ __forceinline__ int channel_of(const HeadsParams &p, int sl, int s, bool halves) {
-    const int i = 4 * sl + (s & 3);
-    return halves && i < p.rot / 2 ? (s < 4 ? i : i + p.rot / 2) : 2 * i + (s >> 2);
+// Group code of eight values side by side, next to each other in a lane.
+template <int BITS> __device__ __forceinline__ uint2 encode(const float (&x)[8], float offset, float scale) {
+    constexpr float TOP = (float)((1 << BITS) - 1), ROUND = 12582912.0f;  // 1.5 * 2^23: adding it rounds to whole numbers
+    if (!(scale > 0.0f)) return make_uint2(0, 0);
+    const float inv = __frcp_rn(scale);
+    float q[8], far = 0.0f;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+        // off by two roundings: 2^-22 of at most 255, below 1e-4
+        q[s] = fminf(fmaxf(__fmul_rn(__fsub_rn(x[s], offset), inv), 0.0f), TOP);
+        far = fmaxf(far, fabsf(q[s] - (__fadd_rn(q[s], ROUND) - ROUND)));
+    }
+    if (far > 0.4999f) {
+#pragma unroll
+        for (int s = 0; s < 8; ++s) q[s] = fminf(fmaxf(__fdiv_rn(__fsub_rn(x[s], offset), scale), 0.0f), TOP);
+    }
+    uint32_t code[2] = {0, 0};
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+        const uint32_t c = __float_as_uint(__fadd_rn(q[s], ROUND)) & 255u;
+        code[BITS == 4 ? 0 : s >> 2] |= c << (BITS == 4 ? 4 * s : 8 * (s & 3));
+    }
+    return make_uint2(code[0], code[1]);
 }
 
-// The eight values of a lane, as they come.
-template <typename S> struct Eight {
-    Pack<4, S> a, b;
-};
+// Two values of a 16-bit type at once.
+template <typename T> __device__ __forceinline__ uint32_t two(float x, float y);
+template <> __device__ __forceinline__ uint32_t two<__half>(float x, float y) {
+    const __half2 v = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <> __device__ __forceinline__ uint32_t two<__nv_bfloat16>(float x, float y) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+// Four values in a row.
+template <typename T> __device__ __forceinline__ void store_four(T *dst, const float *x) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(dst) = make_float4(x[0], x[1], x[2], x[3]);
+    else *reinterpret_cast<uint2 *>(dst) = make_uint2(two<T>(x[0], x[1]), two<T>(x[2], x[3]));
+}
 
-// VEC: D and rot are multiples of 8 and rows allow accesses of four elements.
-template <typename S, typename T, int BITS, bool VEC>
-__global__ void __launch_bounds__(32 * HEADS_WARPS) kv_append_heads_kernel(const __grid_constant__ HeadsParams p) {
-    __shared__ float exchange[BITS ? HEADS_WARPS : 1][BITS ? 256 : 1];
-    const int lane = (int)(threadIdx.x & 31), warp = (int)(threadIdx.x >> 5);
-    const int sl = lane & (p.seg - 1), at_once = 32 / p.seg;
-    const int heads = p.q_heads + 2 * p.kv_heads, step = (int)gridDim.y * HEADS_WARPS * at_once;
-    const int h_first = ((int)blockIdx.y * HEADS_WARPS + warp) * at_once + lane / p.seg;
-    const int t0 = (int)blockIdx.x * p.per_block, t1 = min(t0 + p.per_block, p.tokens);
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) check_rows(p.batch, p.tokens);
+// SEG: lanes of a head where D and rot are multiples of 8 and rows allow accesses of four elements; 0: any other
+// case, p.seg lanes.
+template <typename S, typename T, int BITS, int SEG>
+__global__ void __launch_bounds__(32 * HEADS_WARPS, HEADS_RESIDENT) kv_append_heads_kernel(const __grid_constant__ HeadsParams p) {
+    __shared__ __align__(16) float exchange[BITS ? HEADS_WARPS : 1][BITS ? 256 : 4];
+    constexpr bool VEC = SEG > 0;
+    const int lane = (int)(threadIdx.x & 31), warp = (int)(threadIdx.x >> 5), seg = VEC ? SEG : p.seg;
+    const unsigned unit = blockIdx.x * HEADS_WARPS + warp;
+    if (unit == 0 && lane == 0) check_rows(p.batch, p.tokens);
+    const long long t_first = (long long)(unit / (unsigned)p.parts) * p.run;
+    if (t_first >= p.tokens) return;
+    const int t0 = (int)t_first, t1 = min(t0 + p.run, p.tokens);
+    const int sl = lane & (seg - 1), at_once = 32 / seg, sub = lane / seg;
+    // a token's heads, at_once of one kind at a time: queries, keys, values
+    const int q_items = (p.q_heads + at_once - 1) / at_once, kv_items = (p.kv_heads + at_once - 1) / at_once;
+    const int items = q_items + 2 * kv_items, part = (int)(unit % (unsigned)p.parts);
+    const bool mine = 8 * sl < p.head_dim, turned = 2 * 4 * sl < p.rot;  // (VEC) this lane's channels exist, are rotated
+    const bool apart = turned && !p.interleaved;                        // (VEC) pairs rot / 2 apart
 
-    auto source = [&](int t, int h) -> const S * {
-        if (h < p.q_heads) return static_cast<const S *>(p.q) + t * p.q_ts + h * p.q_hs;
-        h -= p.q_heads;
-        if (h < p.kv_heads) return static_cast<const S *>(p.k) + t * p.k_ts + h * p.k_hs;
-        return static_cast<const S *>(p.v) + t * p.v_ts + (h - p.kv_heads) * p.v_hs;
+    // Channels of value s of the lane. VEC: two fours side by side; else pair 4 sl + s / 2, first or second.
+    const int first_turned = apart ? 4 * sl : 8 * sl, second_turned = apart ? 4 * sl + p.rot / 2 : 8 * sl + 4;
+    auto channel = [&](int s, bool is_v) {
+        const int i = 4 * sl + (s >> 1);
+        return !is_v && !p.interleaved && i < p.rot / 2 ? i + (s & 1) * (p.rot / 2) : 2 * i + (s & 1);
     };
-    // values are apart (pairs rot / 2 apart) for queries and keys, side by side for values
-    auto load = [&](Eight<S> &e, int t, int h) {
-        if (h >= heads) return;
-        const S *src = source(t, h);
-        const bool halves = !p.interleaved && h < p.q_heads + p.kv_heads;
+    struct Eight {
+        Pack<4, S> a, b;
+    };
+    // the token's rows of q, k and v, this lane's heads first
+    const S *q_row = nullptr, *k_row = nullptr, *v_row = nullptr;
+    auto token = [&](int t) {
+        q_row = static_cast<const S *>(p.q) + (long long)t * p.q_ts;
+        k_row = static_cast<const S *>(p.k) + (long long)t * p.k_ts;
+        v_row = static_cast<const S *>(p.v) + (long long)t * p.v_ts;
+    };
+    auto load = [&](Eight &e, int i) {
+        const bool is_q = i < q_items, is_v = i >= q_items + kv_items;
+        const int h = (i - (is_q ? 0 : is_v ? q_items + kv_items : q_items)) * at_once + sub;
+        const S *src = (is_q ? q_row : is_v ? v_row : k_row) + (long long)h * (is_q ? p.q_hs : is_v ? p.v_hs : p.k_hs);
+        const bool have = h < (is_q ? p.q_heads : p.kv_heads);
         if constexpr (VEC) {
-            if (8 * sl >= p.head_dim) return;
-            const bool apart = halves && 8 * sl < p.rot;
-            e.a.load(src + (apart ? 4 * sl : 8 * sl));
-            e.b.load(src + (apart ? 4 * sl + p.rot / 2 : 8 * sl + 4));
+#pragma unroll
+            for (int k = 0; k < Pack<4, S>::N; ++k) e.a.raw[k] = e.b.raw[k] = typename Pack<4, S>::R{};
+            if (!have || !mine) return;
+            e.a.load(src + (is_v ? 8 * sl : first_turned));
+            e.b.load(src + (is_v ? 8 * sl + 4 : second_turned));
         } else {
 #pragma unroll
             for (int s = 0; s < 8; ++s) {
-                const int c = channel_of(p, sl, s, halves);
-                if (c >= p.head_dim) continue;
-                if (s < 4) e.a.e[s] = src[c];
-                else e.b.e[s - 4] = src[c];
+                const int c = channel(s, is_v);
+                (s < 4 ? e.a.e[s & 3] : e.b.e[s & 3]) = have && c < p.head_dim ? src[c] : from_f<S>(0.0f);
             }
         }
     };
-    // the channels of the two packs, in VEC form
-    auto store_row = [&](T *dst, const float (&x)[8], bool halves) {
+    auto store_row = [&](T *dst, const float (&x)[8], bool is_v) {
         if constexpr (VEC) {
-            if (8 * sl >= p.head_dim) return;
-            const bool apart = halves && 8 * sl < p.rot;
-            Pack<4, T> a, b;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                a.e[k] = from_f<T>(apart ? x[k] : x[(k >> 1) + 4 * (k & 1)]);
-                b.e[k] = from_f<T>(apart ? x[4 + k] : x[2 + (k >> 1) + 4 * (k & 1)]);
-            }
-            a.store(dst + (apart ? 4 * sl : 8 * sl));
-            b.store(dst + (apart ? 4 * sl + p.rot / 2 : 8 * sl + 4));
+            if (!mine) return;
+            store_four<T>(dst + (is_v ? 8 * sl : first_turned), x);
+            store_four<T>(dst + (is_v ? 8 * sl + 4 : second_turned), x + 4);
         } else {
 #pragma unroll
             for (int s = 0; s < 8; ++s) {
-                const int c = channel_of(p, sl, s, halves);
+                const int c = channel(s, is_v);
                 if (c < p.head_dim) dst[c] = from_f<T>(x[s]);
             }
         }
@@ -118,8 +164,9 @@ __global__ void __launch_bounds__(32 * HEADS_WARPS) kv_append_heads_kernel(const
     TokenWalk walk;
     walk.start(t0);
     float cs[4], sn[4];
-    bool turn = false;     // the token's heads are normalised and rotated
-    bool cached = false;   // and its key and value written
+    bool turn = false;    // the token's heads are normalised and rotated
+    bool cached = false;  // and its key and value written
+    long long at = 0, pairs = 0;
     auto place = [&](int t) {
         walk.step(p.batch, t);
         turn = walk.pos >= 0;
@@ -128,9 +175,12 @@ __global__ void __launch_bounds__(32 * HEADS_WARPS) kv_append_heads_kernel(const
             if (p.batch.status) *p.batch.status = MGC_CUDA_GATHER_OOB;
             turn = cached = false;
         }
+        at = cached ? walk.at(p.page_stride, p.token_stride) : 0;
+        if (BITS) pairs = cached ? walk.at(p.z.page_stride, p.z.token_stride) : 0;
         if (!turn || !p.rot) return;
         const float *c = p.cos + (long long)walk.pos * p.table_row, *s = p.sin + (long long)walk.pos * p.table_row;
-        if (VEC && 8 * sl < p.rot) {
+        if constexpr (VEC) {
+            if (!turned) return;
             Pack<4, float> x, y;
             x.load(c + 4 * sl);
             y.load(s + 4 * sl);
@@ -139,7 +189,7 @@ __global__ void __launch_bounds__(32 * HEADS_WARPS) kv_append_heads_kernel(const
                 cs[k] = x.e[k];
                 sn[k] = y.e[k];
             }
-        } else if (!VEC) {
+        } else {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int i = 4 * sl + k;
@@ -148,158 +198,157 @@ __global__ void __launch_bounds__(32 * HEADS_WARPS) kv_append_heads_kernel(const
             }
         }
     };
-    auto finish = [&](const Eight<S> &e, int t, int h) {
-        const bool is_q = h < p.q_heads, is_k = !is_q && h < p.q_heads + p.kv_heads, is_v = !is_q && !is_k && h < heads;
-        const bool halves = !p.interleaved && !is_v;
+    auto rotate = [&](float &x1, float &x2, int k) {
+        const float a = __fsub_rn(__fmul_rn(x1, cs[k]), __fmul_rn(x2, sn[k])), b = __fadd_rn(__fmul_rn(x2, cs[k]), __fmul_rn(x1, sn[k]));
+        x1 = a;
+        x2 = b;
+    };
+    // kind 0: queries, 1: keys, 2: values
+    auto finish = [&](const Eight &e, int t, int i, auto kind) {
+        constexpr bool IS_Q = decltype(kind)::value == 0, IS_V = decltype(kind)::value == 2;
+        const int h = i * at_once + sub;
+        const bool there = h < (IS_Q ? p.q_heads : p.kv_heads);
         float x[8];
-        if constexpr (VEC) {
-            const bool mine = h < heads && 8 * sl < p.head_dim, apart = halves && 8 * sl < p.rot;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float a = mine ? to_f(e.a.e[k]) : 0.0f, b = mine ? to_f(e.b.e[k]) : 0.0f;
-                if (apart) {
-                    x[k] = a;
-                    x[4 + k] = b;
+        for (int s = 0; s < 8; ++s) x[s] = to_f(s < 4 ? e.a.e[s & 3] : e.b.e[s & 3]);
+        if constexpr (!IS_V) {
+            const float *weight = IS_Q ? p.q_norm : p.k_norm;
+            if (turn && weight) {
+                double sum = 0.0;
+#pragma unroll
+                for (int s = 0; s < 8; ++s) sum = fma((double)x[s], (double)x[s], sum);
+#pragma unroll
+                for (int d = 1; d < (VEC ? SEG : 32); d <<= 1)
+                    if (VEC || d < seg) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+                const float r = inverse_root(fma(sum, p.inv_dim, p.eps));
+                if constexpr (VEC) {
+                    if (mine) {
+                        Pack<4, float> a, b;
+                        a.load(weight + first_turned);
+                        b.load(weight + second_turned);
+#pragma unroll
+                        for (int s = 0; s < 8; ++s) x[s] = __fmul_rn(__fmul_rn(x[s], r), s < 4 ? a.e[s & 3] : b.e[s & 3]);
+                    }
                 } else {
-                    x[(k >> 1) + 4 * (k & 1)] = a;
-                    x[2 + (k >> 1) + 4 * (k & 1)] = b;
+#pragma unroll
+                    for (int s = 0; s < 8; ++s) {
+                        const int c = channel(s, false);
+                        if (c < p.head_dim) x[s] = __fmul_rn(__fmul_rn(x[s], r), __ldg(weight + c));
+                    }
                 }
             }
-        } else {
+            if (turn && p.rot) {
+                if constexpr (VEC) {
+                    if (apart) {
 #pragma unroll
-            for (int s = 0; s < 8; ++s) {
-                const bool mine = h < heads && channel_of(p, sl, s, halves) < p.head_dim;
-                x[s] = mine ? to_f(s < 4 ? e.a.e[s] : e.b.e[s - 4]) : 0.0f;
-            }
-        }
-        const float *weight = is_q ? p.q_norm : is_k ? p.k_norm : nullptr;
-        if (turn && (p.q_norm || p.k_norm)) {  // (the same branch for the whole warp)
-            double sum = 0.0;
+                        for (int k = 0; k < 4; ++k) rotate(x[k], x[4 + k], k);
+                    } else if (turned) {
 #pragma unroll
-            for (int s = 0; s < 8; ++s) sum += (double)x[s] * (double)x[s];
-            for (int d = 1; d < p.seg; d <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-            if (weight) {
-                const float r = inverse_root(sum / p.head_dim + p.eps);
+                        for (int k = 0; k < 4; ++k) rotate(x[2 * k], x[2 * k + 1], k);
+                    }
+                } else {
 #pragma unroll
-                for (int s = 0; s < 8; ++s) {
-                    const int c = channel_of(p, sl, s, halves);
-                    if (c < p.head_dim) x[s] = __fmul_rn(__fmul_rn(x[s], r), __ldg(weight + c));
+                    for (int k = 0; k < 4; ++k)
+                        if (4 * sl + k < p.rot / 2) rotate(x[2 * k], x[2 * k + 1], k);
                 }
             }
         }
-        if (turn && !is_v && (VEC ? 8 * sl < p.rot : p.rot > 0)) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (!VEC && 4 * sl + k >= p.rot / 2) continue;
-                const float x1 = x[k], x2 = x[4 + k];
-                x[k] = __fsub_rn(__fmul_rn(x1, cs[k]), __fmul_rn(x2, sn[k]));
-                x[4 + k] = __fadd_rn(__fmul_rn(x2, cs[k]), __fmul_rn(x1, sn[k]));
-            }
-        }
-        if (is_q) store_row(static_cast<T *>(p.q_out) + t * p.qo_ts + h * p.qo_hs, x, halves);
-        if constexpr (BITS == 0) {
-            if ((is_k || is_v) && cached) {
-                const int kh = h - p.q_heads - (is_v ? p.kv_heads : 0);
-                T *row = static_cast<T *>(is_k ? p.k_pages : p.v_pages) + walk.row(p.batch, p.page_stride, p.token_stride) +
-                         kh * p.head_stride;
-                store_row(row, x, halves);
-            }
+        if constexpr (IS_Q) {
+            if (there) store_row(static_cast<T *>(p.q_out) + t * p.qo_ts + h * p.qo_hs, x, false);
+        } else if constexpr (BITS == 0) {
+            if (there && cached) store_row(static_cast<T *>(IS_V ? p.v_pages : p.k_pages) + at + h * p.head_stride, x, IS_V);
         } else {
-            const bool some = h + at_once > p.q_heads && h < heads;
-            if (!cached || !__any_sync(0xFFFFFFFFu, some && (is_k || is_v))) return;
+            if (!cached) return;
             // channels 8 sl .. 8 sl + 7 side by side
-            if (!VEC || (p.rot && !p.interleaved)) {
+            if (!VEC || (!IS_V && p.rot && !p.interleaved)) {
                 float *row = exchange[warp] + (lane - sl) * 8;
                 __syncwarp();
+                if constexpr (VEC) {
+                    *reinterpret_cast<float4 *>(row + first_turned) = make_float4(x[0], x[1], x[2], x[3]);
+                    *reinterpret_cast<float4 *>(row + second_turned) = make_float4(x[4], x[5], x[6], x[7]);
+                } else {
 #pragma unroll
-                for (int s = 0; s < 8; ++s) {
-                    const int c = channel_of(p, sl, s, halves);
-                    if (c < p.head_dim) row[c] = x[s];
+                    for (int s = 0; s < 8; ++s) {
+                        const int c = channel(s, IS_V);
+                        if (c < p.head_dim) row[c] = x[s];
+                    }
                 }
                 __syncwarp();
 #pragma unroll
-                for (int s = 0; s < 8; ++s) x[s] = row[8 * sl + s];
-            } else {
-                float y[8];
-#pragma unroll
-                for (int s = 0; s < 8; ++s) y[s] = x[(s >> 1) + 4 * (s & 1)];
-#pragma unroll
-                for (int s = 0; s < 8; ++s) x[s] = y[s];
+                for (int s = 0; s < 8; s += 4) {
+                    const float4 y = *reinterpret_cast<const float4 *>(row + 8 * sl + s);
+                    x[s] = y.x;
+                    x[s + 1] = y.y;
+                    x[s + 2] = y.z;
+                    x[s + 3] = y.w;
+                }
             }
-            const bool mine = 8 * sl < p.head_dim;
             float lo = INFINITY, hi = -INFINITY, bad = 0.0f;
             if (mine) {
 #pragma unroll
                 for (int s = 0; s < 8; ++s) {
                     lo = fminf(lo, x[s]);
                     hi = fmaxf(hi, x[s]);
-                    bad = bad + x[s] * 0.0f;  // NaN if one is not finite
+                    bad = fmaf(x[s], 0.0f, bad);  // NaN if one is not finite
                 }
             }
-            const int span = p.z.group == p.head_dim ? p.seg : p.z.group / 8;  // lanes of a group
-            for (int d = 1; d < span; d <<= 1) {
+            const int span = p.z.groups == 1 ? seg : p.z.group / 8;  // lanes of a group
+#pragma unroll
+            for (int d = 1; d < (VEC ? SEG : 32); d <<= 1) {
+                if (d >= span) break;
                 lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, d));
                 hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, d));
                 bad = bad + __shfl_xor_sync(0xFFFFFFFFu, bad, d);
             }
-            if (!mine || !(is_k || is_v)) return;
+            if (!mine || !there) return;
             constexpr float TOP = (float)((1 << BITS) - 1), MOST = 65504.0f;
             lo = fminf(fmaxf(lo, -MOST), MOST);
             hi = fminf(fmaxf(hi, -MOST), MOST);
             __half offset = __float2half_rn(lo);
             const float o = __half2float(offset);
             __half scale = __float2half_rn(__fmul_rn(__fsub_rn(hi, o), 1.0f / TOP));
-            const float st = __half2float(scale);
-            uint32_t code[2] = {0, 0};
+            uint2 code = encode<BITS>(x, o, __half2float(scale));
             if (bad != 0.0f) {
                 scale = offset = __float2half_rn(__int_as_float(0x7FC00000));
-            } else if (st > 0.0f) {
-#pragma unroll
-                for (int s = 0; s < 8; ++s) {
-                    const float y = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[s], o), st)), 0.0f), TOP);
-                    code[BITS == 4 ? 0 : s >> 2] |= (uint32_t)y << (BITS == 4 ? 4 * s : 8 * (s & 3));
-                }
+                code = make_uint2(0, 0);
             }
-            const int kh = h - p.q_heads - (is_v ? p.kv_heads : 0);
-            uint8_t *row = static_cast<uint8_t *>(is_k ? p.k_pages : p.v_pages) + walk.row(p.batch, p.page_stride, p.token_stride) +
-                           kh * p.head_stride + sl * BITS;
-            if constexpr (BITS == 4) *reinterpret_cast<uint32_t *>(row) = code[0];
-            else *reinterpret_cast<uint2 *>(row) = make_uint2(code[0], code[1]);
-            if (sl % (p.z.group / 8) == 0) {
-                __half2 *pair = const_cast<__half2 *>(is_k ? p.z.k_scales : p.z.v_scales) +
-                                walk.row(p.batch, p.z.page_stride, p.z.token_stride) + kh * p.z.head_stride + 8 * sl / p.z.group;
-                *pair = __halves2half2(scale, offset);
-            }
+            uint8_t *row = static_cast<uint8_t *>(IS_V ? p.v_pages : p.k_pages) + at + h * p.head_stride + sl * BITS;
+            if constexpr (BITS == 4) *reinterpret_cast<uint32_t *>(row) = code.x;
+            else *reinterpret_cast<uint2 *>(row) = code;
+            const int group = p.z.groups == 1 ? 0 : 8 * sl / p.z.group;
+            if (8 * sl == group * p.z.group)
+                const_cast<__half2 *>(IS_V ? p.z.v_scales : p.z.k_scales)[pairs + h * p.z.head_stride + group] = __halves2half2(scale, offset);
         }
     };
 
     for (int t = t0; t < t1; ++t) {
-        Eight<S> now, next;
-        // the whole warp runs while one of its heads is there
-        int h = h_first;
-        load(now, t, h);
+        Eight now, next;
+        token(t);
+        load(now, part);
         place(t);
-        while (h - lane / p.seg < heads) {
-            if (h + step - lane / p.seg < heads) load(next, t, h + step);
-            finish(now, t, h);
+        for (int i = part; i < items; i += p.parts) {
+            if (i + p.parts < items) load(next, i + p.parts);
+            if (i < q_items) finish(now, t, i, std::integral_constant<int, 0>());
+            else if (i < q_items + kv_items) finish(now, t, i - q_items, std::integral_constant<int, 1>());
+            else finish(now, t, i - q_items - kv_items, std::integral_constant<int, 2>());
             now = next;
-            h += step;
         }
     }
 }
 
 template <typename S, typename T, int BITS> inline int launch_heads(HeadsParams &p, bool vec, cudaStream_t stream) {
     p.seg = p.head_dim <= 64 ? 8 : p.head_dim <= 128 ? 16 : 32;
-    const int heads = p.q_heads + 2 * p.kv_heads;
-    // few tokens: a token's heads over several blocks; many: runs of consecutive tokens
-    const int64_t slots = (int64_t)sm_count() * 8, parts = ceil_div(heads, HEADS_WARPS * (32 / p.seg));
-    int64_t split = slots / p.tokens;
-    split = split < 1 ? 1 : split > parts ? parts : split;
-    if (split > 65535) split = 65535;
-    p.per_block = (int)ceil_div(p.tokens, slots / split);
-    const dim3 grid((unsigned)ceil_div(p.tokens, p.per_block), (unsigned)split);
-    if (vec) kv_append_heads_kernel<S, T, BITS, true><<<grid, 32 * HEADS_WARPS, 0, stream>>>(p);
-    else kv_append_heads_kernel<S, T, BITS, false><<<grid, 32 * HEADS_WARPS, 0, stream>>>(p);
+    const TokenRuns r = runs_of(p.tokens, ceil_div(p.q_heads, 32 / p.seg) + 2 * ceil_div(p.kv_heads, 32 / p.seg), HEADS_WARPS, HEADS_RESIDENT);
+    p.run = r.run;
+    p.parts = r.parts;
+    p.inv_dim = 1.0 / p.head_dim;
+    auto go = [&](auto seg) {
+        kv_append_heads_kernel<S, T, BITS, decltype(seg)::value><<<r.blocks, 32 * HEADS_WARPS, 0, stream>>>(p);
+    };
+    if (!vec) go(std::integral_constant<int, 0>());
+    else if (p.seg == 8) go(std::integral_constant<int, 8>());
+    else if (p.seg == 16) go(std::integral_constant<int, 16>());
+    else go(std::integral_constant<int, 32>());
     return check_launch("kv_append_heads_kernel");
 }
 
@@ -348,7 +397,8 @@ inline int append_heads(const mgc_cuda_kv_append_heads_args &a, cudaStream_t str
                      rows(b.v, b.v_token_stride, b.v_head_stride, ss) &&
                      (!b.q || (rows(b.q, b.q_token_stride, b.q_head_stride, ss) && rows(b.q_out, b.qo_token_stride, b.qo_head_stride, ts))) &&
                      (codes || (rows(c.k, c.page_stride, c.token_stride, ts) && rows(c.v, c.head_stride, 0, ts))) &&
-                     (!p.rot || (aligned(b.cos, 16) && aligned(b.sin, 16) && b.table_row % 4 == 0));
+                     (!p.rot || (aligned(b.cos, 16) && aligned(b.sin, 16) && b.table_row % 4 == 0)) &&
+                     (!a.q_norm || aligned(a.q_norm, 16)) && (!a.k_norm || aligned(a.k_norm, 16));
     auto types = [&](auto src, auto page) {
         using S = decltype(src);
         using T = decltype(page);

@@ -17,58 +17,81 @@ struct ReadParams {
     long long k_ts, k_hs, v_ts, v_hs;
     int kv_heads, head_dim;
     int seg;  // lanes of a head, eight channels each
-    int tokens, per_block;
+    int tokens, run, parts;
 };
 
-// Eight consecutive codes as floats.
-template <int BITS> __device__ __forceinline__ void eight_codes(const uint8_t *p, float (&x)[8]) {
-    if constexpr (BITS == 4) {
-        const uint32_t w = *reinterpret_cast<const uint32_t *>(p);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = (float)(w >> 4 * i & 15);
-    } else {
-        const uint2 w = *reinterpret_cast<const uint2 *>(p);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = (float)((i < 4 ? w.x : w.y) >> 8 * (i & 3) & 255);
+// Eight consecutive codes as they are stored, and as floats: put into the mantissa of 2^23, which comes off
+// exactly (a conversion instruction takes a quarter of the rate).
+template <int BITS> struct EightCodes;
+template <> struct EightCodes<4> {
+    uint32_t w;
+    __device__ __forceinline__ void load(const uint8_t *p) { w = __ldg(reinterpret_cast<const unsigned int *>(p)); }
+    __device__ __forceinline__ float operator[](int i) const { return __uint_as_float((w >> 4 * i & 15u) | 0x4B000000u) - 8388608.0f; }
+};
+template <> struct EightCodes<8> {
+    uint2 w;
+    __device__ __forceinline__ void load(const uint8_t *p) { w = __ldg(reinterpret_cast<const uint2 *>(p)); }
+    __device__ __forceinline__ float operator[](int i) const {
+        return __uint_as_float(__byte_perm(i < 4 ? w.x : w.y, 0x4B000000u, 0x7650 | (i & 3))) - 8388608.0f;
     }
-}
+};
+
+constexpr int READ_WARPS = 4, READ_RESIDENT = 8;
 
 template <typename T, int BITS, bool VEC>
-__global__ void __launch_bounds__(128) kv_read_kernel(const __grid_constant__ ReadParams p) {
-    const int lane = (int)(threadIdx.x & 31), warp = (int)(threadIdx.x >> 5);
-    const int sl = lane & (p.seg - 1), at_once = 32 / p.seg;
-    const int step = (int)gridDim.y * 4 * at_once, h0 = ((int)blockIdx.y * 4 + warp) * at_once + lane / p.seg;
-    const int t0 = (int)blockIdx.x * p.per_block, t1 = min(t0 + p.per_block, p.tokens);
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) check_rows(p.batch, p.tokens);
+__global__ void __launch_bounds__(32 * READ_WARPS, READ_RESIDENT) kv_read_kernel(const __grid_constant__ ReadParams p) {
+    const int lane = (int)(threadIdx.x & 31);
+    const unsigned unit = blockIdx.x * READ_WARPS + threadIdx.x / 32;
+    const int sl = lane & (p.seg - 1), at_once = 32 / p.seg, part = (int)(unit % (unsigned)p.parts);
+    const long long t_first = (long long)(unit / (unsigned)p.parts) * p.run;
+    if (unit == 0 && lane == 0) check_rows(p.batch, p.tokens);
+    if (t_first >= p.tokens) return;
+    const int t0 = (int)t_first, t1 = min(t0 + p.run, p.tokens);
+    const int h0 = part * at_once + lane / p.seg, step = p.parts * at_once;
+    const bool mine = 8 * sl < p.head_dim;
+    const int group = 8 * sl / p.z.group;
     TokenWalk walk;
     walk.start(t0);
     for (int t = t0; t < t1; ++t) {
         walk.step(p.batch, t);
         const bool there = walk.page >= 0;
-        const long long codes = there ? walk.row(p.batch, p.page_stride, p.token_stride) : 0;
-        const long long pairs = there ? walk.row(p.batch, p.z.page_stride, p.z.token_stride) : 0;
-        if (8 * sl >= p.head_dim) continue;  // (the next step's lanes meet again)
-        for (int h = h0; h < 2 * p.kv_heads; h += step) {
-            const bool is_v = h >= p.kv_heads;
-            const int kh = is_v ? h - p.kv_heads : h;
-            float x[8], scale = 0.0f, offset = 0.0f;
+        const long long codes = there ? walk.at(p.page_stride, p.token_stride) + sl * BITS : 0;
+        const long long pairs = there ? walk.at(p.z.page_stride, p.z.token_stride) + group : 0;
+        // two heads' keys and values in flight
+        constexpr int BATCH = 2;
+        for (int h = h0; h - lane / p.seg < p.kv_heads; h += BATCH * step) {
+            EightCodes<BITS> c[BATCH][2];
+            __half2 so[BATCH][2];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-            if (there) {
-                eight_codes<BITS>((is_v ? p.v_pages : p.k_pages) + codes + kh * p.head_stride + sl * BITS, x);
-                const float2 so = __half22float2((is_v ? p.z.v_scales : p.z.k_scales)[pairs + kh * p.z.head_stride + 8 * sl / p.z.group]);
-                scale = so.x;
-                offset = so.y;
+            for (int i = 0; i < BATCH; ++i) {
+                const int kh = h + i * step;
+                so[i][0] = so[i][1] = __floats2half2_rn(0.0f, 0.0f);
+                c[i][0] = c[i][1] = EightCodes<BITS>{};
+                if (there && mine && kh < p.kv_heads) {
+                    c[i][0].load(p.k_pages + codes + kh * p.head_stride);
+                    c[i][1].load(p.v_pages + codes + kh * p.head_stride);
+                    so[i][0] = __ldg(p.z.k_scales + pairs + kh * p.z.head_stride);
+                    so[i][1] = __ldg(p.z.v_scales + pairs + kh * p.z.head_stride);
+                }
             }
-            T *dst = static_cast<T *>(is_v ? p.v_out : p.k_out) + t * (is_v ? p.v_ts : p.k_ts) + kh * (is_v ? p.v_hs : p.k_hs) + 8 * sl;
-            Pack<8, T> y;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y.e[i] = from_f<T>(fmaf(scale, x[i], offset));
-            if constexpr (VEC) {
-                y.store(dst);
-            } else {
+            for (int i = 0; i < BATCH; ++i) {
+                const int kh = h + i * step;
+                if (!mine || kh >= p.kv_heads) continue;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) dst[i] = y.e[i];
+                for (int v = 0; v < 2; ++v) {
+                    const float2 s = __half22float2(so[i][v]);
+                    Pack<8, T> y;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y.e[e] = from_f<T>(fmaf(s.x, c[i][v][e], s.y));
+                    T *dst = static_cast<T *>(v ? p.v_out : p.k_out) + t * (v ? p.v_ts : p.k_ts) + kh * (v ? p.v_hs : p.k_hs) + 8 * sl;
+                    if constexpr (VEC) {
+                        y.store(dst);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) dst[e] = y.e[e];
+                    }
+                }
             }
         }
     }
@@ -76,13 +99,11 @@ __global__ void __launch_bounds__(128) kv_read_kernel(const __grid_constant__ Re
 
 template <typename T, int BITS> inline int launch_read(ReadParams &p, bool vec, cudaStream_t stream) {
     p.seg = p.head_dim <= 64 ? 8 : p.head_dim <= 128 ? 16 : 32;
-    const int64_t slots = (int64_t)sm_count() * 16, parts = ceil_div(2 * p.kv_heads, 4 * (32 / p.seg));
-    int64_t split = slots / p.tokens;
-    split = split < 1 ? 1 : split > parts ? parts : split;
-    p.per_block = (int)ceil_div(p.tokens, slots / split);
-    const dim3 grid((unsigned)ceil_div(p.tokens, p.per_block), (unsigned)split);
-    if (vec) kv_read_kernel<T, BITS, true><<<grid, 128, 0, stream>>>(p);
-    else kv_read_kernel<T, BITS, false><<<grid, 128, 0, stream>>>(p);
+    const TokenRuns r = runs_of(p.tokens, ceil_div(p.kv_heads, 32 / p.seg), READ_WARPS, READ_RESIDENT);
+    p.run = r.run;
+    p.parts = r.parts;
+    if (vec) kv_read_kernel<T, BITS, true><<<r.blocks, 32 * READ_WARPS, 0, stream>>>(p);
+    else kv_read_kernel<T, BITS, false><<<r.blocks, 32 * READ_WARPS, 0, stream>>>(p);
     return check_launch("kv_read_kernel");
 }
 

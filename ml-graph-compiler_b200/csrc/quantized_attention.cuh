@@ -177,6 +177,14 @@ template <typename C> inline int launch_quantized(const QuantParams &p, const Qu
     return check_launch("quantized_attention_kernel");
 }
 
+// x / d = x * magic >> shift for 0 <= x < 2^31: with s = ceil(log2 d), ceil(2^(31 + s) / d) fits 32 bits and is exact.
+inline void division(int64_t d, uint32_t &magic, int &shift) {
+    int s = 0;
+    while ((1ll << s) < d) ++s;
+    shift = 31 + s;
+    magic = (uint32_t)(((1ull << shift) + (uint64_t)d - 1) / (uint64_t)d);
+}
+
 // The sequences that are expanded: values to plain pages, attention over them, some key heads at a time.
 inline int attend_expanded(const mgc_cuda_paged_attention_args &a, const QuantParams &p, const QuantPlan &s, char *space, cudaStream_t stream) {
     const mgc_cuda_paged &c = a.paged;
@@ -192,9 +200,16 @@ inline int attend_expanded(const mgc_cuda_paged_attention_args &a, const QuantPa
         e.kv_lens = const_cast<int32_t *>(x.paged.kv_lens);
         e.slots = s.slots;
         e.page = s.page;
+        e.code_page = p.code_page;
+        e.code_token = p.code_token;
+        e.pair_page = p.pair_page;
+        e.pair_token = p.pair_token;
+        e.per_page = p.a.batch.page_size / s.page;
+        division(e.per_page, e.per_magic, e.per_shift);
+        e.page_magic = s.page > 128 ? 0 : (uint32_t)(65536 / s.page + (65536 % s.page != 0));
         e.h0 = h0;
         e.heads = n;
-        const dim3 grid((unsigned)s.slots, (unsigned)n, (unsigned)c.batch);
+        const dim3 grid((unsigned)ceil_div(s.slots, s.page < 64 ? 64 / s.page : 1), (unsigned)n, (unsigned)c.batch);
         auto go = [&](auto type) {
             using T = decltype(type);
             if (p.z.bits == 4) quantized_expand_kernel<T, 4><<<grid, 256, 0, stream>>>(e);
@@ -224,6 +239,11 @@ inline int attend_quantized(const mgc_cuda_paged_attention_quantized_args &a, cu
     if (s.total() && (!b.workspace || b.workspace_bytes < s.total() || !aligned(b.workspace, 16)))
         return fail(MGC_CUDA_NEEDS_WORKSPACE, "%s: needs %lld bytes of workspace (16-byte aligned), got %lld", what,
                     (long long)s.total(), (long long)(b.workspace ? b.workspace_bytes : 0));
+    division(c.page_size, p.page_magic, p.page_shift);
+    p.code_page = (uint32_t)(c.page_stride / 16);
+    p.code_token = (uint32_t)(c.token_stride / 16);
+    p.pair_page = (uint32_t)a.quantized.page_stride;
+    p.pair_token = (uint32_t)a.quantized.token_stride;
     char *space = static_cast<char *>(b.workspace);
     p.a.rows_left = s.rows_left;
     p.a.kv_left = s.heads ? s.slots * s.page : 0;
@@ -238,15 +258,6 @@ inline int attend_quantized(const mgc_cuda_paged_attention_quantized_args &a, cu
         p.a.part_ml = reinterpret_cast<float2 *>(p.a.part + rows * p.a.head_dim);
         p.a.cut = reinterpret_cast<CutUnit *>(p.a.part_ml + rows);
     }
-    // division by the page size: with s = ceil(log2 d), ceil(2^(31 + s) / d) fits 32 bits and is exact below 2^31
-    int shift = 0;
-    while ((1ll << shift) < c.page_size) ++shift;
-    p.page_shift = 31 + shift;
-    p.page_magic = (uint32_t)(((1ull << (31 + shift)) + (uint64_t)c.page_size - 1) / (uint64_t)c.page_size);
-    p.code_page = (uint32_t)(c.page_stride / 16);
-    p.code_token = (uint32_t)(c.token_stride / 16);
-    p.pair_page = (uint32_t)a.quantized.page_stride;
-    p.pair_token = (uint32_t)a.quantized.token_stride;
     const int chunk = 16 / elem_size(c.dtype);
     p.q_wide = aligned(b.q, 16) && b.q_token_stride % chunk == 0 && b.q_head_stride % chunk == 0;
     return with_config(c.dtype, a.quantized, c.head_dim, s.nb, [&](auto config) { return launch_quantized(p, s, config, stream); });

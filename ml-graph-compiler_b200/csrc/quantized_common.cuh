@@ -26,14 +26,16 @@ struct Quantized {
 // Packed tokens one after the other: which sequence and position, and where its cache rows are. All
 // lanes of a warp step together.
 struct TokenWalk {
-    int b, end, n;      // sequence, its end among the packed tokens, its cached positions
-    int held, page;     // page looked up last
-    int pos;            // position; negative: in no sequence, or no cached position
+    int b, end, n;   // sequence, its end among the packed tokens, its cached positions
+    int page, row;   // where the position is: page (-1: none), row in it
+    int pos;         // position; negative: in no sequence, or no cached position
+    int held;        // page of the sequence; -1: not looked up
     __device__ __forceinline__ void start(int t0) {
         b = -1;
         end = t0;
         n = 0;
         held = page = -1;
+        row = 0;
     }
     __device__ __forceinline__ void step(const Batch &d, int t) {
         if (t >= end) {
@@ -47,17 +49,38 @@ struct TokenWalk {
             held = -1;
         }
         pos = n - (end - t);
-        if (pos >= 0 && (held < 0 || pos / d.page_size != held)) {
+        if (pos < 0) {
+            held = page = -1;
+        } else if (held < 0) {
             held = pos / d.page_size;
+            row = pos - held * d.page_size;
             page = page_of(d, b, held);
+        } else if (++row == d.page_size) {
+            row = 0;
+            page = page_of(d, b, ++held);
         }
-        if (pos < 0) page = held = -1;
     }
     // Offset of the token's row in pages of these strides (page >= 0).
-    __device__ __forceinline__ long long row(const Batch &d, long long page_stride, long long token_stride) const {
-        return (long long)page * page_stride + (long long)(pos - held * d.page_size) * token_stride;
+    __device__ __forceinline__ long long at(long long page_stride, long long token_stride) const {
+        return (long long)page * page_stride + (long long)row * token_stride;
     }
 };
+
+// Warps of a launch over packed tokens: each takes a run of consecutive ones, or, when they are few, a part of
+// one token's heads.
+struct TokenRuns {
+    int run, parts;  // tokens of a run; parts of a token's heads
+    unsigned blocks;
+};
+inline TokenRuns runs_of(int64_t tokens, int64_t most_parts, int warps, int resident) {
+    const int64_t slots = (int64_t)sm_count() * resident * warps;
+    TokenRuns r;
+    const int64_t parts = slots / tokens;
+    r.parts = (int)(parts < 1 ? 1 : parts > most_parts ? most_parts : parts);
+    r.run = (int)ceil_div(tokens * r.parts, slots);
+    r.blocks = (unsigned)ceil_div(ceil_div(tokens, r.run) * r.parts, warps);
+    return r;
+}
 
 // Tells of rows of q_starts past the packed tokens (one thread of a launch).
 __device__ __forceinline__ void check_rows(const Batch &d, int tokens) {
