@@ -48,11 +48,25 @@ constexpr int HEADS_WARPS = 4, HEADS_RESIDENT = 8;
 // the rounding to fp32 is the exact root's but for one case in 2^18.
 __device__ __forceinline__ float inverse_root(double m) {
     if (!(m > 1e-30 && m < 1e30)) return (float)(1.0 / sqrt(m));
-    const double r = (double)rsqrtf((float)m);
-    return (float)(r * (1.5 - 0.5 * m * r * r));
+    float a;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"((float)m));
+    const double r = (double)a;
+    return (float)(r * fma(-0.5 * m * r, r, 1.5));
 }
 
-// Group code of eight values side by side, next to each other in a lane.
+// Least and greatest, NaN if one is.
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+// Codes of eight values side by side.
 template <int BITS> __device__ __forceinline__ uint2 encode(const float (&x)[8], float offset, float scale) {
     constexpr float TOP = (float)((1 << BITS) - 1), ROUND = 12582912.0f;  // 1.5 * 2^23: adding it rounds to whole numbers
     if (!(scale > 0.0f)) return make_uint2(0, 0);
@@ -61,19 +75,19 @@ template <int BITS> __device__ __forceinline__ uint2 encode(const float (&x)[8],
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
         // off by two roundings: 2^-22 of at most 255, below 1e-4
-        q[s] = fminf(fmaxf(__fmul_rn(__fsub_rn(x[s], offset), inv), 0.0f), TOP);
-        far = fmaxf(far, fabsf(q[s] - (__fadd_rn(q[s], ROUND) - ROUND)));
+        const float y = fminf(fmaxf(__fmul_rn(__fsub_rn(x[s], offset), inv), 0.0f), TOP);
+        q[s] = __fadd_rn(y, ROUND);
+        far = fmaxf(far, fabsf(y - (q[s] - ROUND)));
     }
     if (far > 0.4999f) {
 #pragma unroll
-        for (int s = 0; s < 8; ++s) q[s] = fminf(fmaxf(__fdiv_rn(__fsub_rn(x[s], offset), scale), 0.0f), TOP);
+        for (int s = 0; s < 8; ++s) q[s] = __fadd_rn(fminf(fmaxf(__fdiv_rn(__fsub_rn(x[s], offset), scale), 0.0f), TOP), ROUND);
     }
-    uint32_t code[2] = {0, 0};
+    // ROUND's own bits, shifted alike, come off the sum at once
+    constexpr uint32_t BASE = 0x4B400000u, ALL = BITS == 4 ? BASE * 0x11111111u : BASE * 0x01010101u;
+    uint32_t code[2] = {0u - ALL, 0u - ALL};
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
-        const uint32_t c = __float_as_uint(__fadd_rn(q[s], ROUND)) & 255u;
-        code[BITS == 4 ? 0 : s >> 2] |= c << (BITS == 4 ? 4 * s : 8 * (s & 3));
-    }
+    for (int s = 0; s < 8; ++s) code[BITS == 4 ? 0 : s >> 2] += __float_as_uint(q[s]) << (BITS == 4 ? 4 * s : 8 * (s & 3));
     return make_uint2(code[0], code[1]);
 }
 
@@ -108,9 +122,13 @@ __global__ void __launch_bounds__(32 * HEADS_WARPS, HEADS_RESIDENT) kv_append_he
     const int sl = lane & (seg - 1), at_once = 32 / seg, sub = lane / seg;
     // a token's heads, at_once of one kind at a time: queries, keys, values
     const int q_items = (p.q_heads + at_once - 1) / at_once, kv_items = (p.kv_heads + at_once - 1) / at_once;
-    const int items = q_items + 2 * kv_items, part = (int)(unit % (unsigned)p.parts);
+    const int part = (int)(unit % (unsigned)p.parts);
     const bool mine = 8 * sl < p.head_dim, turned = 2 * 4 * sl < p.rot;  // (VEC) this lane's channels exist, are rotated
     const bool apart = turned && !p.interleaved;                        // (VEC) pairs rot / 2 apart
+
+    // codes: the lane's group, the lanes of a group, whether it is the group's first
+    const int group = BITS ? 8 * sl / p.z.group : 0, span = !BITS ? 1 : p.z.groups == 1 ? seg : p.z.group / 8;
+    const bool leads = BITS && 8 * sl == group * p.z.group;
 
     // Channels of value s of the lane. VEC: two fours side by side; else pair 4 sl + s / 2, first or second.
     const int first_turned = apart ? 4 * sl : 8 * sl, second_turned = apart ? 4 * sl + p.rot / 2 : 8 * sl + 4;
@@ -121,22 +139,9 @@ __global__ void __launch_bounds__(32 * HEADS_WARPS, HEADS_RESIDENT) kv_append_he
     struct Eight {
         Pack<4, S> a, b;
     };
-    // the token's rows of q, k and v, this lane's heads first
-    const S *q_row = nullptr, *k_row = nullptr, *v_row = nullptr;
-    auto token = [&](int t) {
-        q_row = static_cast<const S *>(p.q) + (long long)t * p.q_ts;
-        k_row = static_cast<const S *>(p.k) + (long long)t * p.k_ts;
-        v_row = static_cast<const S *>(p.v) + (long long)t * p.v_ts;
-    };
-    auto load = [&](Eight &e, int i) {
-        const bool is_q = i < q_items, is_v = i >= q_items + kv_items;
-        const int h = (i - (is_q ? 0 : is_v ? q_items + kv_items : q_items)) * at_once + sub;
-        const S *src = (is_q ? q_row : is_v ? v_row : k_row) + (long long)h * (is_q ? p.q_hs : is_v ? p.v_hs : p.k_hs);
-        const bool have = h < (is_q ? p.q_heads : p.kv_heads);
+    auto load = [&](Eight &e, const S *src, bool have, bool is_v) {
         if constexpr (VEC) {
-#pragma unroll
-            for (int k = 0; k < Pack<4, S>::N; ++k) e.a.raw[k] = e.b.raw[k] = typename Pack<4, S>::R{};
-            if (!have || !mine) return;
+            if (!have) return;
             e.a.load(src + (is_v ? 8 * sl : first_turned));
             e.b.load(src + (is_v ? 8 * sl + 4 : second_turned));
         } else {
@@ -203,11 +208,9 @@ __global__ void __launch_bounds__(32 * HEADS_WARPS, HEADS_RESIDENT) kv_append_he
         x1 = a;
         x2 = b;
     };
-    // kind 0: queries, 1: keys, 2: values
-    auto finish = [&](const Eight &e, int t, int i, auto kind) {
+    // pair: of the lane's group of the head
+    auto finish = [&](const Eight &e, auto kind, auto *dst, __half2 *pair, bool there) {
         constexpr bool IS_Q = decltype(kind)::value == 0, IS_V = decltype(kind)::value == 2;
-        const int h = i * at_once + sub;
-        const bool there = h < (IS_Q ? p.q_heads : p.kv_heads);
         float x[8];
 #pragma unroll
         for (int s = 0; s < 8; ++s) x[s] = to_f(s < 4 ? e.a.e[s & 3] : e.b.e[s & 3]);
@@ -254,9 +257,9 @@ __global__ void __launch_bounds__(32 * HEADS_WARPS, HEADS_RESIDENT) kv_append_he
             }
         }
         if constexpr (IS_Q) {
-            if (there) store_row(static_cast<T *>(p.q_out) + t * p.qo_ts + h * p.qo_hs, x, false);
+            if (there) store_row(dst, x, false);
         } else if constexpr (BITS == 0) {
-            if (there && cached) store_row(static_cast<T *>(IS_V ? p.v_pages : p.k_pages) + at + h * p.head_stride, x, IS_V);
+            if (there && cached) store_row(dst, x, IS_V);
         } else {
             if (!cached) return;
             // channels 8 sl .. 8 sl + 7 side by side
@@ -283,23 +286,21 @@ __global__ void __launch_bounds__(32 * HEADS_WARPS, HEADS_RESIDENT) kv_append_he
                     x[s + 3] = y.w;
                 }
             }
-            float lo = INFINITY, hi = -INFINITY, bad = 0.0f;
+            float lo = INFINITY, hi = -INFINITY;
             if (mine) {
 #pragma unroll
                 for (int s = 0; s < 8; ++s) {
-                    lo = fminf(lo, x[s]);
-                    hi = fmaxf(hi, x[s]);
-                    bad = fmaf(x[s], 0.0f, bad);  // NaN if one is not finite
+                    lo = min_nan(lo, x[s]);
+                    hi = max_nan(hi, x[s]);
                 }
             }
-            const int span = p.z.groups == 1 ? seg : p.z.group / 8;  // lanes of a group
 #pragma unroll
             for (int d = 1; d < (VEC ? SEG : 32); d <<= 1) {
                 if (d >= span) break;
-                lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, d));
-                hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, d));
-                bad = bad + __shfl_xor_sync(0xFFFFFFFFu, bad, d);
+                lo = min_nan(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, d));
+                hi = max_nan(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, d));
             }
+            const bool bad = !(lo > -INFINITY && hi < INFINITY);  // a value is not finite
             if (!mine || !there) return;
             constexpr float TOP = (float)((1 << BITS) - 1), MOST = 65504.0f;
             lo = fminf(fmaxf(lo, -MOST), MOST);
@@ -308,31 +309,52 @@ __global__ void __launch_bounds__(32 * HEADS_WARPS, HEADS_RESIDENT) kv_append_he
             const float o = __half2float(offset);
             __half scale = __float2half_rn(__fmul_rn(__fsub_rn(hi, o), 1.0f / TOP));
             uint2 code = encode<BITS>(x, o, __half2float(scale));
-            if (bad != 0.0f) {
+            if (bad) {
                 scale = offset = __float2half_rn(__int_as_float(0x7FC00000));
                 code = make_uint2(0, 0);
             }
-            uint8_t *row = static_cast<uint8_t *>(IS_V ? p.v_pages : p.k_pages) + at + h * p.head_stride + sl * BITS;
-            if constexpr (BITS == 4) *reinterpret_cast<uint32_t *>(row) = code.x;
-            else *reinterpret_cast<uint2 *>(row) = code;
-            const int group = p.z.groups == 1 ? 0 : 8 * sl / p.z.group;
-            if (8 * sl == group * p.z.group)
-                const_cast<__half2 *>(IS_V ? p.z.v_scales : p.z.k_scales)[pairs + h * p.z.head_stride + group] = __halves2half2(scale, offset);
+            if constexpr (BITS == 4) *reinterpret_cast<uint32_t *>(dst + sl * 4) = code.x;
+            else *reinterpret_cast<uint2 *>(dst + sl * 8) = code;
+            if (leads) *pair = __halves2half2(scale, offset);
         }
     };
 
-    for (int t = t0; t < t1; ++t) {
+    // One kind's heads of a token (0: queries, 1: keys, 2: values): items i, i + parts, ...
+    auto heads_of = [&](auto kind, const S *src, long long src_hs, auto *dst, long long dst_hs, __half2 *pair, int count, int i) {
+        constexpr bool IS_V = decltype(kind)::value == 2;
+        const int step = p.parts * at_once;
+        int h = i * at_once + sub;
+        src += h * src_hs;
+        dst += h * dst_hs;
+        pair += h * p.z.head_stride + group;
+        const long long src_step = step * src_hs, dst_step = step * dst_hs, pair_step = BITS ? step * p.z.head_stride : 0;
         Eight now, next;
-        token(t);
-        load(now, part);
-        place(t);
-        for (int i = part; i < items; i += p.parts) {
-            if (i + p.parts < items) load(next, i + p.parts);
-            if (i < q_items) finish(now, t, i, std::integral_constant<int, 0>());
-            else if (i < q_items + kv_items) finish(now, t, i - q_items, std::integral_constant<int, 1>());
-            else finish(now, t, i - q_items - kv_items, std::integral_constant<int, 2>());
-            now = next;
+#pragma unroll
+        for (int k = 0; k < Pack<4, S>::N; ++k) now.a.raw[k] = now.b.raw[k] = next.a.raw[k] = next.b.raw[k] = typename Pack<4, S>::R{};
+        load(now, src, h < count && (mine || !VEC), IS_V);
+        for (; h - sub < count; h += step, now = next) {
+            src += src_step;
+            if (h - sub + step < count) load(next, src, h + step < count && (mine || !VEC), IS_V);
+            finish(now, kind, dst, pair, h < count);
+            dst += dst_step;
+            pair += pair_step;
         }
+    };
+    // the first item of a kind with so many before it that is this part's
+    auto first_item = [&](int before) {
+        const int x = (part - before) % p.parts;
+        return x < 0 ? x + p.parts : x;
+    };
+    const int k_first = first_item(q_items), v_first = first_item(q_items + kv_items);
+    for (int t = t0; t < t1; ++t) {
+        place(t);
+        using Page = std::conditional_t<BITS != 0, uint8_t, T>;
+        heads_of(std::integral_constant<int, 0>(), static_cast<const S *>(p.q) + (long long)t * p.q_ts, p.q_hs,
+                 static_cast<T *>(p.q_out) + (long long)t * p.qo_ts, p.qo_hs, nullptr, p.q_heads, part);
+        heads_of(std::integral_constant<int, 1>(), static_cast<const S *>(p.k) + (long long)t * p.k_ts, p.k_hs,
+                 static_cast<Page *>(p.k_pages) + at, p.head_stride, const_cast<__half2 *>(p.z.k_scales) + pairs, p.kv_heads, k_first);
+        heads_of(std::integral_constant<int, 2>(), static_cast<const S *>(p.v) + (long long)t * p.v_ts, p.v_hs,
+                 static_cast<Page *>(p.v_pages) + at, p.head_stride, const_cast<__half2 *>(p.z.v_scales) + pairs, p.kv_heads, v_first);
     }
 }
 
