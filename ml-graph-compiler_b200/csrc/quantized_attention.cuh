@@ -1,9 +1,10 @@
 // Attention of new tokens over quantised pages (quantized_common.cuh): paged_attention_params.cuh's
 // definition with k_j and v_j the values that the codes stand for. The choice of kernels and the launch.
 //
-// Sequences with few query rows a key head attend over the codes (quantized_mma.cuh). For those with many the
-// values are written to plain pages in the workspace first (quantized_expand.cuh) and the kernels for plain pages
-// attend over them; key heads some at a time where the workspace would be large.
+// Few query rows a key head attend over the codes (quantized_mma.cuh), and fp32 ones always. Of 16-bit calls with
+// many, the values of sequences with many rows are written to plain half pages in the workspace first
+// (quantized_expand.cuh) and the kernels for plain pages attend over them; key heads some at a time where the
+// workspace would be large.
 #pragma once
 
 #include "quantized_expand.cuh"
@@ -18,7 +19,7 @@ inline int check_attend_quantized(const mgc_cuda_paged_attention_quantized_args 
     // the kernel multiplies strides by page numbers and rows in 32 bits
     const int64_t most = 0xFFFFFFFFll;
     auto fits = [&](int64_t page, int64_t token) { return page <= most && token <= most / c.page_size; };
-    if (!fits(c.page_stride / 16, c.token_stride / 16) || !fits(a.quantized.page_stride, a.quantized.token_stride))
+    if (!fits(c.page_stride, c.token_stride) || !fits(a.quantized.page_stride, a.quantized.token_stride))
         return fail(MGC_CUDA_UNSUPPORTED, "%s: a page does not fit 32 bits", what);
     return MGC_CUDA_OK;
 }
@@ -40,7 +41,7 @@ struct QuantPlan {
     int64_t total() const { return heads ? 2 * pages_bytes + index_bytes + inner + workspace : workspace; }
 };
 
-// More query rows a key head than this take the way over plain pages.
+// Sequences with more query rows a key head than this take the way over plain pages, where a call has one.
 constexpr int64_t DIRECT_ROWS = 64;
 constexpr int64_t EXPANDED_BYTES = 1ll << 30;  // of plain pages at a time
 
@@ -120,14 +121,19 @@ inline QuantPlan quant_plan_of(const mgc_cuda_paged_attention_quantized_args &a)
         }
         s.workspace = (int64_t)s.ctas * (2 * unit_rows * (c.head_dim * 4 + 8) + (int64_t)sizeof(CutUnit));
     }
-    // Rows of 16 bytes are what those kernels take; bf16 queries go over half pages, in the tcgen05 kernel only:
-    // values rounded to bf16 once more left 0.5 % of error in the output of 4-bit pages, half 0.17 %, which is bf16's
-    // own rounding of the output
+    // Over plain pages: rows of 16 bytes are what those kernels take. bf16 queries go over half pages, in the tcgen05
+    // kernel only: values rounded to bf16 once more left 0.5 % of error in the output of 4-bit pages, half 0.17 %, which is
+    // bf16's own rounding of the output. fp32 codes take two products a value where plain fp32 pages take three of half
+    // the depth: 96 rows over 8 x 2048 keys of 8 heads 76 us and 349 us.
     auto rows16 = [&](const void *q, int64_t x, int64_t y) { return aligned(q, 16) && x * es % 16 == 0 && y * es % 16 == 0; };
-    if (rows <= DIRECT_ROWS || !rows16(a.attention.q, a.attention.q_token_stride, a.attention.q_head_stride) ||
+    if (rows <= DIRECT_ROWS || c.dtype == MGC_F32 || !rows16(a.attention.q, a.attention.q_token_stride, a.attention.q_head_stride) ||
         !rows16(a.attention.out, a.attention.o_token_stride, a.attention.o_head_stride) ||
         (c.dtype == MGC_BF16 && (c.head_dim > 128 || c.page_size % 8)))
         return s;
+    // In 10 ps at 128 channels, measured over 1 to 32 sequences of 500 to 8192 keys: a key of a key head takes 7 for 16 rows
+    // over codes, 12 to be expanded and 18 for 256 rows over plain pages, whose four kernels take 25 us for a start.
+    const double keys = (double)c.batch * (double)most * (double)c.kv_heads * width_of(c.head_dim) / 128;
+    if (7 * keys * (double)ceil_div(rows, 16) < 2.5e6 + keys * (12 + 18 * (double)ceil_div(rows, 256))) return s;
     // Plain pages of the cache's size, or of a divisor that the tcgen05 kernel takes (paged_umma.cuh): 128, or a power of
     // two from 8 to 64
     int64_t page = c.page_size;
@@ -194,8 +200,8 @@ inline int attend_expanded(const mgc_cuda_paged_attention_args &a, const QuantPa
         ExpandParams e;
         e.a = p.a;
         e.z = p.z;
-        e.k = x.paged.k;
-        e.v = x.paged.v;
+        e.k = static_cast<__half *>(x.paged.k);
+        e.v = static_cast<__half *>(x.paged.v);
         e.table = const_cast<int32_t *>(x.paged.block_table);
         e.kv_lens = const_cast<int32_t *>(x.paged.kv_lens);
         e.slots = s.slots;
@@ -210,13 +216,9 @@ inline int attend_expanded(const mgc_cuda_paged_attention_args &a, const QuantPa
         e.h0 = h0;
         e.heads = n;
         const dim3 grid((unsigned)ceil_div(s.slots, s.page < 64 ? 64 / s.page : 1), (unsigned)n, (unsigned)c.batch);
-        auto go = [&](auto type) {
-            using T = decltype(type);
-            if (p.z.bits == 4) quantized_expand_kernel<T, 4><<<grid, 256, 0, stream>>>(e);
-            else quantized_expand_kernel<T, 8><<<grid, 256, 0, stream>>>(e);
-            return check_launch("quantized_expand_kernel");
-        };
-        MGC_CHECK(c.dtype == MGC_F32 ? go(float()) : go(__half()));
+        if (p.z.bits == 4) quantized_expand_kernel<4><<<grid, 256, 0, stream>>>(e);
+        else quantized_expand_kernel<8><<<grid, 256, 0, stream>>>(e);
+        MGC_CHECK(check_launch("quantized_expand_kernel"));
         MGC_CHECK(attend(x, c.dtype, stream));
     }
     return MGC_CUDA_OK;
@@ -240,8 +242,8 @@ inline int attend_quantized(const mgc_cuda_paged_attention_quantized_args &a, cu
         return fail(MGC_CUDA_NEEDS_WORKSPACE, "%s: needs %lld bytes of workspace (16-byte aligned), got %lld", what,
                     (long long)s.total(), (long long)(b.workspace ? b.workspace_bytes : 0));
     division(c.page_size, p.page_magic, p.page_shift);
-    p.code_page = (uint32_t)(c.page_stride / 16);
-    p.code_token = (uint32_t)(c.token_stride / 16);
+    p.code_page = (uint32_t)c.page_stride;
+    p.code_token = (uint32_t)c.token_stride;
     p.pair_page = (uint32_t)a.quantized.page_stride;
     p.pair_token = (uint32_t)a.quantized.token_stride;
     char *space = static_cast<char *>(b.workspace);

@@ -7,8 +7,8 @@
 //
 // Pages of `page` positions (the cache's page size or a divisor), one head's rows side by side; sequence b's
 // positions from page * s on are page b * slots + s. Rows that no token sees are zero, so that whatever the cache
-// holds there is not met again; a missing page stays missing. Values are fp32, rounded once to the pages' type:
-// fp32, or half for 16-bit queries, held within its range.
+// holds there is not met again; a missing page stays missing. Values are halves, rounded once and held within
+// half's range.
 #pragma once
 
 #include "kv_read.cuh"
@@ -20,7 +20,7 @@ namespace paged {
 struct ExpandParams {
     QuantAttend a;
     Quantized z;
-    void *k, *v;        // [batch * slots][heads][page][head_dim]
+    __half *k, *v;      // [batch * slots][heads][page][head_dim]
     int32_t *table;     // [batch][slots]
     int32_t *kv_lens;   // [batch]: 0 for sequences that are left to the kernels for codes
     int slots, page, h0, heads;
@@ -30,15 +30,7 @@ struct ExpandParams {
     int per_shift;
 };
 
-// Eight codes' values in order: fp32 rounded once, or halves by one fused operation (rounded once, too), held within
-// half's range.
-template <int BITS> __device__ __forceinline__ void expand_eight(const EightCodes<BITS> &c, __half2 so, float *dst) {
-    const float2 s = __half22float2(so);
-    Pack<8, float> y;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y.e[e] = fmaf(s.x, c[e], s.y);
-    y.store(dst);
-}
+// Eight codes' values in order, by one fused operation each (rounded once), held within half's range.
 template <int BITS> __device__ __forceinline__ void expand_eight(const EightCodes<BITS> &c, __half2 so, __half *dst) {
     const __half2 s = __low2half2(so), o = __high2half2(so), most = __float2half2_rn(65504.0f), least = __float2half2_rn(-65504.0f);
     auto value = [&](uint32_t code, uint32_t bias) {  // of a pair of codes in the mantissas of 1024 or 64
@@ -64,7 +56,7 @@ template <int BITS> __device__ __forceinline__ void expand_eight(const EightCode
 constexpr int EXPAND_ROWS = 4;  // of a thread, in flight together
 
 // Block (64 positions, or one page of more; head; sequence): a thread takes eight channels of every few rows.
-template <typename T, int BITS>
+template <int BITS>
 __global__ void __launch_bounds__(256) quantized_expand_kernel(const __grid_constant__ ExpandParams p) {
     const int h = (int)blockIdx.y, b = (int)blockIdx.z, tid = (int)threadIdx.x, kh = p.h0 + h;
     const Sequence seq = load_sequence(static_cast<const AttendParams &>(p.a), b);
@@ -106,7 +98,7 @@ __global__ void __launch_bounds__(256) quantized_expand_kernel(const __grid_cons
             so[i][0] = so[i][1] = __floats2half2_rn(0.0f, 0.0f);
             if (page >= 0 && j >= lo && j < hi) {
                 const int in_page = row + (slot - (int)((unsigned long long)(unsigned)slot * p.per_magic >> p.per_shift) * p.per_page) * p.page;
-                const unsigned long long at = ((unsigned long long)(unsigned)page * p.code_page + (uint32_t)in_page * p.code_token) * 16;
+                const unsigned long long at = (unsigned long long)(unsigned)page * p.code_page + (uint32_t)in_page * p.code_token;
                 const unsigned long long pair = (unsigned long long)(unsigned)page * p.pair_page + (uint32_t)in_page * p.pair_token;
                 code[i][0].load(k_pages + at);
                 code[i][1].load(v_pages + at);
@@ -118,8 +110,8 @@ __global__ void __launch_bounds__(256) quantized_expand_kernel(const __grid_cons
 #pragma unroll
         for (int i = 0; i < EXPAND_ROWS; ++i) {
             if (to[i] < 0) continue;
-            expand_eight<BITS>(code[i][0], so[i][0], static_cast<T *>(p.k) + (first + to[i]) * p.a.head_dim + c * 8);
-            expand_eight<BITS>(code[i][1], so[i][1], static_cast<T *>(p.v) + (first + to[i]) * p.a.head_dim + c * 8);
+            expand_eight<BITS>(code[i][0], so[i][0], p.k + (first + to[i]) * p.a.head_dim + c * 8);
+            expand_eight<BITS>(code[i][1], so[i][1], p.v + (first + to[i]) * p.a.head_dim + c * 8);
         }
     }
 }

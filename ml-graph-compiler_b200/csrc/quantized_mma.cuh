@@ -24,8 +24,10 @@
 //    the same order of keys, and movmatrix turns weights [key][row] into the second product's operand.
 //  * rows are padded so that both reads are free of bank conflicts (QuantConfig).
 //  * scales and offsets: lane l reads key l's a step ahead and leaves them as floats in shared memory.
-//  * weights times scales are halves 2^14 times as large (paged_attention_params.cuh's reasons), relative to
-//    S_g, a power of two at or above the group's scales so far: tokens' scales may differ by far.
+//  * weights are 2^(score - reference + 11): the reference moves when a score passes it by 4, and not otherwise, so
+//    a step needs no maximum over the lanes; halves then hold them from 2^15 down (paged_attention_params.cuh).
+//  * weights times scales are relative to S_g, a power of two at or above the group's scales so far: tokens'
+//    scales may differ by far.
 //  * query rows are scaled by a power of two into half's range (bf16 and fp32 have more exponent).
 #pragma once
 
@@ -59,13 +61,21 @@ template <typename T_, int BITS_, int DP_, int NB_, bool ONE_> struct QuantConfi
     static constexpr int PAIRS = KW * GS * 8;    // bytes of a step's scales and offsets of K or V
     static constexpr int ORED = DP + 4;
     static constexpr int RED = WARPS * R * (ORED + 2) * 4;
-    static constexpr int SMEM = RING + WARPS * 2 * PAIRS > RED ? RING + WARPS * 2 * PAIRS : RED;
+    static constexpr int Q_AT = RING + WARPS * 2 * PAIRS > RED ? RING + WARPS * 2 * PAIRS : RED;
+    static constexpr int Q = NB * (DP / 32) * 32 * 16;  // bytes of Q's fragments (their upper halves)
+    static constexpr int SMEM = Q_AT + Q * (F32 ? 2 : 1);
     // blocks of an SM, by shared memory and by registers (128 threads of 128, 168 or 255)
     static constexpr int BY_SMEM = 232448 / (SMEM + 1024 + 64);
     static constexpr int BY_REGS = (NB > 1 && DP > 64) || (F32 && DP > 128) ? 2 : DP > 128 || (F32 && DP * NB > 64) ? 3 : 4;
     static constexpr int RESIDENT = BY_SMEM < BY_REGS ? BY_SMEM : BY_REGS;
 };
 
+// a b with a zero accumulator.
+__device__ __forceinline__ void mma16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -167,23 +177,27 @@ struct QuantParams {
     int q_wide;             // rows of q allow 16-byte loads
     uint32_t page_magic;    // j / page_size = j * page_magic >> page_shift for 0 <= j < 2^31
     int page_shift;
-    // strides that fit 32 bits: of codes in 16 bytes, of scales in pairs
+    // strides that fit 32 bits: of codes in bytes, of scales in pairs
     uint32_t code_page, code_token, pair_page, pair_token;
 };
 
 // EVEN: the CTA takes an even share of all units' keys (paged_work.cuh); else one unit's keys.
+__device__ __forceinline__ int lane_id() { return (int)(threadIdx.x & 31); }
 template <typename C, bool EVEN>
 __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_kernel(const __grid_constant__ QuantParams params) {
     using T = typename C::T;
     constexpr int BITS = C::BITS, DP = C::DP, NB = C::NB, R = C::R, BN = C::BN, KW = C::KW, PITCH = C::PITCH, CPR = C::CPR;
     constexpr int SLABS = C::SLABS, GS = C::GS, STAGES = C::STAGES;
-    constexpr float LIFT = Weight<__half>::LIFT;
+    constexpr float LIFT = Weight<__half>::LAZY_LIFT, MOST = LIFT + Weight<__half>::LAZY, FRESH = 1e30f;
     using KCodes = Key<BITS, C::F32>;
     using VCodes = Key<BITS, true>;
     const QuantAttend &p = params.a;
     const Quantized &z = params.z;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint32_t there[C::WARPS][STAGES];  // keys of a stage that were loaded
+    __shared__ float row_scale[R], row_sum[R][GS];  // of Q's rows: what takes a score to base 2, the groups' sums
+    __shared__ RowRange row_sees[R];
+    uint4 *q_upper = reinterpret_cast<uint4 *>(smem + C::Q_AT) + lane_id(), *q_lower = q_upper + C::Q / 16;
     const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g4 = lane >> 2, t4 = lane & 3;
     const int key0 = g4 & 1 ? C::second(g4 >> 1) : C::first(g4 >> 1);  // row of fragment key g4 among its eight
@@ -196,7 +210,7 @@ __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_k
         const int rows = seq.nq * p.group, tiles = k_hi > k_lo ? (k_hi - k_lo + BN - 1) / BN : 0;
         // this lane's part of a copied row: chunk lane % CPR of row lane / CPR of those copied at once
         constexpr int AT_ONCE = KW / CPR;
-        const int part = lane % CPR, copied = min(16, row_bytes - part * 16);
+        const int part = lane % CPR, copied = max(0, min(16, row_bytes - part * 16));
         const uint8_t *kp = static_cast<const uint8_t *>(p.k_pages) + kh * p.head_stride + part * 16;
         const uint8_t *vp = static_cast<const uint8_t *>(p.v_pages) + kh * p.head_stride + part * 16;
         const __half2 *ksp = z.k_scales + kh * z.head_stride, *vsp = z.v_scales + kh * z.head_stride;
@@ -227,22 +241,21 @@ __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_k
             }
             return x;
         };
+        const long long v_past_k = vp - kp;
         auto load_stage = [&](int it, Place x) {
             uint8_t *st = ring + (it % STAGES) * C::STAGE;
             const unsigned mask = __ballot_sync(0xFFFFFFFFu, x.page >= 0);
             if (lane == 0) there[warp][it % STAGES] = mask;
-            const uint32_t dst = smem_u32(st + (lane / CPR) * PITCH + part * 16);
+            const uint32_t dst = smem_u32(st + (lane / CPR) * PITCH + part * 16), in_page = (uint32_t)x.row * params.code_token;
 #pragma unroll
             for (int i = 0; i < CPR; ++i) {
-                const int page = __shfl_sync(0xFFFFFFFFu, x.page, i * AT_ONCE + lane / CPR);
-                const uint32_t row = (uint32_t)__shfl_sync(0xFFFFFFFFu, x.row, i * AT_ONCE + lane / CPR);
-                const int bytes = page >= 0 ? copied : 0;
-                const unsigned long long o =
-                    page >= 0 ? ((unsigned long long)(unsigned)page * params.code_page + row * params.code_token) * 16 : 0;
-                if (copied > 0) {
-                    cp_async16(dst + i * AT_ONCE * PITCH, kp + o, bytes);
-                    cp_async16(dst + i * AT_ONCE * PITCH + C::CODES, vp + o, bytes);
-                }
+                const unsigned page = (unsigned)__shfl_sync(0xFFFFFFFFu, x.page, i * AT_ONCE + lane / CPR);
+                const uint32_t row = __shfl_sync(0xFFFFFFFFu, in_page, i * AT_ONCE + lane / CPR);
+                const int bytes = (int)page >= 0 ? copied : 0;
+                // (a page that is not there: nothing is read)
+                const uint8_t *src = kp + (unsigned long long)page * params.code_page + row;
+                cp_async16(dst + i * AT_ONCE * PITCH, src, bytes);
+                cp_async16(dst + i * AT_ONCE * PITCH + C::CODES, src + v_past_k, bytes);
             }
         };
         // key l's pairs of a step into registers
@@ -265,20 +278,16 @@ __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_k
 #pragma unroll
         for (int it = 0; it < STAGES; ++it) at[it] = fetch(it);
 #pragma unroll
-        for (int it = 0; it < STAGES; ++it) at[it] = checked(it, at[it]);
-#pragma unroll
         for (int it = 0; it < STAGES - 1; ++it) {
+            at[it] = checked(it, at[it]);
             if (it < tiles) load_stage(it, at[it]);
             cp_async_commit();
         }
         load_pairs(at[0]);
-        // fragments of Q (row 8 nb + g4, channels 32 i + 8 t4 .. + 7 in Key's order), times a power of two; what
-        // rows 2 t4 and 2 t4 + 1 need: that power's inverse times the scale, the groups' sums
-        uint32_t qh[DP / 32][NB][4], ql[C::F32 ? DP / 32 : 1][NB][4];
-        float rs[NB][2], qs[NB][2][GS];
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            const int row = row0 + 8 * nb + g4;
+        // Fragments of Q (row 8 nb + g4, channels 32 i + 8 t4 .. + 7 in KCodes's order), times a power of two, left in
+        // shared memory by warp nb: in registers they cost a fifth more instructions
+        if (warp < NB) {
+            const int nb = warp, row = row0 + 8 * nb + g4;
             const T *q = static_cast<const T *>(p.q) + (long long)(seq.start + row / p.group) * p.q_ts +
                          (long long)(kh * p.group + row % p.group) * p.q_hs;
             float top = 0.0f;
@@ -306,35 +315,38 @@ __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_k
             int up = e == 0 || e == 255 ? 0 : (C::F32 ? 13 : 8) + 127 - e;
             up = max(min(up, 126), -126);
             const float f = __uint_as_float((uint32_t)(127 + up) << 23);
-            const float scale = p.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
             float sum[GS];
 #pragma unroll
             for (int x = 0; x < GS; ++x) sum[x] = 0.0f;
 #pragma unroll
             for (int i = 0; i < DP / 32; ++i) {
+                uint32_t h[4], l[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const float a = to_f(raw[i].e[KCodes::channel(k, 0)]) * f, c = to_f(raw[i].e[KCodes::channel(k, 1)]) * f;
-                    qh[i][nb][k] = pack2<__half>(a, c);
-                    if constexpr (C::F32) {
-                        const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&qh[i][nb][k]));
-                        ql[i][nb][k] = pack2<__half>(a - h.x, c - h.y);
-                    }
+                    h[k] = pack2<__half>(a, c);
+                    const float2 hf = __half22float2(*reinterpret_cast<const __half2 *>(&h[k]));
+                    l[k] = pack2<__half>(a - hf.x, c - hf.y);
                     sum[C::ONE ? 0 : i / 2] += a + c;
                 }
+                q_upper[(nb * (DP / 32) + i) * 32] = make_uint4(h[0], h[1], h[2], h[3]);
+                if constexpr (C::F32) q_lower[(nb * (DP / 32) + i) * 32] = make_uint4(l[0], l[1], l[2], l[3]);
             }
-            rs[nb][0] = __shfl_sync(0xFFFFFFFFu, scale, 8 * t4);
-            rs[nb][1] = __shfl_sync(0xFFFFFFFFu, scale, 8 * t4 + 4);
 #pragma unroll
             for (int x = 0; x < GS; ++x) {
                 sum[x] += __shfl_xor_sync(0xFFFFFFFFu, sum[x], 1);
                 sum[x] += __shfl_xor_sync(0xFFFFFFFFu, sum[x], 2);
-                qs[nb][0][x] = __shfl_sync(0xFFFFFFFFu, sum[x], 8 * t4);
-                qs[nb][1][x] = __shfl_sync(0xFFFFFFFFu, sum[x], 8 * t4 + 4);
+                if (t4 == 0) row_sum[8 * nb + g4][x] = sum[x] * KCodes::UNIT;  // scores are made in units of UNIT
+            }
+            if (t4 == 0) {
+                row_scale[8 * nb + g4] = p.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23) * (1.0f / KCodes::UNIT);
+                row_sees[8 * nb + g4] = row_range(p, seq, row);
             }
         }
-        RowRange see[NB][2];
-        float o[SLABS][4][NB][4], off[NB][2][GS], m[NB][2], l[NB][2], top_scale[GS];
+        __syncthreads();
+        // what rows 2 t4 and 2 t4 + 1 need
+        float rs[NB][2], qs[NB][2][GS];
+        float o[SLABS][4][NB][4], off[NB][2][GS], ref[NB][2], l[NB][2], top_scale[GS];
 #pragma unroll
         for (int x = 0; x < GS; ++x) top_scale[x] = 1.0f / 16777216.0f;  // the least scale that half has
 #pragma unroll
@@ -349,11 +361,14 @@ __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_k
         for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                see[nb][e] = row_range(p, seq, row0 + 8 * nb + 2 * t4 + e);
-                m[nb][e] = -INFINITY;
+                rs[nb][e] = row_scale[8 * nb + 2 * t4 + e];
+                ref[nb][e] = FRESH;  // LIFT less the reference
                 l[nb][e] = 0.0f;
 #pragma unroll
-                for (int x = 0; x < GS; ++x) off[nb][e][x] = 0.0f;
+                for (int x = 0; x < GS; ++x) {
+                    qs[nb][e][x] = row_sum[8 * nb + 2 * t4 + e][x];
+                    off[nb][e][x] = 0.0f;
+                }
             }
         }
 
@@ -361,6 +376,8 @@ __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_k
             cp_async_wait<STAGES - 2>();
             __syncwarp();
             // (the slot's last readers were this warp's lanes, a step ago)
+            // the page looked up in the last step is first looked at here
+            at[STAGES - 1] = checked(it + STAGES - 1, at[STAGES - 1]);
             if (it + STAGES - 1 < tiles) load_stage(it + STAGES - 1, at[STAGES - 1]);
             cp_async_commit();
             const int j0 = k_lo + it * BN + warp * KW;
@@ -368,13 +385,15 @@ __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_k
             const Place next = fetch(it + STAGES);
             // key l's scales: K's, and V's relative to S, a power of two at or above all so far (scales that are
             // not finite make their own NaN)
+            bool odd = false;
 #pragma unroll
             for (int x = 0; x < GS; ++x) {
                 float2 k = __half22float2(*reinterpret_cast<const __half2 *>(&kraw[x]));
                 float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&vraw[x]));
-                const uint32_t mine = __float_as_uint(v.x) & 0x7FFFFFFFu;
-                const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, mine < 0x7F800000u ? mine : 0u);
-                if (most > __float_as_uint(top_scale[x])) {
+                odd = odd || fmaf(v.x, 0.0f, v.y * 0.0f) != 0.0f;
+                const float mine = fabsf(v.x) < INFINITY ? fabsf(v.x) : 0.0f;
+                if (__any_sync(0xFFFFFFFFu, mine > top_scale[x])) {
+                    const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(mine));
                     const float now = __uint_as_float((most + 0x7FFFFFu) & 0xFF800000u), ratio = top_scale[x] / now;
                     top_scale[x] = now;
 #pragma unroll
@@ -390,7 +409,6 @@ __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_k
                     }
                 }
                 k.y = fmaf(KCodes::MID, k.x, k.y);
-                k.x *= 1.0f / KCodes::UNIT;
                 v.y = fmaf(VCodes::MID, v.x, v.y);
                 v.x *= __uint_as_float((254u << 23) - __float_as_uint(top_scale[x]));  // 1 / S, S from 2^-24 to 2^16
                 kpair[lane * GS + x] = k;
@@ -400,26 +418,25 @@ __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_k
             load_pairs(at[1]);
 #pragma unroll
             for (int x = 0; x + 1 < STAGES; ++x) at[x] = at[x + 1];
-            at[STAGES - 1] = checked(it + STAGES, next);
+            at[STAGES - 1] = next;
             __syncwarp();
             if (j0 >= k_hi) continue;
             const uint8_t *st = ring + (it % STAGES) * C::STAGE;
             const int k_at = key0 * PITCH + t4 * BITS;
 
             // ---- scores ----
-            float s[2][NB][4];
+            float s[2][NB][4], acc[2][NB][4];
+            // (channels past the head width: whatever is there is finite and the query has zeros)
 #pragma unroll
-            for (int mt = 0; mt < 2; ++mt) {
-                const int ra = 16 * mt + key0, rb = ra + 8;
-                float acc[NB][4];
+            for (int i = 0; i < DP / 32; ++i) {
+                uint4 qh[NB], ql[NB];
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[nb][e] = s[mt][nb][e] = 0.0f;
+                    qh[nb] = q_upper[(nb * (DP / 32) + i) * 32];
+                    if constexpr (C::F32) ql[nb] = q_lower[(nb * (DP / 32) + i) * 32];
                 }
-                // (channels past the head width: whatever is there is finite and the query has zeros)
 #pragma unroll
-                for (int i = 0; i < DP / 32; ++i) {
+                for (int mt = 0; mt < 2; ++mt) {
                     KCodes a, c;  // channels 32 i + 8 t4: BITS bytes a lane
                     a.load(st + k_at + 16 * mt * PITCH + i * 4 * BITS);
                     c.load(st + k_at + (16 * mt + 8) * PITCH + i * 4 * BITS);
@@ -429,31 +446,31 @@ __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_k
                     const uint32_t a0[4] = {ha[0], hc[0], ha[1], hc[1]}, a1[4] = {ha[2], hc[2], ha[3], hc[3]};
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
-                        mma16<__half>(acc[nb], a0, qh[i][nb][0], qh[i][nb][1]);
-                        mma16<__half>(acc[nb], a1, qh[i][nb][2], qh[i][nb][3]);
+                        // (the first of a group; fp32 calls add up every 64 channels, as the instruction truncates its sums)
+                        if (i == 0 || (!(i & 1) && (!C::ONE || C::F32))) mma16_first(acc[mt][nb], a0, qh[nb].x, qh[nb].y);
+                        else mma16<__half>(acc[mt][nb], a0, qh[nb].x, qh[nb].y);
+                        mma16<__half>(acc[mt][nb], a1, qh[nb].z, qh[nb].w);
                         if constexpr (C::F32) {
-                            mma16<__half>(acc[nb], a0, ql[i][nb][0], ql[i][nb][1]);
-                            mma16<__half>(acc[nb], a1, ql[i][nb][2], ql[i][nb][3]);
+                            mma16<__half>(acc[mt][nb], a0, ql[nb].x, ql[nb].y);
+                            mma16<__half>(acc[mt][nb], a1, ql[nb].z, ql[nb].w);
                         }
                     }
-                    // a group's end (fp32: every 64 channels, the instruction truncates its sums)
-                    const bool ends = i + 1 == DP / 32 || (!C::ONE && (i & 1));
-                    if (ends || (C::F32 && (i & 1))) {
-                        const int x = C::ONE ? 0 : i / 2;
-                        const float2 pa = kpair[ra * GS + x], pb = kpair[rb * GS + x];
+                }
+                const bool ends = i + 1 == DP / 32 || (!C::ONE && (i & 1));
+                if (ends || (C::F32 && (i & 1))) {
+                    const int x = C::ONE ? 0 : i / 2;
+#pragma unroll
+                    for (int mt = 0; mt < 2; ++mt) {
+                        const float2 pa = kpair[(16 * mt + key0) * GS + x], pb = kpair[(16 * mt + key0 + 8) * GS + x];
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb) {
-                            s[mt][nb][0] = fmaf(pa.x, acc[nb][0], s[mt][nb][0]);
-                            s[mt][nb][1] = fmaf(pa.x, acc[nb][1], s[mt][nb][1]);
-                            s[mt][nb][2] = fmaf(pb.x, acc[nb][2], s[mt][nb][2]);
-                            s[mt][nb][3] = fmaf(pb.x, acc[nb][3], s[mt][nb][3]);
-                            if (ends) {
-                                s[mt][nb][0] = fmaf(pa.y, qs[nb][0][x], s[mt][nb][0]);
-                                s[mt][nb][1] = fmaf(pa.y, qs[nb][1][x], s[mt][nb][1]);
-                                s[mt][nb][2] = fmaf(pb.y, qs[nb][0][x], s[mt][nb][2]);
-                                s[mt][nb][3] = fmaf(pb.y, qs[nb][1][x], s[mt][nb][3]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float2 &pair = e < 2 ? pa : pb;
+                                if (i == (C::ONE && !C::F32 ? DP / 32 - 1 : 1)) s[mt][nb][e] = pair.x * acc[mt][nb][e];
+                                else s[mt][nb][e] = fmaf(pair.x, acc[mt][nb][e], s[mt][nb][e]);
+                                if (ends) s[mt][nb][e] = fmaf(pair.y, qs[nb][e & 1][x], s[mt][nb][e]);
                             }
-                            acc[nb][0] = acc[nb][1] = acc[nb][2] = acc[nb][3] = 0.0f;
                         }
                     }
                 }
@@ -470,7 +487,8 @@ __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_k
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int r = 16 * mt + key0 + (e < 2 ? 0 : 8), j = j0 + r;
-                            if (j < see[nb][e & 1].lo || j >= see[nb][e & 1].hi || !(loaded >> r & 1)) {
+                            const RowRange see = row_sees[8 * nb + 2 * t4 + (e & 1)];
+                            if (j < see.lo || j >= see.hi || !(loaded >> r & 1)) {
                                 hidden |= 1u << (8 * nb + 4 * mt + e);
                                 s[mt][nb][e] = -INFINITY;
                             }
@@ -478,55 +496,71 @@ __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_k
                     }
                 }
             }
-            bool moved = false;
-            float fall[NB][2];
+            // exponents; a row whose reference they pass by more than LAZY, or that has none yet
+            float e_[2][NB][4];
+            bool passed = false;
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float x = fmaxf(fmaxf(s[0][nb][e], s[0][nb][e + 2]), fmaxf(s[1][nb][e], s[1][nb][e + 2]));
-                    x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 4));
-                    x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 8));
-                    x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 16));
-                    x = fmaxf(x, m[nb][e]);
-                    // weights 2^(rs s - rs m); nothing seen yet: subtract 0. The products are rounded on their own, so
-                    // that a maximum that stays leaves the row as it is (paged_mma.cuh)
-                    const float y = x == -INFINITY ? 0.0f : __fmul_rn(x, rs[nb][e]);
-                    fall[nb][e] = ex2(__fmul_rn(m[nb][e], rs[nb][e]) - y);
-                    moved = moved || fall[nb][e] != 1.0f;
-                    m[nb][e] = x;
-                    float sum = 0.0f;
 #pragma unroll
                     for (int mt = 0; mt < 2; ++mt) {
-#pragma unroll
-                        for (int k = 0; k < 4; k += 2) {
-                            s[mt][nb][e + k] = ex2(fmaf(s[mt][nb][e + k], rs[nb][e], LIFT - y));
-                            sum += s[mt][nb][e + k];
-                        }
+                        e_[mt][nb][e] = fmaf(s[mt][nb][e], rs[nb][e], ref[nb][e]);
+                        e_[mt][nb][e + 2] = fmaf(s[mt][nb][e + 2], rs[nb][e], ref[nb][e]);
                     }
-                    l[nb][e] = fmaf(l[nb][e], fall[nb][e], sum);
+                    passed = passed || fmaxf(fmaxf(e_[0][nb][e], e_[0][nb][e + 2]), fmaxf(e_[1][nb][e], e_[1][nb][e + 2])) > MOST;
                 }
             }
-            if (__any_sync(0xFFFFFFFFu, moved)) {
+            if (__any_sync(0xFFFFFFFFu, passed)) {
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
+                    float fall[2];
 #pragma unroll
-                    for (int x = 0; x < GS; ++x) {
-                        off[nb][0][x] *= fall[nb][0];
-                        off[nb][1][x] *= fall[nb][1];
+                    for (int e = 0; e < 2; ++e) {
+                        float x = fmaxf(fmaxf(s[0][nb][e], s[0][nb][e + 2]), fmaxf(s[1][nb][e], s[1][nb][e + 2]));
+                        x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 4));
+                        x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 8));
+                        x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 16));
+                        fall[e] = 1.0f;
+                        if (x > -INFINITY && fmaf(x, rs[nb][e], ref[nb][e]) > MOST) {
+                            const float now = LIFT - __fmul_rn(x, rs[nb][e]);
+                            if (ref[nb][e] != FRESH) fall[e] = ex2(now - ref[nb][e]);
+                            ref[nb][e] = now;
+                        }
+                        l[nb][e] *= fall[e];
+#pragma unroll
+                        for (int y = 0; y < GS; ++y) off[nb][e][y] *= fall[e];
+#pragma unroll
+                        for (int mt = 0; mt < 2; ++mt) {
+                            e_[mt][nb][e] = fmaf(s[mt][nb][e], rs[nb][e], ref[nb][e]);
+                            e_[mt][nb][e + 2] = fmaf(s[mt][nb][e + 2], rs[nb][e], ref[nb][e]);
+                        }
                     }
 #pragma unroll
                     for (int x = 0; x < SLABS; ++x) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            o[x][j][nb][0] *= fall[nb][0];
-                            o[x][j][nb][1] *= fall[nb][1];
-                            o[x][j][nb][2] *= fall[nb][0];
-                            o[x][j][nb][3] *= fall[nb][1];
+                            o[x][j][nb][0] *= fall[0];
+                            o[x][j][nb][1] *= fall[1];
+                            o[x][j][nb][2] *= fall[0];
+                            o[x][j][nb][3] *= fall[1];
                         }
                     }
                 }
             }
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[mt][nb][e] = ex2(e_[mt][nb][e]);
+                        l[nb][e & 1] += s[mt][nb][e];
+                    }
+                }
+            }
+            // a scale that is not finite, of a key that some row does not see: 0 times it is left out
+            const bool careful = __any_sync(0xFFFFFFFFu, odd) && !whole;
             // ---- values ----
             uint32_t bh[2][NB][2], bl[C::F32 ? 2 : 1][NB][2];
 #pragma unroll
@@ -540,7 +574,7 @@ __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_k
                         for (int nb = 0; nb < NB; ++nb) {
                             const float (&u)[4] = s[mt][nb];
                             float w[4] = {u[0] * pa.x, u[1] * pa.x, u[2] * pb.x, u[3] * pb.x};
-                            if (hidden) {  // 0 times what is not finite
+                            if (careful) {
                                 const uint32_t hide = hidden >> (8 * nb + 4 * mt);
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
@@ -637,7 +671,7 @@ __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_k
                             make_float2(fmaf(up, o[x][j][nb][e], add), fmaf(up, o[x][j][nb][2 + e], add));
                 }
                 if (g4 == 0) {
-                    sm[r] = __fmul_rn(m[nb][e], rs[nb][e]);
+                    sm[r] = ref[nb][e] == FRESH ? -INFINITY : LIFT - ref[nb][e];
                     sl[r] = l[nb][e];
                 }
             }
