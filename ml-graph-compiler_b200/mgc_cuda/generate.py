@@ -26,7 +26,7 @@ if __package__ in (None, ""):
 import torch  # noqa: E402
 
 from mgc_cuda.native import check, library  # noqa: E402
-from mgc_cuda.paged import check_status, kv_append, paged_attention  # noqa: E402
+from mgc_cuda.paged import Cache, check_status, kv_append, paged_attention, quantized_pages  # noqa: E402
 
 ACT_NONE, ACT_GELU_TANH = 0, 4  # MGC_ACT_*
 FP32, TF32 = 0, 1  # MGC_PREC_*
@@ -65,12 +65,15 @@ class Pages:
 
 
 class Gpt2:
-    """A GPT-2 decoder in fp32 over a paged cache of fp32, float16 or bfloat16."""
+    """A GPT-2 decoder in fp32 over a paged cache of fp32, float16 or bfloat16, or, with ``cache_bits``, of 4 or 8 bits."""
 
     def __init__(self, layers: int = 12, d: int = 768, heads: int = 12, vocab: int = 50257, max_pos: int = 1024, *,
-                 cache_dtype: torch.dtype = torch.float32, precision: int = TF32, seed: int = 3, device: str = "cuda") -> None:
+                 cache_dtype: torch.dtype = torch.float32, cache_bits: int = 0, precision: int = TF32, seed: int = 3,
+                 device: str = "cuda") -> None:
+        if cache_bits and cache_dtype != torch.float32:
+            raise ValueError("a cache is of cache_dtype or of cache_bits")
         self.layers, self.d, self.heads, self.vocab, self.max_pos = layers, d, heads, vocab, max_pos
-        self.cache_dtype, self.precision, self.device = cache_dtype, precision, torch.device(device)
+        self.cache_dtype, self.cache_bits, self.precision, self.device = cache_dtype, cache_bits, precision, torch.device(device)
         self.lib = library()
         g = torch.Generator(device=device).manual_seed(seed)
 
@@ -86,8 +89,11 @@ class Gpt2:
         ]
         self.ln = (1 + normal(d), normal(d))
 
-    def cache(self, pages: int, page_size: int) -> list[tuple[torch.Tensor, torch.Tensor]]:
+    def cache(self, pages: int, page_size: int) -> list[tuple[Cache, Cache]]:
         """(k, v) pages of every layer."""
+        if self.cache_bits:
+            return [tuple(quantized_pages(pages, page_size, self.heads, self.d // self.heads, bits=self.cache_bits, device=self.device)
+                          for _ in range(2)) for _ in range(self.layers)]  # type: ignore[misc]
         shape = (pages, page_size, self.heads, self.d // self.heads)
         return [tuple(torch.empty(shape, dtype=self.cache_dtype, device=self.device) for _ in range(2))  # type: ignore[misc]
                 for _ in range(self.layers)]
@@ -117,7 +123,7 @@ class Gpt2:
                                      1.0, act, 0.0, 0.0, precision, self._stream()), "mgc_cuda_gemm", self.lib)
         return y[:, :n]
 
-    def step(self, ids: torch.Tensor, new: list[int], pages: Pages, cache: list[tuple[torch.Tensor, torch.Tensor]],
+    def step(self, ids: torch.Tensor, new: list[int], pages: Pages, cache: list[tuple[Cache, Cache]],
              status: torch.Tensor | None = None) -> torch.Tensor:
         """``ids`` [sum(new)]: the next ``new[b]`` tokens of every sequence. Caches them and returns the
         logits [batch, vocab] after each sequence's last token (of sequences with new tokens)."""
@@ -132,7 +138,7 @@ class Gpt2:
         for block, (k_cache, v_cache) in zip(self.blocks, cache):
             qkv = self._product(self._norm(x, block["ln1"]), *block["qkv"]).view(tokens, 3 * heads, d // heads)
             q, k, v = qkv[:, :heads], qkv[:, heads : 2 * heads], qkv[:, 2 * heads :]
-            # learned positions: nothing to rotate; q comes back in the cache's type
+            # learned positions: nothing to rotate; q comes back in the cache's type (a quantised one's calls take fp32)
             same = self.cache_dtype == torch.float32
             turned = kv_append(k, v, k_cache, v_cache, *at, q=None if same else q, status=status)
             o = paged_attention(q if same else turned, k_cache, v_cache, *at, max_q=max_q, max_kv=max_kv, status=status)
@@ -202,10 +208,13 @@ def main(argv: list[str] | None = None) -> int:
     ap.add_argument("--tokens", type=int, default=32)
     ap.add_argument("--layers", type=int, default=12)
     ap.add_argument("--page-size", type=int, default=16)
-    ap.add_argument("--cache", choices=["float32", "float16", "bfloat16"], default="float32")
+    ap.add_argument("--cache", choices=["float32", "float16", "bfloat16", "int8", "int4"], default="float32")
     ap.add_argument("--check", action="store_true", help="compare the last logits with a plain computation")
     args = ap.parse_args(argv)
-    model = Gpt2(layers=args.layers, cache_dtype=getattr(torch, args.cache))
+    bits = {"int8": 8, "int4": 4}.get(args.cache, 0)
+    if bits and args.check:
+        ap.error("--check compares with unquantised keys and values")
+    model = Gpt2(layers=args.layers, cache_dtype=torch.float32 if bits else getattr(torch, args.cache), cache_bits=bits)
     g = torch.Generator().manual_seed(0)
     prompts = [torch.randint(model.vocab, (max(1, args.prompt - 7 * b),), generator=g).tolist() for b in range(args.batch)]
     out, seconds, logits = generate(model, prompts, args.tokens, page_size=args.page_size)
