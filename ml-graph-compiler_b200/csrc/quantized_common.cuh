@@ -66,19 +66,20 @@ struct TokenWalk {
     }
 };
 
-// Warps of a launch over packed tokens: each takes a run of consecutive ones, or, when they are few, a part of
-// one token's heads.
+// Warps of a launch over packed tokens: each takes a run of consecutive ones, and, when runs would be shorter than
+// three tokens, a part of the tokens' heads, so that whole runs fill the GPU evenly.
 struct TokenRuns {
     int run, parts;  // tokens of a run; parts of a token's heads
     unsigned blocks;
 };
 inline TokenRuns runs_of(int64_t tokens, int64_t most_parts, int warps, int resident) {
     const int64_t slots = (int64_t)sm_count() * resident * warps;
+    int64_t parts = 1;
+    while (parts < most_parts && ceil_div(tokens * parts, slots) < 3) parts = 2 * parts < most_parts ? 2 * parts : most_parts;
     TokenRuns r;
-    const int64_t parts = slots / tokens;
-    r.parts = (int)(parts < 1 ? 1 : parts > most_parts ? most_parts : parts);
-    r.run = (int)ceil_div(tokens * r.parts, slots);
-    r.blocks = (unsigned)ceil_div(ceil_div(tokens, r.run) * r.parts, warps);
+    r.parts = (int)parts;
+    r.run = (int)ceil_div(tokens * parts, slots);
+    r.blocks = (unsigned)ceil_div(ceil_div(tokens, r.run) * parts, warps);
     return r;
 }
 
