@@ -42,7 +42,10 @@ struct HeadsParams {
     double inv_dim;
 };
 
-constexpr int HEADS_WARPS = 4, HEADS_RESIDENT = 8;
+constexpr int HEADS_WARPS = 4;
+// Blocks of an SM: 64 registers do for 16-bit sources into plain pages (19466 tokens, 48 heads of 128: 121 us, with 80
+// 128 us), the others want 80 (4 bits 154 us, with 64 164 us; fp32 sources of 80 channels 22.8 and 24.8 us).
+template <typename S, int BITS> constexpr int HEADS_RESIDENT = BITS == 0 && sizeof(S) == 2 ? 8 : 6;
 
 // (mean + eps)^-1/2 as fp32. In fp32's range one Newton step from the hardware's root leaves 2^-43, so that
 // the rounding to fp32 is the exact root's but for one case in 2^18.
@@ -110,7 +113,7 @@ template <typename T> __device__ __forceinline__ void store_four(T *dst, const f
 // SEG: lanes of a head where D and rot are multiples of 8 and rows allow accesses of four elements; 0: any other
 // case, p.seg lanes.
 template <typename S, typename T, int BITS, int SEG>
-__global__ void __launch_bounds__(32 * HEADS_WARPS, HEADS_RESIDENT) kv_append_heads_kernel(const __grid_constant__ HeadsParams p) {
+__global__ void __launch_bounds__(32 * HEADS_WARPS, HEADS_RESIDENT<S, BITS>) kv_append_heads_kernel(const __grid_constant__ HeadsParams p) {
     __shared__ __align__(16) float exchange[BITS ? HEADS_WARPS : 1][BITS ? 256 : 4];
     constexpr bool VEC = SEG > 0;
     const int lane = (int)(threadIdx.x & 31), warp = (int)(threadIdx.x >> 5), seg = VEC ? SEG : p.seg;
@@ -360,7 +363,7 @@ __global__ void __launch_bounds__(32 * HEADS_WARPS, HEADS_RESIDENT) kv_append_he
 
 template <typename S, typename T, int BITS> inline int launch_heads(HeadsParams &p, bool vec, cudaStream_t stream) {
     p.seg = p.head_dim <= 64 ? 8 : p.head_dim <= 128 ? 16 : 32;
-    const TokenRuns r = runs_of(p.tokens, ceil_div(p.q_heads, 32 / p.seg) + 2 * ceil_div(p.kv_heads, 32 / p.seg), HEADS_WARPS, HEADS_RESIDENT);
+    const TokenRuns r = runs_of(p.tokens, ceil_div(p.q_heads, 32 / p.seg) + 2 * ceil_div(p.kv_heads, 32 / p.seg), HEADS_WARPS, HEADS_RESIDENT<S, BITS>);
     p.run = r.run;
     p.parts = r.parts;
     p.inv_dim = 1.0 / p.head_dim;

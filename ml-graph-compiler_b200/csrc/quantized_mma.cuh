@@ -336,10 +336,10 @@ __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_k
             for (int x = 0; x < GS; ++x) {
                 sum[x] += __shfl_xor_sync(0xFFFFFFFFu, sum[x], 1);
                 sum[x] += __shfl_xor_sync(0xFFFFFFFFu, sum[x], 2);
-                if (t4 == 0) row_sum[8 * nb + g4][x] = sum[x] * KCodes::UNIT;  // scores are made in units of UNIT
+                if (t4 == 0) row_sum[8 * nb + g4][x] = sum[x];
             }
             if (t4 == 0) {
-                row_scale[8 * nb + g4] = p.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23) * (1.0f / KCodes::UNIT);
+                row_scale[8 * nb + g4] = p.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
                 row_sees[8 * nb + g4] = row_range(p, seq, row);
             }
         }
@@ -409,6 +409,7 @@ __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_k
                     }
                 }
                 k.y = fmaf(KCodes::MID, k.x, k.y);
+                k.x *= 1.0f / KCodes::UNIT;
                 v.y = fmaf(VCodes::MID, v.x, v.y);
                 v.x *= __uint_as_float((254u << 23) - __float_as_uint(top_scale[x]));  // 1 / S, S from 2^-24 to 2^16
                 kpair[lane * GS + x] = k;
@@ -522,8 +523,10 @@ __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_k
                         x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 8));
                         x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 16));
                         fall[e] = 1.0f;
-                        if (x > -INFINITY && fmaf(x, rs[nb][e], ref[nb][e]) > MOST) {
-                            const float now = LIFT - __fmul_rn(x, rs[nb][e]);
+                        // (products rounded on their own: scores past 2^24 would leave the fused one's rest as an exponent)
+                        const float top = __fmul_rn(x, rs[nb][e]);
+                        if (x > -INFINITY && top + ref[nb][e] > MOST) {
+                            const float now = LIFT - top;
                             if (ref[nb][e] != FRESH) fall[e] = ex2(now - ref[nb][e]);
                             ref[nb][e] = now;
                         }
@@ -532,8 +535,8 @@ __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_k
                         for (int y = 0; y < GS; ++y) off[nb][e][y] *= fall[e];
 #pragma unroll
                         for (int mt = 0; mt < 2; ++mt) {
-                            e_[mt][nb][e] = fmaf(s[mt][nb][e], rs[nb][e], ref[nb][e]);
-                            e_[mt][nb][e + 2] = fmaf(s[mt][nb][e + 2], rs[nb][e], ref[nb][e]);
+                            e_[mt][nb][e] = __fmul_rn(s[mt][nb][e], rs[nb][e]) + ref[nb][e];
+                            e_[mt][nb][e + 2] = __fmul_rn(s[mt][nb][e + 2], rs[nb][e]) + ref[nb][e];
                         }
                     }
 #pragma unroll

@@ -135,7 +135,8 @@ def kv_append(
 
     Over a quantised cache they are of one type, that of ``q_out`` too. A group of channels takes its least
     value as the offset and its range over 2^bits - 1 as the scale, rounded to float16 (values past +-65504 are
-    held there), and the nearest codes; one that is not finite makes its group read as NaN."""
+    held there), and the nearest codes; one that is not finite makes its group read as NaN. No two new tokens may
+    have the same place in the cache: one's codes could meet the other's scale."""
     return (_EXT or _binding()).kv_append(k, v, k_cache, v_cache, block_table, kv_lens, q_starts, q, cos, sin, interleaved,
                                           q_out, status, q_norm, k_norm, eps)
 

@@ -390,6 +390,42 @@ def test_rows_of_q_starts_that_q_does_not_have() -> None:
 
 
 @pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("qs,ks", [([1, 1], [9000, 40]), ([200, 3], [900, 40])])
+def test_outputs_at_odd_elements(dtype, qs, ks) -> None:
+    """Rows of out that allow single elements only, keys that would be cut into pieces."""
+    x = QuantizedBatch(qs, ks, heads=4, kv_heads=2, dim=64, page=16, dtype=dtype, bits=4)
+    room = torch.full((sum(qs), 4, 67), 5.0, dtype=x.q.dtype, device="cuda")
+    out = room[..., 1:65]
+    assert paged.paged_attention(x.q, *x.operands, max_q=max(qs), max_kv=max(ks), out=out) is out
+    compare(out, *attention(x, 64**-0.5))
+    assert bool((room[..., 0] == 5.0).all()) and bool((room[..., 65:] == 5.0).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_queries_of_every_size(dtype, bits) -> None:
+    """Rows of queries from 1e-30 to 1e30, the softmax flat or on one key: half's range does not show."""
+    for qs, ks in (([6], [50]), ([120], [300])):
+        x = QuantizedBatch(qs, ks, heads=2, kv_heads=1, dim=64, page=16, dtype=dtype, bits=bits)
+        size = torch.tensor([1e-30, 1e-6, 1.0, 1e5, 1e20, 1e30], device="cuda").repeat(qs[0] // 6)[:, None, None]
+        x.q = (x.q.float() * size).to(x.q.dtype)
+        got = attend(x)
+        want, _ = attention(x, 64**-0.5)
+        # one key's weight is 1 to rounding for the large rows, all weights are equal to 1e-5 for the small ones; those
+        # in between have the ordinary bound
+        plain, bound = attention(x, 64**-0.5)
+        rows = size[:, 0, 0].reshape(-1)
+        middle = (rows > 1e-7) & (rows < 1e3)
+        compare(got[middle], plain[middle], bound[middle])
+        flat, peak = rows < 1e-7, rows > 1e3
+        v = values(x.v.codes[x.slots[0]], x.v.scales[x.slots[0]], bits)
+        most = float(v.abs().max())
+        r = ROUND[dtype]
+        assert float((got[flat].double() - want[flat]).abs().max()) <= most * (4 * r + 1e-5)
+        assert float((got[peak].double() - want[peak]).abs().max()) <= most * (4 * r + 1e-5)
+
+
+@pytest.mark.parametrize("dtype", ALL)
 @pytest.mark.parametrize("bits", [4, 8])
 def test_long_contexts(dtype, bits) -> None:
     agree(QuantizedBatch([1], [30011], heads=8, kv_heads=2, dim=128, page=64, dtype=dtype, bits=bits, spread=1.5))
