@@ -261,6 +261,10 @@ inline int attend_quantized(const mgc_cuda_paged_attention_quantized_args &a, cu
         p.a.cut = reinterpret_cast<CutUnit *>(p.a.part_ml + rows);
     }
     const int chunk = 16 / elem_size(c.dtype);
+    p.slabs = (int)ceil_div(c.head_dim, 64);
+    for (int x = 0; x < 4; ++x) p.group_of[x] = 64 * x < p.a.head_dim ? 64 * x / p.z.group : 0;
+    p.pairs_wide = p.z.groups == 2 && c.head_dim == 128 && aligned(p.z.k_scales, 8) && aligned(p.z.v_scales, 8) &&
+                   p.z.page_stride % 2 == 0 && p.z.token_stride % 2 == 0 && p.z.head_stride % 2 == 0;
     p.q_wide = aligned(b.q, 16) && b.q_token_stride % chunk == 0 && b.q_head_stride % chunk == 0;
     return with_config(c.dtype, a.quantized, c.head_dim, s.nb, [&](auto config) { return launch_quantized(p, s, config, stream); });
 }

@@ -175,6 +175,8 @@ struct QuantParams {
     QuantAttend a;
     Quantized z;
     int q_wide;             // rows of q allow 16-byte loads
+    int pairs_wide;         // two groups, whose pairs allow 8-byte loads
+    int slabs, group_of[4]; // of 64 channels; their groups
     uint32_t page_magic;    // j / page_size = j * page_magic >> page_shift for 0 <= j < 2^31
     int page_shift;
     // strides that fit 32 bits: of codes in bytes, of scales in pairs
@@ -262,13 +264,23 @@ __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_k
         uint32_t kraw[GS], vraw[GS];
         auto load_pairs = [&](Place x) {
             const unsigned long long o = (unsigned long long)(unsigned)x.page * params.pair_page + (uint32_t)x.row * params.pair_token;
+            const unsigned int *k = reinterpret_cast<const unsigned int *>(ksp + o), *v = reinterpret_cast<const unsigned int *>(vsp + o);
 #pragma unroll
-            for (int s = 0; s < GS; ++s) {
-                kraw[s] = vraw[s] = 0u;
-                const int g = GS == 1 ? 0 : 64 * s / z.group;
-                if (x.page >= 0 && 64 * s < p.head_dim) {
-                    kraw[s] = __ldg(reinterpret_cast<const unsigned int *>(ksp + o + g));
-                    vraw[s] = __ldg(reinterpret_cast<const unsigned int *>(vsp + o + g));
+            for (int s = 0; s < GS; ++s) kraw[s] = vraw[s] = 0u;
+            if (x.page >= 0) {
+                if (GS == 2 && params.pairs_wide) {
+                    const uint2 a = __ldg(reinterpret_cast<const uint2 *>(k)), b = __ldg(reinterpret_cast<const uint2 *>(v));
+                    kraw[0] = a.x;
+                    kraw[GS - 1] = a.y;
+                    vraw[0] = b.x;
+                    vraw[GS - 1] = b.y;
+                } else {
+#pragma unroll
+                    for (int s = 0; s < GS; ++s) {
+                        if (s >= params.slabs) break;
+                        kraw[s] = __ldg(k + params.group_of[s]);
+                        vraw[s] = __ldg(v + params.group_of[s]);
+                    }
                 }
             }
         };
@@ -565,87 +577,93 @@ __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_k
             // a scale that is not finite, of a key that some row does not see: 0 times it is left out
             const bool careful = __any_sync(0xFFFFFFFFu, odd) && !whole;
             // ---- values ----
-            uint32_t bh[2][NB][2], bl[C::F32 ? 2 : 1][NB][2];
+            // CAREFUL: hidden weights leave out what they would be multiplied by
+            auto values = [&](auto careful_) {
+                constexpr bool CAREFUL = decltype(careful_)::value;
+                uint32_t bh[2][NB][2], bl[C::F32 ? 2 : 1][NB][2];
 #pragma unroll
-            for (int x = 0; x < SLABS; ++x) {
-                if (x == 0 || !C::ONE) {  // a group's weights
-                    const int y = C::ONE ? 0 : x;
+                for (int x = 0; x < SLABS; ++x) {
+                    if (x == 0 || !C::ONE) {  // a group's weights
+                        const int y = C::ONE ? 0 : x;
+#pragma unroll
+                        for (int mt = 0; mt < 2; ++mt) {
+                            const float2 pa = vpair[(16 * mt + key0) * GS + y], pb = vpair[(16 * mt + key0 + 8) * GS + y];
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb) {
+                                const float (&u)[4] = s[mt][nb];
+                                float w[4] = {u[0] * pa.x, u[1] * pa.x, u[2] * pb.x, u[3] * pb.x};
+                                if constexpr (CAREFUL) {
+                                    const uint32_t hide = hidden >> (8 * nb + 4 * mt);
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) {
+                                        w[e] = hide >> e & 1 ? 0.0f : w[e];
+                                        off[nb][e & 1][y] += hide >> e & 1 ? 0.0f : u[e] * (e < 2 ? pa.y : pb.y);
+                                    }
+                                } else {
+                                    off[nb][0][y] = fmaf(u[0], pa.y, fmaf(u[2], pb.y, off[nb][0][y]));
+                                    off[nb][1][y] = fmaf(u[1], pa.y, fmaf(u[3], pb.y, off[nb][1][y]));
+                                }
+                                const uint32_t h0 = pack2<__half>(w[0], w[1]), h1 = pack2<__half>(w[2], w[3]);
+                                bh[mt][nb][0] = movmatrix(h0);
+                                bh[mt][nb][1] = movmatrix(h1);
+                                if constexpr (C::F32) {
+                                    const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&h0));
+                                    const float2 f1 = __half22float2(*reinterpret_cast<const __half2 *>(&h1));
+                                    bl[mt][nb][0] = movmatrix(pack2<__half>(w[0] - f0.x, w[1] - f0.y));
+                                    bl[mt][nb][1] = movmatrix(pack2<__half>(w[2] - f1.x, w[3] - f1.y));
+                                }
+                            }
+                        }
+                    }
+                    float sum[C::F32 ? 4 : 1][NB][4];
+                    if constexpr (C::F32) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb) sum[j][nb][0] = sum[j][nb][1] = sum[j][nb][2] = sum[j][nb][3] = 0.0f;
+                        }
+                    }
 #pragma unroll
                     for (int mt = 0; mt < 2; ++mt) {
-                        const float2 pa = vpair[(16 * mt + key0) * GS + y], pb = vpair[(16 * mt + key0 + 8) * GS + y];
+                        // eight channels from 64 x + 8 g4 on of four keys: BITS bytes a lane
+                        VCodes key[4];
 #pragma unroll
-                        for (int nb = 0; nb < NB; ++nb) {
-                            const float (&u)[4] = s[mt][nb];
-                            float w[4] = {u[0] * pa.x, u[1] * pa.x, u[2] * pb.x, u[3] * pb.x};
-                            if (careful) {
-                                const uint32_t hide = hidden >> (8 * nb + 4 * mt);
+                        for (int k = 0; k < 4; ++k)
+                            key[k].load(st + C::CODES + (k & 1 ? C::second(t4) : C::first(t4)) * PITCH + g4 * BITS + (16 * mt + 8 * (k >> 1)) * PITCH + x * 8 * BITS);
+                        auto tile = [&](auto index) {
+                            constexpr int J = decltype(index)::value;
+                            uint32_t a[4];
+                            VCodes::template two_rows<J>(key[0], key[1], a[0], a[1]);
+                            VCodes::template two_rows<J>(key[2], key[3], a[2], a[3]);
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    w[e] = hide >> e & 1 ? 0.0f : w[e];
-                                    off[nb][e & 1][y] += hide >> e & 1 ? 0.0f : u[e] * (e < 2 ? pa.y : pb.y);
+                            for (int nb = 0; nb < NB; ++nb) {
+                                if constexpr (C::F32) {
+                                    mma16<__half>(sum[J][nb], a, bh[mt][nb][0], bh[mt][nb][1]);
+                                    mma16<__half>(sum[J][nb], a, bl[mt][nb][0], bl[mt][nb][1]);
+                                } else {
+                                    mma16<__half>(o[x][J][nb], a, bh[mt][nb][0], bh[mt][nb][1]);
                                 }
-                            } else {
-                                off[nb][0][y] = fmaf(u[0], pa.y, fmaf(u[2], pb.y, off[nb][0][y]));
-                                off[nb][1][y] = fmaf(u[1], pa.y, fmaf(u[3], pb.y, off[nb][1][y]));
                             }
-                            const uint32_t h0 = pack2<__half>(w[0], w[1]), h1 = pack2<__half>(w[2], w[3]);
-                            bh[mt][nb][0] = movmatrix(h0);
-                            bh[mt][nb][1] = movmatrix(h1);
-                            if constexpr (C::F32) {
-                                const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&h0));
-                                const float2 f1 = __half22float2(*reinterpret_cast<const __half2 *>(&h1));
-                                bl[mt][nb][0] = movmatrix(pack2<__half>(w[0] - f0.x, w[1] - f0.y));
-                                bl[mt][nb][1] = movmatrix(pack2<__half>(w[2] - f1.x, w[3] - f1.y));
+                        };
+                        tile(std::integral_constant<int, 0>());
+                        tile(std::integral_constant<int, 1>());
+                        tile(std::integral_constant<int, 2>());
+                        tile(std::integral_constant<int, 3>());
+                    }
+                    if constexpr (C::F32) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) o[x][j][nb][e] += sum[j][nb][e];
                             }
                         }
                     }
                 }
-                float sum[C::F32 ? 4 : 1][NB][4];
-                if constexpr (C::F32) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-#pragma unroll
-                        for (int nb = 0; nb < NB; ++nb) sum[j][nb][0] = sum[j][nb][1] = sum[j][nb][2] = sum[j][nb][3] = 0.0f;
-                    }
-                }
-#pragma unroll
-                for (int mt = 0; mt < 2; ++mt) {
-                    // eight channels from 64 x + 8 g4 on of four keys: BITS bytes a lane
-                    VCodes key[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        key[k].load(st + C::CODES + (k & 1 ? C::second(t4) : C::first(t4)) * PITCH + g4 * BITS + (16 * mt + 8 * (k >> 1)) * PITCH + x * 8 * BITS);
-                    auto tile = [&](auto index) {
-                        constexpr int J = decltype(index)::value;
-                        uint32_t a[4];
-                        VCodes::template two_rows<J>(key[0], key[1], a[0], a[1]);
-                        VCodes::template two_rows<J>(key[2], key[3], a[2], a[3]);
-#pragma unroll
-                        for (int nb = 0; nb < NB; ++nb) {
-                            if constexpr (C::F32) {
-                                mma16<__half>(sum[J][nb], a, bh[mt][nb][0], bh[mt][nb][1]);
-                                mma16<__half>(sum[J][nb], a, bl[mt][nb][0], bl[mt][nb][1]);
-                            } else {
-                                mma16<__half>(o[x][J][nb], a, bh[mt][nb][0], bh[mt][nb][1]);
-                            }
-                        }
-                    };
-                    tile(std::integral_constant<int, 0>());
-                    tile(std::integral_constant<int, 1>());
-                    tile(std::integral_constant<int, 2>());
-                    tile(std::integral_constant<int, 3>());
-                }
-                if constexpr (C::F32) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-#pragma unroll
-                        for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) o[x][j][nb][e] += sum[j][nb][e];
-                        }
-                    }
-                }
-            }
+            };
+            if (careful) values(std::true_type());
+            else values(std::false_type());
         }
         if (missing && p.batch.status) *p.batch.status = MGC_CUDA_GATHER_OOB;
         cp_async_wait<0>();
