@@ -94,16 +94,6 @@ template <int BITS> __device__ __forceinline__ uint2 encode(const float (&x)[8],
     return make_uint2(code[0], code[1]);
 }
 
-// Two values of a 16-bit type at once.
-template <typename T> __device__ __forceinline__ uint32_t two(float x, float y);
-template <> __device__ __forceinline__ uint32_t two<__half>(float x, float y) {
-    const __half2 v = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t *>(&v);
-}
-template <> __device__ __forceinline__ uint32_t two<__nv_bfloat16>(float x, float y) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
-    return *reinterpret_cast<const uint32_t *>(&v);
-}
 // Four values in a row.
 template <typename T> __device__ __forceinline__ void store_four(T *dst, const float *x) {
     if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(dst) = make_float4(x[0], x[1], x[2], x[3]);

@@ -20,19 +20,30 @@ struct ReadParams {
     int tokens, run, parts;
 };
 
-// Eight consecutive codes as they are stored, and as floats: put into the mantissa of 2^23, which comes off
-// exactly (a conversion instruction takes a quarter of the rate).
+// Eight consecutive codes as they are stored, and as the floats scale * code + offset. A code is put into the
+// mantissa of 2^23, which comes off exactly (a conversion instruction takes a quarter of the rate); a nibble further up
+// stays there, 16^k times as large, and the scale is as much smaller: the product is the same.
 template <int BITS> struct EightCodes;
 template <> struct EightCodes<4> {
     uint32_t w;
     __device__ __forceinline__ void load(const uint8_t *p) { w = __ldg(reinterpret_cast<const unsigned int *>(p)); }
-    __device__ __forceinline__ float operator[](int i) const { return __uint_as_float((w >> 4 * i & 15u) | 0x4B000000u) - 8388608.0f; }
+    __device__ __forceinline__ void values(float2 so, float (&x)[8]) const {
+        const uint32_t up = w >> 16;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int k = i & 3;
+            const float code = __uint_as_float(((i < 4 ? w : up) & 15u << 4 * k) | 0x4B000000u) - 8388608.0f;
+            x[i] = fmaf(k == 0 ? so.x : k == 1 ? so.x * 0.0625f : k == 2 ? so.x * 0.00390625f : so.x * 0.000244140625f, code, so.y);
+        }
+    }
 };
 template <> struct EightCodes<8> {
     uint2 w;
     __device__ __forceinline__ void load(const uint8_t *p) { w = __ldg(reinterpret_cast<const uint2 *>(p)); }
-    __device__ __forceinline__ float operator[](int i) const {
-        return __uint_as_float(__byte_perm(i < 4 ? w.x : w.y, 0x4B000000u, 0x7650 | (i & 3))) - 8388608.0f;
+    __device__ __forceinline__ void values(float2 so, float (&x)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            x[i] = fmaf(so.x, __uint_as_float(__byte_perm(i < 4 ? w.x : w.y, 0x4B000000u, 0x7650 | (i & 3))) - 8388608.0f, so.y);
     }
 };
 
@@ -50,13 +61,32 @@ __global__ void __launch_bounds__(32 * READ_WARPS, READ_RESIDENT) kv_read_kernel
     const int h0 = part * at_once + lane / p.seg, step = p.parts * at_once;
     const bool mine = 8 * sl < p.head_dim;
     const int group = 8 * sl / p.z.group;
+    auto put = [&](T *dst, const EightCodes<BITS> &c, __half2 pair) {
+        float x[8];
+        c.values(__half22float2(pair), x);
+        if constexpr (VEC) {
+            if constexpr (sizeof(T) == 2) {
+                *reinterpret_cast<uint4 *>(dst) = make_uint4(two<T>(x[0], x[1]), two<T>(x[2], x[3]), two<T>(x[4], x[5]), two<T>(x[6], x[7]));
+            } else {
+                *reinterpret_cast<float4 *>(dst) = make_float4(x[0], x[1], x[2], x[3]);
+                *reinterpret_cast<float4 *>(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dst[e] = from_f<T>(x[e]);
+        }
+    };
     TokenWalk walk;
     walk.start(t0);
     for (int t = t0; t < t1; ++t) {
         walk.step(p.batch, t);
         const bool there = walk.page >= 0;
-        const long long codes = there ? walk.at(p.page_stride, p.token_stride) + sl * BITS : 0;
-        const long long pairs = there ? walk.at(p.z.page_stride, p.z.token_stride) + group : 0;
+        const long long codes = (there ? walk.at(p.page_stride, p.token_stride) : 0) + h0 * p.head_stride + sl * BITS;
+        const long long pairs = (there ? walk.at(p.z.page_stride, p.z.token_stride) : 0) + h0 * p.z.head_stride + group;
+        const uint8_t *k = p.k_pages + codes, *v = p.v_pages + codes;
+        const __half2 *ks = p.z.k_scales + pairs, *vs = p.z.v_scales + pairs;
+        T *k_dst = static_cast<T *>(p.k_out) + (long long)t * p.k_ts + h0 * p.k_hs + 8 * sl;
+        T *v_dst = static_cast<T *>(p.v_out) + (long long)t * p.v_ts + h0 * p.v_hs + 8 * sl;
         // two heads' keys and values in flight
         constexpr int BATCH = 2;
         for (int h = h0; h - lane / p.seg < p.kv_heads; h += BATCH * step) {
@@ -64,34 +94,27 @@ __global__ void __launch_bounds__(32 * READ_WARPS, READ_RESIDENT) kv_read_kernel
             __half2 so[BATCH][2];
 #pragma unroll
             for (int i = 0; i < BATCH; ++i) {
-                const int kh = h + i * step;
                 so[i][0] = so[i][1] = __floats2half2_rn(0.0f, 0.0f);
                 c[i][0] = c[i][1] = EightCodes<BITS>{};
-                if (there && mine && kh < p.kv_heads) {
-                    c[i][0].load(p.k_pages + codes + kh * p.head_stride);
-                    c[i][1].load(p.v_pages + codes + kh * p.head_stride);
-                    so[i][0] = __ldg(p.z.k_scales + pairs + kh * p.z.head_stride);
-                    so[i][1] = __ldg(p.z.v_scales + pairs + kh * p.z.head_stride);
+                if (there && mine && h + i * step < p.kv_heads) {
+                    c[i][0].load(k);
+                    c[i][1].load(v);
+                    so[i][0] = __ldg(ks);
+                    so[i][1] = __ldg(vs);
                 }
+                k += step * p.head_stride;
+                v += step * p.head_stride;
+                ks += step * p.z.head_stride;
+                vs += step * p.z.head_stride;
             }
 #pragma unroll
             for (int i = 0; i < BATCH; ++i) {
-                const int kh = h + i * step;
-                if (!mine || kh >= p.kv_heads) continue;
-#pragma unroll
-                for (int v = 0; v < 2; ++v) {
-                    const float2 s = __half22float2(so[i][v]);
-                    Pack<8, T> y;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) y.e[e] = from_f<T>(fmaf(s.x, c[i][v][e], s.y));
-                    T *dst = static_cast<T *>(v ? p.v_out : p.k_out) + t * (v ? p.v_ts : p.k_ts) + kh * (v ? p.v_hs : p.k_hs) + 8 * sl;
-                    if constexpr (VEC) {
-                        y.store(dst);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) dst[e] = y.e[e];
-                    }
+                if (mine && h + i * step < p.kv_heads) {
+                    put(k_dst, c[i][0], so[i][0]);
+                    put(v_dst, c[i][1], so[i][1]);
                 }
+                k_dst += step * p.k_hs;
+                v_dst += step * p.v_hs;
             }
         }
     }

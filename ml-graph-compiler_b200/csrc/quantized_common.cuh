@@ -17,6 +17,16 @@
 namespace mgc {
 namespace paged {
 
+// Two values of a 16-bit type at once.
+template <typename T> __device__ __forceinline__ uint32_t two(float x, float y);
+template <> __device__ __forceinline__ uint32_t two<__half>(float x, float y) {
+    const __half2 v = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <> __device__ __forceinline__ uint32_t two<__nv_bfloat16>(float x, float y) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
 struct Quantized {
     const __half2 *k_scales, *v_scales;
     long long page_stride, token_stride, head_stride;  // pairs
