@@ -15,6 +15,11 @@
 //
 // Codes: the quotient by the group's scale is taken as a product with its inverse, and only where that lies next to
 // the border between two codes (one value in some thousand) as the definition's division.
+//
+// 19466 tokens of 48 heads x 128 in bf16, normalised and rotated: 121 us into plain pages (478 MB, 4.0 TB/s, 61 % of the
+// copy bandwidth), 153 us into 4-bit ones (2.5 TB/s). Issue bounds it: some 160 instructions for two heads' 256
+// values, 90 of them the norm's (sums in fp64), 300 where codes are made; the SMs issue in 62 % of their cycles.
+// Tried: 64 and 96 registers (HEADS_RESIDENT), one loop over all kinds of heads (twice the instructions).
 #pragma once
 
 #include <type_traits>
