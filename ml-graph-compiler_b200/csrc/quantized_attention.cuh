@@ -104,7 +104,8 @@ inline QuantPlan quant_plan_of(const mgc_cuda_paged_attention_quantized_args &a)
     s.row_tiles = (int)ceil_div(rows, unit_rows);
     s.live_rows = (int)(rows < unit_rows ? rows : unit_rows);
     const int64_t units = c.batch * c.kv_heads * s.row_tiles;
-    int64_t most = a.attention.max_kv;
+    const int64_t capacity = c.table_pages * c.page_size;
+    int64_t most = a.attention.max_kv < capacity ? a.attention.max_kv : capacity;
     if (a.attention.window > 0 && a.attention.window + max_q < most) most = a.attention.window + max_q;
     // the kernel that adds pieces stores four elements at once
     const int es = elem_size(c.dtype);
@@ -139,7 +140,6 @@ inline QuantPlan quant_plan_of(const mgc_cuda_paged_attention_quantized_args &a)
     int64_t page = c.page_size;
     if (page % 128 == 0) page = 128;
     else if (page % 8 == 0) page &= -page;
-    const int64_t capacity = c.table_pages * c.page_size;
     const int64_t longest = a.attention.max_kv < capacity ? (a.attention.max_kv < 1 ? 1 : a.attention.max_kv) : capacity;
     const int64_t per_seq = ceil_div(longest, page);
     const int64_t head_bytes = c.batch * per_seq * page * c.head_dim * es;

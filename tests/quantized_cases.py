@@ -3,13 +3,16 @@ definition in 64 bits with the error that a kernel is allowed."""
 
 from __future__ import annotations
 
+import copy
 import math
+import struct
 
 import numpy as np
 import torch
 
 from paged_cases import DTYPES, ROUND
 
+from mgc_cuda.native import library
 from mgc_cuda.paged import QuantizedPages, quantized_pages
 
 
@@ -206,4 +209,28 @@ def rotated(x: torch.Tensor, cos, sin, pos, interleaved: bool) -> torch.Tensor:
     c, s = cos[pos][:, None], sin[pos][:, None]
     y[..., a] = x[..., a] * c - x[..., b] * s
     y[..., b] = x[..., b] * c + x[..., a] * s
+    return y
+
+
+def workspace(x: QuantizedBatch, max_q: int, max_kv: int, window: int = 0) -> int:
+    """Bytes of workspace of a call: those of plain pages are in it where values are expanded first."""
+    k, s, q = x.k.codes, x.k.scales, x.q
+    fields = [k.data_ptr(), x.v.codes.data_ptr(), k.shape[0], k.stride(0), k.stride(1), k.stride(2), {"f32": 0, "f16": 7, "bf16": 8}[x.name],
+              k.shape[2], q.shape[2], k.shape[1], x.block_table.data_ptr(), x.block_table.stride(0), x.block_table.shape[1],
+              x.kv_lens.data_ptr(), x.q_starts.data_ptr(), len(x.qs), q.shape[0], 0, q.data_ptr(), q.stride(0), q.stride(1), q.shape[1],
+              q.data_ptr(), q.stride(0), q.stride(1), max_q, max_kv]
+    data = struct.pack(f"={len(fields)}q", *fields) + struct.pack("=d", 0.125) + struct.pack("=4q", 1, window, 0, 0)
+    data += struct.pack("=7q", x.bits, q.shape[2] // s.shape[3], s.data_ptr(), x.v.scales.data_ptr(), s.stride(0) // 2, s.stride(1) // 2,
+                        s.stride(2) // 2)
+    return library().mgc_cuda_paged_attention_quantized_workspace(data)
+
+
+def widened(x: QuantizedBatch) -> QuantizedBatch:
+    """The same batch with a block table of so many pages (none of them there) that a call without max_kv counts on long
+    contexts: with many query rows values are then expanded to plain pages first."""
+    width = max(1, (64 if x.q.shape[2] <= 64 else 128 if x.q.shape[2] <= 128 else 256) // 64)
+    positions = 6_000_000 // (len(x.qs) * x.k.codes.shape[2] * width)
+    y = copy.copy(x)
+    more = -(-positions // x.page)
+    y.block_table = torch.cat((x.block_table, torch.full((len(x.qs), more), -1, dtype=torch.int32, device=x.block_table.device)), 1)
     return y

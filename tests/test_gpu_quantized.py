@@ -13,7 +13,7 @@ torch = pytest.importorskip("torch")
 from mgc_cuda import paged  # noqa: E402
 from mgc_cuda._errors import GraphError  # noqa: E402
 from paged_cases import DTYPES, ROUND, PagedBatch, angles  # noqa: E402
-from quantized_cases import QuantizedBatch, attention, compare, normed, quantise, rotated, values  # noqa: E402
+from quantized_cases import QuantizedBatch, attention, compare, normed, quantise, rotated, values, widened, workspace  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -64,7 +64,7 @@ def test_append_writes_the_definition_s_codes(src, bits, dim, group, rot, interl
         qs, ks = [1, 37, 0, 5], [9, 37, 4, 70]
         x = QuantizedBatch(qs, ks, heads=6, kv_heads=2, dim=dim, page=16, dtype=src, bits=bits, group=group, layout=layout)
         before = [[t.clone() for t in (c.codes, c.scales)] for c in (x.k, x.v)]
-        q, k, v, got = append(x, qs, ks, src=src, norm=norm, rot=rot, interleaved=interleaved, seed=dim + rot, odd=odd)
+        q, k, v, got = append(x, qs, ks, src=src, norm=norm, rot=rot, interleaved=interleaved, seed=dim + rot, odd=odd, in_place=layout == "tokens")
         assert got.dtype == DTYPES[src]
         assert bool(((got.double() - q.double()).abs() <= ROUND[src] * q.double().abs() + 2.0**-25).all())
         for c, want, old in ((x.k, k, before[0]), (x.v, v, before[1])):
@@ -218,8 +218,26 @@ def attend(x: QuantizedBatch, **kw):
     return out
 
 
+def expands(x: QuantizedBatch) -> bool:
+    """Whether a call without max_kv goes over plain pages."""
+    capacity = x.block_table.shape[1] * x.page
+    return workspace(x, max(x.qs), capacity) >= 4 * len(x.qs) * capacity * x.q.shape[2]
+
+
+def many_rows(x: QuantizedBatch) -> bool:
+    """Whether there is a way over plain pages: 16 bits, rows enough (288: 18 units of codes against 48 of pages; sequences
+    of at most 64 stay on the codes), rows of q in 16 bytes; bf16 with the tcgen05 kernel alone; a head's pages in 1 GiB."""
+    return (x.name != "f32" and max(x.qs) * x.share >= 288 and x.q.data_ptr() % 16 == 0 and x.q.stride(0) % 8 == 0 and
+            not (x.name == "bf16" and (x.q.shape[2] > 128 or x.page % 8)) and x.k.codes.shape[2] > 1)
+
+
 def agree(x: QuantizedBatch, causal: bool = True, window: int = 0, **kw) -> None:
-    compare(attend(x, causal=causal, window=window, **kw), *attention(x, x.q.shape[2] ** -0.5, causal, window))
+    want, bound = attention(x, x.q.shape[2] ** -0.5, causal, window)
+    compare(attend(x, causal=causal, window=window, **kw), want, bound)
+    if many_rows(x) and not kw and not window:
+        y = widened(x)
+        assert expands(y)
+        compare(attend(y, causal=causal, max_q=max(x.qs), max_kv=None), want, bound)
 
 
 @pytest.mark.parametrize("dtype", ALL)
@@ -243,7 +261,7 @@ def test_head_groups(dtype, bits, heads, kv_heads) -> None:
 @pytest.mark.parametrize("dim,group", [(16, 16), (32, 32), (48, 48), (64, 64), (80, 80), (96, 96), (112, 112), (128, 64), (128, 128), (144, 144),
                                        (192, 64), (192, 192), (256, 64), (256, 128), (256, 256)])
 def test_head_widths_and_groups(dtype, bits, dim, group) -> None:
-    for qs, ks in (([1, 1], [150, 33]), ([5, 3], [150, 33]), ([130, 3], [150, 33])):
+    for qs, ks in (([1, 1], [150, 33]), ([5, 3], [150, 33]), ([150, 3], [150, 33])):
         agree(QuantizedBatch(qs, ks, heads=4, kv_heads=2, dim=dim, page=16, dtype=dtype, bits=bits, group=group, seed=dim, spread=1.7))
 
 
@@ -251,7 +269,7 @@ def test_head_widths_and_groups(dtype, bits, dim, group) -> None:
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("page", [1, 3, 8, 16, 24, 32, 48, 64, 100, 128, 256, 512])
 def test_page_sizes(dtype, bits, page) -> None:
-    for qs, ks in (([1, 1], [601, 130]), ([140, 70], [601, 130])):
+    for qs, ks in (([1, 1], [601, 130]), ([150, 70], [601, 130])):
         agree(QuantizedBatch(qs, ks, heads=4, kv_heads=2, dim=64, page=page, dtype=dtype, bits=bits, seed=page))
         agree(QuantizedBatch(qs, ks, heads=4, kv_heads=2, dim=128, page=page, dtype=dtype, bits=bits, seed=page))
 
@@ -261,7 +279,7 @@ def test_page_sizes(dtype, bits, page) -> None:
 @pytest.mark.parametrize("layout", ["heads", "tokens", "joint"])
 def test_cache_layouts_and_query_strides(dtype, bits, layout) -> None:
     for packed in (True, False):
-        for qs in ([1, 1], [200, 30]):
+        for qs in ([1, 1], [200, 30]):  # 600 rows: both ways
             for dim in (64, 80):
                 agree(QuantizedBatch(qs, [300, 31], heads=6, kv_heads=2, dim=dim, page=16, dtype=dtype, bits=bits, layout=layout, packed=packed))
     x = QuantizedBatch([1, 1], [300, 31], heads=6, kv_heads=2, dim=64, page=16, dtype=dtype, bits=bits, layout=layout)
@@ -286,6 +304,73 @@ def test_cache_layouts_and_query_strides(dtype, bits, layout) -> None:
 def test_ragged_batches(dtype, bits, qs, ks, causal) -> None:
     for kv_heads, dim in ((4, 64), (1, 128)):
         agree(QuantizedBatch(qs, ks, heads=4, kv_heads=kv_heads, dim=dim, page=16, dtype=dtype, bits=bits), causal=causal)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_many_rows_over_plain_pages(dtype, bits) -> None:
+    """What a batch may hold, in calls that expand values first: windows, missing pages, NaN, lengths past the table, rows
+    that no sequence has, sequences longer than max_kv says, single tokens beside chunks, key heads in passes."""
+
+    def batch(qs, ks, **kw):
+        return QuantizedBatch(qs, ks, **{**dict(heads=4, kv_heads=2, dim=64, page=16, dtype=dtype, bits=bits), **kw})
+
+    kw = dict(max_kv=None)
+    # windows that leave pages out, whose entries and rows hold anything
+    x = batch([300, 200, 1], [900, 333, 100])
+    # (the rule counts on the window's keys: a wide one)
+    want, bound = attention(x, 64**-0.5, True, 250)
+    for b, (nq, nk) in enumerate(zip(x.qs, x.ks)):
+        first = max(0, nk - nq - 250 + 1)
+        page, row = (t[:first] for t in x.slots[b])
+        for c in (x.k, x.v):
+            c.scales[page, row] = math.nan
+        x.block_table[b, : first // 16] = -1
+    compare(attend(widened(x), window=250, **kw), want, bound)
+    compare(attend(x, window=250), want, bound)
+    # missing pages
+    x = batch([300, 3, 290], [333, 90, 400])
+    present = [torch.ones(n, dtype=torch.bool, device="cuda") for n in x.ks]
+    for b, page, number in ((0, 3, -1), (0, 20, 10**6), (1, 0, -7), (2, 24, 10**9)):
+        x.block_table[b, page] = number
+        present[b][16 * page : 16 * page + 16] = False
+    y = widened(x)
+    assert expands(y)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = paged.paged_attention(y.q, *y.operands, max_q=300, status=status)
+    assert int(status) == 1
+    compare(got, *attention(x, 64**-0.5, present=present))
+    # NaN at the last but one position, and a group of one head
+    for what in ("k", "v"):
+        x = batch([300, 290], [300, 360], dim=128)
+        page, row = x.slots[0]
+        getattr(x, what).scales[page[298], row[298], :] = math.nan
+        page, row = x.slots[1]
+        getattr(x, what).scales[page[358], row[358], 1, 1] = math.nan
+        agree(x)
+    # lengths past the block table
+    x = batch([300, 2], [304, 40])
+    x.block_table = x.block_table[:, :19].contiguous()
+    x.kv_lens = i32(400, 40)
+    compare(paged.paged_attention(x.q, *x.operands, max_q=300, max_kv=400), *attention(x, 64**-0.5, lens=[400, 40]))
+    # rows that no sequence has
+    x = batch([300, 140], [330, 140])
+    want, bound = attention(x, 64**-0.5)
+    y = widened(x)
+    y.q = torch.cat((torch.full_like(x.q[:2], 9.0), x.q, torch.full_like(x.q[:3], math.nan)))
+    y.q_starts = x.q_starts + 2
+    out = torch.full_like(y.q, math.nan)
+    paged.paged_attention(y.q, *y.operands, max_q=300, out=out)
+    assert bool((out[:2] == 0).all()) and bool((out[-3:] == 0).all())
+    compare(out[2:-3], want, bound)
+    # a sequence longer than max_kv says, one that fits, single tokens
+    x = batch([700, 500, 1, 3], [6000, 1500, 900, 20], kv_heads=4, heads=8, dim=128)
+    compare(attend(x, max_kv=4000), *attention(x, 128**-0.5))
+    # key heads in two passes: 2^21 positions of 64 channels take 512 MiB a head
+    x = batch([300], [400], kv_heads=3, heads=3)
+    x.block_table = torch.nn.functional.pad(x.block_table, (0, (1 << 17) - x.block_table.shape[1]), value=-1)
+    assert expands(x) and workspace(x, 300, 1 << 21) < 3 * (1 << 29)
+    compare(attend(x, **kw), *attention(x, 64**-0.5))
 
 
 @pytest.mark.parametrize("dtype", ALL)
@@ -519,6 +604,29 @@ def test_graphs_and_other_streams(qs, ks) -> None:
         got = [attend(x) for x in batches]
     for a, b in zip(got, outs):
         assert torch.equal(a, b)
+
+
+def test_graphs_of_calls_that_expand() -> None:
+    x = [widened(QuantizedBatch([300, 1], [700, 90], heads=4, kv_heads=2, dim=64, page=16, dtype="bf16", bits=4, seed=s)) for s in (1, 2)]
+    assert all(expands(y) for y in x)
+    graphs, outs = [], []
+    for y in x:
+        attend(y, max_kv=None)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(paged.paged_attention(y.q, *y.operands, max_q=300))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in x]
+    for y in x:
+        y.q.mul_(0.5)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for y, out in zip(x, outs):
+        compare(out, *attention(y, 64**-0.5))
 
 
 def test_refusals() -> None:
