@@ -27,7 +27,7 @@ inline int check_attend_quantized(const mgc_cuda_paged_attention_quantized_args 
 // How a call runs.
 struct QuantPlan {
     int nb = 1;          // eights of query rows of a unit
-    int row_tiles = 1;
+    int row_tiles = 1, splits = 1;  // CTAs of a cluster that share a unit's keys
     bool even = false, interleaved = false;
     int ctas = 0, live_rows = 1;
     int64_t workspace = 0;  // of the part over codes
@@ -112,8 +112,16 @@ inline QuantPlan quant_plan_of(const mgc_cuda_paged_attention_quantized_args &a)
     const bool wide = aligned(a.attention.out, 4 * es) && a.attention.o_token_stride % 4 == 0 && a.attention.o_head_stride % 4 == 0;
     const int resident = with_config(c.dtype, a.quantized, c.head_dim, s.nb, [](auto config) { return decltype(config)::RESIDENT; });
     const int64_t slots = (int64_t)sm_count() * resident;
-    // Even shares cost a second kernel and the pieces' way through memory, some 500 keys' worth of time
-    if (wide && most > 512 + most * units / slots) {
+    // Few units: up to 8 CTAs of a cluster take equal parts of a unit's keys (one sequence of 1000 keys, 8 key heads of 128:
+    // 8.7 us, even shares 11.4). From an eighth of the GPU's blocks on clusters wait for room on one part of the GPU
+    // (16 x 500 keys of 12 key heads 15.9 us, a block a unit 9.7).
+    int64_t splits = units * 8 <= slots ? MAX_CLUSTER : 1;
+    if (splits > ceil_div(most, 128)) splits = most < 1 ? 1 : ceil_div(most, 128);
+    s.splits = (int)splits;
+    // Even shares leave no SM idle when sequences differ or 8 parts are too few; their second kernel and the pieces' way
+    // through memory take some 500 keys' worth of time
+    if (wide && most / splits > 512 + most * units / slots) {
+        s.splits = 1;
         s.even = true;
         s.ctas = (int)slots;
         if (slots >= c.kv_heads && slots / c.kv_heads * c.kv_heads * 20 >= slots * 19) {
@@ -170,17 +178,35 @@ inline int64_t attend_quantized_workspace(const mgc_cuda_paged_attention_quantiz
 
 template <typename C> inline int launch_quantized(const QuantParams &p, const QuantPlan &s, C, cudaStream_t stream) {
     if (s.even) {
-        auto kernel = quantized_attention_kernel<C, true>;
+        auto kernel = quantized_attention_kernel<C, WORK_EVEN>;
         MGC_CHECK(raise_smem_ceiling((const void *)kernel));
         kernel<<<(unsigned)s.ctas, C::THREADS, C::SMEM, stream>>>(p);
         MGC_CHECK(check_launch("quantized_attention_kernel"));
         return launch_after(paged_combine_units_kernel<typename C::T, C::R>, dim3((unsigned)s.ctas, (unsigned)s.live_rows), p.a,
                             s.interleaved ? p.a.kv_heads : 1, stream);
     }
-    auto kernel = quantized_attention_kernel<C, false>;
+    const unsigned units = (unsigned)(p.a.batch.batch * p.a.kv_heads * s.row_tiles);
+    if (s.splits == 1) {
+        auto kernel = quantized_attention_kernel<C, WORK_UNIT>;
+        MGC_CHECK(raise_smem_ceiling((const void *)kernel));
+        kernel<<<units, C::THREADS, C::SMEM, stream>>>(p);
+        return check_launch("quantized_attention_kernel");
+    }
+    auto kernel = quantized_attention_kernel<C, WORK_CLUSTER>;
     MGC_CHECK(raise_smem_ceiling((const void *)kernel));
-    kernel<<<(unsigned)(p.a.batch.batch * p.a.kv_heads * s.row_tiles), C::THREADS, C::SMEM, stream>>>(p);
-    return check_launch("quantized_attention_kernel");
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(units, (unsigned)s.splits);
+    cfg.blockDim = dim3(C::THREADS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = attr[0].val.clusterDim.z = 1;
+    attr[0].val.clusterDim.y = (unsigned)s.splits;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    MGC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+    return MGC_CUDA_OK;
 }
 
 // x / d = x * magic >> shift for 0 <= x < 2^31: with s = ceil(log2 d), ceil(2^(31 + s) / d) fits 32 bits and is exact.
@@ -238,6 +264,7 @@ inline int attend_quantized(const mgc_cuda_paged_attention_quantized_args &a, cu
         return fail(MGC_CUDA_UNSUPPORTED, "%s: %lld tokens of %d heads a key head", what, (long long)c.tokens, p.a.group);
     p.a.row_tiles = s.row_tiles;
     p.a.interleaved = s.interleaved;
+    p.a.splits = s.splits;
     if (s.total() && (!b.workspace || b.workspace_bytes < s.total() || !aligned(b.workspace, 16)))
         return fail(MGC_CUDA_NEEDS_WORKSPACE, "%s: needs %lld bytes of workspace (16-byte aligned), got %lld", what,
                     (long long)s.total(), (long long)(b.workspace ? b.workspace_bytes : 0));

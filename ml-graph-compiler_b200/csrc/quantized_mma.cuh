@@ -191,11 +191,14 @@ struct QuantParams {
     uint32_t code_page, code_token, pair_page, pair_token;
 };
 
-// EVEN: the CTA takes an even share of all units' keys (paged_work.cuh); else one unit's keys.
 __device__ __forceinline__ int lane_id() { return (int)(threadIdx.x & 31); }
-template <typename C, bool EVEN>
+// What a CTA takes: one unit's keys; the part of them that its rank in a cluster names; an even share of all units'
+// keys (paged_work.cuh).
+enum QuantWork { WORK_UNIT, WORK_CLUSTER, WORK_EVEN };
+template <typename C, int WORK>
 __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_kernel(const __grid_constant__ QuantParams params) {
     using T = typename C::T;
+    constexpr bool EVEN = WORK == WORK_EVEN;
     constexpr int BITS = C::BITS, DP = C::DP, NB = C::NB, R = C::R, BN = C::BN, KW = C::KW, PITCH = C::PITCH, CPR = C::CPR;
     constexpr int SLABS = C::SLABS, GS = C::GS, STAGES = C::STAGES;
     constexpr float LIFT = Weight<__half>::LAZY_LIFT, MOST = LIFT + Weight<__half>::LAZY, FRESH = 1e30f;
@@ -707,9 +710,9 @@ __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_k
         }
         __syncthreads();
         const int quads = p.head_dim / 4, live = min(R, rows - row0);
-        for (int x = tid; x < live * quads; x += C::THREADS) {
-            const int r = x / quads, c = x - r * quads;
-            float top = sm[r], sum = 0.0f;
+        auto warps_sum = [&](int r, int c, float &top, float &sum) {
+            top = sm[r];
+            sum = 0.0f;
 #pragma unroll
             for (int w = 1; w < C::WARPS; ++w) top = fmaxf(top, sm[w * R + r]);
             float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -723,22 +726,72 @@ __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_k
                 a.z += f * y.z;
                 a.w += f * y.w;
             }
-            if (!EVEN || slot < 0) {
-                const float inv = sum > 0.0f ? 1.0f / sum : sum != sum ? sum : 0.0f;
-                const int row = row0 + r;
-                T *out = static_cast<T *>(p.out) + (long long)(seq.start + row / p.group) * p.o_ts +
-                         (long long)(kh * p.group + row % p.group) * p.o_hs + c * 4;
-                out[0] = from_f<T>(a.x * inv);
-                out[1] = from_f<T>(a.y * inv);
-                out[2] = from_f<T>(a.z * inv);
-                out[3] = from_f<T>(a.w * inv);
-            } else {
-                const long long at = ((long long)blockIdx.x * 2 + slot) * R + r;
-                *reinterpret_cast<float4 *>(p.part + at * p.head_dim + c * 4) = a;
-                if (c == 0) p.part_ml[at] = make_float2(top, sum);
+            return a;
+        };
+        auto put = [&](int r, int c, float4 a, float sum) {
+            const float inv = sum > 0.0f ? 1.0f / sum : sum != sum ? sum : 0.0f;
+            const int row = row0 + r;
+            T *out = static_cast<T *>(p.out) + (long long)(seq.start + row / p.group) * p.o_ts +
+                     (long long)(kh * p.group + row % p.group) * p.o_hs + c * 4;
+            out[0] = from_f<T>(a.x * inv);
+            out[1] = from_f<T>(a.y * inv);
+            out[2] = from_f<T>(a.z * inv);
+            out[3] = from_f<T>(a.w * inv);
+        };
+        if constexpr (WORK != WORK_CLUSTER) {
+            for (int x = tid; x < live * quads; x += C::THREADS) {
+                const int r = x / quads, c = x - r * quads;
+                float top, sum;
+                const float4 a = warps_sum(r, c, top, sum);
+                if (!EVEN || slot < 0) {
+                    put(r, c, a, sum);
+                } else {
+                    const long long at = ((long long)blockIdx.x * 2 + slot) * R + r;
+                    *reinterpret_cast<float4 *>(p.part + at * p.head_dim + c * 4) = a;
+                    if (c == 0) p.part_ml[at] = make_float2(top, sum);
+                }
             }
+            __syncthreads();
+        } else {
+            // this CTA's sum over its first warp's rows (each four read and written by one thread), then the cluster's
+            float own_top = -INFINITY, own_sum = 0.0f;  // of row tid
+            if (tid < live) warps_sum(tid, 0, own_top, own_sum);
+            for (int x = tid; x < live * quads; x += C::THREADS) {
+                const int r = x / quads, c = x - r * quads;
+                float top, sum;
+                const float4 a = warps_sum(r, c, top, sum);
+                *reinterpret_cast<float4 *>(red + r * C::ORED + c * 4) = a;
+            }
+            __syncthreads();
+            if (tid < live) {
+                sm[tid] = own_top;
+                sl[tid] = own_sum;
+            }
+            cluster_barrier();
+            const uint32_t a_red = smem_u32(red), a_m = smem_u32(sm), a_l = smem_u32(sl);
+            for (int x = (int)blockIdx.y * C::THREADS + tid; x < live * quads; x += p.splits * C::THREADS) {
+                const int r = x / quads, c = x - r * quads;
+                float mk[MAX_CLUSTER], top = -INFINITY, sum = 0.0f;
+#pragma unroll
+                for (int k = 0; k < MAX_CLUSTER; ++k) mk[k] = k < p.splits ? ld_cluster(a_m + r * 4, k) : -INFINITY;
+#pragma unroll
+                for (int k = 0; k < MAX_CLUSTER; ++k) top = fmaxf(top, mk[k]);
+                float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int k = 0; k < MAX_CLUSTER; ++k) {
+                    if (k >= p.splits) break;
+                    const float f = top == -INFINITY ? 0.0f : ex2(mk[k] - top);
+                    const float4 v = ld_cluster4(a_red + (r * C::ORED + c * 4) * 4, k);
+                    sum += f * ld_cluster(a_l + r * 4, k);
+                    a.x += f * v.x;
+                    a.y += f * v.y;
+                    a.z += f * v.z;
+                    a.w += f * v.w;
+                }
+                put(r, c, a, sum);
+            }
+            cluster_barrier();  // every partial read before the next tile or the exit reuses it
         }
-        __syncthreads();
     };
 
     if constexpr (EVEN) {
@@ -769,11 +822,14 @@ __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_k
         const int b = (int)(u / (unsigned)p.row_tiles);
         const Sequence seq = load_sequence(p, b);
         if (tid == 0) check_sequence(p, b);
-        zero_outside_rows<T>(p, (int)blockIdx.x, (int)gridDim.x, warp, C::WARPS, lane);
+        zero_outside_rows<T>(p, (int)(blockIdx.y * gridDim.x + blockIdx.x), (int)(gridDim.x * gridDim.y), warp, C::WARPS, lane);
         for (int tile = tile0; tile * R < seq.nq * p.group; tile += p.row_tiles) {
             int first, lo, hi;
-            unit_length<R, BN>(p, seq, tile, first, lo, hi);
-            piece(b, kh, seq, tile * R, lo, hi, -1);
+            const int length = unit_length<R, BN>(p, seq, tile, first, lo, hi);
+            // this CTA's part of the tiles that some row of the unit sees
+            const int per = WORK == WORK_CLUSTER ? (length + p.splits - 1) / p.splits * BN : length * BN;
+            const int k_lo = lo + (WORK == WORK_CLUSTER ? (int)blockIdx.y * per : 0);
+            piece(b, kh, seq, tile * R, k_lo, min(hi, k_lo + per), -1);
         }
     }
 }
