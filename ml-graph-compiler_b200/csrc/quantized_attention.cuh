@@ -75,10 +75,9 @@ inline mgc_cuda_paged_attention_args expanded_args(const mgc_cuda_paged_attentio
 inline int width_of(int64_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 
 // Calls `go` with the configuration of a type, width, row tile and grouping.
-template <typename F> inline auto with_config(int64_t dtype, const mgc_cuda_quantized &z, int64_t head_dim, int nb, F go) {
-    auto widths = [&](auto type, auto b) {
+template <int BITS, typename F> inline auto with_config(int64_t dtype, const mgc_cuda_quantized &z, int64_t head_dim, int nb, F go) {
+    auto widths = [&](auto type) {
         using T = decltype(type);
-        constexpr int BITS = decltype(b)::value;
         const int dp = width_of(head_dim);
         if (dp == 64) return nb > 1 ? go(QuantConfig<T, BITS, 64, 2, true>()) : go(QuantConfig<T, BITS, 64, 1, true>());
         const bool one = z.group == head_dim;
@@ -86,11 +85,8 @@ template <typename F> inline auto with_config(int64_t dtype, const mgc_cuda_quan
         if (one) return nb > 1 ? go(QuantConfig<T, BITS, 128, 2, true>()) : go(QuantConfig<T, BITS, 128, 1, true>());
         return nb > 1 ? go(QuantConfig<T, BITS, 128, 2, false>()) : go(QuantConfig<T, BITS, 128, 1, false>());
     };
-    auto types = [&](auto b) {
-        if (dtype == MGC_F32) return widths(float(), b);
-        return dtype == MGC_F16 ? widths(__half(), b) : widths(__nv_bfloat16(), b);
-    };
-    return z.bits == 4 ? types(std::integral_constant<int, 4>()) : types(std::integral_constant<int, 8>());
+    if (dtype == MGC_F32) return widths(float());
+    return dtype == MGC_F16 ? widths(__half()) : widths(__nv_bfloat16());
 }
 
 inline QuantPlan quant_plan_of(const mgc_cuda_paged_attention_quantized_args &a) {
@@ -110,7 +106,9 @@ inline QuantPlan quant_plan_of(const mgc_cuda_paged_attention_quantized_args &a)
     // the kernel that adds pieces stores four elements at once
     const int es = elem_size(c.dtype);
     const bool wide = aligned(a.attention.out, 4 * es) && a.attention.o_token_stride % 4 == 0 && a.attention.o_head_stride % 4 == 0;
-    const int resident = with_config(c.dtype, a.quantized, c.head_dim, s.nb, [](auto config) { return decltype(config)::RESIDENT; });
+    auto held = [](auto config) { return decltype(config)::RESIDENT; };
+    const int resident = a.quantized.bits == 4 ? with_config<4>(c.dtype, a.quantized, c.head_dim, s.nb, held)
+                                               : with_config<8>(c.dtype, a.quantized, c.head_dim, s.nb, held);
     const int64_t slots = (int64_t)sm_count() * resident;
     // Few units: up to 8 CTAs of a cluster take equal parts of a unit's keys (one sequence of 1000 keys, 8 key heads of 128:
     // 8.7 us, even shares 11.4). From an eighth of the GPU's blocks on clusters wait for room on one part of the GPU
@@ -176,38 +174,8 @@ inline int64_t attend_quantized_workspace(const mgc_cuda_paged_attention_quantiz
     return a.attention.paged.tokens == 0 || a.attention.paged.batch == 0 ? 0 : quant_plan_of(a).total();
 }
 
-template <typename C> inline int launch_quantized(const QuantParams &p, const QuantPlan &s, C, cudaStream_t stream) {
-    if (s.even) {
-        auto kernel = quantized_attention_kernel<C, WORK_EVEN>;
-        MGC_CHECK(raise_smem_ceiling((const void *)kernel));
-        kernel<<<(unsigned)s.ctas, C::THREADS, C::SMEM, stream>>>(p);
-        MGC_CHECK(check_launch("quantized_attention_kernel"));
-        return launch_after(paged_combine_units_kernel<typename C::T, C::R>, dim3((unsigned)s.ctas, (unsigned)s.live_rows), p.a,
-                            s.interleaved ? p.a.kv_heads : 1, stream);
-    }
-    const unsigned units = (unsigned)(p.a.batch.batch * p.a.kv_heads * s.row_tiles);
-    if (s.splits == 1) {
-        auto kernel = quantized_attention_kernel<C, WORK_UNIT>;
-        MGC_CHECK(raise_smem_ceiling((const void *)kernel));
-        kernel<<<units, C::THREADS, C::SMEM, stream>>>(p);
-        return check_launch("quantized_attention_kernel");
-    }
-    auto kernel = quantized_attention_kernel<C, WORK_CLUSTER>;
-    MGC_CHECK(raise_smem_ceiling((const void *)kernel));
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(units, (unsigned)s.splits);
-    cfg.blockDim = dim3(C::THREADS);
-    cfg.dynamicSmemBytes = C::SMEM;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = attr[0].val.clusterDim.z = 1;
-    attr[0].val.clusterDim.y = (unsigned)s.splits;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    MGC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
-    return MGC_CUDA_OK;
-}
+// The kernels for codes of BITS bits, compiled in files of their own (quantized_4.cu, quantized_8.cu).
+template <int BITS> int launch_codes(const QuantParams &p, const QuantPlan &s, int64_t dtype, const mgc_cuda_quantized &z, cudaStream_t stream);
 
 // x / d = x * magic >> shift for 0 <= x < 2^31: with s = ceil(log2 d), ceil(2^(31 + s) / d) fits 32 bits and is exact.
 inline void division(int64_t d, uint32_t &magic, int &shift) {
@@ -293,7 +261,7 @@ inline int attend_quantized(const mgc_cuda_paged_attention_quantized_args &a, cu
     p.pairs_wide = p.z.groups == 2 && c.head_dim == 128 && aligned(p.z.k_scales, 8) && aligned(p.z.v_scales, 8) &&
                    p.z.page_stride % 2 == 0 && p.z.token_stride % 2 == 0 && p.z.head_stride % 2 == 0;
     p.q_wide = aligned(b.q, 16) && b.q_token_stride % chunk == 0 && b.q_head_stride % chunk == 0;
-    return with_config(c.dtype, a.quantized, c.head_dim, s.nb, [&](auto config) { return launch_quantized(p, s, config, stream); });
+    return a.quantized.bits == 4 ? launch_codes<4>(p, s, c.dtype, a.quantized, stream) : launch_codes<8>(p, s, c.dtype, a.quantized, stream);
 }
 
 }  // namespace paged
