@@ -584,7 +584,8 @@ paged_attention_umma_kernel(const __grid_constant__ AttendParams p, const __grid
                         v[i] = as_pages<T, O>(v[i], __uint_as_float((uint32_t)(127 + up) << 23));
                         // rows 32 / CHUNKS i .. of the warp are these lanes': theirs takes the scale along
                         const int mine = __shfl_sync(0xFFFFFFFFu, up, (lane * CHUNKS) % 32);
-                        if (lane * CHUNKS / 32 == i) scale_log2 = p.scale_log2 * __uint_as_float((uint32_t)(127 - mine) << 23);
+                        if (lane * CHUNKS / 32 == i)  // (not 0, which times the -inf of hidden keys would be NaN)
+                            scale_log2 = fmaxf(p.scale_log2 * __uint_as_float((uint32_t)(127 - mine) << 23), 1.2e-38f);
                     }
                 }
 #pragma unroll

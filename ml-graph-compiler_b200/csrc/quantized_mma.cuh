@@ -191,7 +191,6 @@ struct QuantParams {
     uint32_t code_page, code_token, pair_page, pair_token;
 };
 
-__device__ __forceinline__ int lane_id() { return (int)(threadIdx.x & 31); }
 // What a CTA takes: one unit's keys; the part of them that its rank in a cluster names; an even share of all units'
 // keys (paged_work.cuh).
 enum QuantWork { WORK_UNIT, WORK_CLUSTER, WORK_EVEN };
@@ -210,7 +209,7 @@ __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_k
     __shared__ uint32_t there[C::WARPS][STAGES];  // keys of a stage that were loaded
     __shared__ float row_scale[R], row_sum[R][GS];  // of Q's rows: what takes a score to base 2, the groups' sums
     __shared__ RowRange row_sees[R];
-    uint4 *q_upper = reinterpret_cast<uint4 *>(smem + C::Q_AT) + lane_id(), *q_lower = q_upper + C::Q / 16;
+    uint4 *q_upper = reinterpret_cast<uint4 *>(smem + C::Q_AT) + (threadIdx.x & 31), *q_lower = q_upper + C::Q / 16;
     const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g4 = lane >> 2, t4 = lane & 3;
     const int key0 = g4 & 1 ? C::second(g4 >> 1) : C::first(g4 >> 1);  // row of fragment key g4 among its eight
@@ -362,7 +361,8 @@ __global__ void __launch_bounds__(C::THREADS, C::RESIDENT) quantized_attention_k
                 if (t4 == 0) row_sum[8 * nb + g4][x] = sum[x];
             }
             if (t4 == 0) {
-                row_scale[8 * nb + g4] = p.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
+                // (not 0, which times the -inf of hidden keys would be NaN)
+                row_scale[8 * nb + g4] = fmaxf(p.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23), 1.2e-38f);
                 row_sees[8 * nb + g4] = row_range(p, seq, row);
             }
         }

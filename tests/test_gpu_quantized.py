@@ -531,6 +531,18 @@ def test_sizes_of_values_that_differ_by_thousands(dtype) -> None:
         agree(x)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_scale_that_vanishes(dtype) -> None:
+    """Scores that are 0 in fp32: weights are equal, and hidden keys stay hidden."""
+    for qs, ks in (([3, 1], [40, 200]), ([300, 2], [333, 90])):
+        x = QuantizedBatch(qs, ks, heads=4, kv_heads=2, dim=64, page=16, dtype=dtype, bits=4)
+        x.q = x.q * 1e-25
+        want, bound = attention(x, 1e-25)
+        compare(attend(x, scale=1e-25), want, bound)
+        if many_rows(x):
+            compare(attend(widened(x), scale=1e-25, max_kv=None), want, bound)
+
+
 def test_scale_and_masked_rows_of_every_kind() -> None:
     x = QuantizedBatch([4, 3], [2, 300], heads=4, kv_heads=2, dim=64, page=16, dtype="f16", bits=8)
     compare(attend(x, scale=0.01), *attention(x, 0.01))
