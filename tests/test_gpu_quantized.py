@@ -543,6 +543,45 @@ def test_a_scale_that_vanishes(dtype) -> None:
             compare(attend(widened(x), scale=1e-25, max_kv=None), want, bound)
 
 
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("bits", [4, 8])
+def test_a_long_tail_far_below_one_key(dtype, bits) -> None:
+    """One key 17 above 16383 others, whose weights are 2^-24.5 of its own, with a value of 0: the output is theirs."""
+    for qs in ([1], [2]):
+        x = QuantizedBatch(qs, [16384], heads=2, kv_heads=1, dim=64, page=64, dtype=dtype, bits=bits, gain=0.05)
+        x.q[:] = x.q[:1, :1]
+        q = x.q[0, 0].float()
+        page, row = (t[100] for t in x.slots[0])
+        x.v.scales[page, row] = 0.0
+        x.k.codes[page, row, 0], x.k.scales[page, row, 0] = quantise(q * (17.0 * 8.0 / float(q.square().sum())), bits, 64)
+        agree(x)
+
+
+def test_offsets_that_pass_32_bits() -> None:
+    """Pages 2 GiB apart: codes 4 GiB and scales 4 GiB from the first page."""
+    dim, page, far = 64, 16, 1 << 31
+
+    def pages():
+        codes = torch.empty(2 * far + (1 << 20), dtype=torch.uint8, device="cuda").as_strided((3, page, 2, dim // 2), (far, 64, 32, 1))
+        scales = torch.empty(far + (1 << 20), dtype=torch.float16, device="cuda").as_strided((3, page, 2, 1, 2), (far // 2, 4, 2, 2, 1))
+        return paged.QuantizedPages(codes, scales, 4)
+
+    x = QuantizedBatch([20, 1], [20, 11], heads=4, kv_heads=2, dim=dim, page=page, dtype="f16", bits=4)
+    x.k, x.v = pages(), pages()
+    x.block_table = torch.tensor([[2, 0], [1, -1]], dtype=torch.int32, device="cuda")
+    x.slots = [(torch.tensor([2] * 16 + [0] * 4, device="cuda"), torch.tensor([*range(16), *range(4)], device="cuda")),
+               (torch.full((11,), 1, device="cuda"), torch.arange(11, device="cuda"))]
+    k, v = (torch.randn(31, 2, dim, device="cuda").half() for _ in range(2))
+    at = (x.block_table, x.kv_lens, i32(0, 20, 31))
+    paged.kv_append(k, v, x.k, x.v, *at)
+    got = paged.kv_read(x.k, x.v, *at, rows=31)
+    for src, back, c in ((k, got[0], x.k), (v, got[1], x.v)):
+        codes, scales = quantise(src.float(), 4, dim)
+        assert torch.equal(back, values(codes, scales, 4, torch.float32).half())
+        assert torch.equal(c.codes[x.slots[0]], codes[:20]) and torch.equal(c.scales[x.slots[1]], scales[20:])
+    compare(attend(x), *attention(x, dim**-0.5))
+
+
 def test_scale_and_masked_rows_of_every_kind() -> None:
     x = QuantizedBatch([4, 3], [2, 300], heads=4, kv_heads=2, dim=64, page=16, dtype="f16", bits=8)
     compare(attend(x, scale=0.01), *attention(x, 0.01))
